@@ -1,4 +1,4 @@
-"""ctypes binding of include/mi_moe.h (one function per exported symbol)."""
+"""ctypes binding of include/mi_moe.h and include/mi_moe_layer.h (one function per exported symbol)."""
 import ctypes as C
 import os
 
@@ -9,6 +9,8 @@ SCORE_SOFTMAX_THEN_TOPK_RENORM = 0
 SCORE_SOFTMAX_THEN_TOPK = 1
 SCORE_TOPK_THEN_SOFTMAX = 2
 DTYPE_BF16, DTYPE_F16, DTYPE_F32 = 0, 1, 2
+SCORING_SOFTMAX, SCORING_SIGMOID = 0, 1
+GROUP_SCORE_MAX, GROUP_SCORE_TOP2 = 0, 1
 N_STAGES = 6
 N_KERNEL_TIMES = 8
 KERNEL_NAMES = ("gate_up_tiles256", "gate_up_tiles128", "gate_up_tiles64", "gate_up_streamed",
@@ -31,6 +33,12 @@ EXPORTS = (
     "mi_moe_debug_kernel_count", "mi_moe_debug_kernel_name", "mi_moe_debug_kernel_launches", "mi_moe_debug_plan_forward", "mi_moe_debug_plan_grouped",
     "mi_moe_debug_side_streams_created", "mi_moe_debug_tile_rule",
     "mi_moe_router_logits_workspace_size", "mi_moe_router_logits",
+)
+# and include/mi_moe_layer.h
+LAYER_EXPORTS = (
+    "mi_moe_add_rms_norm", "mi_moe_add_rms_norm_rows8", "mi_moe_add_rms_norm_grad_workspace_size", "mi_moe_add_rms_norm_grad",
+    "mi_moe_forward_routed", "mi_moe_select_experts", "mi_moe_select_experts_grad",
+    "mi_moe_quantized_linear_rows8_workspace_size", "mi_moe_quantized_linear_rows8",
 )
 
 
@@ -121,6 +129,15 @@ def load_library():
         "mi_moe_dequantize_typed": [vp, vp, vp, i64, i64, i32, i32, i32, vp, vp],
         "mi_moe_dequantize_native": [vp, vp, vp, i64, i64, i32, i32, i32, vp, vp],
         "mi_moe_quantized_linear_typed": [vp, vp, vp, vp, vp, i64, i32, i32, i32, i32, i32, vp, vp, sz, vp],
+        "mi_moe_add_rms_norm": [vp, vp, vp, C.c_float, i64, i32, i32, vp, vp, vp],
+        "mi_moe_add_rms_norm_rows8": [vp, vp, vp, C.c_float, i64, i32, i32, vp, vp, vp, vp],
+        "mi_moe_add_rms_norm_grad_workspace_size": [i64, i32, C.POINTER(sz)],
+        "mi_moe_add_rms_norm_grad": [vp, vp, vp, vp, C.c_float, i64, i32, i32, vp, vp, vp, sz, vp],
+        "mi_moe_forward_routed": [vp, vp, vp, vp, i64, vp, vp, sz, C.POINTER(DebugOut), vp],
+        "mi_moe_select_experts": [vp, i32, vp, i64, i32, i32, i32, i32, i32, i32, i32, C.c_float, vp, vp, i32, vp],
+        "mi_moe_select_experts_grad": [vp, i32, vp, i32, vp, i64, i32, i32, i32, i32, C.c_float, vp, vp],
+        "mi_moe_quantized_linear_rows8_workspace_size": [i64, i32, C.POINTER(sz)],
+        "mi_moe_quantized_linear_rows8": [vp, vp, vp, vp, vp, vp, i64, i32, i32, i32, i32, i32, vp, vp, sz, vp],
         "mi_moe_debug_plan_forward": [C.POINTER(Config), i64, C.c_char_p, sz],
         "mi_moe_debug_tile_rule": [C.POINTER(Config), i64, C.POINTER(i32), C.POINTER(i32)],
         "mi_moe_debug_plan_grouped": [i32, i32, i32, i32, i64, i32, i64, i64, i32, i32, C.c_char_p, sz],

@@ -1,6 +1,6 @@
 // C ABI of libmi_moe: validation, workspace carving and the launch sequence of the block.
-// Declarations and the reference interfaces they replace: include/mi_moe.h.
-#include "../../include/mi_moe.h"
+// Declarations and the reference interfaces they replace: include/mi_moe.h, include/mi_moe_layer.h.
+#include "../../include/mi_moe_layer.h"
 
 #include <atomic>
 #include <cstdarg>
@@ -577,7 +577,7 @@ static void grouped_args(const mi_moe_config &c, const mi_moe_weights &w, const 
 static int forward_impl(mi_moe_handle h, const uint16_t *x_in, int64_t T, uint16_t *out, void *workspace,
                         size_t workspace_bytes, const mi_moe_debug_out *dbg, hipStream_t st,
                         hipEvent_t *ev, const uint16_t *norm_weight = nullptr, float eps = 0.f,
-                        KernelTimer *kt = nullptr) {
+                        KernelTimer *kt = nullptr, const uint32_t *given_idx = nullptr, const uint16_t *given_w = nullptr) {
   const uint16_t *x = x_in;
   if (!h) return fail("forward: handle is NULL");
   if (T < 0) return fail("forward: negative token count");
@@ -608,7 +608,7 @@ static int forward_impl(mi_moe_handle h, const uint16_t *x_in, int64_t T, uint16
     if (ev) MI_HIP(hipEventRecord(ev[++stage], st));     \
   } while (0)
   if (ev) MI_HIP(hipEventRecord(ev[0], st));
-  const bool fused_router = router_fused_applies(T, c.n_experts, c.top_k);
+  const bool fused_router = !given_idx && router_fused_applies(T, c.n_experts, c.top_k);
   const bool mid = f.mid, raw_codes = mid || f.pieces;
   uint32_t *const tile_lists = f.tiled && !raw_codes ? f.mtiles : nullptr;
   const int tile_cap = f.max_mtiles, tile_from = f.tmr;
@@ -624,7 +624,7 @@ static int forward_impl(mi_moe_handle h, const uint16_t *x_in, int64_t T, uint16
   // registers anyway, or by a kernel of its own (light batches pair the rows beside their streamed segments)
   const bool paired = c.bits == 4;
   const bool streamed_first = f.tiled && !f.heavy && !ev && !mid;  // light batches start their streamed segments first
-  const bool pair_in_router = f.tiled && paired && !raw_codes && !streamed_first && !fused_router && !plain_config(c) &&
+  const bool pair_in_router = f.tiled && paired && !raw_codes && !streamed_first && !fused_router && !given_idx && !plain_config(c) &&
                               router_logits_pairs_rows(T, c.hidden);
   if (fused_router) {
     // decode: one launch for the three stages (the stage times then all land in the first)
@@ -642,7 +642,9 @@ static int forward_impl(mi_moe_handle h, const uint16_t *x_in, int64_t T, uint16
     // included; a block's phases follow each other, and there are T / 32 blocks) 41.3 / 41.9 / 45.2 / 49.5.
     const int64_t logit_work = T * (int64_t)c.hidden * ((c.n_experts + 127) / 128);
     const bool i8_pays = f.router_scratch && logit_work >= (int64_t)3 << 20;
-    if (i8_pays && logit_work >= (int64_t)12 << 20 && router_tile_applies(T, c.hidden, c.n_experts, c.top_k)) {
+    if (given_idx) {
+      MI_HIP(launch_check_routing(given_idx, given_w, T, c.n_experts, c.top_k, f.topk_idx, f.topk_w, st));
+    } else if (i8_pays && logit_work >= (int64_t)12 << 20 && router_tile_applies(T, c.hidden, c.n_experts, c.top_k)) {
       // logits and selection in one kernel (the stage times both land in the first)
       MI_HIP(launch_router_tile(x, h->w.router_w, h->w.router_bias, T, c.hidden, c.n_experts, c.top_k, c.score_mode,
                                 f.logits, f.topk_idx, f.topk_w, f.router_scratch, st, pair_in_router ? f.xperm : nullptr));
@@ -933,6 +935,119 @@ int mi_moe_forward_residual(mi_moe_handle h, const uint16_t *x, const uint16_t *
   return forward_impl(h, x, T, out, workspace, workspace_bytes, dbg, static_cast<hipStream_t>(stream), nullptr,
                       norm_weight, eps);
 } MI_CATCH("forward_residual")
+
+int mi_moe_forward_routed(mi_moe_handle h, const uint16_t *x, const uint32_t *topk_idx, const uint16_t *topk_w, int64_t T, uint16_t *out, void *workspace,
+                          size_t workspace_bytes, const mi_moe_debug_out *dbg, void *stream) try {
+  if (T > 0 && (!topk_idx || !topk_w)) return fail("forward_routed: topk_idx and topk_w must be non-NULL");
+  return forward_impl(h, x, T, out, workspace, workspace_bytes, dbg, static_cast<hipStream_t>(stream), nullptr, nullptr, 0.f, nullptr, topk_idx, topk_w);
+} MI_CATCH("forward_routed")
+
+static int check_dtype(const char *who, int32_t dtype);
+
+static int check_norm(const char *who, float eps, int64_t T, int32_t hidden, int32_t dtype) {
+  if (T < 0 || T > (int64_t)1 << 30) return fail("%s: row count out of range", who);
+  if (hidden < 1 || hidden > kNormMostHidden) return fail("%s: hidden must be in [1, %d], got %d", who, kNormMostHidden, hidden);
+  if (!(eps >= 0.f)) return fail("%s: eps must be non-negative", who);
+  return check_dtype(who, dtype);
+}
+
+int mi_moe_add_rms_norm(const void *x, const void *residual, const void *weight, float eps, int64_t T, int32_t hidden, int32_t dtype, void *sum, void *y,
+                        void *stream) try {
+  if (check_norm("add_rms_norm", eps, T, hidden, dtype)) return 1;
+  if (T == 0) return 0;
+  if (!x || !weight || !y) return fail("add_rms_norm: x, weight and y must be non-NULL");
+  if (residual && !sum) return fail("add_rms_norm: sum must be non-NULL where a residual is added");
+  MI_HIP(launch_add_rms_norm(x, residual, weight, eps, T, hidden, dtype, sum, y, nullptr, static_cast<hipStream_t>(stream)));
+  return 0;
+} MI_CATCH("add_rms_norm")
+
+int mi_moe_add_rms_norm_rows8(const void *x, const void *residual, const void *weight, float eps, int64_t T, int32_t hidden, int32_t dtype, void *sum,
+                              void *rows8, float *row_scales, void *stream) try {
+  if (check_norm("add_rms_norm_rows8", eps, T, hidden, dtype)) return 1;
+  if (T == 0) return 0;
+  if (!x || !weight || !rows8 || !row_scales) return fail("add_rms_norm_rows8: x, weight, rows8 and row_scales must be non-NULL");
+  if (residual && !sum) return fail("add_rms_norm_rows8: sum must be non-NULL where a residual is added");
+  MI_HIP(launch_add_rms_norm(x, residual, weight, eps, T, hidden, dtype, sum, rows8, row_scales, static_cast<hipStream_t>(stream)));
+  return 0;
+} MI_CATCH("add_rms_norm_rows8")
+
+int mi_moe_add_rms_norm_grad_workspace_size(int64_t T, int32_t hidden, size_t *bytes) try {
+  if (!bytes) return fail("add_rms_norm_grad_workspace_size: bytes is NULL");
+  if (T < 0 || T > (int64_t)1 << 30 || hidden < 1 || hidden > kNormMostHidden) return fail("add_rms_norm_grad_workspace_size: bad sizes");
+  *bytes = norm_grad_bytes(T, hidden);
+  return 0;
+} MI_CATCH("add_rms_norm_grad_workspace_size")
+
+int mi_moe_add_rms_norm_grad(const void *dy, const void *sum, const void *dsum, const void *weight, float eps, int64_t T, int32_t hidden, int32_t dtype,
+                             void *dx, void *dweight, void *workspace, size_t workspace_bytes, void *stream) try {
+  if (check_norm("add_rms_norm_grad", eps, T, hidden, dtype)) return 1;
+  if (!dweight) return fail("add_rms_norm_grad: dweight must be non-NULL");
+  if (T > 0 && (!dy || !sum || !weight || !dx)) return fail("add_rms_norm_grad: dy, sum, weight and dx must be non-NULL");
+  const size_t need = norm_grad_bytes(T, hidden);
+  if (T > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need))
+    return fail("add_rms_norm_grad: workspace must be 16-byte aligned and hold %zu bytes, got %zu", need, workspace ? workspace_bytes : 0);
+  MI_HIP(launch_norm_grad(dy, sum, dsum, weight, eps, T, hidden, dtype, dx, dweight, static_cast<float *>(workspace), static_cast<hipStream_t>(stream)));
+  return 0;
+} MI_CATCH("add_rms_norm_grad")
+
+static int check_select(const char *who, int32_t dtype, int32_t w_dtype, int64_t T, int32_t n_experts, int32_t top_k, int32_t scoring, float scale) {
+  if (check_dtype(who, dtype) || check_dtype(who, w_dtype)) return 1;
+  if (T < 0 || T > (int64_t)1 << 30) return fail("%s: token count out of range", who);
+  if (n_experts < 1 || n_experts > 512) return fail("%s: n_experts must be in [1, 512], got %d", who, n_experts);
+  if (top_k < 1 || top_k > n_experts || top_k > 32) return fail("%s: top_k must be in [1, min(n_experts, 32)], got %d", who, top_k);
+  if (scoring != MI_MOE_SCORING_SOFTMAX && scoring != MI_MOE_SCORING_SIGMOID) return fail("%s: unknown scoring %d", who, scoring);
+  if (!(scale - scale == 0.f)) return fail("%s: scale must be finite", who);
+  return 0;
+}
+
+int mi_moe_select_experts(const void *logits, int32_t dtype, const float *bias, int64_t T, int32_t n_experts, int32_t top_k, int32_t scoring, int32_t n_groups,
+                          int32_t top_groups, int32_t group_score, int32_t renormalize, float scale, uint32_t *topk_idx, void *topk_w, int32_t w_dtype,
+                          void *stream) try {
+  if (check_select("select_experts", dtype, w_dtype, T, n_experts, top_k, scoring, scale)) return 1;
+  if (n_groups < 1 || n_groups > 64 || n_experts % n_groups)
+    return fail("select_experts: n_groups must be in [1, 64] and divide n_experts (%d), got %d", n_experts, n_groups);
+  if (top_groups < 1 || top_groups > n_groups) return fail("select_experts: top_groups must be in [1, n_groups], got %d", top_groups);
+  if (top_k > top_groups * (n_experts / n_groups))
+    return fail("select_experts: top_k (%d) is more than the open groups hold (%d)", top_k, top_groups * (n_experts / n_groups));
+  if (group_score != MI_MOE_GROUP_SCORE_MAX && group_score != MI_MOE_GROUP_SCORE_TOP2) return fail("select_experts: unknown group_score %d", group_score);
+  if (T == 0) return 0;
+  if (!logits || !topk_idx || !topk_w) return fail("select_experts: logits, topk_idx and topk_w must be non-NULL");
+  const SelectArgs a{logits, bias, T, n_experts, top_k, scoring, n_groups, top_groups, group_score, renormalize, scale, topk_idx, topk_w, w_dtype};
+  MI_HIP(launch_select_experts(a, dtype, static_cast<hipStream_t>(stream)));
+  return 0;
+} MI_CATCH("select_experts")
+
+int mi_moe_select_experts_grad(const void *dw, int32_t w_dtype, const void *logits, int32_t dtype, const uint32_t *topk_idx, int64_t T, int32_t n_experts,
+                               int32_t top_k, int32_t scoring, int32_t renormalize, float scale, void *dlogits, void *stream) try {
+  if (check_select("select_experts_grad", dtype, w_dtype, T, n_experts, top_k, scoring, scale)) return 1;
+  if (T == 0) return 0;
+  if (!dw || !logits || !topk_idx || !dlogits) return fail("select_experts_grad: dw, logits, topk_idx and dlogits must be non-NULL");
+  const SelectGradArgs a{dw, logits, topk_idx, T, n_experts, top_k, scoring, renormalize, scale, dlogits, w_dtype};
+  MI_HIP(launch_select_grad(a, dtype, static_cast<hipStream_t>(stream)));
+  return 0;
+} MI_CATCH("select_experts_grad")
+
+int mi_moe_quantized_linear_rows8_workspace_size(int64_t M, int32_t K, size_t *bytes) try {
+  if (!bytes) return fail("quantized_linear_rows8_workspace_size: bytes is NULL");
+  if (M < 0 || K <= 0 || M * (int64_t)K > (int64_t)1 << 40) return fail("quantized_linear_rows8_workspace_size: bad sizes");
+  *bytes = 0;
+  return 0;
+} MI_CATCH("quantized_linear_rows8_workspace_size")
+
+int mi_moe_quantized_linear_rows8(const void *x, const float *row_scales, const uint32_t *w, const void *scales, const void *biases, const void *linear_bias,
+                                  int64_t M, int32_t N, int32_t K, int32_t group_size, int32_t bits, int32_t dtype, void *y, void *workspace,
+                                  size_t workspace_bytes, void *stream) try {
+  if (check_dtype("quantized_linear_rows8", dtype)) return 1;
+  if (bits != 4 && bits != 8) return fail("quantized_linear_rows8: bits must be 4 or 8, got %d", bits);
+  if (group_size != 32 && group_size != 64 && group_size != 128) return fail("quantized_linear_rows8: group_size must be 32, 64 or 128, got %d", group_size);
+  if (N < 1 || K < 1 || K % group_size) return fail("quantized_linear_rows8: N must be positive and K a positive multiple of group_size, got N = %d, K = %d", N, K);
+  if (M < 0 || M > (int64_t)1 << 30) return fail("quantized_linear_rows8: row count out of range");
+  if (M == 0) return 0;
+  if (!x || !row_scales || !w || !scales || !biases || !y) return fail("quantized_linear_rows8: x, row_scales, w, scales, biases and y must be non-NULL");
+  const Rows8Args a{static_cast<const signed char *>(x), row_scales, w, scales, biases, linear_bias, y, M, N, K, group_size};
+  MI_HIP(launch_qmm_rows8(a, bits, dtype, static_cast<hipStream_t>(stream)));
+  return 0;
+} MI_CATCH("quantized_linear_rows8")
 
 int mi_moe_rms_norm(const uint16_t *x, const uint16_t *weight, float eps, int64_t T, int32_t hidden,
                     uint16_t *out, void *stream) try {

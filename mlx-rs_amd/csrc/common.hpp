@@ -446,5 +446,47 @@ hipError_t launch_dequantize(const uint32_t *q, const void *s, const void *b,
                              int64_t rows, int64_t cols, int group, int bits, void *out, int dt, bool native_out,
                              hipStream_t st);
 hipError_t launch_add_row_bias(void *y, const void *bias, int64_t M, int N, int dt, hipStream_t st);
+// The residual's addition and the norm behind it (norm.hip); dt: mi_moe_dtype.  scales: rows in eight bits, or nullptr.
+hipError_t launch_add_rms_norm(const void *x, const void *r, const void *w, float eps, int64_t T, int H, int dt, void *sum, void *y, float *scales,
+                               hipStream_t st);
+size_t norm_grad_bytes(int64_t T, int H);  // parts
+hipError_t launch_norm_grad(const void *dy, const void *h, const void *dh, const void *w, float eps, int64_t T, int H, int dt, void *dx, void *dw,
+                            float *parts, hipStream_t st);
+constexpr int kNormMostHidden = 32768;  // a row stays in the registers of 1024 threads
+// Experts from logits (select.hip); scoring, group_score: mi_moe_scoring, mi_moe_group_score.
+struct SelectArgs {
+  const void *logits;
+  const float *bias;
+  int64_t T;
+  int E, k, scoring, groups, top_groups, group_score, renormalize;
+  float scale;
+  uint32_t *idx;
+  void *w;
+  int w_dtype;
+};
+hipError_t launch_select_experts(const SelectArgs &a, int dt, hipStream_t st);
+struct SelectGradArgs {
+  const void *dw, *logits;
+  const uint32_t *idx;
+  int64_t T;
+  int E, k, scoring, renormalize;
+  float scale;
+  void *dlogits;
+  int w_dtype;
+};
+hipError_t launch_select_grad(const SelectGradArgs &a, int dt, hipStream_t st);
+// A caller's routing as the block takes it: k different experts a token.
+hipError_t launch_check_routing(const uint32_t *idx, const uint16_t *w, int64_t T, int E, int k, uint32_t *idx_out, uint16_t *w_out, hipStream_t st);
+// The linear layer on rows in eight bits (qmm_rows8.hip).
+struct Rows8Args {
+  const signed char *x;
+  const float *row_scales;
+  const uint32_t *w;
+  const void *s, *b, *bias;
+  void *y;
+  int64_t M;
+  int N, K, group;
+};
+hipError_t launch_qmm_rows8(const Rows8Args &a, int bits, int dt, hipStream_t st);
 
 }  // namespace mi_moe

@@ -1,0 +1,341 @@
+// The residual's addition and the RMS norm behind it in one pass over the rows, with the normalised rows in the input's type or in
+// eight bits, and the backward pass.
+//
+//   h = round(x + r)   rstd = 1 / sqrt(mean(h^2) + eps)   y = round(w (h rstd))
+//   rows in 8 bits: with z = w h rstd, s = max |z| / 127 and q the integer nearest to z / s (ties to even).  rstd has no part in q:
+//     z / s = 127 w h / max |w h|
+//   backward, hat = h rstd: dx = dh + rstd (w dy - hat mean(w dy hat)),  dw = sum over rows of dy hat
+//
+// Contract of the norm: mlx_fast_rms_norm (mlx-rs/src/fast.rs:190-207; nn::RmsNorm, nn/normalization.rs:233-275) on the rounded sum: in bfloat16
+// the bits of mi_moe_rms_norm on x + r.  The square sums are in double (exact products; any order gives the same float).
+#include <type_traits>
+
+#include "common.hpp"
+
+namespace mi_moe {
+
+__device__ __forceinline__ double wave_max_f64(double v) {
+  v = fmax(v, dpp_f64<kDppXor1>(v));
+  v = fmax(v, dpp_f64<kDppXor2>(v));
+  v = fmax(v, dpp_f64<kDppHalfMirror>(v));
+  v = fmax(v, dpp_f64<kDppMirror>(v));
+  return fmax(fmax(readlane_f64(v, 0), readlane_f64(v, 16)), fmax(readlane_f64(v, 32), readlane_f64(v, 48)));
+}
+
+// ---------------------------------------------------------------- eight values of a row
+template <int DT>
+struct Octet {  // as they lie in memory; DT: mi_moe_dtype
+  using Raw = typename std::conditional<DT == 0, uint16_t, typename std::conditional<DT == 1, _Float16, float>::type>::type;
+  Raw v[8];
+  __device__ __forceinline__ float at(int i) const { return as_f32(v[i]); }
+  __device__ __forceinline__ void put(int i, float f) {
+    if constexpr (DT == 0) v[i] = f32_to_bf16(f);
+    else v[i] = (Raw)f;
+  }
+};
+// `n` values at p (8, or fewer at a row's end), in 16-byte accesses that assume no more than the elements' own alignment: a row of an odd number
+// of values starts anywhere.  What is missing is zeros.
+template <int DT>
+__device__ __forceinline__ Octet<DT> load_octet(const void *base, int64_t at, int n) {
+  using Raw = typename Octet<DT>::Raw;
+  const Raw *p = static_cast<const Raw *>(base) + at;
+  Octet<DT> o;
+  if (n >= 8) {
+    __builtin_memcpy(o.v, p, sizeof o.v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o.v[i] = i < n ? p[i] : Raw(0);
+  }
+  return o;
+}
+template <int DT>
+__device__ __forceinline__ void store_octet(void *base, int64_t at, int n, const Octet<DT> &o) {
+  using Raw = typename Octet<DT>::Raw;
+  Raw *p = static_cast<Raw *>(base) + at;
+  if (n >= 8) {
+    __builtin_memcpy(p, o.v, sizeof o.v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) p[i] = o.v[i];
+  }
+}
+
+// 1 / sqrt(mean + eps) from the double square sum: mi_moe_rms_norm's float operations, and double ones where the mean leaves the floats' range
+__device__ __forceinline__ float rstd_of(double ss, int H, float eps) {
+  const double m = ss / (double)H;
+  if (m > 1e-30 && m < 1e37) return 1.0f / sqrtf((float)m + eps);
+  return (float)(1.0 / sqrt(m + (double)eps));
+}
+
+struct NormArgs {
+  const void *x, *r, *w;  // r: or nullptr, then the sum is x
+  float eps;
+  int64_t T;
+  int H;
+  void *sum, *y;  // sum: or nullptr; y: rows in the input's type, or in eight bits
+  float *scales;
+};
+
+// A row goes to TPR threads (a wave and more), CH octets each, and stays in their registers between its sums and its results: memory is passed once.
+template <int DT, int TPR, int CH, bool ROWS8>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void add_rms_norm_kernel(NormArgs a) {
+  constexpr int kRows = TPR < 256 ? 256 / TPR : 1, kWaves = TPR / kWave;
+  __shared__ double part[kRows][kWaves][2];
+  const int t = threadIdx.x % TPR, wave = t / kWave;
+  const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR;
+  if (kWaves == 1 && row >= a.T) return;  // (rows of several waves have a block each: none is outside)
+  const int64_t at = row * a.H;
+  Octet<DT> h[CH];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) h[c] = load_octet<DT>(a.x, at + (c * TPR + t) * 8, a.H - (c * TPR + t) * 8);
+  if (a.r) {
+    Octet<DT> r[CH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) r[c] = load_octet<DT>(a.r, at + (c * TPR + t) * 8, a.H - (c * TPR + t) * 8);
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[c].put(i, h[c].at(i) + r[c].at(i));
+  }
+  double ss = 0.0, most = 0.0;  // most: the largest |w h|; infinite where one of them is infinite or no number
+  if (a.sum) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) store_octet<DT>(a.sum, at + (c * TPR + t) * 8, a.H - (c * TPR + t) * 8, h[c]);
+  }
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss = __builtin_fma((double)h[c].at(i), (double)h[c].at(i), ss);
+  Octet<DT> w[CH];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) w[c] = load_octet<DT>(a.w, (c * TPR + t) * 8, a.H - (c * TPR + t) * 8);
+  if constexpr (ROWS8) {
+    bool finite = true;
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const double p = fabs((double)h[c].at(i) * (double)w[c].at(i));
+        finite &= p < INFINITY;
+        most = p > most ? p : most;
+      }
+    if (!finite) most = INFINITY;
+  }
+  ss = wave_sum_f64(ss);
+  if constexpr (ROWS8) most = wave_max_f64(most);
+  if constexpr (kWaves > 1) {
+    if ((t & (kWave - 1)) == 0) part[0][wave][0] = ss, part[0][wave][1] = most;
+    __syncthreads();
+    ss = 0.0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+      ss += part[0][i][0];
+      if constexpr (ROWS8) most = fmax(most, part[0][i][1]);
+    }
+  }
+  const float rstd = rstd_of(ss, a.H, a.eps);
+  if constexpr (!ROWS8) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[c].put(i, w[c].at(i) * (h[c].at(i) * rstd));
+      store_octet<DT>(a.y, at + (c * TPR + t) * 8, a.H - (c * TPR + t) * 8, h[c]);
+    }
+  } else {
+    // rows of zeros have a scale and codes of zero; rows that hold an infinity or no number a scale that is none, so that what is made of them is none either
+    const bool none = !(most > 0.0 && most < INFINITY), wide = !(most > 1e-30 && most < 1e30);
+    const float inv = none ? 0.f : (float)(127.0 / most);
+    if (t == 0) a.scales[row] = !none ? (float)(most * (double)rstd / 127.0) : most > 0.0 ? NAN : 0.f;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int n = a.H - (c * TPR + t) * 8;
+      uint32_t q[2] = {0, 0};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float v = h[c].at(i) * w[c].at(i) * inv;
+        float k = rintf(v);
+        // the float quotient is up to 2^-15 off (three roundings of a value below 128): where that could change the integer, or the products leave
+        // the floats' range, the exact products decide
+        if (none) k = 0.f;
+        else if (wide || fabsf(v - k) > 0.4999f) k = (float)rint(127.0 * ((double)h[c].at(i) * (double)w[c].at(i)) / most);
+        q[i / 4] |= ((uint32_t)(int)k & 0xffu) << (8 * (i % 4));
+      }
+      unsigned char *const to = static_cast<unsigned char *>(a.y) + at + (c * TPR + t) * 8;
+      if (n >= 8) __builtin_memcpy(to, q, 8);
+      else
+        for (int i = 0; i < n; ++i) to[i] = (unsigned char)(q[i / 4] >> (8 * (i % 4)));
+    }
+  }
+}
+
+template <int DT, int TPR, int CH>
+static hipError_t start_norm(const NormArgs &a, bool rows8, hipStream_t st) {
+  constexpr int block = TPR < 256 ? 256 : TPR, rows = block / TPR;
+  const unsigned grid = (unsigned)((a.T + rows - 1) / rows);
+  if (rows8) add_rms_norm_kernel<DT, TPR, CH, true><<<grid, block, 0, st>>>(a);
+  else add_rms_norm_kernel<DT, TPR, CH, false><<<grid, block, 0, st>>>(a);
+  return hipGetLastError();
+}
+
+template <class F>
+static hipError_t with_dtype(int dt, F f) {
+  if (dt == 0) return f(std::integral_constant<int, 0>{});
+  if (dt == 1) return f(std::integral_constant<int, 1>{});
+  return f(std::integral_constant<int, 2>{});
+}
+
+hipError_t launch_add_rms_norm(const void *x, const void *r, const void *w, float eps, int64_t T, int H, int dt, void *sum, void *y, float *scales,
+                               hipStream_t st) {
+  if (T == 0) return hipSuccess;
+  const NormArgs a{x, r, w, eps, T, H, sum, y, scales};
+  const bool rows8 = scales != nullptr;
+  return with_dtype(dt, [&](auto d) {
+    constexpr int DT = decltype(d)::value;
+    if (H <= 512) return start_norm<DT, 64, 1>(a, rows8, st);
+    if (H <= 1024) return start_norm<DT, 64, 2>(a, rows8, st);
+    if (H <= 2048) return start_norm<DT, 256, 1>(a, rows8, st);
+    if (H <= 4096) return start_norm<DT, 256, 2>(a, rows8, st);
+    if (H <= 8192) return start_norm<DT, 256, 4>(a, rows8, st);
+    if (H <= 16384) return start_norm<DT, 1024, 2>(a, rows8, st);
+    return start_norm<DT, 1024, 4>(a, rows8, st);
+  });
+}
+
+// ---------------------------------------------------------------- backward
+struct NormGradArgs {
+  const void *dy, *h, *dh, *w;  // dh: or nullptr
+  float eps;
+  int64_t T;
+  int H, groups;
+  void *dx, *dw;
+  float *parts;  // [groups, H]: the rows' shares of dw, of every group of rows
+};
+
+// TPR threads have every groups-th row, and their columns' sums for dw in registers; the sums of the groups meet in a second launch, in a fixed order.
+template <int DT, int TPR, int CH>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_grad_kernel(NormGradArgs a) {
+  constexpr int kRows = TPR < 256 ? 256 / TPR : 1, kWaves = TPR / kWave;
+  __shared__ double part[2][kWaves][2];
+  const int t = threadIdx.x % TPR, wave = t / kWave;
+  const int group = blockIdx.x * kRows + threadIdx.x / TPR;
+  if (kWaves == 1 && group >= a.groups) return;
+  Octet<DT> w[CH];
+  float dw[CH][8];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    w[c] = load_octet<DT>(a.w, (c * TPR + t) * 8, a.H - (c * TPR + t) * 8);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) dw[c][i] = 0.f;
+  }
+  int turn = 0;
+  for (int64_t row = group; row < a.T; row += a.groups, turn ^= 1) {
+    const int64_t at = row * a.H;
+    Octet<DT> h[CH], dy[CH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int j = (c * TPR + t) * 8;
+      h[c] = load_octet<DT>(a.h, at + j, a.H - j);
+      dy[c] = load_octet<DT>(a.dy, at + j, a.H - j);
+    }
+    double ss = 0.0, dot = 0.0;  // sums of h^2 and of w dy h
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const double v = h[c].at(i);
+        ss = __builtin_fma(v, v, ss);
+        const double g = DT == 2 ? (double)w[c].at(i) * (double)dy[c].at(i) : (double)(w[c].at(i) * dy[c].at(i));  // (exact either way)
+        dot = __builtin_fma(g, v, dot);
+      }
+    ss = wave_sum_f64(ss);
+    dot = wave_sum_f64(dot);
+    if constexpr (kWaves > 1) {
+      if ((t & (kWave - 1)) == 0) part[turn][wave][0] = ss, part[turn][wave][1] = dot;
+      __syncthreads();  // (one a row: the next row's sums go to the other half)
+      ss = dot = 0.0;
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i) ss += part[turn][i][0], dot += part[turn][i][1];
+    }
+    const float rstd = rstd_of(ss, a.H, a.eps);
+    const float mean = (float)(dot * (double)rstd / (double)a.H);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int j = (c * TPR + t) * 8, n = a.H - j;
+      Octet<DT> add;
+      if (a.dh) add = load_octet<DT>(a.dh, at + j, n);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float hat = h[c].at(i) * rstd, g = dy[c].at(i);
+        dw[c][i] = __builtin_fmaf(g, hat, dw[c][i]);
+        float d = rstd * __builtin_fmaf(-hat, mean, w[c].at(i) * g);
+        if (a.dh) d += add.at(i);
+        h[c].put(i, d);
+      }
+      store_octet<DT>(a.dx, at + j, n, h[c]);
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int j = (c * TPR + t) * 8;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (j + i < a.H) a.parts[(int64_t)group * a.H + j + i] = dw[c][i];
+  }
+}
+
+// dw = the groups' sums: 32 columns a block, every eighth group a thread
+template <int DT>
+__global__ __launch_bounds__(256) void norm_grad_weight_kernel(const float *parts, int groups, int H, void *dw) {
+  __shared__ float sums[8][32];
+  const int col = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5;
+  float s = 0.f;
+  if (col < H)
+    for (int g = slice; g < groups; g += 8) s += parts[(int64_t)g * H + col];
+  sums[slice][threadIdx.x & 31] = s;
+  __syncthreads();
+  if (slice == 0 && col < H) {
+    float v = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v += sums[i][threadIdx.x & 31];
+    Octet<DT> o;
+    o.put(0, v);
+    static_cast<typename Octet<DT>::Raw *>(dw)[col] = o.v[0];
+  }
+}
+
+// groups of rows of the backward pass: what fills the chip, and no more of them than rows
+static int norm_grad_groups(int64_t T, int H) {
+  const int64_t most = H <= 1024 ? 2048 : 512;
+  return (int)(T < most ? T : most);
+}
+size_t norm_grad_bytes(int64_t T, int H) { return (size_t)norm_grad_groups(T, H) * H * sizeof(float); }
+
+template <int DT, int TPR, int CH>
+static hipError_t start_norm_grad(const NormGradArgs &a, hipStream_t st) {
+  constexpr int block = TPR < 256 ? 256 : TPR, rows = block / TPR;
+  norm_grad_kernel<DT, TPR, CH><<<(unsigned)((a.groups + rows - 1) / rows), block, 0, st>>>(a);
+  return hipGetLastError();
+}
+
+hipError_t launch_norm_grad(const void *dy, const void *h, const void *dh, const void *w, float eps, int64_t T, int H, int dt, void *dx, void *dw,
+                            float *parts, hipStream_t st) {
+  const NormGradArgs a{dy, h, dh, w, eps, T, H, norm_grad_groups(T, H), dx, dw, parts};
+  return with_dtype(dt, [&](auto d) {
+    constexpr int DT = decltype(d)::value;
+    hipError_t e = hipSuccess;
+    if (T > 0)
+      e = H <= 512     ? start_norm_grad<DT, 64, 1>(a, st)
+          : H <= 1024  ? start_norm_grad<DT, 64, 2>(a, st)
+          : H <= 2048  ? start_norm_grad<DT, 256, 1>(a, st)
+          : H <= 4096  ? start_norm_grad<DT, 256, 2>(a, st)
+          : H <= 8192  ? start_norm_grad<DT, 256, 4>(a, st)
+          : H <= 16384 ? start_norm_grad<DT, 1024, 2>(a, st)
+                       : start_norm_grad<DT, 1024, 4>(a, st);
+    if (e != hipSuccess) return e;
+    norm_grad_weight_kernel<DT><<<(unsigned)((H + 31) / 32), 256, 0, st>>>(parts, a.groups, H, dw);  // (no rows: zeros)
+    return hipGetLastError();
+  });
+}
+
+}  // namespace mi_moe

@@ -13,7 +13,7 @@ import torch
 
 from . import capi
 from .capi import check, load_library
-from .ops import _need, _ptr, _stream
+from .ops import _need, _ptr, _stream, _together
 
 
 @dataclass
@@ -118,7 +118,19 @@ class SparseMoeBlock:
         check(self._lib.mi_moe_forward_static(self._handle, _ptr(x2), x2.shape[0], _ptr(out), None, _stream()))
         return out.reshape(x.shape)
 
-    def forward(self, x, debug=False, out=None, _norm=None):
+    def forward_routed(self, x, inds, weights, debug=False, out=None):
+        """forward() with a routing of the caller's in place of the block's router: inds int32 and weights bf16 [..., top_k] for x bf16
+        [..., H] (``ops.select_experts``).  A token that names an expert twice gets it once, with the sum of its weights; an id outside the experts
+        contributes nothing."""
+        c = self.config
+        _need(inds, torch.int32, "inds")
+        _need(weights, torch.bfloat16, "weights")
+        if inds.shape != x.shape[:-1] + (c.top_k,) or weights.shape != inds.shape:
+            raise capi.MoeError(f"forward_routed: inds and weights must be {tuple(x.shape[:-1]) + (c.top_k,)}, got {tuple(inds.shape)} and {tuple(weights.shape)}")
+        _together("forward_routed", x, inds, weights)
+        return self.forward(x, debug=debug, out=out, _routing=(inds, weights))
+
+    def forward(self, x, debug=False, out=None, _norm=None, _routing=None):
         """x: bf16 [..., H] -> bf16 [..., H].  With debug=True also returns the routing
         arrays (topk_idx, topk_w, counts, offsets, perm, inv_perm)."""
         _need(x, torch.bfloat16, "x")
@@ -144,7 +156,10 @@ class SparseMoeBlock:
             dbg_struct = capi.DebugOut(*[dbg[n].data_ptr() for n in
                                          ("topk_idx", "topk_w", "counts", "offsets", "perm", "inv_perm")])
         dbg_arg = None if dbg_struct is None else C.byref(dbg_struct)
-        if _norm is None:
+        if _routing is not None:
+            check(self._lib.mi_moe_forward_routed(self._handle, _ptr(x2), _ptr(_routing[0]), _ptr(_routing[1]), T, _ptr(out), _ptr(ws), ws.numel(),
+                                                  dbg_arg, _stream()))
+        elif _norm is None:
             check(self._lib.mi_moe_forward(self._handle, _ptr(x2), T, _ptr(out), _ptr(ws), ws.numel(), dbg_arg,
                                            _stream()))
         else:

@@ -260,6 +260,44 @@ def quantized_linear(x, w, scales, biases, linear_bias=None, transpose=True, gro
     return y if x.dim() == 2 else y.reshape(*x.shape[:-1], N)
 
 
+def quantized_linear_rows8(x, row_scales, w, scales, biases, linear_bias=None, group_size=64, bits=4):
+    """quantized_linear on rows in eight bits (``add_rms_norm_rows8``): y = (row_scales * x) . dequantize(w)^T + linear_bias, each result rounded
+    once.  x: int8 [..., K]; row_scales: float32 [...]; w: int32 [N, K*bits/32]; scales, biases [N, K/group_size] and linear_bias [N] in
+    bfloat16, float16 or float32, which is y's type.  bits 4 or 8.  Returns [..., N]."""
+    lib = load_library()
+    who = "quantized_linear_rows8"
+    _need(x, torch.int8, "x")
+    _need(row_scales, torch.float32, "row_scales")
+    _need(w, torch.int32, "w")
+    dt = _float_dtype(scales, "scales")
+    _need(biases, scales.dtype, "biases")
+    if w.dim() != 2 or x.dim() < 1 or scales.dim() != 2 or biases.dim() != 2:
+        raise capi.MoeError(f"{who}: x must be [..., K], w, scales and biases matrices")
+    if row_scales.shape != x.shape[:-1]:
+        raise capi.MoeError(f"{who}: row_scales must be {tuple(x.shape[:-1])}, got {tuple(row_scales.shape)}")
+    K, N = x.shape[-1], w.shape[0]
+    _check_qmat(who, w, scales, biases, K, True, group_size, bits)
+    if linear_bias is not None:
+        _need(linear_bias, scales.dtype, "linear_bias")
+        if linear_bias.numel() != N:
+            raise capi.MoeError(f"{who}: linear_bias must have {N} elements, got {linear_bias.numel()}")
+    _together(who, x, row_scales, w, scales, biases, linear_bias)
+    M = row_scales.numel()
+    y = torch.empty(x.shape[:-1] + (N,), dtype=scales.dtype, device=x.device)
+    need = _rows8_workspace_bytes(M, K)
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    check(lib.mi_moe_quantized_linear_rows8(_ptr(x), _ptr(row_scales), _ptr(w), _ptr(scales), _ptr(biases), _ptr(linear_bias), M, N, K, group_size, bits, dt,
+                                            _ptr(y), _ptr(ws), need, _stream()))
+    return y
+
+
+@functools.lru_cache(maxsize=1024)
+def _rows8_workspace_bytes(M, K):
+    need = C.c_size_t()
+    check(load_library().mi_moe_quantized_linear_rows8_workspace_size(M, K, C.byref(need)))
+    return need.value
+
+
 def rms_norm(x, weight, eps=1e-5):
     """fast::rms_norm (mlx-rs/src/fast.rs:190-207): weight * x * rsqrt(mean(x^2) + eps) over the last
     axis.  x: bf16 [..., H]; weight: bf16 [H]."""
@@ -273,6 +311,73 @@ def rms_norm(x, weight, eps=1e-5):
     out = torch.empty_like(x2)
     check(lib.mi_moe_rms_norm(_ptr(x2), _ptr(weight), float(eps), x2.shape[0], H, _ptr(out), _stream()))
     return out.reshape(x.shape)
+
+
+def _together(who, *tensors):
+    """Operands of one launch: on the current device, whose current stream takes it."""
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            raise capi.MoeError(f"{who}: an operand is on {t.device}, the current device is cuda:{here}")
+
+
+def _norm_operands(who, x, residual, weight):
+    dt = _float_dtype(x, "x")
+    _need(weight, x.dtype, "weight")
+    if x.dim() < 1 or weight.numel() != x.shape[-1]:
+        raise capi.MoeError(f"{who}: weight must have the {x.shape[-1] if x.dim() else 1} elements of x's last axis, got {weight.numel()}")
+    if residual is not None:
+        _need(residual, x.dtype, "residual")
+        if residual.shape != x.shape:
+            raise capi.MoeError(f"{who}: residual must be {tuple(x.shape)} as x, got {tuple(residual.shape)}")
+    _together(who, x, residual, weight)
+    H = x.shape[-1]
+    return dt, x.numel() // H if H else 0, H
+
+
+def add_rms_norm(x, residual, weight, eps=1e-5):
+    """The residual's addition and the norm behind it in one pass: (y, h) with h = x + residual, rounded, and y = rms_norm(h, weight, eps).
+    x, residual: [..., H] in bfloat16, float16 or float32; weight: [H], the same type.  residual None: h is x.  What stands between
+    two sublayers (mlx-lm/src/models/qwen3.rs:310-325); in bfloat16 the bits of ``rms_norm(x + residual, weight, eps)``."""
+    lib = load_library()
+    dt, T, H = _norm_operands("add_rms_norm", x, residual, weight)
+    y = torch.empty_like(x)
+    h = x if residual is None else torch.empty_like(x)
+    check(lib.mi_moe_add_rms_norm(_ptr(x), _ptr(residual), _ptr(weight), float(eps), T, H, dt, None if residual is None else _ptr(h), _ptr(y),
+                                  _stream()))
+    return y, h
+
+
+def add_rms_norm_rows8(x, residual, weight, eps=1e-5):
+    """add_rms_norm with the normalised rows in eight bits, for ``quantized_linear_rows8``: (rows8 int8 [..., H], row_scales float32 [...], h);
+    rows8 * row_scales stands for the rows, in steps of a 127th of a row's largest value."""
+    lib = load_library()
+    dt, T, H = _norm_operands("add_rms_norm_rows8", x, residual, weight)
+    rows8 = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    h = x if residual is None else torch.empty_like(x)
+    check(lib.mi_moe_add_rms_norm_rows8(_ptr(x), _ptr(residual), _ptr(weight), float(eps), T, H, dt, None if residual is None else _ptr(h), _ptr(rows8),
+                                        _ptr(scales), _stream()))
+    return rows8, scales, h
+
+
+def add_rms_norm_grad(dy, h, weight, eps=1e-5, dh=None):
+    """The backward pass of add_rms_norm: (dx, dweight) from the gradients that arrive at y (dy) and, along the residual, at h (dh; None: none).
+    dx is the gradient of x and of residual alike; dweight is summed over the rows in float32, in an order that does not change."""
+    lib = load_library()
+    dt, T, H = _norm_operands("add_rms_norm_grad", h, dy, weight)
+    if dh is not None:
+        _need(dh, h.dtype, "dh")
+        if dh.shape != h.shape:
+            raise capi.MoeError(f"add_rms_norm_grad: dh must be {tuple(h.shape)} as h, got {tuple(dh.shape)}")
+        _together("add_rms_norm_grad", dh)
+    dx, dweight = torch.empty_like(h), torch.empty_like(weight)
+    need = C.c_size_t()
+    check(lib.mi_moe_add_rms_norm_grad_workspace_size(T, H, C.byref(need)))
+    ws = _workspace(need.value, h.device)
+    check(lib.mi_moe_add_rms_norm_grad(_ptr(dy), _ptr(h), _ptr(dh), _ptr(weight), float(eps), T, H, dt, _ptr(dx), _ptr(dweight), _ptr(ws), ws.numel(),
+                                       _stream()))
+    return dx, dweight
 
 
 def router_logits(x, router_w, router_bias=None):
@@ -315,6 +420,62 @@ def route(x, router_w, top_k, score_mode=capi.SCORE_SOFTMAX_THEN_TOPK_RENORM, ro
                            _ptr(None if router_bias is None else _need(router_bias, torch.float32, "router_bias")),
                            T, H, E, top_k, score_mode, _ptr(inds), _ptr(sc), _ptr(logits), _ptr(ws), ws.numel(), _stream()))
     return (inds, sc, logits) if return_logits else (inds, sc)
+
+
+_SCORINGS = {"softmax": capi.SCORING_SOFTMAX, "sigmoid": capi.SCORING_SIGMOID}
+_GROUP_SCORES = {"max": capi.GROUP_SCORE_MAX, "top2": capi.GROUP_SCORE_TOP2}
+
+
+def _choice(who, table, value, name):
+    if value not in table:
+        raise capi.MoeError(f"{who}: {name} must be one of {sorted(table)}, got {value!r}")
+    return table[value]
+
+
+def select_experts(logits, top_k, scoring="softmax", bias=None, n_groups=1, top_groups=1, group_score="max", renormalize=True, scale=1.0,
+                   dtype=torch.bfloat16):
+    """Experts of every token from the router's logits, for routers that ``route`` does not cover: (inds int32 [..., k], best first, weights
+    [..., k] of ``dtype``).  logits: [..., E] in bfloat16, float16 or float32.  Scores are ``scoring`` ("softmax" over the experts, or
+    "sigmoid") of the logits; ``bias`` (float32 [E]) is added for the choice alone; of ``n_groups`` runs of experts the best ``top_groups`` are open, by
+    their largest key or by the sum of their two largest scores (``group_score`` "max" / "top2"); ties go to the lower id.  Weights: the chosen
+    scores, divided by their sum with ``renormalize``, times ``scale``.  ``SparseMoeBlock.forward_routed`` takes the results."""
+    lib = load_library()
+    dt = _float_dtype(logits, "logits")
+    if dtype not in _DTYPES:
+        raise capi.MoeError(f"select_experts: dtype must be bfloat16, float16 or float32, got {dtype}")
+    if logits.dim() < 1:
+        raise capi.MoeError("select_experts: logits must be [..., E]")
+    E = logits.shape[-1]
+    if bias is not None:
+        _need(bias, torch.float32, "bias")
+        if bias.numel() != E:
+            raise capi.MoeError(f"select_experts: bias must have {E} elements, got {bias.numel()}")
+    _together("select_experts", logits, bias)
+    T = logits.numel() // E if E else 0
+    shape = logits.shape[:-1] + (max(int(top_k), 0),)
+    inds = torch.empty(shape, dtype=torch.int32, device=logits.device)
+    weights = torch.empty(shape, dtype=dtype, device=logits.device)
+    check(lib.mi_moe_select_experts(_ptr(logits), dt, _ptr(bias), T, E, top_k, _choice("select_experts", _SCORINGS, scoring, "scoring"), n_groups, top_groups,
+                                    _choice("select_experts", _GROUP_SCORES, group_score, "group_score"), int(bool(renormalize)), float(scale), _ptr(inds),
+                                    _ptr(weights), _DTYPES[dtype], _stream()))
+    return inds, weights
+
+
+def select_experts_grad(dweights, logits, inds, scoring="softmax", renormalize=True, scale=1.0):
+    """The gradient of select_experts' weights with respect to the logits, the choice taken as given: dlogits, of logits' shape and type.
+    dweights: [..., k] in bfloat16, float16 or float32; inds: what select_experts returned."""
+    lib = load_library()
+    dt, wt = _float_dtype(logits, "logits"), _float_dtype(dweights, "dweights")
+    _need(inds, torch.int32, "inds")
+    if logits.dim() < 1 or inds.shape[:-1] != logits.shape[:-1] or inds.dim() != logits.dim() or dweights.shape != inds.shape:
+        raise capi.MoeError(f"select_experts_grad: inds and dweights must be {tuple(logits.shape[:-1])} + (k,), got {tuple(inds.shape)} and {tuple(dweights.shape)}")
+    _together("select_experts_grad", logits, dweights, inds)
+    E = logits.shape[-1]
+    dlogits = torch.empty_like(logits)
+    check(lib.mi_moe_select_experts_grad(_ptr(dweights), wt, _ptr(logits), dt, _ptr(inds), logits.numel() // E if E else 0, E, inds.shape[-1],
+                                         _choice("select_experts_grad", _SCORINGS, scoring, "scoring"), int(bool(renormalize)), float(scale), _ptr(dlogits),
+                                         _stream()))
+    return dlogits
 
 
 def dispatch(expert_of_pair, n_experts):

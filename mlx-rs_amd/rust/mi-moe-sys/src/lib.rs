@@ -4,6 +4,8 @@
 
 use std::os::raw::{c_char, c_int, c_void};
 
+pub mod layer;
+
 #[repr(C)]
 pub struct mi_moe_s {
     _private: [u8; 0],

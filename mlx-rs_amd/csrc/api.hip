@@ -1030,7 +1030,7 @@ int mi_moe_select_experts_grad(const void *dw, int32_t w_dtype, const void *logi
 int mi_moe_quantized_linear_rows8_workspace_size(int64_t M, int32_t K, size_t *bytes) try {
   if (!bytes) return fail("quantized_linear_rows8_workspace_size: bytes is NULL");
   if (M < 0 || K <= 0 || M * (int64_t)K > (int64_t)1 << 40) return fail("quantized_linear_rows8_workspace_size: bad sizes");
-  *bytes = 0;
+  *bytes = rows8_workspace_bytes(M, K);
   return 0;
 } MI_CATCH("quantized_linear_rows8_workspace_size")
 
@@ -1045,7 +1045,7 @@ int mi_moe_quantized_linear_rows8(const void *x, const float *row_scales, const 
   if (M == 0) return 0;
   if (!x || !row_scales || !w || !scales || !biases || !y) return fail("quantized_linear_rows8: x, row_scales, w, scales, biases and y must be non-NULL");
   const Rows8Args a{static_cast<const signed char *>(x), row_scales, w, scales, biases, linear_bias, y, M, N, K, group_size};
-  MI_HIP(launch_qmm_rows8(a, bits, dtype, static_cast<hipStream_t>(stream)));
+  MI_HIP(launch_qmm_rows8(a, bits, dtype, workspace, workspace_bytes, static_cast<hipStream_t>(stream)));
   return 0;
 } MI_CATCH("quantized_linear_rows8")
 

@@ -487,6 +487,7 @@ struct Rows8Args {
   int64_t M;
   int N, K, group;
 };
-hipError_t launch_qmm_rows8(const Rows8Args &a, int bits, int dt, hipStream_t st);
+size_t rows8_workspace_bytes(int64_t M, int K);
+hipError_t launch_qmm_rows8(const Rows8Args &a, int bits, int dt, void *workspace, size_t workspace_bytes, hipStream_t st);
 
 }  // namespace mi_moe

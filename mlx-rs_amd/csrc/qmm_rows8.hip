@@ -5,7 +5,8 @@
 // the sums over a group are integers and exact; what is in float is a term or two a group.  (The layer on 16-bit rows: mlx-rs/src/nn/quantized.rs:363-386.)
 #include <type_traits>
 
-#include "common.hpp"
+#include "lds_copies.hpp"
+#include "qmm_codes_dev.hpp"
 
 namespace mi_moe {
 
@@ -25,6 +26,8 @@ template <int BITS>
 struct Centre {
   static constexpr float value = BITS == 4 ? 8.f : 128.f, of_codes = BITS == 4 ? 16.f : 1.f;  // of_codes: what centred_bytes multiplies them by
 };
+
+constexpr int kRows8Few = 16;  // rows up to which the kernel without preparation runs
 
 template <int DT>
 using Value = typename std::conditional<DT == 0, uint16_t, typename std::conditional<DT == 1, _Float16, float>::type>::type;
@@ -77,6 +80,259 @@ __global__ __launch_bounds__(256) void rows8_plain_kernel(Rows8Args a) {
   }
 }
 
+// ---------------------------------------------------------------- many rows: tiles on the int8 matrix cores
+// Rows as the matrix instructions take them: for every 16 rows and 64 K values a tile of 1024 bytes, 16 a lane (row l % 16, part kb = l / 16 of the values), in the
+// order in which the lane that holds the same values of a weight row has them after unpacking:
+//   8-bit codes                16 consecutive values
+//   4-bit codes                the words 2 kb and 2 kb + 1 of the eight, of each the even nibbles, then the odd ones
+//   groups of 32 (two a tile)  8 values of each, 8 kb .. 8 kb + 7 of the group, in that order within a word
+// and the group sums, four groups of 16 rows a tile of 64 floats (lane: row l % 16, group 4 q + kb; zeros past the last group).
+__host__ __device__ constexpr int64_t row_tiles(int64_t M) { return (M + 15) / 16; }
+constexpr size_t rows8_tiles_bytes(int64_t M, int K) { return (size_t)row_tiles(M) * 16 * K; }
+constexpr size_t rows8_sums_bytes(int64_t M, int K, int group) { return (size_t)row_tiles(M) * ((K / group + 3) / 4) * 256; }
+
+__device__ __forceinline__ int32_t byte_sum(uint32_t v, int32_t c) { return __builtin_amdgcn_sdot4((int32_t)v, 0x01010101, c, false); }
+// eight bytes in their order to the even ones, then the odd ones
+__device__ __forceinline__ uint2 evens_odds(uint2 v) {
+  return make_uint2(__builtin_amdgcn_perm(v.y, v.x, 0x06040200u), __builtin_amdgcn_perm(v.y, v.x, 0x07050301u));
+}
+
+// A wave makes the tiles of 16 rows and four groups.
+template <int BITS, int GROUP>
+__global__ __launch_bounds__(256) void rows8_prepare_kernel(const signed char *x, int64_t M, int K, uint4 *tiles, float *sums) {
+  constexpr int NT = GROUP * 4 / 64;  // tiles of four groups
+  const int lane = lane_id(), kb = lane >> 4, quads = (K / GROUP + 3) / 4, n_tiles = K / 64;
+  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), mt = unit / quads;
+  const int q = (int)(unit % quads);
+  if (mt >= row_tiles(M)) return;
+  const int64_t row = mt * 16 + (lane & 15);
+  int32_t sum[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    const int kt = q * NT + i;
+    uint2 a = make_uint2(0, 0), b = a;
+    if (kt < n_tiles && row < M) {
+      const signed char *const p = x + row * K + kt * 64;
+      a = *reinterpret_cast<const uint2 *>(p + (GROUP == 32 ? 8 * kb : 16 * kb));
+      b = *reinterpret_cast<const uint2 *>(p + (GROUP == 32 ? 32 + 8 * kb : 16 * kb + 8));
+    }
+    if constexpr (GROUP == 32) {
+      sum[2 * i] = byte_sum(a.y, byte_sum(a.x, 0));
+      sum[2 * i + 1] = byte_sum(b.y, byte_sum(b.x, 0));
+    } else {
+      sum[i * 64 / GROUP] = byte_sum(b.y, byte_sum(b.x, byte_sum(a.y, byte_sum(a.x, sum[i * 64 / GROUP]))));
+    }
+    if constexpr (BITS == 4) a = evens_odds(a), b = evens_odds(b);
+    if (kt < n_tiles) tiles[(mt * n_tiles + kt) * 64 + lane] = make_uint4(a.x, a.y, b.x, b.y);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    sum[i] += __shfl_xor(sum[i], 16);
+    sum[i] += __shfl_xor(sum[i], 32);
+  }
+  sums[(mt * quads + q) * 64 + lane] = (float)(kb == 0 ? sum[0] : kb == 1 ? sum[1] : kb == 2 ? sum[2] : sum[3]);
+}
+
+typedef int32_t i32x2_t __attribute__((ext_vector_type(2)));
+
+// the operand of a lane's 8- or 16-byte piece of codes
+template <int BITS>
+__device__ __forceinline__ i32x4_t operand_of(uint2 lo, uint2 hi) {  // 8-bit: 16 codes; 4-bit: lo, two words
+  if constexpr (BITS == 8) {
+    return i32x4_t{(int32_t)(lo.x ^ 0x80808080u), (int32_t)(lo.y ^ 0x80808080u), (int32_t)(hi.x ^ 0x80808080u), (int32_t)(hi.y ^ 0x80808080u)};
+  } else {
+    auto even = [](uint32_t w) { return (int32_t)(((w << 4) & 0xf0f0f0f0u) ^ 0x80808080u); };
+    auto odd = [](uint32_t w) { return (int32_t)((w & 0xf0f0f0f0u) ^ 0x80808080u); };
+    return i32x4_t{even(lo.x), odd(lo.x), even(lo.y), odd(lo.y)};
+  }
+}
+
+// y = rows x weights in tiles of 16 MI WM rows and 16 NI WN columns, a wave 16 MI x 16 NI of them.  A stage is 128 K values: the rows' tiles and the codes are copied straight
+// into LDS, one stage ahead.  Codes: 64 or 128 bytes of a weight row a stage, its 16-byte pieces in an order turned by the row, so that the lanes' reads meet all banks.
+// A group is one matrix instruction a 16 x 16 tile (two for 128 values, one of half the depth for 32), whose integer sums are exact; then a conversion and a
+// multiply-add a result.  That vector work, 32 cycles a tile and 64 values, is what bounds it: twice the instruction's own 16.  The biases' terms are a product over
+// the groups by the float32 matrix instructions, four groups a time.
+template <int DT, int BITS, int GROUP, int MI, int NI, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, 2) void rows8_tiles_kernel(Rows8Args a, const uint4 *tiles, const float *sums, int n_mtiles, int n_ntiles) {
+  constexpr int kWaves = WM * WN, ROWS = 16 * MI * WM, COLS = 16 * NI * WN;
+  constexpr int CODES = 128 * BITS / 8, PIECES = CODES / 16;  // bytes and 16-byte pieces of a weight row's stage
+  constexpr int A_BYTES = ROWS * 128, STAGE = A_BYTES + COLS * CODES;
+  constexpr int GS = 128 / GROUP, PERIOD = GROUP / 32;  // groups of a stage; stages of four groups
+  extern __shared__ __align__(16) unsigned char lds_raw[];
+  const int xcd = blockIdx.x & 7, j = blockIdx.x >> 3, nt = j / n_mtiles * 8 + xcd;  // an XCD takes every eighth column tile and all row tiles of it
+  if (nt >= n_ntiles) return;
+  const int64_t mt0 = (int64_t)(j % n_mtiles) * (MI * WM);
+  const int n0 = nt * COLS;
+  const int lane = lane_id(), ln = lane & 15, kb = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+  const int K = a.K, n_stages = K / 128, G = K / GROUP, quads = (G + 3) / 4, row_bytes = K * BITS / 8;
+  const int64_t x_bytes = (row_tiles(a.M) - mt0) * K * 16, w_bytes = (int64_t)(a.N - n0) * row_bytes;
+  const i32x4_t xr = words_of(reinterpret_cast<const char *>(tiles) + mt0 * K * 16, (uint32_t)(x_bytes < INT32_MAX ? x_bytes : INT32_MAX));
+  const i32x4_t wr = words_of(reinterpret_cast<const char *>(a.w) + (int64_t)n0 * row_bytes, (uint32_t)(w_bytes < INT32_MAX ? w_bytes : INT32_MAX));
+  // copies: 1024 bytes an instruction; of the rows tile (i / 2) of 16 and half i % 2 of the stage, of the codes 1024 / CODES weight rows
+  constexpr int A_COPIES = MI * WM * 2, B_ROWS = 1024 / CODES, B_COPIES = COLS / B_ROWS;
+  static_assert(A_COPIES % kWaves == 0 && B_COPIES % kWaves == 0);
+  const int brow = lane / PIECES;
+  auto turn = [](int row) { return PIECES == 4 ? (row >> 2) & 3 : (row >> 1) & 7; };
+  auto copy_stage = [&](int t) __attribute__((always_inline)) {
+    const uint32_t to = (uint32_t)(t & 1) * STAGE;
+#pragma unroll
+    for (int u = 0; u < A_COPIES / kWaves; ++u) {
+      const int i = u * kWaves + wave;
+      copy_to_lds(xr, lane * 16, (i >> 1) * (K * 16) + t * 2048 + (i & 1) * 1024, to + i * 1024);
+    }
+#pragma unroll
+    for (int u = 0; u < B_COPIES / kWaves; ++u) {
+      const int i = u * kWaves + wave, row = i * B_ROWS + brow;
+      copy_to_lds(wr, row * row_bytes + ((lane % PIECES) ^ turn(row)) * 16, t * CODES, to + A_BYTES + i * 1024);
+    }
+  };
+  using T = Value<DT>;
+  struct Scales { T v[GS]; };
+  const T *sp[NI], *bp[NI];
+#pragma unroll
+  for (int n = 0; n < NI; ++n) {
+    const int64_t col = n0 + (wn * NI + n) * 16 + ln;  // (columns outside: the last one's, not stored)
+    sp[n] = static_cast<const T *>(a.s) + (col < a.N ? col : a.N - 1) * G;
+    bp[n] = static_cast<const T *>(a.b) + (col < a.N ? col : a.N - 1) * G;
+  }
+  const float *sump[MI];
+#pragma unroll
+  for (int m = 0; m < MI; ++m) {
+    const int64_t mt = mt0 + wm * MI + m;
+    sump[m] = sums + (mt < row_tiles(a.M) ? mt : row_tiles(a.M) - 1) * quads * 64 + lane;
+  }
+  Scales next[NI];
+  T qs[NI], qb[NI];
+  float qx[MI];
+  auto load_scales = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+    for (int n = 0; n < NI; ++n) __builtin_memcpy(next[n].v, __builtin_assume_aligned(sp[n] + t * GS, sizeof(Scales) < 16 ? sizeof(Scales) : 16), sizeof(Scales));
+    if (t % PERIOD == 0) {
+      const int q = t / PERIOD, g = 4 * q + kb < G ? 4 * q + kb : G - 1;
+#pragma unroll
+      for (int n = 0; n < NI; ++n) qs[n] = sp[n][g], qb[n] = bp[n][g];
+#pragma unroll
+      for (int m = 0; m < MI; ++m) qx[m] = sump[m][q * 64];
+    }
+  };
+  f32x4_t acc[MI][NI];
+#pragma unroll
+  for (int m = 0; m < MI; ++m)
+#pragma unroll
+    for (int n = 0; n < NI; ++n) acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  copy_stage(0);
+  load_scales(0);
+#pragma unroll 1
+  for (int t = 0; t < n_stages; ++t) {
+    wait_copies<0>();
+    block_barrier();
+    float s[NI][GS];
+#pragma unroll
+    for (int n = 0; n < NI; ++n)
+#pragma unroll
+      for (int g = 0; g < GS; ++g) s[n][g] = as_f32(next[n].v[g]);
+    if (t % PERIOD == 0) {
+#pragma unroll
+      for (int n = 0; n < NI; ++n) {
+        constexpr float k = Centre<BITS>::of_codes;
+        const float beta = __builtin_fmaf(k * Centre<BITS>::value, as_f32(qs[n]), k * as_f32(qb[n]));
+#pragma unroll
+        for (int m = 0; m < MI; ++m) acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(qx[m], beta, acc[m][n], 0, 0, 0);
+      }
+    }
+    if (t + 1 < n_stages) {
+      load_scales(t + 1);
+      copy_stage(t + 1);
+    }
+    const unsigned char *const at = lds_raw + (t & 1) * STAGE;
+    constexpr int HP = GROUP == 128 ? 2 : 1;  // halves of the stage whose integer sums are one
+#pragma unroll
+    for (int h0 = 0; h0 < 2; h0 += HP) {
+      i32x4_t xa[HP][MI], wb[HP][NI];
+#pragma unroll
+      for (int p = 0; p < HP; ++p) {
+        const int h = h0 + p;
+#pragma unroll
+        for (int m = 0; m < MI; ++m) xa[p][m] = *reinterpret_cast<const i32x4_t *>(at + ((wm * MI + m) * 2 + h) * 1024 + lane * 16);
+#pragma unroll
+        for (int n = 0; n < NI; ++n) {
+          const int row = (wn * NI + n) * 16 + ln;
+          const unsigned char *const r = at + A_BYTES + row * CODES;
+          auto piece = [&](int byte) { return r + (((byte >> 4) ^ turn(row)) << 4) + (byte & 15); };
+          uint2 lo, hi = make_uint2(0, 0);
+          if constexpr (BITS == 8 && GROUP != 32) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(piece(h * 64 + 16 * kb));
+            lo = make_uint2(v.x, v.y), hi = make_uint2(v.z, v.w);
+          } else if constexpr (BITS == 8) {
+            lo = *reinterpret_cast<const uint2 *>(piece(h * 64 + 8 * kb));
+            hi = *reinterpret_cast<const uint2 *>(piece(h * 64 + 32 + 8 * kb));
+          } else if constexpr (GROUP != 32) {
+            lo = *reinterpret_cast<const uint2 *>(piece(h * 32 + 8 * kb));
+          } else {
+            lo = make_uint2(*reinterpret_cast<const uint32_t *>(piece(h * 32 + 4 * kb)), *reinterpret_cast<const uint32_t *>(piece(h * 32 + 16 + 4 * kb)));
+          }
+          wb[p][n] = operand_of<BITS>(lo, hi);
+        }
+      }
+      const i32x4_t zero = {0, 0, 0, 0};
+      auto add = [&](f32x4_t &to, float scale, i32x4_t d) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) to[i] = __builtin_fmaf(scale, (float)d[i], to[i]);
+      };
+#pragma unroll
+      for (int m = 0; m < MI; ++m)
+#pragma unroll
+        for (int n = 0; n < NI; ++n) {
+          if constexpr (GROUP == 32) {
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              const i32x2_t x2 = {xa[0][m][2 * g], xa[0][m][2 * g + 1]}, w2 = {wb[0][n][2 * g], wb[0][n][2 * g + 1]};
+              add(acc[m][n], s[n][2 * h0 + g], __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, x2), __builtin_bit_cast(long, w2), zero, 0, 0, 0));
+            }
+          } else {
+            i32x4_t d = __builtin_amdgcn_mfma_i32_16x16x64_i8(xa[0][m], wb[0][n], zero, 0, 0, 0);
+            if constexpr (HP == 2) d = __builtin_amdgcn_mfma_i32_16x16x64_i8(xa[1][m], wb[1][n], d, 0, 0, 0);
+            add(acc[m][n], s[n][HP == 2 ? 0 : h0], d);
+          }
+        }
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MI; ++m)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t row = (mt0 + wm * MI + m) * 16 + 4 * kb + i;
+      if (row >= a.M) continue;
+      const float scale = a.row_scales[row] / Centre<BITS>::of_codes;
+#pragma unroll
+      for (int n = 0; n < NI; ++n) {
+        const int col = n0 + (wn * NI + n) * 16 + ln;
+        if (col >= a.N) continue;
+        float v = acc[m][n][i] * scale;
+        if (a.bias) v += as_f32(static_cast<const T *>(a.bias)[col]);
+        static_cast<T *>(a.y)[row * a.N + col] = value_of<DT>(v);
+      }
+    }
+}
+
+template <int DT, int BITS, int GROUP>
+static hipError_t start_tiles(const Rows8Args &a, void *workspace, hipStream_t st) {
+  uint4 *const tiles = static_cast<uint4 *>(workspace);
+  float *const sums = reinterpret_cast<float *>(static_cast<char *>(workspace) + rows8_tiles_bytes(a.M, a.K));
+  const int64_t units = row_tiles(a.M) * ((a.K / GROUP + 3) / 4);
+  if (units > (int64_t)4 * INT32_MAX) return hipErrorInvalidValue;
+  rows8_prepare_kernel<BITS, GROUP><<<(unsigned)((units + 3) / 4), 256, 0, st>>>(a.x, a.M, a.K, tiles, sums);
+  if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  constexpr int MI = 4, NI = 4, WM = 2, WN = 2, ROWS = 16 * MI * WM, COLS = 16 * NI * WN, lds = 2 * (ROWS * 128 + COLS * 128 * BITS / 8);
+  const int64_t n_mtiles = (a.M + ROWS - 1) / ROWS, n_ntiles = (a.N + COLS - 1) / COLS, grid = (n_ntiles + 7) / 8 * 8 * n_mtiles;
+  if (grid > INT32_MAX) return hipErrorInvalidValue;
+  rows8_tiles_kernel<DT, BITS, GROUP, MI, NI, WM, WN><<<(unsigned)grid, 64 * WM * WN, lds, st>>>(a, tiles, sums, (int)n_mtiles, (int)n_ntiles);
+  return hipGetLastError();
+}
+
+size_t rows8_workspace_bytes(int64_t M, int K) { return M <= kRows8Few || K % 128 ? 0 : rows8_tiles_bytes(M, K) + rows8_sums_bytes(M, K, 32); }
+
 template <int DT, int BITS>
 static hipError_t start_plain(const Rows8Args &a, hipStream_t st) {
   auto start = [&](auto rows) {
@@ -89,15 +345,22 @@ static hipError_t start_plain(const Rows8Args &a, hipStream_t st) {
   return a.M == 1 ? start(std::integral_constant<int, 1>{}) : start(std::integral_constant<int, 8>{});
 }
 
-hipError_t launch_qmm_rows8(const Rows8Args &a, int bits, int dt, hipStream_t st) {
+hipError_t launch_qmm_rows8(const Rows8Args &a, int bits, int dt, void *workspace, size_t workspace_bytes, hipStream_t st) {
   if (a.M == 0) return hipSuccess;
-  auto with_bits = [&](auto d) {
-    constexpr int DT = decltype(d)::value;
-    return bits == 4 ? start_plain<DT, 4>(a, st) : start_plain<DT, 8>(a, st);
+  auto even = [](const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
+  const size_t need = rows8_workspace_bytes(a.M, a.K);
+  const bool tiles = need && workspace && even(workspace) && workspace_bytes >= need && a.K <= 1 << 20 && even(a.x) && even(a.w) && even(a.s) && even(a.b);
+  auto with_bits = [&](auto d, auto b) {
+    constexpr int DT = decltype(d)::value, BITS = decltype(b)::value;
+    if (!tiles) return start_plain<DT, BITS>(a, st);
+    if (a.group == 32) return start_tiles<DT, BITS, 32>(a, workspace, st);
+    if (a.group == 64) return start_tiles<DT, BITS, 64>(a, workspace, st);
+    return start_tiles<DT, BITS, 128>(a, workspace, st);
   };
-  if (dt == 0) return with_bits(std::integral_constant<int, 0>{});
-  if (dt == 1) return with_bits(std::integral_constant<int, 1>{});
-  return with_bits(std::integral_constant<int, 2>{});
+  auto with_dtype = [&](auto d) { return bits == 4 ? with_bits(d, std::integral_constant<int, 4>{}) : with_bits(d, std::integral_constant<int, 8>{}); };
+  if (dt == 0) return with_dtype(std::integral_constant<int, 0>{});
+  if (dt == 1) return with_dtype(std::integral_constant<int, 1>{});
+  return with_dtype(std::integral_constant<int, 2>{});
 }
 
 }  // namespace mi_moe

@@ -188,114 +188,157 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void rows8_tiles_kernel(Rows8Args 
     }
   };
   using T = Value<DT>;
-  struct Scales { T v[GS]; };
-  const T *sp[NI], *bp[NI];
-#pragma unroll
-  for (int n = 0; n < NI; ++n) {
-    const int64_t col = n0 + (wn * NI + n) * 16 + ln;  // (columns outside: the last one's, not stored)
-    sp[n] = static_cast<const T *>(a.s) + (col < a.N ? col : a.N - 1) * G;
-    bp[n] = static_cast<const T *>(a.b) + (col < a.N ? col : a.N - 1) * G;
+  // Scales and biases, a window of 16 bytes a column (8 groups, or 4 of float32) at a time: a piece a thread, loaded a window ahead and laid into LDS in the window's last
+  // stage but one.  (Each lane loading its own, a few bytes a stage: 16 lines of 128 bytes a load, 83 KB a stage through an L1 of 32, and 205 us for 4096 x 4096 x 4096.)
+  constexpr int WINDOW = 16 / sizeof(T), WSTAGES = WINDOW / GS;
+  static_assert(2 * COLS == 64 * kWaves);
+  unsigned char *const scales_at = lds_raw + 2 * STAGE;
+  const T *piece_row;
+  {
+    const int64_t col = n0 + (int)threadIdx.x % COLS;  // (columns outside: the last one's, not stored)
+    piece_row = static_cast<const T *>(threadIdx.x < COLS ? a.s : a.b) + (col < a.N ? col : a.N - 1) * G;
   }
+  struct __align__(16) Window { T v[WINDOW]; };
+  Window window;
+  auto load_window = [&](int w) __attribute__((always_inline)) {
+    const int g = w * WINDOW;
+    if (g + WINDOW <= G) {
+      __builtin_memcpy(window.v, piece_row + g, 16);  // (rows of scales start anywhere)
+    } else {
+#pragma unroll
+      for (int i = 0; i < WINDOW; ++i) window.v[i] = piece_row[g + i < G ? g + i : G - 1];
+    }
+  };
+  auto put_window = [&](int w) __attribute__((always_inline)) {
+    *reinterpret_cast<Window *>(scales_at + (w & 1) * (COLS * 32) + threadIdx.x * 16) = window;
+  };
   const float *sump[MI];
 #pragma unroll
   for (int m = 0; m < MI; ++m) {
     const int64_t mt = mt0 + wm * MI + m;
     sump[m] = sums + (mt < row_tiles(a.M) ? mt : row_tiles(a.M) - 1) * quads * 64 + lane;
   }
-  Scales next[NI];
-  T qs[NI], qb[NI];
   float qx[MI];
-  auto load_scales = [&](int t) __attribute__((always_inline)) {
+  auto load_sums = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
-    for (int n = 0; n < NI; ++n) __builtin_memcpy(next[n].v, __builtin_assume_aligned(sp[n] + t * GS, sizeof(Scales) < 16 ? sizeof(Scales) : 16), sizeof(Scales));
-    if (t % PERIOD == 0) {
-      const int q = t / PERIOD, g = 4 * q + kb < G ? 4 * q + kb : G - 1;
-#pragma unroll
-      for (int n = 0; n < NI; ++n) qs[n] = sp[n][g], qb[n] = bp[n][g];
-#pragma unroll
-      for (int m = 0; m < MI; ++m) qx[m] = sump[m][q * 64];
-    }
+    for (int m = 0; m < MI; ++m) qx[m] = sump[m][t / PERIOD * 64];
   };
   f32x4_t acc[MI][NI];
 #pragma unroll
   for (int m = 0; m < MI; ++m)
 #pragma unroll
     for (int n = 0; n < NI; ++n) acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  // Integer sums start at the bits of 1.5 * 2^23, where a float's step is one: below 2^22 (128 products of 2^14 at most are 2^21) they leave the bits of that number
+  // and the sum, and a subtraction in place of a conversion, which is a quarter as fast.
+  constexpr float kWhole = 12582912.f;
+  constexpr int kWholeBits = 0x4b400000;
+  i32x4_t whole = {kWholeBits, kWholeBits, kWholeBits, kWholeBits};
+  asm("" : "+v"(whole));  // (a literal is not among the instruction's operands)
   copy_stage(0);
-  load_scales(0);
+  load_sums(0);
+  load_window(0);
+  put_window(0);
+  load_window(1);
 #pragma unroll 1
   for (int t = 0; t < n_stages; ++t) {
     wait_copies<0>();
     block_barrier();
+    const int w = t / WSTAGES;
+    const unsigned char *const mine = scales_at + (w & 1) * (COLS * 32) + (wn * NI * 16 + ln) * 16;  // this lane's columns: every 16th
     float s[NI][GS];
 #pragma unroll
-    for (int n = 0; n < NI; ++n)
+    for (int n = 0; n < NI; ++n) {
+      T v[GS];
+      __builtin_memcpy(v, __builtin_assume_aligned(mine + n * 256 + t % WSTAGES * (int)sizeof v, sizeof v), sizeof v);
 #pragma unroll
-      for (int g = 0; g < GS; ++g) s[n][g] = as_f32(next[n].v[g]);
+      for (int g = 0; g < GS; ++g) s[n][g] = as_f32(v[g]);
+    }
     if (t % PERIOD == 0) {
+      const int g = (t / PERIOD * 4 + kb) % WINDOW * (int)sizeof(T);
 #pragma unroll
       for (int n = 0; n < NI; ++n) {
         constexpr float k = Centre<BITS>::of_codes;
-        const float beta = __builtin_fmaf(k * Centre<BITS>::value, as_f32(qs[n]), k * as_f32(qb[n]));
+        const float beta = __builtin_fmaf(k * Centre<BITS>::value, as_f32(*reinterpret_cast<const T *>(mine + n * 256 + g)),
+                                          k * as_f32(*reinterpret_cast<const T *>(mine + COLS * 16 + n * 256 + g)));
 #pragma unroll
         for (int m = 0; m < MI; ++m) acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(qx[m], beta, acc[m][n], 0, 0, 0);
       }
     }
+    if ((t + 1) % WSTAGES == 0) {  // (what was loaded a window ago is there: every stage waits for all loads before it)
+      put_window(w + 1);
+      load_window(w + 2);
+    }
     if (t + 1 < n_stages) {
-      load_scales(t + 1);
+      if ((t + 1) % PERIOD == 0) load_sums(t + 1);
       copy_stage(t + 1);
     }
     const unsigned char *const at = lds_raw + (t & 1) * STAGE;
-    constexpr int HP = GROUP == 128 ? 2 : 1;  // halves of the stage whose integer sums are one
-#pragma unroll
-    for (int h0 = 0; h0 < 2; h0 += HP) {
-      i32x4_t xa[HP][MI], wb[HP][NI];
-#pragma unroll
-      for (int p = 0; p < HP; ++p) {
-        const int h = h0 + p;
-#pragma unroll
-        for (int m = 0; m < MI; ++m) xa[p][m] = *reinterpret_cast<const i32x4_t *>(at + ((wm * MI + m) * 2 + h) * 1024 + lane * 16);
-#pragma unroll
-        for (int n = 0; n < NI; ++n) {
-          const int row = (wn * NI + n) * 16 + ln;
-          const unsigned char *const r = at + A_BYTES + row * CODES;
-          auto piece = [&](int byte) { return r + (((byte >> 4) ^ turn(row)) << 4) + (byte & 15); };
-          uint2 lo, hi = make_uint2(0, 0);
-          if constexpr (BITS == 8 && GROUP != 32) {
-            const uint4 v = *reinterpret_cast<const uint4 *>(piece(h * 64 + 16 * kb));
-            lo = make_uint2(v.x, v.y), hi = make_uint2(v.z, v.w);
-          } else if constexpr (BITS == 8) {
-            lo = *reinterpret_cast<const uint2 *>(piece(h * 64 + 8 * kb));
-            hi = *reinterpret_cast<const uint2 *>(piece(h * 64 + 32 + 8 * kb));
-          } else if constexpr (GROUP != 32) {
-            lo = *reinterpret_cast<const uint2 *>(piece(h * 32 + 8 * kb));
-          } else {
-            lo = make_uint2(*reinterpret_cast<const uint32_t *>(piece(h * 32 + 4 * kb)), *reinterpret_cast<const uint32_t *>(piece(h * 32 + 16 + 4 * kb)));
-          }
-          wb[p][n] = operand_of<BITS>(lo, hi);
-        }
+    struct Half {  // the operands of 64 values
+      i32x4_t x[MI], w[NI];
+      uint2 lo[NI], hi[NI];
+    };
+    Half half[2];
+    auto read_x = [&](int h, int m) __attribute__((always_inline)) {
+      half[h].x[m] = *reinterpret_cast<const i32x4_t *>(at + ((wm * MI + m) * 2 + h) * 1024 + lane * 16);
+    };
+    auto read_w = [&](int h, int n) __attribute__((always_inline)) {
+      const int row = (wn * NI + n) * 16 + ln;
+      const unsigned char *const r = at + A_BYTES + row * CODES;
+      auto piece = [&](int byte) { return r + (((byte >> 4) ^ turn(row)) << 4) + (byte & 15); };
+      uint2 &lo = half[h].lo[n], &hi = half[h].hi[n];
+      hi = make_uint2(0, 0);
+      if constexpr (BITS == 8 && GROUP != 32) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(piece(h * 64 + 16 * kb));
+        lo = make_uint2(v.x, v.y), hi = make_uint2(v.z, v.w);
+      } else if constexpr (BITS == 8) {
+        lo = *reinterpret_cast<const uint2 *>(piece(h * 64 + 8 * kb));
+        hi = *reinterpret_cast<const uint2 *>(piece(h * 64 + 32 + 8 * kb));
+      } else if constexpr (GROUP != 32) {
+        lo = *reinterpret_cast<const uint2 *>(piece(h * 32 + 8 * kb));
+      } else {
+        lo = make_uint2(*reinterpret_cast<const uint32_t *>(piece(h * 32 + 4 * kb)), *reinterpret_cast<const uint32_t *>(piece(h * 32 + 16 + 4 * kb)));
       }
-      const i32x4_t zero = {0, 0, 0, 0};
-      auto add = [&](f32x4_t &to, float scale, i32x4_t d) __attribute__((always_inline)) {
+    };
+    auto unpack = [&](int h, int n) __attribute__((always_inline)) { half[h].w[n] = operand_of<BITS>(half[h].lo[n], half[h].hi[n]); };
+    // The tiles one after the other, each multiplied LEAD steps before its sums are converted and scaled: written out in the order in which it is to run (the compiler's own
+    // order has a multiply's results used right behind it: 195.7 us for 4096 x 4096 x 4096, 4-bit, groups of 64).
+    constexpr int PER = GROUP == 32 ? 2 : 1, HALVES = GROUP == 128 ? 1 : 2, TILES = MI * NI, STEPS = HALVES * TILES * PER, LEAD = 3;
+    i32x4_t d[LEAD + 1];
+    auto multiply = [&](int k) __attribute__((always_inline)) {
+      const int h = k / (TILES * PER), m = k / PER % TILES / NI, n = k / PER % NI, g = k % PER;
+      if constexpr (GROUP == 32) {
+        const i32x2_t x2 = {half[h].x[m][2 * g], half[h].x[m][2 * g + 1]}, w2 = {half[h].w[n][2 * g], half[h].w[n][2 * g + 1]};
+        d[k % (LEAD + 1)] = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, x2), __builtin_bit_cast(long, w2), whole, 0, 0, 0);
+      } else {
+        d[k % (LEAD + 1)] = __builtin_amdgcn_mfma_i32_16x16x64_i8(half[h].x[m], half[h].w[n], whole, 0, 0, 0);
+        if constexpr (GROUP == 128) d[k % (LEAD + 1)] = __builtin_amdgcn_mfma_i32_16x16x64_i8(half[1].x[m], half[1].w[n], d[k % (LEAD + 1)], 0, 0, 0);
+      }
+    };
+    auto scale = [&](int k) __attribute__((always_inline)) {
+      const int h = k / (TILES * PER), m = k / PER % TILES / NI, n = k / PER % NI, g = k % PER;
+      const i32x4_t v = d[k % (LEAD + 1)];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) to[i] = __builtin_fmaf(scale, (float)d[i], to[i]);
-      };
+      for (int i = 0; i < 4; ++i) acc[m][n][i] = __builtin_fmaf(s[n][h * PER + g], __int_as_float(v[i]) - kWhole, acc[m][n][i]);
+    };
 #pragma unroll
-      for (int m = 0; m < MI; ++m)
+    for (int h = 0; h < (GROUP == 128 ? 2 : 1); ++h) {
 #pragma unroll
-        for (int n = 0; n < NI; ++n) {
-          if constexpr (GROUP == 32) {
+      for (int n = 0; n < NI; ++n) read_w(h, n);
 #pragma unroll
-            for (int g = 0; g < 2; ++g) {
-              const i32x2_t x2 = {xa[0][m][2 * g], xa[0][m][2 * g + 1]}, w2 = {wb[0][n][2 * g], wb[0][n][2 * g + 1]};
-              add(acc[m][n], s[n][2 * h0 + g], __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, x2), __builtin_bit_cast(long, w2), zero, 0, 0, 0));
-            }
-          } else {
-            i32x4_t d = __builtin_amdgcn_mfma_i32_16x16x64_i8(xa[0][m], wb[0][n], zero, 0, 0, 0);
-            if constexpr (HP == 2) d = __builtin_amdgcn_mfma_i32_16x16x64_i8(xa[1][m], wb[1][n], d, 0, 0, 0);
-            add(acc[m][n], s[n][HP == 2 ? 0 : h0], d);
-          }
-        }
+      for (int m = 0; m < MI; ++m) read_x(h, m);
+#pragma unroll
+      for (int n = 0; n < NI; ++n) unpack(h, n);
+    }
+#pragma unroll
+    for (int k = 0; k < STEPS + LEAD; ++k) {
+      if constexpr (HALVES == 2) {  // the second half's operands: read during the first steps, unpacked ahead of their own
+        if (k < NI) read_w(1, k);
+        if (k < MI) read_x(1, k);
+        if (k >= TILES * PER - NI && k < TILES * PER) unpack(1, k - (TILES * PER - NI));
+      }
+      if (k < STEPS) multiply(k);
+      if (k >= LEAD) scale(k - LEAD);
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 #pragma unroll
@@ -324,10 +367,13 @@ static hipError_t start_tiles(const Rows8Args &a, void *workspace, hipStream_t s
   if (units > (int64_t)4 * INT32_MAX) return hipErrorInvalidValue;
   rows8_prepare_kernel<BITS, GROUP><<<(unsigned)((units + 3) / 4), 256, 0, st>>>(a.x, a.M, a.K, tiles, sums);
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-  constexpr int MI = 4, NI = 4, WM = 2, WN = 2, ROWS = 16 * MI * WM, COLS = 16 * NI * WN, lds = 2 * (ROWS * 128 + COLS * 128 * BITS / 8);
+  constexpr int MI = 4, NI = 4, WM = 2, WN = 2, ROWS = 16 * MI * WM, COLS = 16 * NI * WN, lds = 2 * (ROWS * 128 + COLS * 128 * BITS / 8) + 2 * COLS * 32;
   const int64_t n_mtiles = (a.M + ROWS - 1) / ROWS, n_ntiles = (a.N + COLS - 1) / COLS, grid = (n_ntiles + 7) / 8 * 8 * n_mtiles;
   if (grid > INT32_MAX) return hipErrorInvalidValue;
-  rows8_tiles_kernel<DT, BITS, GROUP, MI, NI, WM, WN><<<(unsigned)grid, 64 * WM * WN, lds, st>>>(a, tiles, sums, (int)n_mtiles, (int)n_ntiles);
+  const auto kernel = &rows8_tiles_kernel<DT, BITS, GROUP, MI, NI, WM, WN>;
+  static std::atomic<uint64_t> allowed{0};
+  if (hipError_t e = allow_lds(reinterpret_cast<const void *>(kernel), lds, allowed); e != hipSuccess) return e;
+  kernel<<<(unsigned)grid, 64 * WM * WN, lds, st>>>(a, tiles, sums, (int)n_mtiles, (int)n_ntiles);
   return hipGetLastError();
 }
 

@@ -44,6 +44,10 @@ def truth(x, sx, w, s, b, lb, group, bits):
     return (y if lb is None else y + lb.double()), size * sx.double()[:, None]
 
 
+# products whose tiles fill the chip, with last tiles of every kind
+TILED = [(257, 3000, 512), (520, 5000, 256), (1300, 4111, 128), (900, 2500, 896), (2100, 4000, 384), (1000, 4096, 512), (256, 4096, 1024)]
+
+
 def check(y, args, group, bits):
     x, sx, w, s, b, lb = args
     ref, size = truth(x, sx, w, s, b, lb, group, bits)
@@ -74,6 +78,15 @@ SHAPES = [(1, 1, 128), (1, 17, 256), (1, 1000, 2048), (2, 64, 384), (7, 33, 640)
 @pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_linear(dtype, bits, group, M, N, K):
+    args = layer(M, N, K, bits, group, dtype, bias=(M + N) % 2 == 1)
+    check(run(args, group, bits), args, group, bits)
+
+
+@pytest.mark.parametrize("M,N,K", TILED)
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_in_tiles(dtype, bits, group, M, N, K):
     args = layer(M, N, K, bits, group, dtype, bias=(M + N) % 2 == 1)
     check(run(args, group, bits), args, group, bits)
 

@@ -28,6 +28,14 @@ struct Octet {  // as they lie in memory; DT: mi_moe_dtype
   using Raw = typename std::conditional<DT == 0, uint16_t, typename std::conditional<DT == 1, _Float16, float>::type>::type;
   Raw v[8];
   __device__ __forceinline__ float at(int i) const { return as_f32(v[i]); }
+  __device__ __forceinline__ void put2(int i, float lo, float hi) {  // i: even
+    if constexpr (DT == 0) {
+      const uint32_t p = cvt_pk_bf16(lo, hi);
+      v[i] = (uint16_t)p, v[i + 1] = (uint16_t)(p >> 16);
+    } else {
+      v[i] = (Raw)lo, v[i + 1] = (Raw)hi;
+    }
+  }
   __device__ __forceinline__ void put(int i, float f) {
     if constexpr (DT == 0) v[i] = f32_to_bf16(f);
     else v[i] = (Raw)f;
@@ -96,7 +104,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void add_rms_norm_kernel(Nor
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) h[c].put(i, h[c].at(i) + r[c].at(i));
+      for (int i = 0; i < 8; i += 2) h[c].put2(i, h[c].at(i) + r[c].at(i), h[c].at(i + 1) + r[c].at(i + 1));
   }
   double ss = 0.0, most = 0.0;  // most: the largest |w h|; infinite where one of them is infinite or no number
   if (a.sum) {
@@ -139,7 +147,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void add_rms_norm_kernel(Nor
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) h[c].put(i, w[c].at(i) * (h[c].at(i) * rstd));
+      for (int i = 0; i < 8; i += 2) h[c].put2(i, w[c].at(i) * (h[c].at(i) * rstd), w[c].at(i + 1) * (h[c].at(i + 1) * rstd));
       store_octet<DT>(a.y, at + (c * TPR + t) * 8, a.H - (c * TPR + t) * 8, h[c]);
     }
   } else {
@@ -207,19 +215,19 @@ struct NormGradArgs {
   const void *dy, *h, *dh, *w;  // dh: or nullptr
   float eps;
   int64_t T;
-  int H, groups;
-  void *dx, *dw;
-  float *parts;  // [groups, H]: the rows' shares of dw, of every group of rows
+  int H;
+  void *dx;
+  float *parts;  // [blocks, H]: every block's sums over its rows
 };
 
-// TPR threads have every groups-th row, and their columns' sums for dw in registers; the sums of the groups meet in a second launch, in a fixed order.
+// A block has every blocks-th row (rows of up to 1024 values: a wave each, four at a time), the next one's loads under way while it works on one, and its columns' sums for dw in
+// registers; the sums of the blocks meet in a second launch, in a fixed order.  Bound by memory: what the forward pass reads and writes, and the blocks' sums twice.
 template <int DT, int TPR, int CH>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_grad_kernel(NormGradArgs a) {
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR, 4) void norm_grad_kernel(NormGradArgs a) {
   constexpr int kRows = TPR < 256 ? 256 / TPR : 1, kWaves = TPR / kWave;
   __shared__ double part[2][kWaves][2];
-  const int t = threadIdx.x % TPR, wave = t / kWave;
-  const int group = blockIdx.x * kRows + threadIdx.x / TPR;
-  if (kWaves == 1 && group >= a.groups) return;
+  const int t = threadIdx.x % TPR, wave = t / kWave, which = threadIdx.x / TPR;
+  const int64_t step = (int64_t)gridDim.x * kRows;
   Octet<DT> w[CH];
   float dw[CH][8];
 #pragma unroll
@@ -228,24 +236,24 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_grad_kernel(NormGr
 #pragma unroll
     for (int i = 0; i < 8; ++i) dw[c][i] = 0.f;
   }
-  int turn = 0;
-  for (int64_t row = group; row < a.T; row += a.groups, turn ^= 1) {
-    const int64_t at = row * a.H;
-    Octet<DT> h[CH], dy[CH];
+  int64_t row = (int64_t)blockIdx.x * kRows + which;
+  for (int turn = 0; row < a.T; row += step, turn ^= 1) {  // (rows of several waves: the same for all of the block's)
+    struct { Octet<DT> h[CH], dy[CH], dh[CH]; } R;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int j = (c * TPR + t) * 8;
-      h[c] = load_octet<DT>(a.h, at + j, a.H - j);
-      dy[c] = load_octet<DT>(a.dy, at + j, a.H - j);
+      R.h[c] = load_octet<DT>(a.h, row * a.H + j, a.H - j);
+      R.dy[c] = load_octet<DT>(a.dy, row * a.H + j, a.H - j);
+      if (a.dh) R.dh[c] = load_octet<DT>(a.dh, row * a.H + j, a.H - j);
     }
     double ss = 0.0, dot = 0.0;  // sums of h^2 and of w dy h
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const double v = h[c].at(i);
+        const double v = R.h[c].at(i);
         ss = __builtin_fma(v, v, ss);
-        const double g = DT == 2 ? (double)w[c].at(i) * (double)dy[c].at(i) : (double)(w[c].at(i) * dy[c].at(i));  // (exact either way)
+        const double g = DT == 2 ? (double)w[c].at(i) * (double)R.dy[c].at(i) : (double)(w[c].at(i) * R.dy[c].at(i));  // (exact either way)
         dot = __builtin_fma(g, v, dot);
       }
     ss = wave_sum_f64(ss);
@@ -261,79 +269,108 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_grad_kernel(NormGr
     const float mean = (float)(dot * (double)rstd / (double)a.H);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const int j = (c * TPR + t) * 8, n = a.H - j;
-      Octet<DT> add;
-      if (a.dh) add = load_octet<DT>(a.dh, at + j, n);
+      const int j = (c * TPR + t) * 8;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float hat = h[c].at(i) * rstd, g = dy[c].at(i);
-        dw[c][i] = __builtin_fmaf(g, hat, dw[c][i]);
-        float d = rstd * __builtin_fmaf(-hat, mean, w[c].at(i) * g);
-        if (a.dh) d += add.at(i);
-        h[c].put(i, d);
+      for (int i = 0; i < 8; i += 2) {
+        float d[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float hat = R.h[c].at(i + k) * rstd, g = R.dy[c].at(i + k);
+          dw[c][i + k] = __builtin_fmaf(g, hat, dw[c][i + k]);
+          d[k] = rstd * __builtin_fmaf(-hat, mean, w[c].at(i + k) * g);
+          if (a.dh) d[k] += R.dh[c].at(i + k);
+        }
+        R.h[c].put2(i, d[0], d[1]);
       }
-      store_octet<DT>(a.dx, at + j, n, h[c]);
+      store_octet<DT>(a.dx, row * a.H + j, a.H - j, R.h[c]);
     }
+  }
+  float *const to = a.parts + (int64_t)blockIdx.x * a.H;
+  if constexpr (kRows > 1) {  // the block's rows' sums, one after the other
+    __shared__ float meet[kRows - 1][CH * TPR * 8];
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (which > 0) meet[which - 1][(c * 8 + i) * TPR + t] = dw[c][i];
+    __syncthreads();
+    if (which > 0) return;
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int r = 0; r < kRows - 1; ++r) dw[c][i] += meet[r][(c * 8 + i) * TPR + t];
   }
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     const int j = (c * TPR + t) * 8;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (j + i < a.H) a.parts[(int64_t)group * a.H + j + i] = dw[c][i];
+      if (j + i < a.H) to[j + i] = dw[c][i];
   }
 }
 
-// dw = the groups' sums: 32 columns a block, every eighth group a thread
+// dw = the blocks' sums: 16 columns a block, every 64th block's sums a thread
 template <int DT>
-__global__ __launch_bounds__(256) void norm_grad_weight_kernel(const float *parts, int groups, int H, void *dw) {
-  __shared__ float sums[8][32];
-  const int col = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5;
+__global__ __launch_bounds__(1024) void norm_grad_weight_kernel(const float *parts, int blocks, int H, void *dw) {
+  __shared__ float sums[64][17];
+  const int c = threadIdx.x & 15, col = blockIdx.x * 16 + c, slice = threadIdx.x >> 4;
   float s = 0.f;
-  if (col < H)
-    for (int g = slice; g < groups; g += 8) s += parts[(int64_t)g * H + col];
-  sums[slice][threadIdx.x & 31] = s;
+  if (col < H) {
+#pragma unroll 4
+    for (int g = slice; g < blocks; g += 64) s += parts[(int64_t)g * H + col];
+  }
+  sums[slice][c] = s;
   __syncthreads();
-  if (slice == 0 && col < H) {
-    float v = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v += sums[i][threadIdx.x & 31];
-    Octet<DT> o;
-    o.put(0, v);
-    static_cast<typename Octet<DT>::Raw *>(dw)[col] = o.v[0];
+  if (threadIdx.x < 256) {  // 16 threads a column, four sums each, then a tree
+    const int cc = threadIdx.x >> 4, q = threadIdx.x & 15;
+    float v = (sums[q][cc] + sums[q + 16][cc]) + (sums[q + 32][cc] + sums[q + 48][cc]);
+    v += __uint_as_float(dpp_u32<kDppXor1>(__float_as_uint(v)));
+    v += __uint_as_float(dpp_u32<kDppXor2>(__float_as_uint(v)));
+    v += __uint_as_float(dpp_u32<kDppHalfMirror>(__float_as_uint(v)));
+    v += __uint_as_float(dpp_u32<kDppMirror>(__float_as_uint(v)));
+    if (q == 0 && blockIdx.x * 16 + cc < H) {
+      Octet<DT> o;
+      o.put(0, v);
+      static_cast<typename Octet<DT>::Raw *>(dw)[blockIdx.x * 16 + cc] = o.v[0];
+    }
   }
 }
 
-// groups of rows of the backward pass: what fills the chip, and no more of them than rows
-static int norm_grad_groups(int64_t T, int H) {
-  const int64_t most = H <= 1024 ? 2048 : 512;
-  return (int)(T < most ? T : most);
+// Blocks of the backward pass: what the chip holds at once (of 1024 threads one a CU), and rows enough for each that its sums for dw are little beside them.  us, bf16, 256 / 512 / 768 / 1024
+// blocks: 1000 x 2048 12.0, 12.8, 15.0, 18.0; 4096 x 4096 42.8, 37.5, 41.0, 41.8; 16384 x 1024 51.3, 36.0, 29.8, 32.1; float32 2048 x 8192 51.5, 62.8, 72.3, 82.7.  (The next row's loads
+// ahead of a row's sums cost registers, and with them waves: 46.3, 39.1, 44.0, 45.7 for 4096 x 4096.)
+static int norm_grad_blocks(int64_t T, int H) {
+  const int64_t rows = H <= 1024 ? (T + 3) / 4 : T, most = H <= 1024 ? 768 : H <= 4096 ? 512 : 256;
+  const int64_t few = rows / 5 > 256 ? rows / 5 : 256, blocks = few < most ? few : most;
+  return (int)(rows < blocks ? rows : blocks);
 }
-size_t norm_grad_bytes(int64_t T, int H) { return (size_t)norm_grad_groups(T, H) * H * sizeof(float); }
+size_t norm_grad_bytes(int64_t T, int H) { return (size_t)norm_grad_blocks(T, H) * H * sizeof(float); }
 
 template <int DT, int TPR, int CH>
-static hipError_t start_norm_grad(const NormGradArgs &a, hipStream_t st) {
-  constexpr int block = TPR < 256 ? 256 : TPR, rows = block / TPR;
-  norm_grad_kernel<DT, TPR, CH><<<(unsigned)((a.groups + rows - 1) / rows), block, 0, st>>>(a);
+static hipError_t start_norm_grad(const NormGradArgs &a, int blocks, hipStream_t st) {
+  norm_grad_kernel<DT, TPR, CH><<<(unsigned)blocks, TPR < 256 ? 256 : TPR, 0, st>>>(a);
   return hipGetLastError();
 }
 
 hipError_t launch_norm_grad(const void *dy, const void *h, const void *dh, const void *w, float eps, int64_t T, int H, int dt, void *dx, void *dw,
                             float *parts, hipStream_t st) {
-  const NormGradArgs a{dy, h, dh, w, eps, T, H, norm_grad_groups(T, H), dx, dw, parts};
+  const NormGradArgs a{dy, h, dh, w, eps, T, H, dx, parts};
+  const int blocks = norm_grad_blocks(T, H);
   return with_dtype(dt, [&](auto d) {
     constexpr int DT = decltype(d)::value;
     hipError_t e = hipSuccess;
     if (T > 0)
-      e = H <= 512     ? start_norm_grad<DT, 64, 1>(a, st)
-          : H <= 1024  ? start_norm_grad<DT, 64, 2>(a, st)
-          : H <= 2048  ? start_norm_grad<DT, 256, 1>(a, st)
-          : H <= 4096  ? start_norm_grad<DT, 256, 2>(a, st)
-          : H <= 8192  ? start_norm_grad<DT, 256, 4>(a, st)
-          : H <= 16384 ? start_norm_grad<DT, 1024, 2>(a, st)
-                       : start_norm_grad<DT, 1024, 4>(a, st);
+      e = H <= 512     ? start_norm_grad<DT, 64, 1>(a, blocks, st)
+          : H <= 1024  ? start_norm_grad<DT, 64, 2>(a, blocks, st)
+          : H <= 2048  ? start_norm_grad<DT, 256, 1>(a, blocks, st)
+          : H <= 4096  ? start_norm_grad<DT, 512, 1>(a, blocks, st)
+          : H <= 8192  ? start_norm_grad<DT, 1024, 1>(a, blocks, st)
+          : H <= 16384 ? start_norm_grad<DT, 1024, 2>(a, blocks, st)
+                       : start_norm_grad<DT, 1024, 4>(a, blocks, st);
     if (e != hipSuccess) return e;
-    norm_grad_weight_kernel<DT><<<(unsigned)((H + 31) / 32), 256, 0, st>>>(parts, a.groups, H, dw);  // (no rows: zeros)
+    norm_grad_weight_kernel<DT><<<(unsigned)((H + 15) / 16), 1024, 0, st>>>(parts, blocks, H, dw);  // (no rows: zeros)
     return hipGetLastError();
   });
 }

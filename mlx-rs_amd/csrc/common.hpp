@@ -452,7 +452,7 @@ hipError_t launch_add_rms_norm(const void *x, const void *r, const void *w, floa
 size_t norm_grad_bytes(int64_t T, int H);  // parts
 hipError_t launch_norm_grad(const void *dy, const void *h, const void *dh, const void *w, float eps, int64_t T, int H, int dt, void *dx, void *dw,
                             float *parts, hipStream_t st);
-constexpr int kNormMostHidden = 32768;  // a row stays in the registers of 1024 threads
+constexpr int kNormMostHidden = 32768;
 // Experts from logits (select.hip); scoring, group_score: mi_moe_scoring, mi_moe_group_score.
 struct SelectArgs {
   const void *logits;

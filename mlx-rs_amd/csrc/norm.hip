@@ -76,6 +76,53 @@ __device__ __forceinline__ float rstd_of(double ss, int H, float eps) {
   return (float)(1.0 / sqrt(m + (double)eps));
 }
 
+// the codes of an octet in eight bits; most: the row's largest |w h|, inv = 127 / most
+template <int DT>
+__device__ __forceinline__ void put_codes(unsigned char *to, int n, const Octet<DT> &h, const Octet<DT> &w, double most) {
+  // rows of zeros have a scale and codes of zero; rows that hold an infinity or no number a scale that is none, so that what is made of them is none either
+  const bool none = !(most > 0.0 && most < INFINITY), wide = !(most > 1e-30 && most < 1e30);
+  const float inv = none ? 0.f : (float)(127.0 / most);
+  uint32_t q[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float v = h.at(i) * w.at(i) * inv;
+    float k = rintf(v);
+    // the float quotient is up to 2^-15 off (three roundings of a value below 128): where that could change the integer, or the products leave
+    // the floats' range, the exact products decide
+    if (none) k = 0.f;
+    else if (wide || fabsf(v - k) > 0.4999f) k = (float)rint(127.0 * ((double)h.at(i) * (double)w.at(i)) / most);
+    q[i / 4] |= ((uint32_t)(int)k & 0xffu) << (8 * (i % 4));
+  }
+  if (n >= 8) __builtin_memcpy(to, q, 8);
+  else
+    for (int i = 0; i < n; ++i) to[i] = (unsigned char)(q[i / 4] >> (8 * (i % 4)));
+}
+__device__ __forceinline__ float scale_of(double most, float rstd) {
+  return most > 0.0 && most < INFINITY ? (float)(most * (double)rstd / 127.0) : most > 0.0 ? NAN : 0.f;
+}
+// the largest |w h| of an octet and `most`, infinite where one is infinite or no number
+template <int DT>
+__device__ __forceinline__ double largest(double most, const Octet<DT> &h, const Octet<DT> &w) {
+  bool finite = true;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const double p = fabs((double)h.at(i) * (double)w.at(i));
+    finite &= p < INFINITY;
+    most = p > most ? p : most;
+  }
+  return finite ? most : INFINITY;
+}
+// a block's sums and largest values, in the order of its waves
+template <int WAVES>
+__device__ __forceinline__ void meet(double (&part)[WAVES][2], double &sum, double &other, bool is_sum) {
+  if ((threadIdx.x & (kWave - 1)) == 0) part[threadIdx.x / kWave % WAVES][0] = sum, part[threadIdx.x / kWave % WAVES][1] = other;
+  __syncthreads();
+  sum = 0.0;
+  other = 0.0;
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) sum += part[i][0], other = is_sum ? other + part[i][1] : fmax(other, part[i][1]);
+}
+
 struct NormArgs {
   const void *x, *r, *w;  // r: or nullptr, then the sum is x
   float eps;
@@ -89,8 +136,8 @@ struct NormArgs {
 template <int DT, int TPR, int CH, bool ROWS8>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void add_rms_norm_kernel(NormArgs a) {
   constexpr int kRows = TPR < 256 ? 256 / TPR : 1, kWaves = TPR / kWave;
-  __shared__ double part[kRows][kWaves][2];
-  const int t = threadIdx.x % TPR, wave = t / kWave;
+  __shared__ double part[kWaves][2];
+  const int t = threadIdx.x % TPR;
   const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR;
   if (kWaves == 1 && row >= a.T) return;  // (rows of several waves have a block each: none is outside)
   const int64_t at = row * a.H;
@@ -119,29 +166,12 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void add_rms_norm_kernel(Nor
 #pragma unroll
   for (int c = 0; c < CH; ++c) w[c] = load_octet<DT>(a.w, (c * TPR + t) * 8, a.H - (c * TPR + t) * 8);
   if constexpr (ROWS8) {
-    bool finite = true;
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const double p = fabs((double)h[c].at(i) * (double)w[c].at(i));
-        finite &= p < INFINITY;
-        most = p > most ? p : most;
-      }
-    if (!finite) most = INFINITY;
+    for (int c = 0; c < CH; ++c) most = largest<DT>(most, h[c], w[c]);
   }
   ss = wave_sum_f64(ss);
   if constexpr (ROWS8) most = wave_max_f64(most);
-  if constexpr (kWaves > 1) {
-    if ((t & (kWave - 1)) == 0) part[0][wave][0] = ss, part[0][wave][1] = most;
-    __syncthreads();
-    ss = 0.0;
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-      ss += part[0][i][0];
-      if constexpr (ROWS8) most = fmax(most, part[0][i][1]);
-    }
-  }
+  if constexpr (kWaves > 1) meet<kWaves>(part, ss, most, false);
   const float rstd = rstd_of(ss, a.H, a.eps);
   if constexpr (!ROWS8) {
 #pragma unroll
@@ -151,30 +181,58 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void add_rms_norm_kernel(Nor
       store_octet<DT>(a.y, at + (c * TPR + t) * 8, a.H - (c * TPR + t) * 8, h[c]);
     }
   } else {
-    // rows of zeros have a scale and codes of zero; rows that hold an infinity or no number a scale that is none, so that what is made of them is none either
-    const bool none = !(most > 0.0 && most < INFINITY), wide = !(most > 1e-30 && most < 1e30);
-    const float inv = none ? 0.f : (float)(127.0 / most);
-    if (t == 0) a.scales[row] = !none ? (float)(most * (double)rstd / 127.0) : most > 0.0 ? NAN : 0.f;
+    if (t == 0) a.scales[row] = scale_of(most, rstd);
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      const int n = a.H - (c * TPR + t) * 8;
-      uint32_t q[2] = {0, 0};
+    for (int c = 0; c < CH; ++c)
+      put_codes<DT>(static_cast<unsigned char *>(a.y) + at + (c * TPR + t) * 8, a.H - (c * TPR + t) * 8, h[c], w[c], most);
+  }
+}
+
+// Rows of more values than 1024 threads hold octets: passed twice, the second time through the caches.
+constexpr int kLong = 1024;
+template <int DT, bool ROWS8>
+__global__ __launch_bounds__(kLong) void add_rms_norm_long_kernel(NormArgs a) {
+  __shared__ double part[kLong / kWave][2];
+  const int64_t at = (int64_t)blockIdx.x * a.H;
+  double ss = 0.0, most = 0.0;
+#pragma unroll 1
+  for (int j = threadIdx.x * 8; j < a.H; j += kLong * 8) {
+    Octet<DT> h = load_octet<DT>(a.x, at + j, a.H - j);
+    if (a.r) {
+      const Octet<DT> r = load_octet<DT>(a.r, at + j, a.H - j);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float v = h[c].at(i) * w[c].at(i) * inv;
-        float k = rintf(v);
-        // the float quotient is up to 2^-15 off (three roundings of a value below 128): where that could change the integer, or the products leave
-        // the floats' range, the exact products decide
-        if (none) k = 0.f;
-        else if (wide || fabsf(v - k) > 0.4999f) k = (float)rint(127.0 * ((double)h[c].at(i) * (double)w[c].at(i)) / most);
-        q[i / 4] |= ((uint32_t)(int)k & 0xffu) << (8 * (i % 4));
-      }
-      unsigned char *const to = static_cast<unsigned char *>(a.y) + at + (c * TPR + t) * 8;
-      if (n >= 8) __builtin_memcpy(to, q, 8);
-      else
-        for (int i = 0; i < n; ++i) to[i] = (unsigned char)(q[i / 4] >> (8 * (i % 4)));
+      for (int i = 0; i < 8; i += 2) h.put2(i, h.at(i) + r.at(i), h.at(i + 1) + r.at(i + 1));
+    }
+    if (a.sum) store_octet<DT>(a.sum, at + j, a.H - j, h);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss = __builtin_fma((double)h.at(i), (double)h.at(i), ss);
+    if constexpr (ROWS8) most = largest<DT>(most, h, load_octet<DT>(a.w, j, a.H - j));
+  }
+  ss = wave_sum_f64(ss);
+  if constexpr (ROWS8) most = wave_max_f64(most);
+  meet<kLong / kWave>(part, ss, most, false);
+  const float rstd = rstd_of(ss, a.H, a.eps);
+  if (ROWS8 && threadIdx.x == 0) a.scales[blockIdx.x] = scale_of(most, rstd);
+  const void *const from = a.r ? a.sum : a.x;  // (a thread's own octets)
+#pragma unroll 1
+  for (int j = threadIdx.x * 8; j < a.H; j += kLong * 8) {
+    Octet<DT> h = load_octet<DT>(from, at + j, a.H - j);
+    const Octet<DT> w = load_octet<DT>(a.w, j, a.H - j);
+    if constexpr (ROWS8) {
+      put_codes<DT>(static_cast<unsigned char *>(a.y) + at + j, a.H - j, h, w, most);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) h.put2(i, w.at(i) * (h.at(i) * rstd), w.at(i + 1) * (h.at(i + 1) * rstd));
+      store_octet<DT>(a.y, at + j, a.H - j, h);
     }
   }
+}
+
+template <int DT>
+static hipError_t start_norm_long(const NormArgs &a, bool rows8, hipStream_t st) {
+  if (rows8) add_rms_norm_long_kernel<DT, true><<<(unsigned)a.T, kLong, 0, st>>>(a);
+  else add_rms_norm_long_kernel<DT, false><<<(unsigned)a.T, kLong, 0, st>>>(a);
+  return hipGetLastError();
 }
 
 template <int DT, int TPR, int CH>
@@ -205,8 +263,7 @@ hipError_t launch_add_rms_norm(const void *x, const void *r, const void *w, floa
     if (H <= 2048) return start_norm<DT, 256, 1>(a, rows8, st);
     if (H <= 4096) return start_norm<DT, 256, 2>(a, rows8, st);
     if (H <= 8192) return start_norm<DT, 256, 4>(a, rows8, st);
-    if (H <= 16384) return start_norm<DT, 1024, 2>(a, rows8, st);
-    return start_norm<DT, 1024, 4>(a, rows8, st);
+    return start_norm_long<DT>(a, rows8, st);
   });
 }
 
@@ -226,7 +283,7 @@ template <int DT, int TPR, int CH>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR, 4) void norm_grad_kernel(NormGradArgs a) {
   constexpr int kRows = TPR < 256 ? 256 / TPR : 1, kWaves = TPR / kWave;
   __shared__ double part[2][kWaves][2];
-  const int t = threadIdx.x % TPR, wave = t / kWave, which = threadIdx.x / TPR;
+  const int t = threadIdx.x % TPR, which = threadIdx.x / TPR;
   const int64_t step = (int64_t)gridDim.x * kRows;
   Octet<DT> w[CH];
   float dw[CH][8];
@@ -258,13 +315,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR, 4) void norm_grad_kernel(Nor
       }
     ss = wave_sum_f64(ss);
     dot = wave_sum_f64(dot);
-    if constexpr (kWaves > 1) {
-      if ((t & (kWave - 1)) == 0) part[turn][wave][0] = ss, part[turn][wave][1] = dot;
-      __syncthreads();  // (one a row: the next row's sums go to the other half)
-      ss = dot = 0.0;
-#pragma unroll
-      for (int i = 0; i < kWaves; ++i) ss += part[turn][i][0], dot += part[turn][i][1];
-    }
+    if constexpr (kWaves > 1) meet<kWaves>(part[turn], ss, dot, true);  // (one barrier a row: the next row's sums go to the other half)
     const float rstd = rstd_of(ss, a.H, a.eps);
     const float mean = (float)(dot * (double)rstd / (double)a.H);
 #pragma unroll
@@ -311,6 +362,49 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR, 4) void norm_grad_kernel(Nor
   }
 }
 
+// Rows of more values than 1024 threads hold octets: passed twice, and the sums for dw kept where they go.
+template <int DT>
+__global__ __launch_bounds__(kLong) void norm_grad_long_kernel(NormGradArgs a) {
+  __shared__ double part[2][kLong / kWave][2];
+  float *const to = a.parts + (int64_t)blockIdx.x * a.H;
+  int turn = 0;
+#pragma unroll 1
+  for (int64_t row = blockIdx.x; row < a.T; row += gridDim.x, turn ^= 1) {
+    const int64_t at = row * a.H;
+    double ss = 0.0, dot = 0.0;
+#pragma unroll 1
+    for (int j = threadIdx.x * 8; j < a.H; j += kLong * 8) {
+      const Octet<DT> h = load_octet<DT>(a.h, at + j, a.H - j), dy = load_octet<DT>(a.dy, at + j, a.H - j), w = load_octet<DT>(a.w, j, a.H - j);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const double v = h.at(i);
+        ss = __builtin_fma(v, v, ss);
+        dot = __builtin_fma((double)w.at(i) * (double)dy.at(i), v, dot);
+      }
+    }
+    ss = wave_sum_f64(ss);
+    dot = wave_sum_f64(dot);
+    meet<kLong / kWave>(part[turn], ss, dot, true);
+    const float rstd = rstd_of(ss, a.H, a.eps);
+    const float mean = (float)(dot * (double)rstd / (double)a.H);
+#pragma unroll 1
+    for (int j = threadIdx.x * 8; j < a.H; j += kLong * 8) {
+      Octet<DT> h = load_octet<DT>(a.h, at + j, a.H - j), dh;
+      const Octet<DT> dy = load_octet<DT>(a.dy, at + j, a.H - j), w = load_octet<DT>(a.w, j, a.H - j);
+      if (a.dh) dh = load_octet<DT>(a.dh, at + j, a.H - j);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float hat = h.at(i) * rstd, g = dy.at(i);
+        if (j + i < a.H) to[j + i] = row == blockIdx.x ? g * hat : __builtin_fmaf(g, hat, to[j + i]);
+        float d = rstd * __builtin_fmaf(-hat, mean, w.at(i) * g);
+        if (a.dh) d += dh.at(i);
+        h.put(i, d);
+      }
+      store_octet<DT>(a.dx, at + j, a.H - j, h);
+    }
+  }
+}
+
 // dw = the blocks' sums: 16 columns a block, every 64th block's sums a thread
 template <int DT>
 __global__ __launch_bounds__(1024) void norm_grad_weight_kernel(const float *parts, int blocks, int H, void *dw) {
@@ -354,6 +448,12 @@ static hipError_t start_norm_grad(const NormGradArgs &a, int blocks, hipStream_t
   return hipGetLastError();
 }
 
+template <int DT>
+static hipError_t start_norm_grad_long(const NormGradArgs &a, int blocks, hipStream_t st) {
+  norm_grad_long_kernel<DT><<<(unsigned)blocks, kLong, 0, st>>>(a);
+  return hipGetLastError();
+}
+
 hipError_t launch_norm_grad(const void *dy, const void *h, const void *dh, const void *w, float eps, int64_t T, int H, int dt, void *dx, void *dw,
                             float *parts, hipStream_t st) {
   const NormGradArgs a{dy, h, dh, w, eps, T, H, dx, parts};
@@ -367,8 +467,7 @@ hipError_t launch_norm_grad(const void *dy, const void *h, const void *dh, const
           : H <= 2048  ? start_norm_grad<DT, 256, 1>(a, blocks, st)
           : H <= 4096  ? start_norm_grad<DT, 512, 1>(a, blocks, st)
           : H <= 8192  ? start_norm_grad<DT, 1024, 1>(a, blocks, st)
-          : H <= 16384 ? start_norm_grad<DT, 1024, 2>(a, blocks, st)
-                       : start_norm_grad<DT, 1024, 4>(a, blocks, st);
+                       : start_norm_grad_long<DT>(a, blocks, st);
     if (e != hipSuccess) return e;
     norm_grad_weight_kernel<DT><<<(unsigned)((H + 15) / 16), 1024, 0, st>>>(parts, blocks, H, dw);  // (no rows: zeros)
     return hipGetLastError();

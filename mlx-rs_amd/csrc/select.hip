@@ -59,63 +59,66 @@ struct SelectKernelArgs {
   int size, lanes_log2, slots;  // experts of a group; lanes of a group; a lane's experts
 };
 
-// A wave a token.  A group of experts goes to a run of lanes, consecutive experts to a lane, so that lanes and slots are in the order of the ids.
-template <int DT, class Key, int S>
-__global__ __launch_bounds__(256) void select_experts_kernel(SelectKernelArgs p) {
-  const SelectArgs &a = p.a;
-  const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (t >= a.T) return;
-  const int lane = lane_id(), g = lane >> p.lanes_log2, from = (lane & ((1 << p.lanes_log2) - 1)) * p.slots;
-  const Logit<DT> *const row = static_cast<const Logit<DT> *>(a.logits) + t * a.E;
+// A token's experts in a wave.  A group of experts goes to a run of lanes, consecutive experts to a lane, so that lanes and slots are in the order of the ids.
+template <int S>
+struct Slots {
   float l[S];
-  double v[S];  // scores, then scores with the bias
-  Key key[S];
   bool on[S];
-#pragma unroll
-  for (int j = 0; j < S; ++j) {
-    on[j] = j < p.slots && from + j < p.size && g < a.groups;
-    l[j] = on[j] ? as_f32(row[g * p.size + from + j]) : -INFINITY;
-  }
-  float most = -INFINITY;  // (fmaxf passes over what is no number)
-  double total = 0.0;
+  int base;  // id of slot 0
+};
+
+// merges the two largest of two disjoint sets
+template <class T>
+__device__ __forceinline__ void merge_two(T &t1, T &t2, T o1, T o2) {
+  t2 = fmax(fmin(t1, o1), fmax(t2, o2));
+  t1 = fmax(t1, o1);
+}
+__device__ __forceinline__ float f32_of(uint32_t u) { return __uint_as_float(u); }
+
+// Everything in double, u64 keys: any logits and biases.  Lane r gets the r-th expert's id and score.
+template <int S>
+__device__ __forceinline__ void select_exact(const SelectKernelArgs &p, const Slots<S> &x, int g, uint32_t &id, double &score) {
+  const SelectArgs &a = p.a;
+  const int lane = lane_id();
+  double v[S], s[S];
   if (a.scoring == 0) {
+    float most = -INFINITY;  // (fmaxf passes over what is no number)
 #pragma unroll
-    for (int j = 0; j < S; ++j) most = fmaxf(most, l[j]);
+    for (int j = 0; j < S; ++j) most = fmaxf(most, x.l[j]);
     most = wave_max_f32(most);
+    double total = 0.0;
 #pragma unroll
     for (int j = 0; j < S; ++j) {
-      v[j] = most == -INFINITY ? 0.0 : exp((double)l[j] - (double)most);
-      total += v[j] == v[j] || l[j] == l[j] ? v[j] : 0.0;
+      v[j] = most == -INFINITY ? 0.0 : exp((double)x.l[j] - (double)most);
+      total += v[j] == v[j] || x.l[j] == x.l[j] ? v[j] : 0.0;
     }
     total = wave_sum_f64(total);
 #pragma unroll
-    for (int j = 0; j < S; ++j) v[j] = l[j] != l[j] ? NAN : total > 0.0 || total != total ? v[j] / total : 0.0;
+    for (int j = 0; j < S; ++j) v[j] = x.l[j] != x.l[j] ? NAN : total > 0.0 || total != total ? v[j] / total : 0.0;
   } else {
 #pragma unroll
-    for (int j = 0; j < S; ++j) v[j] = sigmoid64(l[j]);
+    for (int j = 0; j < S; ++j) v[j] = sigmoid64(x.l[j]);
   }
-  double s[S];
+  uint64_t key[S];
 #pragma unroll
   for (int j = 0; j < S; ++j) {
     s[j] = v[j];
-    if (a.bias && on[j]) v[j] += (double)a.bias[g * p.size + from + j];
-    if (l[j] == -INFINITY) v[j] = -INFINITY;
-    if constexpr (sizeof(Key) == 8) key[j] = on[j] ? key_of(v[j]) : 0;
-    else key[j] = on[j] ? key_of(l[j]) : 0;
+    if (a.bias && x.on[j]) v[j] += (double)a.bias[x.base + j];
+    if (x.l[j] == -INFINITY) v[j] = -INFINITY;
+    key[j] = !x.on[j] ? 0 : a.bias ? key_of(v[j]) : key_of((double)x.l[j]);
   }
   if (a.groups > 1) {
     double t1 = -INFINITY, t2 = -INFINITY;  // the two largest of the group
 #pragma unroll
     for (int j = 0; j < S; ++j) {
-      double x = a.group_score == 0 && sizeof(Key) == 4 ? (double)l[j] : v[j];
-      if (!on[j] || x != x) x = -INFINITY;
-      t2 = fmax(t2, fmin(t1, x));
-      t1 = fmax(t1, x);
+      double y = a.group_score == 0 && !a.bias ? (double)x.l[j] : v[j];
+      if (!x.on[j] || y != y) y = -INFINITY;
+      t2 = fmax(t2, fmin(t1, y));
+      t1 = fmax(t1, y);
     }
     for (int d = 0; d < p.lanes_log2; ++d) {
       const double o1 = __shfl_xor(t1, 1 << d), o2 = __shfl_xor(t2, 1 << d);
-      t2 = fmax(fmin(t1, o1), fmax(t2, o2));
-      t1 = fmax(t1, o1);
+      merge_two(t1, t2, o1, o2);
     }
     const uint64_t mine = key_of(a.group_score == 0 || p.size == 1 ? t1 : t1 + t2);
     int before = 0;
@@ -127,55 +130,485 @@ __global__ __launch_bounds__(256) void select_experts_kernel(SelectKernelArgs p)
 #pragma unroll
       for (int j = 0; j < S; ++j) key[j] = 0;
   }
-  uint32_t id = 0;
-  double score = 0.0;
   for (int r = 0; r < a.k; ++r) {
-    Key best = 0;
+    uint64_t best = 0;
     int at = 0;
     double sv = 0.0;
 #pragma unroll
     for (int j = 0; j < S; ++j)
       if (key[j] > best) best = key[j], at = j, sv = s[j];
-    const Key top = wave_max_key(best);
+    const uint64_t top = wave_max_key(best);
     const int owner = __builtin_ctzll(__ballot(best == top));
     if (lane == owner)
 #pragma unroll
       for (int j = 0; j < S; ++j)
         if (j == at) key[j] = 0;
-    const uint32_t chosen = (uint32_t)__builtin_amdgcn_readlane(g * p.size + from + at, owner);
+    const uint32_t chosen = (uint32_t)__builtin_amdgcn_readlane(x.base + at, owner);
     const double its = readlane_f64(sv, owner);
     if (lane == r) id = chosen, score = its;
   }
+}
+
+// The keys and the groups' ranks in float where that decides them: float scores are within kNear / 4 of the exact ones (exp and reciprocal to 2^-22 of their values, an
+// exponent off by 2^-24 of itself, of scores of one at most, a sum to 2^-22), biased keys within 2^-24 of their size more.  Where two keys that follow each other in the choice, or two groups' ranks, are nearer than
+// that allows, or something is not finite, the token goes through select_exact (one in some hundred); without a bias the logits are exact keys.  Scores of the chosen are in double, a lane each.
+constexpr float kNear = 0x1p-19f, kNearOfSize = 0x1p-21f;
+
+// SUM: softmax scores that are not renormalised, whose denominator is over all experts.  KEYS: float scores decide something (a bias, or groups ranked by two scores).
+template <int DT, int S, bool KEYS, bool SUM>
+__global__ __launch_bounds__(256) void select_experts_kernel(SelectKernelArgs p) {
+  const SelectArgs &a = p.a;
+  const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (t >= a.T) return;
+  const int lane = lane_id(), g = lane >> p.lanes_log2, from = (lane & ((1 << p.lanes_log2) - 1)) * p.slots;
+  const Logit<DT> *const row = static_cast<const Logit<DT> *>(a.logits) + t * a.E;
+  Slots<S> x;
+  x.base = g * p.size + from;
+#pragma unroll
+  for (int j = 0; j < S; ++j) {
+    x.on[j] = j < p.slots && from + j < p.size && g < a.groups;
+    x.l[j] = x.on[j] ? as_f32(row[x.base + j]) : -INFINITY;
+  }
+  float b[S];
+  bool odd = false;  // something that floats do not decide
+  if constexpr (KEYS) {
+#pragma unroll
+    for (int j = 0; j < S; ++j) {
+      b[j] = a.bias && x.on[j] ? a.bias[x.base + j] : 0.f;
+      odd |= x.on[j] && not_finite(x.l[j] - x.l[j] + b[j]);
+    }
+  }
+  float most = -INFINITY;
+  if (SUM || (KEYS && a.scoring == 0)) {
+#pragma unroll
+    for (int j = 0; j < S; ++j) most = fmaxf(most, x.l[j]);
+    most = wave_max_f32(most);
+  }
+  double total = 1.0;
+  if constexpr (SUM) {
+    total = 0.0;
+#pragma unroll
+    for (int j = 0; j < S; ++j)
+      if (x.l[j] == x.l[j] && most > -INFINITY) total += exp((double)x.l[j] - (double)most);
+    total = wave_sum_f64(total);
+  }
+  uint32_t key[S];
+#pragma unroll
+  for (int j = 0; j < S; ++j) key[j] = x.on[j] ? key_of(x.l[j]) : 0;
+  if constexpr (KEYS) {
+    float s[S];
+    if (a.scoring == 0) {
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < S; ++j) {
+        s[j] = __expf(x.l[j] - most);
+        sum += s[j];
+      }
+      const float inv = __builtin_amdgcn_rcpf((float)wave_sum_f64((double)sum));
+#pragma unroll
+      for (int j = 0; j < S; ++j) s[j] *= inv;
+    } else {
+#pragma unroll
+      for (int j = 0; j < S; ++j) s[j] = __builtin_amdgcn_rcpf(1.0f + __expf(-x.l[j]));
+    }
+#pragma unroll
+    for (int j = 0; j < S; ++j) {
+      s[j] += b[j];
+      if (a.bias && x.on[j]) key[j] = key_of(s[j]);
+    }
+    if (a.groups > 1) {
+      float t1 = -INFINITY, t2 = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < S; ++j) {
+        const float y = !x.on[j] ? -INFINITY : a.group_score == 0 && !a.bias ? x.l[j] : s[j];
+        t2 = fmaxf(t2, fminf(t1, y));
+        t1 = fmaxf(t1, y);
+      }
+      const int n = p.lanes_log2;
+      auto other = [&](auto ctrl) __attribute__((always_inline)) {
+        constexpr int CTRL = decltype(ctrl)::value;
+        merge_two(t1, t2, f32_of(dpp_u32<CTRL>(__float_as_uint(t1))), f32_of(dpp_u32<CTRL>(__float_as_uint(t2))));
+      };
+      if (n > 0) other(std::integral_constant<int, kDppXor1>{});
+      if (n > 1) other(std::integral_constant<int, kDppXor2>{});
+      if (n > 2) other(std::integral_constant<int, kDppHalfMirror>{});
+      if (n > 3) other(std::integral_constant<int, kDppMirror>{});
+      if (n > 4) merge_two(t1, t2, __shfl_xor(t1, 16), __shfl_xor(t2, 16));
+      if (n > 5) merge_two(t1, t2, __shfl_xor(t1, 32), __shfl_xor(t2, 32));
+      const float mine = a.group_score == 0 || p.size == 1 ? t1 : t1 + t2;
+      const float clear = 2 * kNear + kNearOfSize * wave_max_f32(g >= a.groups ? 0.f : p.size == 1 ? fabsf(t1) : fabsf(t1) + fabsf(t2));
+      int before = 0, maybe = 0;  // groups that are better, and that could be
+      for (int o = 0; o < a.groups; ++o) {
+        const float its = f32_of((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(mine), o << n));
+        before += o != g && its - mine > clear;
+        maybe += o != g && !(mine - its > clear);
+      }
+      odd |= g < a.groups && before < a.top_groups && maybe >= a.top_groups;
+      if (before >= a.top_groups)
+#pragma unroll
+        for (int j = 0; j < S; ++j) key[j] = 0;
+    }
+  } else if (a.groups > 1) {  // by their largest logits, which are exact
+    uint32_t best = 0;
+#pragma unroll
+    for (int j = 0; j < S; ++j) best = key[j] > best ? key[j] : best;
+    for (int d = 0; d < p.lanes_log2; ++d) {
+      const uint32_t o = __shfl_xor(best, 1 << d);
+      best = o > best ? o : best;
+    }
+    if (best == 1u) best = key_of(-INFINITY);  // (no numbers rank as -inf)
+    int before = 0;
+    for (int o = 0; o < a.groups; ++o) {
+      const uint32_t its = (uint32_t)__builtin_amdgcn_readlane((int)best, o << p.lanes_log2);
+      before += its > best || (its == best && o < g);
+    }
+    if (before >= a.top_groups)
+#pragma unroll
+      for (int j = 0; j < S; ++j) key[j] = 0;
+  }
+  uint32_t id = 0;
+  float logit = 0.f;
+  double score = 0.0;
+  bool exact = false;
+  if (!KEYS || !__any(odd)) {
+    float last = 0.f;
+    bool near = false;
+    const int rounds = KEYS && a.bias ? a.k + 1 : a.k;  // (the first that is not chosen has to be clear of the last that is)
+    for (int r = 0; r < rounds; ++r) {
+      uint32_t best = key[0];
+#pragma unroll
+      for (int j = 1; j < S; ++j) best = key[j] > best ? key[j] : best;
+      const uint32_t top = wave_max_u32(best);
+      if (KEYS && a.bias) {
+        if (top == 0) break;  // (no more than were chosen)
+        const float now = f32_of((top >> 31) ? top & 0x7fffffffu : ~top);
+        near |= r > 0 && !(last - now > kNear + kNearOfSize * fabsf(last));
+        last = now;
+      }
+      const int owner = __builtin_ctzll(__ballot(best == top));
+      int at = 0;
+      float l = x.l[0];
+#pragma unroll
+      for (int j = S - 1; j >= 0; --j)
+        if (key[j] == top) at = j, l = x.l[j];
+      const uint32_t chosen = (uint32_t)__builtin_amdgcn_readlane(x.base + at, owner);
+      const float its = f32_of((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(l), owner));
+#pragma unroll
+      for (int j = 0; j < S; ++j)
+        if (lane == owner && j == at) key[j] = 0;
+      if (lane == r) id = chosen, logit = its;
+    }
+    exact = near;
+  } else {
+    exact = true;
+  }
+  const bool mine = lane < a.k;
+  if (KEYS && exact) {
+    select_exact<S>(p, x, g, id, score);
+  } else if (a.scoring == 1) {
+    score = mine ? sigmoid64(logit) : 0.0;
+  } else {
+    if constexpr (!SUM) most = wave_max_f32(mine ? logit : -INFINITY);  // (renormalised: any common factor)
+    score = !mine ? 0.0 : logit != logit ? NAN : most == -INFINITY ? 0.0 : exp((double)logit - (double)most) / total;
+  }
   double w = score;
   if (a.renormalize) {
-    const double sum = wave_sum_f64(lane < a.k ? score : 0.0);
+    const double sum = wave_sum_f64(mine ? score : 0.0);
     w = sum == 0.0 ? 0.0 : score / sum;
   }
+  if (mine) {
+    a.idx[t * a.k + lane] = id;
+    put_value(a.w, t * a.k + lane, a.w_dtype, w * (double)a.scale);
+  }
+}
+
+// ---------------------------------------------------------------- up to 16 groups and 16 choices: a row of 16 lanes a token
+// The same choice with four tokens in a wave and up to 32 experts a lane: what a round of the choice exchanges between lanes stays in a row, and a wave's instructions, which are
+// what bounds the selection, serve four tokens.  What floats do not decide is gone over by the whole wave, a token after the other.  It takes over where there is a wave for each SIMD.  us, a row / a wave a token, bf16 logits
+// but for the groups, 2048, 4096, 8192 tokens:
+//   128 experts, 8 chosen               4.6 / 4.5    4.7 / 5.5    5.3 / 7.7
+//   512, 10                             8.7 / 6.8    8.8 / 10.0   10.8 / 16.4
+//   256, 8, sigmoid, bias               9.2 / 9.3    9.4 / 10.3   10.1 / 15.2
+//   256, 8, sigmoid, bias, 8 groups    13.4 / 11.1  13.5 / 13.4   12.2 / 17.9
+//   512, 16, sigmoid, bias             24.1 / 19.5  25.2 / 25.1   29.2 / 36.6
+// At one token they are 4.6 and 4.0 in the first line, 8.5 and 6.0 in the fourth.  8192 tokens of 256 float32 logits are 8.4 MB, 1.7 us of a copy's traffic: what bounds the choice are its
+// instructions, some 20 for each chosen and two for each expert and chosen, and the double exponentials of the weights; where doubles decide, in half of the fourth line's waves, theirs too.
+constexpr int64_t kSelectWaves = 1024;
+__device__ __forceinline__ uint32_t row_max(uint32_t v) {
+  uint32_t o;
+  o = dpp_u32<kDppXor1>(v); v = o > v ? o : v;
+  o = dpp_u32<kDppXor2>(v); v = o > v ? o : v;
+  o = dpp_u32<kDppHalfMirror>(v); v = o > v ? o : v;
+  o = dpp_u32<kDppMirror>(v); v = o > v ? o : v;
+  return v;
+}
+__device__ __forceinline__ uint32_t row_min(uint32_t v) { return ~row_max(~v); }
+template <class F>
+__device__ __forceinline__ float row_join(float v, F f) {
+  v = f(v, f32_of(dpp_u32<kDppXor1>(__float_as_uint(v))));
+  v = f(v, f32_of(dpp_u32<kDppXor2>(__float_as_uint(v))));
+  v = f(v, f32_of(dpp_u32<kDppHalfMirror>(__float_as_uint(v))));
+  return f(v, f32_of(dpp_u32<kDppMirror>(__float_as_uint(v))));
+}
+__device__ __forceinline__ double row_sum(double v) {
+  v += dpp_f64<kDppXor1>(v);
+  v += dpp_f64<kDppXor2>(v);
+  v += dpp_f64<kDppHalfMirror>(v);
+  return v + dpp_f64<kDppMirror>(v);
+}
+// f(n, v of the lane n places before in the row) for n = 1 .. 15
+template <int N = 1, class F>
+__device__ __forceinline__ void each_other(float v, F f) {
+  if constexpr (N < 16) {
+    f(N, f32_of(dpp_u32<0x120 + N>(__float_as_uint(v))));
+    each_other<N + 1>(v, f);
+  }
+}
+template <int N = 1, class F>
+__device__ __forceinline__ void each_candidate(double v, uint32_t id, F f) {
+  if constexpr (N < 16) {
+    f(dpp_f64<0x120 + N>(v), dpp_u32<0x120 + N>(id));
+    each_candidate<N + 1>(v, id, f);
+  }
+}
+
+// weights of a token's choice from its scores, in the lanes below k; `sum`: of all lanes' scores
+__device__ __forceinline__ void put_choice(const SelectArgs &a, int64_t t, int lane, uint32_t id, double score, double sum) {
+  const double w = !a.renormalize ? score : sum == 0.0 ? 0.0 : score / sum;
   if (lane < a.k) {
     a.idx[t * a.k + lane] = id;
     put_value(a.w, t * a.k + lane, a.w_dtype, w * (double)a.scale);
   }
 }
 
-template <int DT, class Key>
+template <int DT, int S, bool KEYS, bool SUM>
+__global__ __launch_bounds__(256) void select_rows_kernel(SelectKernelArgs p, SelectKernelArgs whole) {  // whole: the layout of a wave a token
+  const SelectArgs &a = p.a;
+  const int64_t t0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 4, t = t0 + (lane_id() >> 4);
+  if (t0 >= a.T) return;
+  const int lane = lane_id() & 15, g = lane >> p.lanes_log2, from = (lane & ((1 << p.lanes_log2) - 1)) * p.slots, base = g * p.size + from;
+  const Logit<DT> *const row = static_cast<const Logit<DT> *>(a.logits) + (t < a.T ? t : a.T - 1) * a.E;  // (tokens outside: the last one's, not stored)
+  const int n_mine = g < a.groups ? (p.size - from < p.slots ? p.size - from : p.slots) : 0;  // this lane's experts
+  float l[S];
+  if (p.slots == S && n_mine == S) {
+    Logit<DT> v[S];
+    __builtin_memcpy(v, row + base, sizeof v);
+#pragma unroll
+    for (int j = 0; j < S; ++j) l[j] = as_f32(v[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < S; ++j) l[j] = j < n_mine ? as_f32(row[base + j]) : -INFINITY;
+  }
+  float b[S];
+  bool odd = false;
+  if constexpr (KEYS) {
+    if (a.bias && p.slots == S && n_mine == S) {
+      __builtin_memcpy(b, a.bias + base, sizeof b);
+    } else {
+#pragma unroll
+      for (int j = 0; j < S; ++j) b[j] = a.bias && j < n_mine ? a.bias[base + j] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < S; ++j) odd |= j < n_mine && not_finite(l[j] - l[j] + b[j]);
+  }
+  auto larger = [](float x, float y) { return fmaxf(x, y); };
+  float most = -INFINITY;
+  if (SUM || (KEYS && a.scoring == 0)) {
+#pragma unroll
+    for (int j = 0; j < S; ++j) most = fmaxf(most, l[j]);
+    most = row_join(most, larger);
+  }
+  double total = 1.0;
+  if constexpr (SUM) {
+    total = 0.0;
+#pragma unroll
+    for (int j = 0; j < S; ++j)
+      if (l[j] == l[j] && most > -INFINITY) total += exp((double)l[j] - (double)most);
+    total = row_sum(total);
+  }
+  uint32_t key[S];
+  if (!KEYS || !a.bias) {
+#pragma unroll
+    for (int j = 0; j < S; ++j) key[j] = j < n_mine ? key_of(l[j]) : 0;
+  }
+  float y[S];  // what groups are ranked by
+#pragma unroll
+  for (int j = 0; j < S; ++j) y[j] = l[j] == l[j] ? l[j] : -INFINITY;  // (no numbers rank as -inf)
+  if constexpr (KEYS) {
+    if (a.bias || a.group_score == 1) {
+      if (a.scoring == 0) {
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < S; ++j) {
+          y[j] = __expf(l[j] - most);
+          sum += y[j];
+        }
+        const float inv = __builtin_amdgcn_rcpf(row_join(sum, [](float u, float v) { return u + v; }));
+#pragma unroll
+        for (int j = 0; j < S; ++j) y[j] = __builtin_fmaf(y[j], inv, b[j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < S; ++j) y[j] = __builtin_amdgcn_rcpf(1.0f + __expf(-l[j])) + b[j];
+      }
+      if (a.bias) {
+#pragma unroll
+        for (int j = 0; j < S; ++j) key[j] = j < n_mine ? key_of(y[j]) : 0;
+      }
+    }
+  }
+  if (a.groups > 1) {
+    float t1 = -INFINITY, t2 = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < S; ++j) {
+      const float v = j < n_mine ? y[j] : -INFINITY;
+      t2 = fmaxf(t2, fminf(t1, v));
+      t1 = fmaxf(t1, v);
+    }
+    const int n = p.lanes_log2;
+    auto other = [&](auto ctrl) __attribute__((always_inline)) {
+      constexpr int CTRL = decltype(ctrl)::value;
+      merge_two(t1, t2, f32_of(dpp_u32<CTRL>(__float_as_uint(t1))), f32_of(dpp_u32<CTRL>(__float_as_uint(t2))));
+    };
+    if (n > 0) other(std::integral_constant<int, kDppXor1>{});
+    if (n > 1) other(std::integral_constant<int, kDppXor2>{});
+    if (n > 2) other(std::integral_constant<int, kDppHalfMirror>{});
+    const float mine = a.group_score == 0 || p.size == 1 ? t1 : t1 + t2;
+    float clear = 0.f;
+    if constexpr (KEYS) clear = 2 * kNear + kNearOfSize * row_join(g >= a.groups ? 0.f : p.size == 1 ? fabsf(t1) : fabsf(t1) + fabsf(t2), larger);
+    int before = 0, maybe = 0;  // lanes of groups that are better, and that could be
+    each_other(mine, [&](int n_back, float its) __attribute__((always_inline)) {
+      const int og = ((lane - n_back) & 15) >> n;
+      const bool another = og != g && og < a.groups;
+      if constexpr (KEYS) {
+        before += another && its - mine > clear;
+        maybe += another && !(mine - its > clear);
+      } else {
+        before += another && (its > mine || (its == mine && og < g));
+      }
+    });
+    if constexpr (KEYS) odd |= g < a.groups && before >> n < a.top_groups && maybe >> n >= a.top_groups;
+    if (before >> n >= a.top_groups)
+#pragma unroll
+      for (int j = 0; j < S; ++j) key[j] = 0;
+  }
+  // With a bias the choice goes on to one more candidate, in a lane as the others, and to the key after that one: where that is clearly below the last of the k, floats have
+  // found the candidates and doubles their order.
+  const int candidates = KEYS && a.bias ? (a.k < 16 ? a.k + 1 : 16) : a.k;
+  uint32_t id = (uint32_t)(a.E + lane);  // (no expert)
+  float last = 0.f, kth = 0.f;
+  bool close = false;
+#pragma unroll 1
+  for (int r = 0; r < candidates + (KEYS && a.bias); ++r) {
+    uint32_t best = key[0];
+#pragma unroll
+    for (int j = 1; j < S; ++j) best = key[j] > best ? key[j] : best;
+    const uint32_t top = row_max(best);
+    if (KEYS && a.bias) {
+      const float now = f32_of((top >> 31) ? top & 0x7fffffffu : ~top);
+      if (r == a.k - 1) kth = now;
+      const float clear = kNear + kNearOfSize * fabsf(r == candidates ? kth : last);
+      if (r == candidates) odd |= top != 0 && !(kth - now > clear);
+      else close |= r > 0 && top != 0 && !(last - now > clear);
+      last = now;
+    }
+    uint32_t at = ~0u;
+#pragma unroll
+    for (int j = S - 1; j >= 0; --j)
+      if (key[j] == top) at = (uint32_t)(base + j);
+    const uint32_t chosen = row_min(at);
+#pragma unroll
+    for (int j = 0; j < S; ++j)
+      if (chosen == (uint32_t)(base + j)) key[j] = 0;
+    if (lane == r && top != 0) id = chosen;
+  }
+  const bool named = id < (uint32_t)a.E;
+  const float logit = named ? as_f32(row[id]) : -INFINITY;
+  double score;
+  if (a.scoring == 1) {
+    score = named ? sigmoid64(logit) : 0.0;
+  } else {
+    if constexpr (!SUM) most = row_join(lane < a.k ? logit : -INFINITY, larger);  // (renormalised: any common factor)
+    score = !named ? 0.0 : logit != logit ? NAN : most == -INFINITY ? 0.0 : exp((double)logit - (double)most) / total;
+  }
+  if constexpr (KEYS) {
+    if (__ballot(close)) {
+      if (a.scoring == 0 && !SUM) {
+        odd |= close;
+      } else {
+        const double v = named && a.bias ? score + (double)a.bias[id] : -INFINITY;
+        int rank = 0;
+        each_candidate(v, id, [&](double its, uint32_t other) __attribute__((always_inline)) { rank += its > v || (its == v && other < id); });
+        if (close) {
+          const int to = ((lane_id() & 48) + rank) * 4;
+          id = (uint32_t)__builtin_amdgcn_ds_permute(to, (int)id);
+          const uint64_t u = (uint64_t)__double_as_longlong(score);
+          score = __longlong_as_double((int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_ds_permute(to, (int)(u >> 32)) << 32 | (uint32_t)__builtin_amdgcn_ds_permute(to, (int)u)));
+        }
+      }
+    }
+  }
+  const double sum = row_sum(lane < a.k ? score : 0.0);
+  uint64_t again = KEYS ? __ballot(odd) : 0;
+  if (t < a.T && (again >> (lane_id() & 48) & 0xffff) == 0) put_choice(a, t, lane, id, score, sum);
+  if constexpr (KEYS) {
+    for (; again; again &= ~((uint64_t)0xffff << (__builtin_ctzll(again) & 48))) {
+      const int64_t tt = t0 + (__builtin_ctzll(again) >> 4);
+      if (tt >= a.T) continue;
+      const Logit<DT> *const its = static_cast<const Logit<DT> *>(a.logits) + tt * a.E;
+      const int wl = lane_id(), wg = wl >> whole.lanes_log2, wf = (wl & ((1 << whole.lanes_log2) - 1)) * whole.slots;
+      Slots<S / 4> x;  // (a wave has four times the lanes)
+      x.base = wg * whole.size + wf;
+#pragma unroll
+      for (int j = 0; j < S / 4; ++j) {
+        x.on[j] = j < whole.slots && wf + j < whole.size && wg < a.groups;
+        x.l[j] = x.on[j] ? as_f32(its[x.base + j]) : -INFINITY;
+      }
+      uint32_t eid = 0;
+      double es = 0.0;
+      select_exact<S / 4>(whole, x, wg, eid, es);
+      put_choice(a, tt, wl, eid, es, wave_sum_f64(wl < a.k ? es : 0.0));
+    }
+  }
+}
+
+template <int DT, bool KEYS, bool SUM>
+static hipError_t start_rows(const SelectKernelArgs &p, const SelectKernelArgs &whole, hipStream_t st) {
+  const unsigned grid = (unsigned)((p.a.T + 15) / 16);
+  if (p.slots <= 4) select_rows_kernel<DT, 4, KEYS, SUM><<<grid, 256, 0, st>>>(p, whole);
+  else if (p.slots <= 8) select_rows_kernel<DT, 8, KEYS, SUM><<<grid, 256, 0, st>>>(p, whole);
+  else if (p.slots <= 16) select_rows_kernel<DT, 16, KEYS, SUM><<<grid, 256, 0, st>>>(p, whole);
+  else select_rows_kernel<DT, 32, KEYS, SUM><<<grid, 256, 0, st>>>(p, whole);
+  return hipGetLastError();
+}
+
+template <int DT, bool KEYS, bool SUM>
 static hipError_t start_select(const SelectKernelArgs &p, hipStream_t st) {
   const unsigned grid = (unsigned)((p.a.T + 3) / 4);
-  if (p.slots <= 1) select_experts_kernel<DT, Key, 1><<<grid, 256, 0, st>>>(p);
-  else if (p.slots <= 2) select_experts_kernel<DT, Key, 2><<<grid, 256, 0, st>>>(p);
-  else if (p.slots <= 4) select_experts_kernel<DT, Key, 4><<<grid, 256, 0, st>>>(p);
-  else if (p.slots <= 8) select_experts_kernel<DT, Key, 8><<<grid, 256, 0, st>>>(p);
-  else select_experts_kernel<DT, Key, 16><<<grid, 256, 0, st>>>(p);
+  if (p.slots <= 1) select_experts_kernel<DT, 1, KEYS, SUM><<<grid, 256, 0, st>>>(p);
+  else if (p.slots <= 2) select_experts_kernel<DT, 2, KEYS, SUM><<<grid, 256, 0, st>>>(p);
+  else if (p.slots <= 4) select_experts_kernel<DT, 4, KEYS, SUM><<<grid, 256, 0, st>>>(p);
+  else if (p.slots <= 8) select_experts_kernel<DT, 8, KEYS, SUM><<<grid, 256, 0, st>>>(p);
+  else select_experts_kernel<DT, 16, KEYS, SUM><<<grid, 256, 0, st>>>(p);
   return hipGetLastError();
 }
 
 hipError_t launch_select_experts(const SelectArgs &a, int dt, hipStream_t st) {
   if (a.T == 0) return hipSuccess;
-  SelectKernelArgs p{a, a.E / a.groups, 6, 0};
-  while ((kWave >> p.lanes_log2) < a.groups) --p.lanes_log2;
-  p.slots = (p.size + (1 << p.lanes_log2) - 1) >> p.lanes_log2;  // 16 at most: 512 experts, and runs of lanes that leave less than half of the wave idle
+  auto layout = [&](int lanes_log2) {
+    SelectKernelArgs p{a, a.E / a.groups, lanes_log2, 0};
+    while (p.lanes_log2 > 0 && (1 << (lanes_log2 - p.lanes_log2)) < a.groups) --p.lanes_log2;  // lanes of a group
+    p.slots = (p.size + (1 << p.lanes_log2) - 1) >> p.lanes_log2;
+    return p;
+  };
+  const SelectKernelArgs p = layout(6), four = layout(4);  // p.slots: 16 at most (512 experts, and runs of lanes that leave less than half of the wave idle)
+  const bool rows = a.groups <= 16 && four.slots <= 32 && a.k <= 16 && a.T >= 4 * kSelectWaves;
+  const bool keys = a.bias || (a.groups > 1 && a.group_score == 1), sum = a.scoring == 0 && !a.renormalize;
   auto start = [&](auto d) {
     constexpr int DT = decltype(d)::value;
-    return a.bias ? start_select<DT, uint64_t>(p, st) : start_select<DT, uint32_t>(p, st);
+    if (rows && keys) return sum ? start_rows<DT, true, true>(four, p, st) : start_rows<DT, true, false>(four, p, st);
+    if (rows) return sum ? start_rows<DT, false, true>(four, p, st) : start_rows<DT, false, false>(four, p, st);
+    if (keys) return sum ? start_select<DT, true, true>(p, st) : start_select<DT, true, false>(p, st);
+    return sum ? start_select<DT, false, true>(p, st) : start_select<DT, false, false>(p, st);
   };
   if (dt == 0) return start(std::integral_constant<int, 0>{});
   if (dt == 1) return start(std::integral_constant<int, 1>{});
@@ -219,19 +652,28 @@ __global__ __launch_bounds__(256) void select_grad_kernel(SelectGradArgs a) {
   }
   const double dot = whole ? wave_sum_f64(inner) : 0.0;
   if (a.scoring == 1) inner *= sigmoid64(-l);
-  for (int c0 = 0; c0 < a.E; c0 += kWave) {
-    const int c = c0 + lane;
-    double v = 0.0;
-    if (whole && c < a.E) {
+  // the row: zeros, and a chosen expert's term (of one named twice the sum, in slot order, by the first) where it belongs
+  __shared__ double rows[4][512];
+  double *const out = rows[threadIdx.x >> 6];
+  for (int c = lane; c < a.E; c += kWave) out[c] = 0.0;
+  double mine = inner;
+  bool first = on;
+  for (int r = 0; r < a.k; ++r) {
+    const uint32_t at = (uint32_t)__builtin_amdgcn_readlane((int)id, r);
+    const double its = readlane_f64(inner, r);
+    if (at == id && r < lane) first = false;
+    if (at == id && r > lane) mine += its;
+  }
+  __builtin_amdgcn_wave_barrier();
+  if (first) out[id] = mine;
+  __builtin_amdgcn_wave_barrier();
+  for (int c = lane; c < a.E; c += kWave) {
+    double v = out[c];
+    if (whole) {
       const float x = as_f32(row[c]);
-      v = x != x ? NAN : most == -INFINITY ? 0.0 : -dot * (exp((double)x - (double)most) / total);
+      v += x != x ? NAN : most == -INFINITY ? 0.0 : -dot * (exp((double)x - (double)most) / total);
     }
-    for (int r = 0; r < a.k; ++r) {
-      const uint32_t at = (uint32_t)__builtin_amdgcn_readlane((int)id, r);
-      const double its = readlane_f64(inner, r);
-      if (at == (uint32_t)c) v += its;
-    }
-    if (c < a.E) put_value(a.dlogits, t * a.E + c, DT, v);
+    put_value(a.dlogits, t * a.E + c, DT, v);
   }
 }
 

@@ -57,6 +57,8 @@ def check(logits, k, scoring="softmax", bias=None, groups=1, top_groups=1, group
     for t, row in enumerate(rows):
         ids, s = choose(row, k, scoring, b, groups, top_groups, group_score)
         assert inds.reshape(-1, k)[t].tolist() == ids, (t, ids)
+        if renormalize and scoring == "softmax":  # (shares of the chosen, which are there also where a softmax over all rounds to zero, as of logits 1e38 below the largest)
+            s = dict(zip(ids, scores_of([row[i] for i in ids], scoring)))
         total = math.fsum(s[i] for i in ids) if renormalize else 1.0
         for j, i in enumerate(ids):
             ref = (0.0 if total == 0 else s[i] / total) * scale
@@ -139,6 +141,73 @@ def test_keys_that_differ_by_less_than_a_float():
     assert inds[0, 0] == 40 and 9 not in inds[0].tolist()[:31]
     # as close as one expert in a thousand draws comes: the rest of the order goes by ids
     assert inds[0, 1:].tolist() == [i for i in range(34) if i not in (9, 40)][:31]
+
+
+def check_many(rows, k, scoring="softmax", bias=None, groups=1, top_groups=1, group_score="max", renormalize=True, scale=1.0):
+    """4099 tokens that repeat `rows`: each repetition in other lanes and beside other tokens, and all with the same result, which the first ones are checked for."""
+    import mlx_rs_amd as m
+    at = torch.arange(4099, device="cuda") % rows.shape[0]
+    args = (k, scoring, bias, groups, top_groups, group_score, renormalize, scale, torch.float32)
+    inds, w = m.ops.select_experts(rows[at], *args)
+    small_inds, small_w = check(rows, *args)
+    assert bool((inds == small_inds[at]).all())
+    assert torch.equal(w.view(torch.int32), w[:rows.shape[0]][at].view(torch.int32))
+    # both are within one rounding of the same number
+    assert torch.allclose(w, small_w[at], rtol=2.0 ** -22, atol=2.0 ** -148, equal_nan=True)
+
+
+# a row of lanes a token: 4, 8, 16 and 32 experts a lane, uneven ones, groups that leave lanes of the row idle, and what only a wave holds (more groups, more chosen)
+MANY = [(1, 1, 1), (8, 1, 8), (17, 1, 16), (64, 1, 15), (65, 1, 14), (100, 1, 16), (128, 1, 8), (200, 1, 8), (256, 1, 16), (257, 1, 5), (500, 1, 16), (512, 1, 10),
+        (16, 4, 2), (256, 8, 8), (160, 8, 6), (9, 3, 3), (300, 5, 16), (512, 2, 8), (126, 9, 4), (16, 16, 2), (512, 16, 16), (64, 64, 8), (64, 1, 17), (102, 17, 6)]
+
+
+@pytest.mark.parametrize("E,groups,k", MANY)
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_many_tokens(dtype, scoring, E, groups, k):
+    gen = torch.Generator().manual_seed(E * 64 + groups + k)
+    rows = (torch.randn(21, E, generator=gen) * 1.5).to(dtype).cuda()
+    bias = (torch.randn(E, generator=gen) * 0.05).cuda()
+    top = groups if groups == 1 else max(groups // 2, -(-k // (E // groups)))
+    for b in (None, bias, torch.zeros_like(bias)):
+        for group_score in ("max", "top2") if groups > 1 else ("max",):
+            for renormalize in (True, False):
+                check_many(rows, k, scoring, b, groups, top, group_score, renormalize, 2.5)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("k", [1, 2, 7, 8, 14, 15, 16])
+def test_many_tokens_with_keys_close_together(k, scoring):
+    """Biases that are minus the score but for steps of 1e-9 to 1e-5: the order, the last that is in and the first that is out are all nearer than floats tell, in some rows."""
+    gen = torch.Generator().manual_seed(k)
+    one = torch.randn(1, 96, generator=gen)
+    s = torch.tensor(scores_of(one[0].tolist(), scoring), dtype=torch.float64)
+    for step in (1e-9, 1e-7, 1e-6, 1e-5):
+        bias = (-s + step * torch.randperm(96, generator=gen).double()).float()
+        rows = (one + step * torch.randn(16, 96, generator=gen)).cuda()
+        check_many(rows, k, scoring, bias.cuda())
+        check_many(rows, min(k, 12), scoring, bias.cuda(), 8, 4, "top2", False)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("biased", [False, True])
+def test_many_tokens_masked(scoring, biased):
+    gen = torch.Generator().manual_seed(5)
+    rows = torch.randn(9, 32, generator=gen)
+    rows[0] = -math.inf
+    rows[1, 3:] = -math.inf
+    rows[2] = torch.finfo(torch.float32).min
+    rows[2, 7] = 1.0
+    rows[3, ::2] = -math.inf
+    rows[4, 5] = math.nan
+    rows[5] = math.nan
+    rows[6, :31] = math.nan
+    rows[7, :16] = -math.inf
+    bias = (torch.randn(32, generator=gen) * 0.5 - 2.0).cuda() if biased else None
+    for groups, top in ((1, 1), (4, 2), (16, 4)):
+        for group_score in ("max", "top2"):
+            for renormalize in (True, False):
+                check_many(rows.cuda(), 5, scoring, bias, groups, top, group_score, renormalize)
 
 
 def gradient(logits, inds, dw, scoring, renormalize, scale):

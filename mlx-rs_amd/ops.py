@@ -206,7 +206,22 @@ def _linear_call():
         return lambda *args: None
     mod.bind(*(C.cast(getattr(lib, n), C.c_void_p).value for n in
                ("mi_moe_quantized_linear_typed", "mi_moe_quantized_matmul_typed", "mi_moe_quantized_matmul_workspace_size")))
+    mod.bind_layer(*(C.cast(getattr(lib, "mi_moe_" + n), C.c_void_p).value for n in
+                     ("add_rms_norm", "add_rms_norm_rows8", "add_rms_norm_grad_workspace_size", "add_rms_norm_grad", "quantized_linear_rows8_workspace_size",
+                      "quantized_linear_rows8", "select_experts", "select_experts_grad")))
     return mod.quantized_linear
+
+
+def _native(name, *args):
+    """The same module's call around another operator: its results, or None for what goes the general way."""
+    out = getattr(getattr(_linear_call(), "__self__", None), name, _general)(*args)
+    if type(out) is int:
+        check(out)
+    return out
+
+
+def _general(*args):
+    return None
 
 
 def quantized_matmul(x, w, scales, biases, transpose=False, group_size=64, bits=4):
@@ -264,6 +279,9 @@ def quantized_linear_rows8(x, row_scales, w, scales, biases, linear_bias=None, g
     """quantized_linear on rows in eight bits (``add_rms_norm_rows8``): y = (row_scales * x) . dequantize(w)^T + linear_bias, each result rounded
     once.  x: int8 [..., K]; row_scales: float32 [...]; w: int32 [N, K*bits/32]; scales, biases [N, K/group_size] and linear_bias [N] in
     bfloat16, float16 or float32, which is y's type.  bits 4 or 8.  Returns [..., N]."""
+    out = _native("quantized_linear_rows8", x, row_scales, w, scales, biases, linear_bias, group_size, bits)
+    if out is not None:
+        return out
     lib = load_library()
     who = "quantized_linear_rows8"
     _need(x, torch.int8, "x")
@@ -339,6 +357,9 @@ def add_rms_norm(x, residual, weight, eps=1e-5):
     """The residual's addition and the norm behind it in one pass: (y, h) with h = x + residual, rounded, and y = rms_norm(h, weight, eps).
     x, residual: [..., H] in bfloat16, float16 or float32; weight: [H], the same type.  residual None: h is x.  What stands between
     two sublayers (mlx-lm/src/models/qwen3.rs:310-325); in bfloat16 the bits of ``rms_norm(x + residual, weight, eps)``."""
+    out = _native("add_rms_norm", x, residual, weight, eps)
+    if out is not None:
+        return out
     lib = load_library()
     dt, T, H = _norm_operands("add_rms_norm", x, residual, weight)
     y = torch.empty_like(x)
@@ -351,6 +372,9 @@ def add_rms_norm(x, residual, weight, eps=1e-5):
 def add_rms_norm_rows8(x, residual, weight, eps=1e-5):
     """add_rms_norm with the normalised rows in eight bits, for ``quantized_linear_rows8``: (rows8 int8 [..., H], row_scales float32 [...], h);
     rows8 * row_scales stands for the rows, in steps of a 127th of a row's largest value."""
+    out = _native("add_rms_norm_rows8", x, residual, weight, eps)
+    if out is not None:
+        return out
     lib = load_library()
     dt, T, H = _norm_operands("add_rms_norm_rows8", x, residual, weight)
     rows8 = torch.empty(x.shape, dtype=torch.int8, device=x.device)
@@ -364,6 +388,9 @@ def add_rms_norm_rows8(x, residual, weight, eps=1e-5):
 def add_rms_norm_grad(dy, h, weight, eps=1e-5, dh=None):
     """The backward pass of add_rms_norm: (dx, dweight) from the gradients that arrive at y (dy) and, along the residual, at h (dh; None: none).
     dx is the gradient of x and of residual alike; dweight is summed over the rows in float32, in an order that does not change."""
+    out = _native("add_rms_norm_grad", dy, h, weight, eps, dh)
+    if out is not None:
+        return out
     lib = load_library()
     dt, T, H = _norm_operands("add_rms_norm_grad", h, dy, weight)
     if dh is not None:
@@ -439,6 +466,9 @@ def select_experts(logits, top_k, scoring="softmax", bias=None, n_groups=1, top_
     "sigmoid") of the logits; ``bias`` (float32 [E]) is added for the choice alone; of ``n_groups`` runs of experts the best ``top_groups`` are open, by
     their largest key or by the sum of their two largest scores (``group_score`` "max" / "top2"); ties go to the lower id.  Weights: the chosen
     scores, divided by their sum with ``renormalize``, times ``scale``.  ``SparseMoeBlock.forward_routed`` takes the results."""
+    out = _native("select_experts", logits, top_k, scoring, bias, n_groups, top_groups, group_score, renormalize, scale, dtype)
+    if out is not None:
+        return out
     lib = load_library()
     dt = _float_dtype(logits, "logits")
     if dtype not in _DTYPES:
@@ -464,6 +494,9 @@ def select_experts(logits, top_k, scoring="softmax", bias=None, n_groups=1, top_
 def select_experts_grad(dweights, logits, inds, scoring="softmax", renormalize=True, scale=1.0):
     """The gradient of select_experts' weights with respect to the logits, the choice taken as given: dlogits, of logits' shape and type.
     dweights: [..., k] in bfloat16, float16 or float32; inds: what select_experts returned."""
+    out = _native("select_experts_grad", dweights, logits, inds, scoring, renormalize, scale)
+    if out is not None:
+        return out
     lib = load_library()
     dt, wt = _float_dtype(logits, "logits"), _float_dtype(dweights, "dweights")
     _need(inds, torch.int32, "inds")

@@ -1029,7 +1029,7 @@ int mi_moe_select_experts_grad(const void *dw, int32_t w_dtype, const void *logi
 
 int mi_moe_quantized_linear_rows8_workspace_size(int64_t M, int32_t K, size_t *bytes) try {
   if (!bytes) return fail("quantized_linear_rows8_workspace_size: bytes is NULL");
-  if (M < 0 || K <= 0 || M * (int64_t)K > (int64_t)1 << 40) return fail("quantized_linear_rows8_workspace_size: bad sizes");
+  if (M < 0 || M > (int64_t)1 << 30 || K <= 0 || M * (int64_t)K > (int64_t)1 << 40) return fail("quantized_linear_rows8_workspace_size: bad sizes");
   *bytes = rows8_workspace_bytes(M, K);
   return 0;
 } MI_CATCH("quantized_linear_rows8_workspace_size")

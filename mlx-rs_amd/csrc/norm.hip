@@ -254,8 +254,20 @@ static hipError_t with_dtype(int dt, F f) {
 hipError_t launch_add_rms_norm(const void *x, const void *r, const void *w, float eps, int64_t T, int H, int dt, void *sum, void *y, float *scales,
                                hipStream_t st) {
   if (T == 0) return hipSuccess;
-  const NormArgs a{x, r, w, eps, T, H, sum, y, scales};
   const bool rows8 = scales != nullptr;
+  constexpr int64_t kMost = (int64_t)1 << 21;  // rows of a launch, which has less than 2^32 threads
+  if (T > kMost) {
+    const int64_t size = dt == 2 ? 4 : 2;
+    auto in = [&](const void *base, int64_t at) { return base ? static_cast<const char *>(base) + at : nullptr; };
+    auto out = [&](void *base, int64_t at) { return base ? static_cast<char *>(base) + at : nullptr; };
+    for (int64_t t = 0; t < T; t += kMost) {
+      const int64_t at = t * H * size;
+      const hipError_t e = launch_add_rms_norm(in(x, at), in(r, at), w, eps, T - t < kMost ? T - t : kMost, H, dt, out(sum, at), out(y, rows8 ? t * H : at), rows8 ? scales + t : nullptr, st);
+      if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+  }
+  const NormArgs a{x, r, w, eps, T, H, sum, y, scales};
   return with_dtype(dt, [&](auto d) {
     constexpr int DT = decltype(d)::value;
     if (H <= 512) return start_norm<DT, 64, 1>(a, rows8, st);

@@ -54,10 +54,19 @@ template <int DT, int BITS>
 static hipError_t start_plain(const Rows8Args &a, hipStream_t st) {
   auto start = [&](auto rows) {
     constexpr int ROWS = decltype(rows)::value;
-    const int64_t waves = (a.M + ROWS - 1) / ROWS * a.N, grid = (waves + 3) / 4;
-    if (grid > INT32_MAX) return hipErrorInvalidValue;
-    rows8_plain_kernel<DT, BITS, ROWS><<<(unsigned)grid, 256, 0, st>>>(a);
-    return hipGetLastError();
+    const int64_t most = ((int64_t)1 << 25) / a.N * ROWS, step = most ? most : ROWS;  // rows of a launch, which has less than 2^32 threads
+    for (int64_t m = 0; m < a.M; m += step) {
+      Rows8Args some = a;
+      some.x = a.x + m * a.K;
+      some.row_scales = a.row_scales + m;
+      some.y = static_cast<Value<DT> *>(a.y) + m * a.N;
+      some.M = a.M - m < step ? a.M - m : step;
+      const int64_t grid = ((some.M + ROWS - 1) / ROWS * a.N + 3) / 4;
+      if (grid >= (int64_t)1 << 24) return hipErrorInvalidValue;
+      rows8_plain_kernel<DT, BITS, ROWS><<<(unsigned)grid, 256, 0, st>>>(some);
+      if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    }
+    return hipSuccess;
   };
   return a.M == 1 ? start(std::integral_constant<int, 1>{}) : start(std::integral_constant<int, 8>{});
 }
@@ -232,7 +241,7 @@ __global__ __launch_bounds__(512, MI * NI <= 4 ? 4 : 2) void rows8_few_kernel(Ro
 template <int DT, int BITS, int GROUP, int MI, int NI>
 static hipError_t start_few(const Rows8Args &a, hipStream_t st) {
   const int64_t wide = (a.N + 16 * NI - 1) / (16 * NI), grid = (a.M + 16 * MI - 1) / (16 * MI) * wide;
-  if (grid > INT32_MAX) return hipErrorInvalidValue;
+  if (grid >= (int64_t)1 << 23) return hipErrorInvalidValue;  // (a launch has less than 2^32 threads)
   rows8_few_kernel<DT, BITS, GROUP, MI, NI><<<(unsigned)grid, 512, 0, st>>>(a, (int)wide);
   return hipGetLastError();
 }
@@ -247,6 +256,19 @@ size_t rows8_workspace_bytes(int64_t M, int K) { return M <= kRows8NoTiles || K 
 
 hipError_t launch_qmm_rows8(const Rows8Args &a, int bits, int dt, void *workspace, size_t workspace_bytes, hipStream_t st) {
   if (a.M == 0) return hipSuccess;
+  // rows of a launch: every kernel's has less than 2^32 threads with these
+  const int64_t by_k = ((int64_t)1 << 34) / a.K, by_n = ((int64_t)1 << 33) / a.N, fit = (by_k < by_n ? by_k : by_n) / 128 * 128, step = fit ? fit : 128;
+  if (a.M > step) {
+    Rows8Args some = a;
+    for (int64_t m = 0; m < a.M; m += step) {
+      some.x = a.x + m * a.K;
+      some.row_scales = a.row_scales + m;
+      some.y = static_cast<char *>(a.y) + m * a.N * (dt == 2 ? 4 : 2);
+      some.M = a.M - m < step ? a.M - m : step;
+      if (hipError_t e = launch_qmm_rows8(some, bits, dt, workspace, workspace_bytes, st); e != hipSuccess) return e;
+    }
+    return hipSuccess;
+  }
   if (!rows8_even(a)) {
     return rows8_with_types(dt, bits, a.group, [&](auto d, auto b, auto) { return start_plain<decltype(d)::value, decltype(b)::value>(a, st); });
   }

@@ -288,7 +288,7 @@ template <int DT, int BITS, int GROUP, int MI, int NI, int WM, int WN, int KS, i
 static hipError_t start_tile(const Rows8Args &a, const uint4 *tiles, const float *sums, hipStream_t st) {
   using L = Rows8Tile<DT, BITS, GROUP, MI, NI, WM, WN, KS, NB>;
   const int64_t n_mtiles = (a.M + L::ROWS - 1) / L::ROWS, n_ntiles = (a.N + L::COLS - 1) / L::COLS, grid = (n_ntiles + 7) / 8 * 8 * n_mtiles;
-  if (grid > INT32_MAX) return hipErrorInvalidValue;
+  if (grid * L::kThreads >= (int64_t)1 << 32) return hipErrorInvalidValue;
   const auto kernel = &rows8_tiles_kernel<DT, BITS, GROUP, MI, NI, WM, WN, KS, NB, OCC>;
   static std::atomic<uint64_t> allowed{0};
   if (hipError_t e = allow_lds(reinterpret_cast<const void *>(kernel), L::LDS, allowed); e != hipSuccess) return e;
@@ -302,7 +302,7 @@ hipError_t launch_rows8_tiles(const Rows8Args &a, Rows8Kind kind, int bits, int 
   uint4 *const tiles = static_cast<uint4 *>(workspace);
   float *const sums = reinterpret_cast<float *>(static_cast<char *>(workspace) + rows8_tiles_bytes(a.M, a.K));
   const int64_t units = row_tiles(a.M) * ((a.K / a.group + 3) / 4);
-  if (units > (int64_t)4 * INT32_MAX) return hipErrorInvalidValue;
+  if (units >= (int64_t)1 << 25) return hipErrorInvalidValue;  // (a launch has less than 2^32 threads)
   return rows8_with_types(dt, bits, a.group, [&](auto d, auto b, auto g) {
     constexpr int DT = decltype(d)::value, BITS = decltype(b)::value, GROUP = decltype(g)::value;
     rows8_prepare_kernel<BITS, GROUP><<<(unsigned)((units + 3) / 4), 256, 0, st>>>(a.x, a.M, a.K, tiles, sums);

@@ -75,12 +75,12 @@ __device__ __forceinline__ void merge_two(T &t1, T &t2, T o1, T o2) {
 }
 __device__ __forceinline__ float f32_of(uint32_t u) { return __uint_as_float(u); }
 
-// Everything in double, u64 keys: any logits and biases.  Lane r gets the r-th expert's id and score.
+// Everything in double, u64 keys: any logits and biases.  Lane r gets the r-th expert's id.
 template <int S>
-__device__ __forceinline__ void select_exact(const SelectKernelArgs &p, const Slots<S> &x, int g, uint32_t &id, double &score) {
+__device__ __forceinline__ void select_exact(const SelectKernelArgs &p, const Slots<S> &x, int g, uint32_t &id) {
   const SelectArgs &a = p.a;
   const int lane = lane_id();
-  double v[S], s[S];
+  double v[S];
   if (a.scoring == 0) {
     float most = -INFINITY;  // (fmaxf passes over what is no number)
 #pragma unroll
@@ -102,7 +102,6 @@ __device__ __forceinline__ void select_exact(const SelectKernelArgs &p, const Sl
   uint64_t key[S];
 #pragma unroll
   for (int j = 0; j < S; ++j) {
-    s[j] = v[j];
     if (a.bias && x.on[j]) v[j] += (double)a.bias[x.base + j];
     if (x.l[j] == -INFINITY) v[j] = -INFINITY;
     key[j] = !x.on[j] ? 0 : a.bias ? key_of(v[j]) : key_of((double)x.l[j]);
@@ -133,10 +132,9 @@ __device__ __forceinline__ void select_exact(const SelectKernelArgs &p, const Sl
   for (int r = 0; r < a.k; ++r) {
     uint64_t best = 0;
     int at = 0;
-    double sv = 0.0;
 #pragma unroll
     for (int j = 0; j < S; ++j)
-      if (key[j] > best) best = key[j], at = j, sv = s[j];
+      if (key[j] > best) best = key[j], at = j;
     const uint64_t top = wave_max_key(best);
     const int owner = __builtin_ctzll(__ballot(best == top));
     if (lane == owner)
@@ -144,15 +142,36 @@ __device__ __forceinline__ void select_exact(const SelectKernelArgs &p, const Sl
       for (int j = 0; j < S; ++j)
         if (j == at) key[j] = 0;
     const uint32_t chosen = (uint32_t)__builtin_amdgcn_readlane(x.base + at, owner);
-    const double its = readlane_f64(sv, owner);
-    if (lane == r) id = chosen, score = its;
+    if (lane == r) id = chosen;
   }
 }
 
 // The keys and the groups' ranks in float where that decides them: float scores are within kNear / 4 of the exact ones (exp and reciprocal to 2^-22 of their values, an
 // exponent off by 2^-24 of itself, of scores of one at most, a sum to 2^-22), biased keys within 2^-24 of their size more.  Where two keys that follow each other in the choice, or two groups' ranks, are nearer than
-// that allows, or something is not finite, the token goes through select_exact (one in some hundred); without a bias the logits are exact keys.  Scores of the chosen are in double, a lane each.
+// that allows, or something is an infinity above zero or no number, the token goes through select_exact (one in some hundred); without a bias the logits are exact keys.  Scores of the chosen
+// are in double, a lane each, of softmax scores that are renormalised from the chosen logits alone: they hold where a softmax over all would round to zero.
 constexpr float kNear = 0x1p-19f, kNearOfSize = 0x1p-21f;
+
+// the key's part that a bias is, minus infinity for an expert that is masked, and whether floats can decide
+__device__ __forceinline__ float with_mask(float l, float bias) { return l == -INFINITY ? -INFINITY : bias; }
+__device__ __forceinline__ bool not_below(float l, float b) { return !(l < INFINITY && b < INFINITY); }
+// what a group's rank may be off by, in kNearOfSize (a rank of minus infinity is that)
+__device__ __forceinline__ float rank_size(float rank, float t1, float t2, bool two) { return rank == -INFINITY ? 0.f : two ? fabsf(t1) + fabsf(t2) : fabsf(t1); }
+
+// score of a chosen expert but for a factor that renormalisation takes out again
+__device__ __forceinline__ double score_of(const SelectArgs &a, float logit, float most, double total) {
+  if (a.scoring == 1) return sigmoid64(logit);
+  return logit != logit ? NAN : most == -INFINITY ? 0.0 : exp((double)logit - (double)most) / total;
+}
+
+// weights of a token's choice from its scores, in the lanes below k; `sum`: of all lanes' scores
+__device__ __forceinline__ void put_choice(const SelectArgs &a, int64_t t, int lane, uint32_t id, double score, double sum) {
+  const double w = !a.renormalize ? score : sum == 0.0 ? 0.0 : score / sum;
+  if (lane < a.k) {
+    a.idx[t * a.k + lane] = id;
+    put_value(a.w, t * a.k + lane, a.w_dtype, w * (double)a.scale);
+  }
+}
 
 // SUM: softmax scores that are not renormalised, whose denominator is over all experts.  KEYS: float scores decide something (a bias, or groups ranked by two scores).
 template <int DT, int S, bool KEYS, bool SUM>
@@ -174,8 +193,8 @@ __global__ __launch_bounds__(256) void select_experts_kernel(SelectKernelArgs p)
   if constexpr (KEYS) {
 #pragma unroll
     for (int j = 0; j < S; ++j) {
-      b[j] = a.bias && x.on[j] ? a.bias[x.base + j] : 0.f;
-      odd |= x.on[j] && not_finite(x.l[j] - x.l[j] + b[j]);
+      b[j] = with_mask(x.l[j], a.bias && x.on[j] ? a.bias[x.base + j] : 0.f);
+      odd |= x.on[j] && not_below(x.l[j], b[j]);
     }
   }
   float most = -INFINITY;
@@ -183,6 +202,7 @@ __global__ __launch_bounds__(256) void select_experts_kernel(SelectKernelArgs p)
 #pragma unroll
     for (int j = 0; j < S; ++j) most = fmaxf(most, x.l[j]);
     most = wave_max_f32(most);
+    if constexpr (KEYS) odd |= a.scoring == 0 && most == -INFINITY;
   }
   double total = 1.0;
   if constexpr (SUM) {
@@ -235,8 +255,9 @@ __global__ __launch_bounds__(256) void select_experts_kernel(SelectKernelArgs p)
       if (n > 3) other(std::integral_constant<int, kDppMirror>{});
       if (n > 4) merge_two(t1, t2, __shfl_xor(t1, 16), __shfl_xor(t2, 16));
       if (n > 5) merge_two(t1, t2, __shfl_xor(t1, 32), __shfl_xor(t2, 32));
-      const float mine = a.group_score == 0 || p.size == 1 ? t1 : t1 + t2;
-      const float clear = 2 * kNear + kNearOfSize * wave_max_f32(g >= a.groups ? 0.f : p.size == 1 ? fabsf(t1) : fabsf(t1) + fabsf(t2));
+      const bool two = a.group_score == 1 && p.size > 1;
+      const float mine = two ? t1 + t2 : t1;
+      const float clear = 2 * kNear + kNearOfSize * wave_max_f32(g >= a.groups ? 0.f : rank_size(mine, t1, t2, two));
       int before = 0, maybe = 0;  // groups that are better, and that could be
       for (int o = 0; o < a.groups; ++o) {
         const float its = f32_of((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(mine), o << n));
@@ -267,8 +288,6 @@ __global__ __launch_bounds__(256) void select_experts_kernel(SelectKernelArgs p)
       for (int j = 0; j < S; ++j) key[j] = 0;
   }
   uint32_t id = 0;
-  float logit = 0.f;
-  double score = 0.0;
   bool exact = false;
   if (!KEYS || !__any(odd)) {
     float last = 0.f;
@@ -287,39 +306,28 @@ __global__ __launch_bounds__(256) void select_experts_kernel(SelectKernelArgs p)
       }
       const int owner = __builtin_ctzll(__ballot(best == top));
       int at = 0;
-      float l = x.l[0];
 #pragma unroll
       for (int j = S - 1; j >= 0; --j)
-        if (key[j] == top) at = j, l = x.l[j];
+        if (key[j] == top) at = j;
       const uint32_t chosen = (uint32_t)__builtin_amdgcn_readlane(x.base + at, owner);
-      const float its = f32_of((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(l), owner));
 #pragma unroll
       for (int j = 0; j < S; ++j)
         if (lane == owner && j == at) key[j] = 0;
-      if (lane == r) id = chosen, logit = its;
+      if (lane == r) id = chosen;
     }
     exact = near;
   } else {
     exact = true;
   }
+  if constexpr (KEYS) {
+    if (exact) select_exact<S>(p, x, g, id);
+  }
   const bool mine = lane < a.k;
-  if (KEYS && exact) {
-    select_exact<S>(p, x, g, id, score);
-  } else if (a.scoring == 1) {
-    score = mine ? sigmoid64(logit) : 0.0;
-  } else {
-    if constexpr (!SUM) most = wave_max_f32(mine ? logit : -INFINITY);  // (renormalised: any common factor)
-    score = !mine ? 0.0 : logit != logit ? NAN : most == -INFINITY ? 0.0 : exp((double)logit - (double)most) / total;
-  }
-  double w = score;
-  if (a.renormalize) {
-    const double sum = wave_sum_f64(mine ? score : 0.0);
-    w = sum == 0.0 ? 0.0 : score / sum;
-  }
-  if (mine) {
-    a.idx[t * a.k + lane] = id;
-    put_value(a.w, t * a.k + lane, a.w_dtype, w * (double)a.scale);
-  }
+  const float logit = mine ? as_f32(row[id]) : -INFINITY;
+  if (!SUM && a.scoring == 0) most = wave_max_f32(logit);
+  const double score = mine ? score_of(a, logit, most, total) : 0.0;
+  const double sum = wave_sum_f64(score);
+  put_choice(a, t, lane, id, score, sum);
 }
 
 // ---------------------------------------------------------------- up to 16 groups and 16 choices: a row of 16 lanes a token
@@ -372,15 +380,6 @@ __device__ __forceinline__ void each_candidate(double v, uint32_t id, F f) {
   }
 }
 
-// weights of a token's choice from its scores, in the lanes below k; `sum`: of all lanes' scores
-__device__ __forceinline__ void put_choice(const SelectArgs &a, int64_t t, int lane, uint32_t id, double score, double sum) {
-  const double w = !a.renormalize ? score : sum == 0.0 ? 0.0 : score / sum;
-  if (lane < a.k) {
-    a.idx[t * a.k + lane] = id;
-    put_value(a.w, t * a.k + lane, a.w_dtype, w * (double)a.scale);
-  }
-}
-
 template <int DT, int S, bool KEYS, bool SUM>
 __global__ __launch_bounds__(256) void select_rows_kernel(SelectKernelArgs p, SelectKernelArgs whole) {  // whole: the layout of a wave a token
   const SelectArgs &a = p.a;
@@ -409,7 +408,10 @@ __global__ __launch_bounds__(256) void select_rows_kernel(SelectKernelArgs p, Se
       for (int j = 0; j < S; ++j) b[j] = a.bias && j < n_mine ? a.bias[base + j] : 0.f;
     }
 #pragma unroll
-    for (int j = 0; j < S; ++j) odd |= j < n_mine && not_finite(l[j] - l[j] + b[j]);
+    for (int j = 0; j < S; ++j) {
+      b[j] = with_mask(l[j], b[j]);
+      odd |= j < n_mine && not_below(l[j], b[j]);
+    }
   }
   auto larger = [](float x, float y) { return fmaxf(x, y); };
   float most = -INFINITY;
@@ -417,6 +419,7 @@ __global__ __launch_bounds__(256) void select_rows_kernel(SelectKernelArgs p, Se
 #pragma unroll
     for (int j = 0; j < S; ++j) most = fmaxf(most, l[j]);
     most = row_join(most, larger);
+    if constexpr (KEYS) odd |= a.scoring == 0 && most == -INFINITY;
   }
   double total = 1.0;
   if constexpr (SUM) {
@@ -472,9 +475,10 @@ __global__ __launch_bounds__(256) void select_rows_kernel(SelectKernelArgs p, Se
     if (n > 0) other(std::integral_constant<int, kDppXor1>{});
     if (n > 1) other(std::integral_constant<int, kDppXor2>{});
     if (n > 2) other(std::integral_constant<int, kDppHalfMirror>{});
-    const float mine = a.group_score == 0 || p.size == 1 ? t1 : t1 + t2;
+    const bool two = a.group_score == 1 && p.size > 1;
+    const float mine = two ? t1 + t2 : t1;
     float clear = 0.f;
-    if constexpr (KEYS) clear = 2 * kNear + kNearOfSize * row_join(g >= a.groups ? 0.f : p.size == 1 ? fabsf(t1) : fabsf(t1) + fabsf(t2), larger);
+    if constexpr (KEYS) clear = 2 * kNear + kNearOfSize * row_join(g >= a.groups ? 0.f : rank_size(mine, t1, t2, two), larger);
     int before = 0, maybe = 0;  // lanes of groups that are better, and that could be
     each_other(mine, [&](int n_back, float its) __attribute__((always_inline)) {
       const int og = ((lane - n_back) & 15) >> n;
@@ -523,19 +527,14 @@ __global__ __launch_bounds__(256) void select_rows_kernel(SelectKernelArgs p, Se
   }
   const bool named = id < (uint32_t)a.E;
   const float logit = named ? as_f32(row[id]) : -INFINITY;
-  double score;
-  if (a.scoring == 1) {
-    score = named ? sigmoid64(logit) : 0.0;
-  } else {
-    if constexpr (!SUM) most = row_join(lane < a.k ? logit : -INFINITY, larger);  // (renormalised: any common factor)
-    score = !named ? 0.0 : logit != logit ? NAN : most == -INFINITY ? 0.0 : exp((double)logit - (double)most) / total;
-  }
+  if (!SUM && a.scoring == 0) most = row_join(lane < a.k ? logit : -INFINITY, larger);
+  double score = named ? score_of(a, logit, most, total) : 0.0;
   if constexpr (KEYS) {
     if (__ballot(close)) {
       if (a.scoring == 0 && !SUM) {
         odd |= close;
       } else {
-        const double v = named && a.bias ? score + (double)a.bias[id] : -INFINITY;
+        const double v = named && a.bias && logit != -INFINITY ? score + (double)a.bias[id] : -INFINITY;
         int rank = 0;
         each_candidate(v, id, [&](double its, uint32_t other) __attribute__((always_inline)) { rank += its > v || (its == v && other < id); });
         if (close) {
@@ -564,9 +563,12 @@ __global__ __launch_bounds__(256) void select_rows_kernel(SelectKernelArgs p, Se
         x.l[j] = x.on[j] ? as_f32(its[x.base + j]) : -INFINITY;
       }
       uint32_t eid = 0;
-      double es = 0.0;
-      select_exact<S / 4>(whole, x, wg, eid, es);
-      put_choice(a, tt, wl, eid, es, wave_sum_f64(wl < a.k ? es : 0.0));
+      select_exact<S / 4>(whole, x, wg, eid);
+      const int from_lane = (int)(tt - t0) * 16;  // (of its row)
+      const float el = wl < a.k ? as_f32(its[eid]) : -INFINITY;
+      const float em = SUM ? f32_of((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(most), from_lane)) : wave_max_f32(el);
+      const double es = wl < a.k ? score_of(a, el, em, SUM ? readlane_f64(total, from_lane) : 1.0) : 0.0;
+      put_choice(a, tt, wl, eid, es, wave_sum_f64(es));
     }
   }
 }
@@ -592,8 +594,21 @@ static hipError_t start_select(const SelectKernelArgs &p, hipStream_t st) {
   return hipGetLastError();
 }
 
+constexpr int64_t kSelectMost = (int64_t)1 << 25;  // tokens of a launch
 hipError_t launch_select_experts(const SelectArgs &a, int dt, hipStream_t st) {
   if (a.T == 0) return hipSuccess;
+  if (a.T > kSelectMost) {  // (a launch has less than 2^32 threads)
+    SelectArgs some = a;
+    const int64_t size = dt == 2 ? 4 : 2, w_size = a.w_dtype == 2 ? 4 : 2;
+    for (int64_t t = 0; t < a.T; t += kSelectMost) {
+      some.logits = static_cast<const char *>(a.logits) + t * a.E * size;
+      some.idx = a.idx + t * a.k;
+      some.w = static_cast<char *>(a.w) + t * a.k * w_size;
+      some.T = a.T - t < kSelectMost ? a.T - t : kSelectMost;
+      if (hipError_t e = launch_select_experts(some, dt, st); e != hipSuccess) return e;
+    }
+    return hipSuccess;
+  }
   auto layout = [&](int lanes_log2) {
     SelectKernelArgs p{a, a.E / a.groups, lanes_log2, 0};
     while (p.lanes_log2 > 0 && (1 << (lanes_log2 - p.lanes_log2)) < a.groups) --p.lanes_log2;  // lanes of a group
@@ -679,6 +694,19 @@ __global__ __launch_bounds__(256) void select_grad_kernel(SelectGradArgs a) {
 
 hipError_t launch_select_grad(const SelectGradArgs &a, int dt, hipStream_t st) {
   if (a.T == 0) return hipSuccess;
+  if (a.T > kSelectMost) {
+    SelectGradArgs some = a;
+    const int64_t size = dt == 2 ? 4 : 2, w_size = a.w_dtype == 2 ? 4 : 2;
+    for (int64_t t = 0; t < a.T; t += kSelectMost) {
+      some.logits = static_cast<const char *>(a.logits) + t * a.E * size;
+      some.dlogits = static_cast<char *>(a.dlogits) + t * a.E * size;
+      some.idx = a.idx + t * a.k;
+      some.dw = static_cast<const char *>(a.dw) + t * a.k * w_size;
+      some.T = a.T - t < kSelectMost ? a.T - t : kSelectMost;
+      if (hipError_t e = launch_select_grad(some, dt, st); e != hipSuccess) return e;
+    }
+    return hipSuccess;
+  }
   const unsigned grid = (unsigned)((a.T + 3) / 4);
   if (dt == 0) select_grad_kernel<0><<<grid, 256, 0, st>>>(a);
   else if (dt == 1) select_grad_kernel<1><<<grid, 256, 0, st>>>(a);

@@ -193,6 +193,21 @@ def test_more_values_than_32_bits_count():
     torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("with_residual", [True, False])
+def test_more_rows_than_a_launch_takes(with_residual):
+    """2^21 rows a launch: the rows around its end and the last ones, as in a call of their own."""
+    import mlx_rs_amd as m
+    T, H = 2 ** 21 + 5, 24
+    x = torch.randn(T, H, device="cuda").to(torch.bfloat16)
+    r = torch.randn(T, H, device="cuda").to(torch.bfloat16) if with_residual else None
+    w = torch.randn(H, device="cuda").to(torch.bfloat16)
+    got = m.ops.add_rms_norm(x, r, w) + m.ops.add_rms_norm_rows8(x, r, w)
+    for part in (slice(0, 9), slice(2 ** 21 - 7, 2 ** 21 + 3), slice(T - 4, T)):
+        some = (x[part].contiguous(), None if r is None else r[part].contiguous(), w)
+        for a, b in zip(got, m.ops.add_rms_norm(*some) + m.ops.add_rms_norm_rows8(*some)):
+            assert torch.equal(a[part], b)
+
+
 def test_refusals():
     import mlx_rs_amd as m
     x = torch.zeros(4, 64, dtype=torch.bfloat16, device="cuda")

@@ -152,6 +152,56 @@ def test_shapes_of_rows_and_no_rows():
     assert m.ops.quantized_linear_rows8(x[:0], sx[:0], w, s, b).shape == (0, 32)
 
 
+@pytest.mark.parametrize("M,N,K,step", [(8192 + 70, 2 ** 20, 128, 8192), (2 ** 16 * 8 + 70, 512, 32, 2 ** 16 * 8)])
+def test_more_rows_than_a_launch_takes(M, N, K, step):
+    """Rows on both sides of where a launch ends, results past 2^32 elements: the bits of a call of their own rows."""
+    import mlx_rs_amd as m
+    w, s, b = m.ops.quantize(torch.randn(N, K, device="cuda"), 32, 4, torch.bfloat16)
+    x = torch.randint(-127, 128, (M, K), device="cuda", dtype=torch.int32).to(torch.int8)
+    sx = torch.rand(M, device="cuda")
+    y = m.ops.quantized_linear_rows8(x, sx, w, s, b, None, 32, 4)
+    for at in (0, step - 64, step, M - 64):
+        some = slice(at, at + 64)
+        part = m.ops.quantized_linear_rows8(x[some].contiguous(), sx[some].contiguous(), w, s, b, None, 32, 4)
+        err, size = (y[some].float() - part.float()).abs(), part.float().abs()
+        # two orders of the same float sums: each rounded once to bfloat16, whose steps are 2^-8 of a value and next to which the sums' own differences are little
+        assert bool((err <= 2.0 ** -7 * size + 1e-3).all())
+    del y
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("M", [17, 100, 600])
+def test_without_room_for_prepared_rows(M):
+    """No workspace, and one that is a byte short: the kernels that need none, never a write outside."""
+    import mlx_rs_amd as m
+    args = layer(M, 640, 512, 4, 64, torch.bfloat16)
+    x, sx, w, s, b, _ = args
+    lib = m.load_library()
+    need = m.ops._rows8_workspace_bytes(M, 512)
+    assert need > 0
+    for room, size in ((None, 0), (torch.full((need + 512,), 77, dtype=torch.uint8, device="cuda"), need - 1)):
+        y = torch.empty(M, 640, dtype=torch.bfloat16, device="cuda")
+        m.capi.check(lib.mi_moe_quantized_linear_rows8(x.data_ptr(), sx.data_ptr(), w.data_ptr(), s.data_ptr(), b.data_ptr(), None, M, 640, 512, 64, 4, 0, y.data_ptr(),
+                                                       None if room is None else room.data_ptr(), size, m.ops._stream()))
+        check(y, args, 64, 4)
+        assert room is None or bool((room == 77).all())
+
+
+def test_the_workspace_ends_where_it_says():
+    import mlx_rs_amd as m
+    lib = m.load_library()
+    for M, N, K, bits, group in ((600, 640, 512, 4, 64), (130, 2048, 384, 8, 32), (257, 4096, 128, 4, 128)):
+        args = layer(M, N, K, bits, group, torch.bfloat16)
+        x, sx, w, s, b, _ = args
+        need = m.ops._rows8_workspace_bytes(M, K)
+        room = torch.full((need + 4096,), 77, dtype=torch.uint8, device="cuda")
+        y = torch.empty(M, N, dtype=torch.bfloat16, device="cuda")
+        m.capi.check(lib.mi_moe_quantized_linear_rows8(x.data_ptr(), sx.data_ptr(), w.data_ptr(), s.data_ptr(), b.data_ptr(), None, M, N, K, group, bits, 0, y.data_ptr(),
+                                                       room.data_ptr(), need, m.ops._stream()))
+        check(y, args, group, bits)
+        assert bool((room[need:] == 77).all())
+
+
 def test_refusals():
     import mlx_rs_amd as m
     x, sx, w, s, b, lb = layer(4, 32, 256, 4, 64, torch.bfloat16, bias=True)

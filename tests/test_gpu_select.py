@@ -300,3 +300,56 @@ def test_refusals():
                  lambda: m.ops.select_experts_grad(x[:3, :2].contiguous(), x, i[:3].contiguous())):
         with pytest.raises(m.MoeError):
             call()
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("T", [5, 4100])
+def test_masked_experts_and_groups_of_a_router(scoring, T):
+    """Experts that every token has masked, by a logit or by a bias of -inf, among others that are close together."""
+    import mlx_rs_amd as m
+    gen = torch.Generator().manual_seed(T)
+    rows = torch.randn(5, 48, generator=gen)
+    rows[:, 40:] = -math.inf
+    bias = torch.randn(48, generator=gen) * 1e-6
+    bias[[3, 17]] = -math.inf
+    bias[24:30] = -math.inf  # all of a group of six
+    at = torch.arange(T) % 5
+    for groups, top, group_score in ((1, 1, "max"), (8, 3, "top2"), (8, 5, "max"), (48, 40, "top2")):
+        for k in (4, 9):
+            for b in (None, bias.cuda()):
+                inds, w = m.ops.select_experts(rows[at].cuda(), k, scoring, b, groups, top, group_score, dtype=torch.float32)
+                small, small_w = check(rows.cuda(), k, scoring, b, groups, top, group_score)
+                assert bool((inds == small[at.cuda()]).all()) and torch.allclose(w, small_w[at.cuda()], rtol=2.0 ** -22, atol=0)
+
+
+def test_weights_of_scores_that_a_softmax_rounds_to_zero():
+    """The expert with all of the softmax is not open: the shares are those of the chosen logits among themselves, whether floats or doubles decide the choice."""
+    logits = torch.full((2, 32), -1000.0)
+    logits[:, 0] = 1000.0
+    logits[:, 9] = -999.0
+    bias = torch.zeros(32)
+    bias[0] = -5.0
+    spread = bias + torch.arange(32) * 1e-3
+    for b in (bias, spread):
+        check(logits.cuda(), 4, "softmax", b.cuda(), 4, 2, "max")
+        check_many(logits.cuda(), 4, "softmax", b.cuda(), 4, 2, "max")
+
+
+def test_more_tokens_than_a_launch_takes():
+    """2^25 and three tokens of 128 experts: results and gradients on both sides of where a launch ends, logits past 2^32 elements."""
+    import mlx_rs_amd as m
+    T, E, k = 2 ** 25 + 3, 128, 2
+    base = torch.randn(4093, E, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
+    logits = torch.empty((T, E), dtype=torch.bfloat16, device="cuda")
+    for i in range(0, T, 4093 * 512):
+        part = logits[i:i + 4093 * 512]
+        part.copy_(base.repeat(512, 1)[:part.shape[0]])
+    inds, w = m.ops.select_experts(logits, k)
+    want_i, want_w = m.ops.select_experts(base, k)
+    dw = torch.randn(T, k, device="cuda").to(torch.bfloat16)
+    d = m.ops.select_experts_grad(dw, logits, inds)
+    for at in (0, 2 ** 25 - 4093, 2 ** 25 - 2, T - 4093):
+        r = torch.arange(at, min(at + 4093, T), device="cuda") % 4093
+        part = slice(at, at + r.numel())
+        assert torch.equal(inds[part], want_i[r]) and torch.equal(w[part], want_w[r])
+        assert torch.equal(d[part], m.ops.select_experts_grad(dw[part].contiguous(), logits[part].contiguous(), inds[part].contiguous()))

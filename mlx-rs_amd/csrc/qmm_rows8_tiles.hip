@@ -8,10 +8,15 @@ namespace mi_moe {
 //   8-bit codes                16 consecutive values
 //   4-bit codes                the words 2 kb and 2 kb + 1 of the eight, of each the even nibbles, then the odd ones
 //   groups of 32 (two a tile)  8 values of each, 8 kb .. 8 kb + 7 of the group, in that order within a word
-// and the group sums, four groups of 16 rows a tile of 64 floats (lane: row l % 16, group 4 q + kb; zeros past the last group).
+// and the group sums of 16 rows, zeros past the last group:
+//   16-bit scales   eight groups a tile of 512 bytes, a lane's (row l % 16) of the groups 2 kb and 2 kb + 1: the sums' multiples of 128 as two bf16 values, then the rests, -64 .. 64 (both are
+//                   exact: a sum is 2^14 at most)
+//   float32 scales  four groups a tile of 64 floats (lane: row l % 16, group 4 q + kb)
 __host__ __device__ constexpr int64_t row_tiles(int64_t M) { return (M + 15) / 16; }
 constexpr size_t rows8_tiles_bytes(int64_t M, int K) { return (size_t)row_tiles(M) * 16 * K; }
-constexpr size_t rows8_sums_bytes(int64_t M, int K, int group) { return (size_t)row_tiles(M) * ((K / group + 3) / 4) * 256; }
+constexpr size_t rows8_sums_bytes(int64_t M, int K, int group) { return (size_t)row_tiles(M) * ((K / group + 7) / 8) * 512; }
+
+__host__ __device__ constexpr int rows8_quads(int G) { return (G + 7) / 8 * 2; }  // fours of groups, in whole eights
 
 // eight bytes in their order to the even ones, then the odd ones
 __device__ __forceinline__ uint2 evens_odds(uint2 v) {
@@ -19,10 +24,10 @@ __device__ __forceinline__ uint2 evens_odds(uint2 v) {
 }
 
 // A wave makes the tiles of 16 rows and four groups.
-template <int BITS, int GROUP>
-__global__ __launch_bounds__(256) void rows8_prepare_kernel(const signed char *x, int64_t M, int K, uint4 *tiles, float *sums) {
+template <int BITS, int GROUP, bool WIDE>
+__global__ __launch_bounds__(256) void rows8_prepare_kernel(const signed char *x, int64_t M, int K, uint4 *tiles, void *sums) {  // WIDE: float32 scales
   constexpr int NT = GROUP * 4 / 64;  // tiles of four groups
-  const int lane = lane_id(), kb = lane >> 4, quads = (K / GROUP + 3) / 4, n_tiles = K / 64;
+  const int lane = lane_id(), kb = lane >> 4, quads = rows8_quads(K / GROUP), n_tiles = K / 64;
   const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), mt = unit / quads;
   const int q = (int)(unit % quads);
   if (mt >= row_tiles(M)) return;
@@ -51,7 +56,12 @@ __global__ __launch_bounds__(256) void rows8_prepare_kernel(const signed char *x
     sum[i] += __shfl_xor(sum[i], 16);
     sum[i] += __shfl_xor(sum[i], 32);
   }
-  sums[(mt * quads + q) * 64 + lane] = (float)(kb == 0 ? sum[0] : kb == 1 ? sum[1] : kb == 2 ? sum[2] : sum[3]);
+  if constexpr (WIDE) {
+    static_cast<float *>(sums)[(mt * quads + q) * 64 + lane] = (float)(kb == 0 ? sum[0] : kb == 1 ? sum[1] : kb == 2 ? sum[2] : sum[3]);
+  } else if (kb < 2) {
+    const int32_t v0 = kb == 0 ? sum[0] : sum[2], v1 = kb == 0 ? sum[1] : sum[3], h0 = (v0 + 64) & ~127, h1 = (v1 + 64) & ~127;
+    static_cast<uint2 *>(sums)[(mt * quads + q) * 32 + lane] = make_uint2(cvt_pk_bf16((float)h0, (float)h1), cvt_pk_bf16((float)(v0 - h0), (float)(v1 - h1)));
+  }
 }
 
 // copy_to_lds with scalars that are the whole wave's, taken back out of the vector registers where the compiler holds them there
@@ -64,30 +74,32 @@ __device__ __forceinline__ void copy_scalars_to_lds(i32x4_t rsrc, uint32_t voff,
 // of a column (a window of 8 groups, or 4 of float32) at a time: a few bytes of each column a stage would be 128 lines of 128 bytes (205 us for 4096 x 4096 x 4096, 4-bit, groups of 64;
 // 149 in windows).  Codes: 64 or 128 bytes of a weight row a stage, its 16-byte pieces in an order turned by the row, so that the lanes' reads meet all banks.
 // A group is one matrix instruction a 16 x 16 tile (two for 128 values, one of half the depth for 32), whose integer sums are exact; then a subtraction and a
-// multiply-add a result.  What bounds it is those, a matrix unit and a vector unit that do not run at once (kWhole).  The biases' terms are a product over
-// the groups by the float32 matrix instructions, four groups a time.
+// multiply-add a result.  What bounds it is those, a matrix unit and a vector unit that do not run at once (kWhole): 4096 x 4096 x 4096, 4-bit, groups of 64, 144 us with the rows' preparation
+// (956 TFLOP/s), groups of 128 1320 TFLOP/s, 32 730.  The biases' terms are a product over the groups as well, eight of them a bf16 instruction: the sums in two exact values, their factors
+// b + 8 s (b + 128 s) in two that leave 2^-18 of the factor, 2^-9 of the result's own rounding to bf16.  (Four groups of float32 a float32 instruction are 32 cycles for 16: 149, 1290 and 670;
+// with float32 scales, whose results keep 24 bits, they remain.)
 template <int DT, int BITS, int GROUP, int MI, int NI, int WM, int WN, int KS, int NB>
 struct Rows8Tile {
   static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves * KS, ROWS = 16 * MI * WM, COLS = 16 * NI * WN;
   static constexpr int CODES = 128 * BITS / 8, PIECES = CODES / 16;                     // bytes and 16-byte pieces of a weight row's stage
-  static constexpr int GS = 128 / GROUP, PERIOD = GROUP / 32;                           // groups of a stage; stages of four groups
+  static constexpr int GS = 128 / GROUP;                                                // groups of a stage
   static constexpr int WINDOW = 16 / (DT == 2 ? 4 : 2), WSTAGES = WINDOW / GS;          // groups and stages of a window
   static constexpr int LW = WSTAGES > KS ? WSTAGES / KS : 1, NW = (NB - 2) / LW + 2;    // a group of waves' own stages in a window; windows in LDS
-  static constexpr int A = ROWS * 128, B = COLS * CODES, SUMS = ROWS * 16, STAGE = A + B + SUMS, SCALES = COLS * 32;
-  static constexpr int SHARE = NB * STAGE + NW * SCALES;                                // of LDS, a group of waves'
+  static constexpr int A = ROWS * 128, B = COLS * CODES, STAGE = A + B, SCALES = COLS * 32, SUMS = ROWS * WINDOW * 4;
+  static constexpr int SHARE = NB * STAGE + NW * (SCALES + SUMS);                       // of LDS, a group of waves'
   static constexpr int MEET = (KS - 1) * ROWS * COLS * 4;                               // where the groups meet, in the same place
   static constexpr int LDS = KS * SHARE > MEET ? KS * SHARE : MEET;
-  static constexpr int A_COPIES = ROWS / 8, B_COPIES = B / 1024, W_COPIES = COLS / 32, S_COPIES = ROWS / 64;
-  static constexpr int COPIES = (A_COPIES + B_COPIES) / kWaves;                         // of a wave and stage, but for windows and sums
+  static constexpr int A_COPIES = ROWS / 8, B_COPIES = B / 1024, W_COPIES = COLS / 32, S_COPIES = SUMS / 1024;
+  static constexpr int COPIES = (A_COPIES + B_COPIES) / kWaves;                         // of a wave and stage, but for windows
   static_assert(A_COPIES % kWaves == 0 && B_COPIES % kWaves == 0 && W_COPIES + S_COPIES <= kWaves && ROWS % 64 == 0);
   static_assert(NB >= 2 && (NW - 1) * LW >= NB - 1 && LDS <= 160 * 1024);
 };
 
 template <int DT, int BITS, int GROUP, int MI, int NI, int WM, int WN, int KS, int NB, int OCC>
-__global__ __launch_bounds__(64 * WM * WN * KS, OCC) void rows8_tiles_kernel(Rows8Args a, const uint4 *tiles, const float *sums, int n_mtiles, int n_ntiles) {
+__global__ __launch_bounds__(64 * WM * WN * KS, OCC) void rows8_tiles_kernel(Rows8Args a, const uint4 *tiles, const char *sums, int n_mtiles, int n_ntiles) {
   using L = Rows8Tile<DT, BITS, GROUP, MI, NI, WM, WN, KS, NB>;
   using T = Value<DT>;
-  constexpr int kWaves = L::kWaves, COLS = L::COLS, CODES = L::CODES, PIECES = L::PIECES, GS = L::GS, PERIOD = L::PERIOD, STAGE = L::STAGE;
+  constexpr int kWaves = L::kWaves, COLS = L::COLS, CODES = L::CODES, PIECES = L::PIECES, GS = L::GS, STAGE = L::STAGE;
   extern __shared__ __align__(16) unsigned char lds_raw[];
   const int xcd = blockIdx.x & 7, j = blockIdx.x >> 3, nt = j / n_mtiles * 8 + xcd;  // an XCD takes every eighth column tile and all row tiles of it
   if (nt >= n_ntiles) return;
@@ -95,19 +107,19 @@ __global__ __launch_bounds__(64 * WM * WN * KS, OCC) void rows8_tiles_kernel(Row
   const int n0 = nt * COLS;
   const int lane = lane_id(), ln = lane & 15, kb = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), share = wave / kWaves, wv = wave % kWaves, wm = wv / WN, wn = wv % WN;
-  const int K = a.K, n_stages = K / 128, G = K / GROUP, quads = (G + 3) / 4, row_bytes = K * BITS / 8, s_row = G * (int)sizeof(T);
+  const int K = a.K, n_stages = K / 128, G = K / GROUP, sums_row = rows8_quads(G) * 256, row_bytes = K * BITS / 8, s_row = G * (int)sizeof(T);
   const uint32_t my_lds = share * L::SHARE, my_scales = my_lds + NB * STAGE;
   auto clip = [](int64_t v) { return (uint32_t)(v < INT32_MAX ? v : INT32_MAX); };
   const int64_t cols_left = a.N - n0, tiles_left = mt_all - mt0;  // (what a descriptor ends behind is zeros)
   const i32x4_t xr = words_of(reinterpret_cast<const char *>(tiles) + mt0 * K * 16, clip(tiles_left * K * 16));
-  const i32x4_t qr = words_of(reinterpret_cast<const char *>(sums) + mt0 * quads * 256, clip(tiles_left * quads * 256));
+  const i32x4_t qr = words_of(sums + mt0 * sums_row, clip(tiles_left * sums_row));
   const i32x4_t wr = words_of(reinterpret_cast<const char *>(a.w) + (int64_t)n0 * row_bytes, clip(cols_left * row_bytes));
   const i32x4_t sr = words_of(static_cast<const char *>(a.s) + (int64_t)n0 * s_row, clip(cols_left * s_row));
   const i32x4_t br = words_of(static_cast<const char *>(a.b) + (int64_t)n0 * s_row, clip(cols_left * s_row));
   auto turn = [](int row) { return PIECES == 4 ? (row >> 2) & 3 : (row >> 1) & 7; };
-  // the stage at which the four groups of q are multiplied with the biases: each of the groups of waves has its turn
+  // the stage at which the groups of the window q are multiplied with the biases: each of the groups of waves has its turn
   auto owner = [&](int q) {
-    const int t = q * PERIOD + q % (PERIOD < KS ? PERIOD : KS);
+    const int t = q * L::WSTAGES + q % (L::WSTAGES < KS ? L::WSTAGES : KS);
     return t < n_stages ? t : n_stages - 1;
   };
   auto copy_stage = [&](int u) __attribute__((always_inline)) {  // this share's u-th
@@ -123,15 +135,20 @@ __global__ __launch_bounds__(64 * WM * WN * KS, OCC) void rows8_tiles_kernel(Row
       const int i = c * kWaves + wv, row = i * (64 / PIECES) + lane / PIECES;
       copy_scalars_to_lds(wr, row * row_bytes + ((lane % PIECES) ^ turn(row)) * 16, t * CODES, to + L::A + i * 1024);
     }
-    if (u % L::LW == 0 && wv < L::W_COPIES) {
-      const bool second = wv >= L::W_COPIES / 2;
-      const int i = second ? wv - L::W_COPIES / 2 : wv;
-      const uint32_t place = my_scales + (uint32_t)(u / L::LW % L::NW) * L::SCALES + wv * 1024;
-      if (second) copy_scalars_to_lds(br, (i * 64 + lane) * s_row, t / L::WSTAGES * 16, place);
-      else copy_scalars_to_lds(sr, (i * 64 + lane) * s_row, t / L::WSTAGES * 16, place);
+    if (u % L::LW == 0) {
+      const int q = t / L::WSTAGES;
+      const uint32_t place = my_scales + (uint32_t)(u / L::LW % L::NW) * (L::SCALES + L::SUMS);
+      if (wv < L::W_COPIES) {
+        const bool second = wv >= L::W_COPIES / 2;
+        const int i = second ? wv - L::W_COPIES / 2 : wv;
+        if (second) copy_scalars_to_lds(br, (i * 64 + lane) * s_row, q * 16, place + wv * 1024);
+        else copy_scalars_to_lds(sr, (i * 64 + lane) * s_row, q * 16, place + wv * 1024);
+      }
+      if (const int i = kWaves - 1 - wv; i < L::S_COPIES && (KS == 1 || owner(q) % KS == share)) {
+        constexpr int LANES = L::WINDOW * 4;  // of a tile of sums
+        copy_scalars_to_lds(qr, (i * (64 / LANES) + lane / LANES) * sums_row + lane % LANES * 16, q * L::WINDOW * 64, place + L::SCALES + i * 1024);
+      }
     }
-    if (const int i = kWaves - 1 - wv; i < L::S_COPIES && t == owner(t / PERIOD))
-      copy_scalars_to_lds(qr, (i * 4 + kb) * (quads * 256) + ln * 16, t / PERIOD * 256, to + L::A + L::B + i * 1024);
   };
   f32x4_t acc[MI][NI];
 #pragma unroll
@@ -154,7 +171,7 @@ __global__ __launch_bounds__(64 * WM * WN * KS, OCC) void rows8_tiles_kernel(Row
     if (KS > 1 && u >= mine) break;  // (the last stage, for some of the shares)
     const int t = u * KS + share;
     const unsigned char *const at = lds_raw + my_lds + u % NB * STAGE;
-    const unsigned char *const scales = lds_raw + my_scales + u / L::LW % L::NW * L::SCALES + (wn * NI * 16 + ln) * 16;  // this lane's columns: every 16th
+    const unsigned char *const scales = lds_raw + my_scales + u / L::LW % L::NW * (L::SCALES + L::SUMS) + (wn * NI * 16 + ln) * 16;  // this lane's columns: every 16th
     struct Half {  // the operands of 64 values
       i32x4_t x[MI], w[NI];
       uint2 lo[NI], hi[NI];
@@ -197,16 +214,42 @@ __global__ __launch_bounds__(64 * WM * WN * KS, OCC) void rows8_tiles_kernel(Row
 #pragma unroll
       for (int g = 0; g < GS; ++g) s[n][g] = as_f32(v[g]);
     }
-    if (const int q = t / PERIOD; t == owner(q)) {
-      const int g = (q * 4 + kb < G ? q * 4 + kb : G - 1) % L::WINDOW * (int)sizeof(T);  // (past the last group the sums are zeros)
+    if (const int q = t / L::WSTAGES; t == owner(q)) {
+      constexpr float k = Centre<BITS>::of_codes;
+      const unsigned char *const my_sums = lds_raw + my_scales + u / L::LW % L::NW * (L::SCALES + L::SUMS) + L::SCALES + wm * MI * L::WINDOW * 64;
+      if constexpr (DT == 2) {
+        const int g = (q * 4 + kb < G ? kb : G - 1 - q * 4) * 4;  // (past the last group the sums are zeros)
 #pragma unroll
-      for (int n = 0; n < NI; ++n) {
-        constexpr float k = Centre<BITS>::of_codes;
-        const float beta = __builtin_fmaf(k * Centre<BITS>::value, as_f32(*reinterpret_cast<const T *>(scales + n * 256 + g)),
-                                          k * as_f32(*reinterpret_cast<const T *>(scales + COLS * 16 + n * 256 + g)));
+        for (int n = 0; n < NI; ++n) {
+          const float beta = __builtin_fmaf(k * Centre<BITS>::value, *reinterpret_cast<const float *>(scales + n * 256 + g),
+                                            k * *reinterpret_cast<const float *>(scales + COLS * 16 + n * 256 + g));
 #pragma unroll
-        for (int m = 0; m < MI; ++m)
-          acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(*reinterpret_cast<const float *>(at + L::A + L::B + (wm * MI + m) * 256 + lane * 4), beta, acc[m][n], 0, 0, 0);
+          for (int m = 0; m < MI; ++m)
+            acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(*reinterpret_cast<const float *>(my_sums + m * 256 + lane * 4), beta, acc[m][n], 0, 0, 0);
+        }
+      } else {
+        const bool there = q * 8 + 2 * kb < G;  // (an even number of groups)
+        i32x4_t sum[MI];
+#pragma unroll
+        for (int m = 0; m < MI; ++m) {
+          const uint2 v = *reinterpret_cast<const uint2 *>(my_sums + m * 512 + lane * 8);
+          sum[m] = i32x4_t{(int32_t)v.x, (int32_t)v.y, (int32_t)v.x, (int32_t)v.y};
+        }
+#pragma unroll
+        for (int n = 0; n < NI; ++n) {
+          T sv[2], bv[2];
+          __builtin_memcpy(sv, __builtin_assume_aligned(scales + n * 256 + 4 * kb, 4), 4);
+          __builtin_memcpy(bv, __builtin_assume_aligned(scales + COLS * 16 + n * 256 + 4 * kb, 4), 4);
+          float beta[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) beta[i] = there ? __builtin_fmaf(k * Centre<BITS>::value, as_f32(sv[i]), k * as_f32(bv[i])) : 0.f;
+          const uint32_t first = cvt_pk_bf16(beta[0], beta[1]);
+          const uint32_t rest = cvt_pk_bf16(beta[0] - __uint_as_float(first << 16), beta[1] - __uint_as_float(first & 0xffff0000u));
+          const i32x4_t b4 = {(int32_t)first, (int32_t)first, (int32_t)rest, (int32_t)rest};
+#pragma unroll
+          for (int m = 0; m < MI; ++m)
+            acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, sum[m]), __builtin_bit_cast(bf16x8_t, b4), acc[m][n], 0, 0, 0);
+        }
       }
     }
     // The tiles one after the other, each multiplied LEAD steps before its sums are scaled: written out in the order in which it is to run (the compiler's own
@@ -285,7 +328,7 @@ __global__ __launch_bounds__(64 * WM * WN * KS, OCC) void rows8_tiles_kernel(Row
 }
 
 template <int DT, int BITS, int GROUP, int MI, int NI, int WM, int WN, int KS, int NB, int OCC>
-static hipError_t start_tile(const Rows8Args &a, const uint4 *tiles, const float *sums, hipStream_t st) {
+static hipError_t start_tile(const Rows8Args &a, const uint4 *tiles, const char *sums, hipStream_t st) {
   using L = Rows8Tile<DT, BITS, GROUP, MI, NI, WM, WN, KS, NB>;
   const int64_t n_mtiles = (a.M + L::ROWS - 1) / L::ROWS, n_ntiles = (a.N + L::COLS - 1) / L::COLS, grid = (n_ntiles + 7) / 8 * 8 * n_mtiles;
   if (grid * L::kThreads >= (int64_t)1 << 32) return hipErrorInvalidValue;
@@ -300,12 +343,12 @@ size_t rows8_tiles_workspace_bytes(int64_t M, int K) { return rows8_tiles_bytes(
 
 hipError_t launch_rows8_tiles(const Rows8Args &a, Rows8Kind kind, int bits, int dt, void *workspace, hipStream_t st) {
   uint4 *const tiles = static_cast<uint4 *>(workspace);
-  float *const sums = reinterpret_cast<float *>(static_cast<char *>(workspace) + rows8_tiles_bytes(a.M, a.K));
-  const int64_t units = row_tiles(a.M) * ((a.K / a.group + 3) / 4);
+  char *const sums = static_cast<char *>(workspace) + rows8_tiles_bytes(a.M, a.K);
+  const int64_t units = row_tiles(a.M) * rows8_quads(a.K / a.group);
   if (units >= (int64_t)1 << 25) return hipErrorInvalidValue;  // (a launch has less than 2^32 threads)
   return rows8_with_types(dt, bits, a.group, [&](auto d, auto b, auto g) {
     constexpr int DT = decltype(d)::value, BITS = decltype(b)::value, GROUP = decltype(g)::value;
-    rows8_prepare_kernel<BITS, GROUP><<<(unsigned)((units + 3) / 4), 256, 0, st>>>(a.x, a.M, a.K, tiles, sums);
+    rows8_prepare_kernel<BITS, GROUP, DT == 2><<<(unsigned)((units + 3) / 4), 256, 0, st>>>(a.x, a.M, a.K, tiles, sums);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     if (kind == Rows8Kind::kTiles64x64) return start_tile<DT, BITS, GROUP, 2, 2, 2, 2, 2, 2, 4>(a, tiles, sums, st);
     if (kind == Rows8Kind::kTiles64x128) return start_tile<DT, BITS, GROUP, 2, 2, 2, 4, 1, 2, 4>(a, tiles, sums, st);

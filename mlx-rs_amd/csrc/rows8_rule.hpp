@@ -15,14 +15,13 @@ struct Rows8Cost {
   // us = start + first K / 4096 + (x - 1) (more K / 4096 + more0), x: blocks of the fullest XCD a CU, at least one
   float start, first, more, more0;
 };
-// Fitted to 110 products (16 to 2048 rows, 1024 to 14336 columns, K = 1024, 2048 and 4096; groups of 64 with 4- and 8-bit codes, of 32 and 128 with 4-bit ones): what the rule takes is 0.7 %
-// slower than the fastest kind on average, 16 % at most.  The times that
-// they stand for, us, 4-bit, K = 4096, in the order of the kinds:
-//   16 x 4096     8.4, 9.0, 12.4, 14.6                      64 x 14336    76, 53, 47, 37, 23.7, 34.3, 46.6
-//   32 x 4096     13.8, 10.6, 14.1, 16.4, 20.6, 31, 42      256 x 4096    87, 59, 46, 36.6, 24.1, 34.6, 47
-//   64 x 4096     24.4, 17.6, 14.5, 19.3, 21.3, 32, 45      512 x 4096    171, 115, 87, 68, 34.1, 37.7, 49.3
-//   128 x 4096    45.4, 31.6, 25.4, 19.9, 22.4, 33, 46      1024 x 4096   337, 226, 171, 134, 58.0, 51.8, 53.9
-//   16 x 14336    25.0, 27.2, 23.0, 28.1                    2048 x 4096   671, 447, 338, 265, 112, 93.3, 83.3
+// Fitted to 110 products (16 to 2048 rows, 1024 to 14336 columns, K = 1024, 2048 and 4096; groups of 64 with 4- and 8-bit codes, of 32 and 128 with 4-bit ones): what the rule takes is 0.5 %
+// slower than the fastest kind on average, 22 % at most.  The times, us, 4-bit, groups of 64, K = 4096, in the order of the kinds:
+//   16 x 4096     8.4, 9.0, 12.4, 14.6                      64 x 14336    76, 53, 47, 37, 22.3, 31.6, 43.6
+//   32 x 4096     13.8, 10.6, 14.1, 16.4, 19.8, 30, 40      256 x 4096    87, 59, 46, 36.6, 23.1, 32.3, 43
+//   64 x 4096     24.4, 17.6, 14.5, 19.3, 20.6, 30, 42      512 x 4096    170, 115, 87, 68, 31.8, 35.6, 46.3
+//   128 x 4096    45.4, 31.6, 25.4, 19.9, 21.3, 31, 42      1024 x 4096   337, 226, 171, 134, 54.8, 48.6, 49.6
+//   16 x 14336    25.0, 27.2, 23.0, 28.1                    2048 x 4096   671, 447, 338, 264, 106, 88.6, 79.5
 constexpr Rows8Cost kRows8Costs[] = {
     {16, 16, false, 3.3f, 5.1f, 6.2f, 0.1f},   {32, 16, false, 3.4f, 6.6f, 7.0f, 0.3f},    {32, 32, false, 3.5f, 10.5f, 11.5f, 1.5f}, {64, 32, false, 4.1f, 15.2f, 15.0f, 2.6f},
     {64, 64, true, 8.7f, 14.5f, 10.3f, 1.7f},  {64, 128, true, 8.5f, 27.5f, 15.0f, 2.0f},  {128, 128, true, 10.5f, 43.0f, 28.0f, 2.0f},

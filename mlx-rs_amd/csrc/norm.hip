@@ -14,6 +14,11 @@
 
 namespace mi_moe {
 
+template <int CTRL>
+__device__ __forceinline__ double dpp_of(double v) { return dpp_f64<CTRL>(v); }
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_of(uint32_t v) { return dpp_u32<CTRL>(v); }
+
 __device__ __forceinline__ double wave_max_f64(double v) {
   v = fmax(v, dpp_f64<kDppXor1>(v));
   v = fmax(v, dpp_f64<kDppXor2>(v));
@@ -66,6 +71,7 @@ __device__ __forceinline__ void store_octet(void *base, int64_t at, int n, const
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (i < n) p[i] = o.v[i];
+    asm volatile("");  // (else the compiler makes one short store of the first value and of the last ones of both branches, and three of the other)
   }
 }
 
@@ -76,22 +82,44 @@ __device__ __forceinline__ float rstd_of(double ss, int H, float eps) {
   return (float)(1.0 / sqrt(m + (double)eps));
 }
 
-// the codes of an octet in eight bits; most: the row's largest |w h|, inv = 127 / most
+// the integer nearest to 127 p / most, ties to even, of a quotient that is within 2^-13 of the half m: by the sign of 127 p - m most, whose products are taken with their rounding errors
+__device__ __forceinline__ float beside_half(float m, double p, double most) {
+  const double a = 127.0 * p, b = (double)m * most, d = (a - b) + (__builtin_fma(127.0, p, -a) - __builtin_fma((double)m, most, -b));
+  return d > 0.0 ? m + 0.5f : d < 0.0 ? m - 0.5f : rintf(m);
+}
+// the codes of an octet in eight bits; most: the row's largest |w h|
 template <int DT>
 __device__ __forceinline__ void put_codes(unsigned char *to, int n, const Octet<DT> &h, const Octet<DT> &w, double most) {
   // rows of zeros have a scale and codes of zero; rows that hold an infinity or no number a scale that is none, so that what is made of them is none either
-  const bool none = !(most > 0.0 && most < INFINITY), wide = !(most > 1e-30 && most < 1e30);
-  const float inv = none ? 0.f : (float)(127.0 / most);
   uint32_t q[2] = {0, 0};
+  if (most > 0.0 && most < INFINITY) {
+    constexpr float kWhole = 12582912.f;  // 1.5 * 2^23: added to a small float, its low bits are the nearest integer, ties to even
+    float v[8], off = 0.f;
+    if (most > 1e-30 && most < 1e30) {
+      const float inv = 127.f * __builtin_amdgcn_rcpf((float)most);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float v = h.at(i) * w.at(i) * inv;
-    float k = rintf(v);
-    // the float quotient is up to 2^-15 off (three roundings of a value below 128): where that could change the integer, or the products leave
-    // the floats' range, the exact products decide
-    if (none) k = 0.f;
-    else if (wide || fabsf(v - k) > 0.4999f) k = (float)rint(127.0 * ((double)h.at(i) * (double)w.at(i)) / most);
-    q[i / 4] |= ((uint32_t)(int)k & 0xffu) << (8 * (i % 4));
+      for (int i = 0; i < 8; ++i) v[i] = h.at(i) * w.at(i) * inv;
+    } else {  // products outside the floats' range
+      const double inv = 127.0 / most;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = (float)((double)h.at(i) * (double)w.at(i) * inv);
+    }
+    uint32_t k[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float t = v[i] + kWhole;
+      off = fmaxf(off, fabsf(v[i] - (t - kWhole)));
+      k[i] = __float_as_uint(t);
+    }
+    // the float quotient is up to 2^-14 off (2^-21.4 of a value below 128: a reciprocal to 2^-23 and five roundings): where that could change an integer, the exact products decide
+    if (off > 0.4999f) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (fabsf(v[i] - rintf(v[i])) > 0.4999f) k[i] = __float_as_uint(kWhole + beside_half(rintf(2.f * v[i]) * 0.5f, (double)h.at(i) * (double)w.at(i), most));
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      q[j] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(k[4 * j + 3], k[4 * j + 2], 0x0c0c0400u), __builtin_amdgcn_perm(k[4 * j + 1], k[4 * j], 0x0c0c0400u), 0x05040100u);
   }
   if (n >= 8) __builtin_memcpy(to, q, 8);
   else
@@ -112,15 +140,40 @@ __device__ __forceinline__ double largest(double most, const Octet<DT> &h, const
   }
   return finite ? most : INFINITY;
 }
-// a block's sums and largest values, in the order of its waves
-template <int WAVES>
-__device__ __forceinline__ void meet(double (&part)[WAVES][2], double &sum, double &other, bool is_sum) {
-  if ((threadIdx.x & (kWave - 1)) == 0) part[threadIdx.x / kWave % WAVES][0] = sum, part[threadIdx.x / kWave % WAVES][1] = other;
-  __syncthreads();
-  sum = 0.0;
-  other = 0.0;
+// The same as the bits of a float where the products are exact floats or nearly so (16-bit types): what is infinite or no number comes out above everything.  Good for a row
+// whose result is a normal float well above the smallest; others (products beyond the floats' range, or below) are gone over in double.
+template <int DT>
+__device__ __forceinline__ uint32_t largest_bits(uint32_t most, const Octet<DT> &h, const Octet<DT> &w) {
 #pragma unroll
-  for (int i = 0; i < WAVES; ++i) sum += part[i][0], other = is_sum ? other + part[i][1] : fmax(other, part[i][1]);
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t p = __float_as_uint(h.at(i) * w.at(i)) & 0x7fffffffu;
+    most = p > most ? p : most;
+  }
+  return most;
+}
+__device__ __forceinline__ bool in_floats(uint32_t bits) { return bits - 0x12800000u < 0x7f800000u - 0x12800000u; }  // 2^-90 and more
+
+// f over the values of WAVES (up to 16) lanes that follow each other, in all of them and in one order
+template <int WAVES, class T, class F>
+__device__ __forceinline__ T join_waves(T v, F f) {
+  if constexpr (WAVES > 1) v = f(v, dpp_of<kDppXor1>(v));
+  if constexpr (WAVES > 2) v = f(v, dpp_of<kDppXor2>(v));
+  if constexpr (WAVES > 4) v = f(v, dpp_of<kDppHalfMirror>(v));
+  if constexpr (WAVES > 8) v = f(v, dpp_of<kDppMirror>(v));
+  return v;
+}
+// a block's sums and largest values from its waves': a lane reads one wave's (all of them in each lane are 64 registers for 16 waves, and what was in those in scratch memory)
+template <int WAVES, bool BOTH = true>
+__device__ __forceinline__ void meet(double (&part)[WAVES][2], double &sum, double &other, bool is_sum) {  // BOTH: `other` too
+  static_assert((WAVES & (WAVES - 1)) == 0 && WAVES <= 16);
+  if ((threadIdx.x & (kWave - 1)) == 0) {
+    part[threadIdx.x / kWave % WAVES][0] = sum;
+    if constexpr (BOTH) part[threadIdx.x / kWave % WAVES][1] = other;
+  }
+  __syncthreads();
+  const int i = threadIdx.x & (WAVES - 1);
+  sum = join_waves<WAVES>(part[i][0], [](double u, double v) { return u + v; });
+  if constexpr (BOTH) other = join_waves<WAVES>(part[i][1], [&](double u, double v) { return is_sum ? u + v : fmax(u, v); });
 }
 
 struct NormArgs {
@@ -132,59 +185,68 @@ struct NormArgs {
   float *scales;
 };
 
-// A row goes to TPR threads (a wave and more), CH octets each, and stays in their registers between its sums and its results: memory is passed once.
-template <int DT, int TPR, int CH, bool ROWS8>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void add_rms_norm_kernel(NormArgs a) {
-  constexpr int kRows = TPR < 256 ? 256 / TPR : 1, kWaves = TPR / kWave;
+// A row goes to TPR threads, an octet each, and stays in their registers between its sums and its results: memory is passed once, which is what bounds it.  One octet rather than two or
+// four: fewer registers, more waves with loads under way.  us, one octet a thread / two (of 8192 values: four), with a residual, values that are read and written each once:
+//   300 x 1024 3.5 / 4.2   16384 x 1024 23.0 / 27.7   777 x 4096 6.8 / 7.9   8192 x 4096 40.5 / 46.0 (6.6 TB/s)   2048 x 8192 22.9 / 30.1   8192 x 8192 93.7 / 119   (bf16)
+//   rows in eight bits: 16384 x 1024 25.6 / 26.5   8192 x 4096 43.5 / 43.8   2048 x 8192 25.5 / 33.8   8192 x 8192 91.7 / 138
+template <int DT, int TPR, bool ROWS8>
+__global__ __launch_bounds__(TPR == kWave ? 256 : TPR, ROWS8 && DT == 1 ? 4 : 8) void add_rms_norm_kernel(NormArgs a) {
+  constexpr int kRows = TPR == kWave ? 4 : 1, kWaves = TPR / kWave;
+  constexpr bool BITS = ROWS8 && DT != 2;  // the largest |w h| as a float's bits
   __shared__ double part[kWaves][2];
+  __shared__ uint32_t part_bits[BITS ? kWaves : 1];
   const int t = threadIdx.x % TPR;
   const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR;
   if (kWaves == 1 && row >= a.T) return;  // (rows of several waves have a block each: none is outside)
-  const int64_t at = row * a.H;
-  Octet<DT> h[CH];
-#pragma unroll
-  for (int c = 0; c < CH; ++c) h[c] = load_octet<DT>(a.x, at + (c * TPR + t) * 8, a.H - (c * TPR + t) * 8);
+  const int64_t at = row * a.H + t * 8;
+  const int n = a.H - t * 8;
+  Octet<DT> h, r, w;
+  if (n >= 8) {  // (all loads under way at once: one branch around them)
+    h = load_octet<DT>(a.x, at, 8);
+    w = load_octet<DT>(a.w, t * 8, 8);
+    if (a.r) r = load_octet<DT>(a.r, at, 8);
+  } else {
+    h = load_octet<DT>(a.x, at, n);
+    w = load_octet<DT>(a.w, t * 8, n);
+    if (a.r) r = load_octet<DT>(a.r, at, n);
+  }
   if (a.r) {
-    Octet<DT> r[CH];
 #pragma unroll
-    for (int c = 0; c < CH; ++c) r[c] = load_octet<DT>(a.r, at + (c * TPR + t) * 8, a.H - (c * TPR + t) * 8);
-#pragma unroll
-    for (int c = 0; c < CH; ++c)
-#pragma unroll
-      for (int i = 0; i < 8; i += 2) h[c].put2(i, h[c].at(i) + r[c].at(i), h[c].at(i + 1) + r[c].at(i + 1));
+    for (int i = 0; i < 8; i += 2) h.put2(i, h.at(i) + r.at(i), h.at(i + 1) + r.at(i + 1));
   }
+  if (a.sum) store_octet<DT>(a.sum, at, n, h);
   double ss = 0.0, most = 0.0;  // most: the largest |w h|; infinite where one of them is infinite or no number
-  if (a.sum) {
 #pragma unroll
-    for (int c = 0; c < CH; ++c) store_octet<DT>(a.sum, at + (c * TPR + t) * 8, a.H - (c * TPR + t) * 8, h[c]);
-  }
-#pragma unroll
-  for (int c = 0; c < CH; ++c)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) ss = __builtin_fma((double)h[c].at(i), (double)h[c].at(i), ss);
-  Octet<DT> w[CH];
-#pragma unroll
-  for (int c = 0; c < CH; ++c) w[c] = load_octet<DT>(a.w, (c * TPR + t) * 8, a.H - (c * TPR + t) * 8);
-  if constexpr (ROWS8) {
-#pragma unroll
-    for (int c = 0; c < CH; ++c) most = largest<DT>(most, h[c], w[c]);
+  for (int i = 0; i < 8; ++i) ss = __builtin_fma((double)h.at(i), (double)h.at(i), ss);
+  uint32_t bits = 0;
+  if constexpr (BITS) {
+    bits = wave_max_u32(largest_bits<DT>(0, h, w));
+    if (kWaves > 1 && (threadIdx.x & (kWave - 1)) == 0) part_bits[threadIdx.x / kWave] = bits;
+  } else if constexpr (ROWS8) {
+    most = wave_max_f64(largest<DT>(0.0, h, w));
   }
   ss = wave_sum_f64(ss);
-  if constexpr (ROWS8) most = wave_max_f64(most);
-  if constexpr (kWaves > 1) meet<kWaves>(part, ss, most, false);
+  if constexpr (kWaves > 1) meet<kWaves, ROWS8 && !BITS>(part, ss, most, false);
+  if constexpr (BITS) {
+    if constexpr (kWaves > 1) bits = join_waves<kWaves>(part_bits[threadIdx.x & (kWaves - 1)], [](uint32_t u, uint32_t v) { return u > v ? u : v; });
+    most = (double)__uint_as_float(bits);
+    if (!in_floats(bits)) {  // (the same in all of the row's threads)
+      most = wave_max_f64(largest<DT>(0.0, h, w));
+      double none = 0.0;
+      if constexpr (kWaves > 1) {
+        __syncthreads();
+        meet<kWaves>(part, none, most, false);
+      }
+    }
+  }
   const float rstd = rstd_of(ss, a.H, a.eps);
   if constexpr (!ROWS8) {
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-#pragma unroll
-      for (int i = 0; i < 8; i += 2) h[c].put2(i, w[c].at(i) * (h[c].at(i) * rstd), w[c].at(i + 1) * (h[c].at(i + 1) * rstd));
-      store_octet<DT>(a.y, at + (c * TPR + t) * 8, a.H - (c * TPR + t) * 8, h[c]);
-    }
+    for (int i = 0; i < 8; i += 2) h.put2(i, w.at(i) * (h.at(i) * rstd), w.at(i + 1) * (h.at(i + 1) * rstd));
+    store_octet<DT>(a.y, at, n, h);
   } else {
     if (t == 0) a.scales[row] = scale_of(most, rstd);
-#pragma unroll
-    for (int c = 0; c < CH; ++c)
-      put_codes<DT>(static_cast<unsigned char *>(a.y) + at + (c * TPR + t) * 8, a.H - (c * TPR + t) * 8, h[c], w[c], most);
+    put_codes<DT>(static_cast<unsigned char *>(a.y) + at, n, h, w, most);
   }
 }
 
@@ -235,12 +297,12 @@ static hipError_t start_norm_long(const NormArgs &a, bool rows8, hipStream_t st)
   return hipGetLastError();
 }
 
-template <int DT, int TPR, int CH>
+template <int DT, int TPR>
 static hipError_t start_norm(const NormArgs &a, bool rows8, hipStream_t st) {
-  constexpr int block = TPR < 256 ? 256 : TPR, rows = block / TPR;
+  constexpr int block = TPR == kWave ? 256 : TPR, rows = block / TPR;
   const unsigned grid = (unsigned)((a.T + rows - 1) / rows);
-  if (rows8) add_rms_norm_kernel<DT, TPR, CH, true><<<grid, block, 0, st>>>(a);
-  else add_rms_norm_kernel<DT, TPR, CH, false><<<grid, block, 0, st>>>(a);
+  if (rows8) add_rms_norm_kernel<DT, TPR, true><<<grid, block, 0, st>>>(a);
+  else add_rms_norm_kernel<DT, TPR, false><<<grid, block, 0, st>>>(a);
   return hipGetLastError();
 }
 
@@ -270,11 +332,11 @@ hipError_t launch_add_rms_norm(const void *x, const void *r, const void *w, floa
   const NormArgs a{x, r, w, eps, T, H, sum, y, scales};
   return with_dtype(dt, [&](auto d) {
     constexpr int DT = decltype(d)::value;
-    if (H <= 512) return start_norm<DT, 64, 1>(a, rows8, st);
-    if (H <= 1024) return start_norm<DT, 64, 2>(a, rows8, st);
-    if (H <= 2048) return start_norm<DT, 256, 1>(a, rows8, st);
-    if (H <= 4096) return start_norm<DT, 256, 2>(a, rows8, st);
-    if (H <= 8192) return start_norm<DT, 256, 4>(a, rows8, st);
+    if (H <= 512) return start_norm<DT, 64>(a, rows8, st);
+    if (H <= 1024) return start_norm<DT, 128>(a, rows8, st);
+    if (H <= 2048) return start_norm<DT, 256>(a, rows8, st);
+    if (H <= 4096) return start_norm<DT, 512>(a, rows8, st);
+    if (H <= 8192) return start_norm<DT, 1024>(a, rows8, st);
     return start_norm_long<DT>(a, rows8, st);
   });
 }
@@ -310,10 +372,16 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR, 4) void norm_grad_kernel(Nor
     struct { Octet<DT> h[CH], dy[CH], dh[CH]; } R;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const int j = (c * TPR + t) * 8;
-      R.h[c] = load_octet<DT>(a.h, row * a.H + j, a.H - j);
-      R.dy[c] = load_octet<DT>(a.dy, row * a.H + j, a.H - j);
-      if (a.dh) R.dh[c] = load_octet<DT>(a.dh, row * a.H + j, a.H - j);
+      const int j = (c * TPR + t) * 8, n = a.H - j;
+      if (n >= 8) {
+        R.h[c] = load_octet<DT>(a.h, row * a.H + j, 8);
+        R.dy[c] = load_octet<DT>(a.dy, row * a.H + j, 8);
+        if (a.dh) R.dh[c] = load_octet<DT>(a.dh, row * a.H + j, 8);
+      } else {
+        R.h[c] = load_octet<DT>(a.h, row * a.H + j, n);
+        R.dy[c] = load_octet<DT>(a.dy, row * a.H + j, n);
+        if (a.dh) R.dh[c] = load_octet<DT>(a.dh, row * a.H + j, n);
+      }
     }
     double ss = 0.0, dot = 0.0;  // sums of h^2 and of w dy h
 #pragma unroll

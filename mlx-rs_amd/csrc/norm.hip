@@ -351,8 +351,9 @@ struct NormGradArgs {
   float *parts;  // [blocks, H]: every block's sums over its rows
 };
 
-// A block has every blocks-th row (rows of up to 1024 values: a wave each, four at a time), the next one's loads under way while it works on one, and its columns' sums for dw in
-// registers; the sums of the blocks meet in a second launch, in a fixed order.  Bound by memory: what the forward pass reads and writes, and the blocks' sums twice.
+// A block has every blocks-th row (rows of up to 1024 values: a wave each, four at a time) and its columns' sums for dw in registers; the sums of the blocks meet in a second launch, in a
+// fixed order.  4096 x 4096, bf16, with the gradient along the residual: 31.8 us, 134 MB at 4.2 TB/s; bound by memory (those, and the blocks' sums written and read, 17 MB) and by the latency of
+// a row, whose loads, sums and barrier follow each other in a block.
 template <int DT, int TPR, int CH>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR, 4) void norm_grad_kernel(NormGradArgs a) {
   constexpr int kRows = TPR < 256 ? 256 / TPR : 1, kWaves = TPR / kWave;
@@ -513,8 +514,8 @@ __global__ __launch_bounds__(1024) void norm_grad_weight_kernel(const float *par
 }
 
 // Blocks of the backward pass: what the chip holds at once (of 1024 threads one a CU), and rows enough for each that its sums for dw are little beside them.  us, bf16, 256 / 512 / 768 / 1024
-// blocks: 1000 x 2048 12.0, 12.8, 15.0, 18.0; 4096 x 4096 42.8, 37.5, 41.0, 41.8; 16384 x 1024 51.3, 36.0, 29.8, 32.1; float32 2048 x 8192 51.5, 62.8, 72.3, 82.7.  (The next row's loads
-// ahead of a row's sums cost registers, and with them waves: 46.3, 39.1, 44.0, 45.7 for 4096 x 4096.)
+// blocks: 1000 x 2048 11.3, 12.4, 15.1, 17.7; 4096 x 4096 34.0, 31.8, 35.9, 38.8; 16384 x 1024 34.0, 27.9, 28.4, 28.5; float32 2048 x 8192 51.5, 61.7, 70.4, 79.2.  (The next row's loads
+// ahead of a row's sums cost registers, and with them waves: 46.3, 39.1, 44.0, 45.7 where 4096 x 4096 took 42.8, 37.5, 41.0, 41.8; so does holding 64 registers, for twice the waves: 48.)
 static int norm_grad_blocks(int64_t T, int H) {
   const int64_t rows = H <= 1024 ? (T + 3) / 4 : T, most = H <= 1024 ? 768 : H <= 4096 ? 512 : 256;
   const int64_t few = rows / 5 > 256 ? rows / 5 : 256, blocks = few < most ? few : most;

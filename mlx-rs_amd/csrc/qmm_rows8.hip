@@ -71,10 +71,125 @@ static hipError_t start_plain(const Rows8Args &a, hipStream_t st) {
   return a.M == 1 ? start(std::integral_constant<int, 1>{}) : start(std::integral_constant<int, 8>{});
 }
 
+// ---------------------------------------------------------------- up to four rows
+__device__ __forceinline__ float wave_sum_in_order(float v) {
+  v += __uint_as_float(dpp_u32<kDppXor1>(__float_as_uint(v)));
+  v += __uint_as_float(dpp_u32<kDppXor2>(__float_as_uint(v)));
+  v += __uint_as_float(dpp_u32<kDppHalfMirror>(__float_as_uint(v)));
+  v += __uint_as_float(dpp_u32<kDppMirror>(__float_as_uint(v)));
+  auto row = [&](int lane) { return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), lane)); };
+  return (row(0) + row(16)) + (row(32) + row(48));
+}
+
+// A wave has two columns; a lane 16 bytes of each column's codes at a time, of one group, which it multiplies four at a time (v_dot4) and scales once; whole lines are loaded and nothing
+// is loaded twice.  What bounds it is memory, for a few thousand columns the latency of a wave's loads.  us, 4-bit, groups of 64, K = 4096 (the matrix instructions below: 6.9, 19.7, 20.3, 7.5, 21.1):
+//   1 x 4096 3.9, 1 x 14336 6.7 (4.9 TB/s), 4 x 14336 12.2, 8 rows would be 8.5 and 22.2; one column a wave 4.0, 7.7, 15.9, four 3.9, 6.8, 12.4 and more registers.
+template <int DT, int BITS, int GROUP, int ROWS>
+__global__ __launch_bounds__(256) void rows8_dot_kernel(Rows8Args a) {
+  using T = Value<DT>;
+  constexpr int COLS = 2, CODES = 128 / BITS, WORDS = CODES / 4;  // a lane's codes of a step, and the words of as many rows' values
+  const int lane = lane_id(), pieces = a.K / CODES, G = a.K / GROUP;
+  const int64_t n0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * COLS;
+  if (n0 >= a.N) return;
+  const uint4 *wp[COLS];
+  const T *sp[COLS], *bp[COLS];
+#pragma unroll
+  for (int c = 0; c < COLS; ++c) {  // columns outside: the last one again, not stored
+    const int64_t n = n0 + c < a.N ? n0 + c : a.N - 1;
+    wp[c] = reinterpret_cast<const uint4 *>(a.w) + n * pieces;
+    sp[c] = static_cast<const T *>(a.s) + n * G;
+    bp[c] = static_cast<const T *>(a.b) + n * G;
+  }
+  struct Step {
+    uint4 w[COLS];
+    T s[COLS], b[COLS];
+    uint4 x[ROWS][WORDS / 4];
+  };
+  auto load = [&](int p, Step &S) __attribute__((always_inline)) {
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) {
+      S.w[c] = wp[c][p];
+      S.s[c] = sp[c][p * CODES / GROUP];
+      S.b[c] = bp[c][p * CODES / GROUP];
+    }
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+      for (int i = 0; i < WORDS / 4; ++i) S.x[r][i] = reinterpret_cast<const uint4 *>(a.x + (r < a.M ? r : a.M - 1) * a.K)[p * (WORDS / 4) + i];
+  };
+  float acc[ROWS][COLS] = {};
+  Step next;
+  if (lane < pieces) load(lane, next);
+#pragma unroll 1
+  for (int p = lane; p < pieces; p += kWave) {
+    const Step S = next;
+    if (p + kWave < pieces) load(p + kWave, next);
+    int32_t x[ROWS][WORDS], sum[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      sum[r] = 0;
+#pragma unroll
+      for (int i = 0; i < WORDS / 4; ++i) {
+        const uint4 v = S.x[r][i];
+        const uint2 lo = BITS == 4 ? evens_odds(make_uint2(v.x, v.y)) : make_uint2(v.x, v.y), hi = BITS == 4 ? evens_odds(make_uint2(v.z, v.w)) : make_uint2(v.z, v.w);
+        x[r][4 * i] = (int32_t)lo.x, x[r][4 * i + 1] = (int32_t)lo.y, x[r][4 * i + 2] = (int32_t)hi.x, x[r][4 * i + 3] = (int32_t)hi.y;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum[r] = byte_sum((uint32_t)x[r][4 * i + k], sum[r]);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) {
+      constexpr float k = Centre<BITS>::of_codes;
+      const float s = as_f32(S.s[c]), beta = __builtin_fmaf(k * Centre<BITS>::value, s, k * as_f32(S.b[c]));
+      int32_t w[WORDS];
+      if constexpr (BITS == 4) {
+        const i32x4_t lo = operand_of<4>(make_uint2(S.w[c].x, S.w[c].y), make_uint2(0, 0)), hi = operand_of<4>(make_uint2(S.w[c].z, S.w[c].w), make_uint2(0, 0));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = lo[j], w[4 + j] = hi[j];
+      } else {
+        const i32x4_t v = operand_of<8>(make_uint2(S.w[c].x, S.w[c].y), make_uint2(S.w[c].z, S.w[c].w));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = v[j];
+      }
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        int32_t d = 0;
+#pragma unroll
+        for (int j = 0; j < WORDS; ++j) d = __builtin_amdgcn_sdot4(x[r][j], w[j], d, false);
+        acc[r][c] = __builtin_fmaf(s, (float)d, __builtin_fmaf(beta, (float)sum[r], acc[r][c]));
+      }
+    }
+  }
+  float mine = 0.f;  // lane r COLS + c: that result
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) {
+      const float v = wave_sum_in_order(acc[r][c]);
+      if (lane == r * COLS + c) mine = v;
+    }
+  const int r = lane / COLS;
+  const int64_t col = n0 + lane % COLS;
+  if (r >= ROWS || r >= a.M || col >= a.N) return;
+  mine *= a.row_scales[r] / Centre<BITS>::of_codes;
+  if (a.bias) mine += as_f32(static_cast<const T *>(a.bias)[col]);
+  static_cast<T *>(a.y)[r * a.N + col] = value_of<DT>(mine);
+}
+
+template <int DT, int BITS, int GROUP, int ROWS>
+static hipError_t start_dot(const Rows8Args &a, hipStream_t st) {
+  const int64_t grid = ((int64_t)a.N + 7) / 8;
+  if (grid >= (int64_t)1 << 24) return hipErrorInvalidValue;  // (a launch has less than 2^32 threads)
+  rows8_dot_kernel<DT, BITS, GROUP, ROWS><<<(unsigned)grid, 256, 0, st>>>(a);
+  return hipGetLastError();
+}
+
 // ---------------------------------------------------------------- few rows
 // A block multiplies 16 MI rows by 16 NI columns; its eight waves share K, every eighth stage of 128 values each, and meet in LDS in a fixed order.  Nothing is prepared: a wave
 // loads its codes, scales and rows straight into registers (a stage ahead), unpacks the codes in the rows' own order, and forms the group sums beside the products
-// (a lane's part of them is an operand of the biases' product as it is).  What bounds it is the latency of the loads, all of which are under way at once.
+// (a lane's part of them is an operand of the biases' product as it is).  What bounds it is the L1 cache's tags: the 16 rows of an operand are 16 lanes that follow each other, 8 bytes of 16 lines
+// each, 48 accesses a load on average (1 x 14336, 4096 values: 32000 accesses a CU in 46000 cycles).  Whole lines through LDS instead, passed to the lanes there: 10.1 us for 8.1 (16 x 4096),
+// 32.3 for 21.9 (16 x 14336).
 template <int DT, int BITS, int GROUP, int MI, int NI>
 __global__ __launch_bounds__(512, MI * NI <= 4 ? 4 : 2) void rows8_few_kernel(Rows8Args a, int wide) {
   using T = Value<DT>;
@@ -271,6 +386,12 @@ hipError_t launch_qmm_rows8(const Rows8Args &a, int bits, int dt, void *workspac
   }
   if (!rows8_even(a)) {
     return rows8_with_types(dt, bits, a.group, [&](auto d, auto b, auto) { return start_plain<decltype(d)::value, decltype(b)::value>(a, st); });
+  }
+  if (a.M <= kRows8Dot) {
+    return rows8_with_types(dt, bits, a.group, [&](auto d, auto b, auto g) {
+      constexpr int DT = decltype(d)::value, BITS = decltype(b)::value, GROUP = decltype(g)::value;
+      return a.M == 1 ? start_dot<DT, BITS, GROUP, 1>(a, st) : a.M == 2 ? start_dot<DT, BITS, GROUP, 2>(a, st) : start_dot<DT, BITS, GROUP, 4>(a, st);
+    });
   }
   const bool words = a.K / a.group * (dt == 2 ? 4 : 2) % 4 == 0;  // (groups of 128, 16-bit scales: an odd number of them starts half of the columns off a word)
   const bool tiles = words && workspace && (reinterpret_cast<uintptr_t>(workspace) & 15u) == 0 && workspace_bytes >= rows8_workspace_bytes(a.M, a.K);

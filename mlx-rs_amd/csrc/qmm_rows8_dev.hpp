@@ -54,6 +54,11 @@ __device__ __forceinline__ i32x4_t operand_of(uint2 lo, uint2 hi) {  // 8-bit: 1
   }
 }
 
+// eight bytes in their order to the even ones, then the odd ones
+__device__ __forceinline__ uint2 evens_odds(uint2 v) {
+  return make_uint2(__builtin_amdgcn_perm(v.y, v.x, 0x06040200u), __builtin_amdgcn_perm(v.y, v.x, 0x07050301u));
+}
+
 template <class F>
 inline hipError_t rows8_with_types(int dt, int bits, int group, F f) {  // f(type, bits, group), each a compile-time constant
   auto with_group = [&](auto d, auto b) {

@@ -18,11 +18,6 @@ constexpr size_t rows8_sums_bytes(int64_t M, int K, int group) { return (size_t)
 
 __host__ __device__ constexpr int rows8_quads(int G) { return (G + 7) / 8 * 2; }  // fours of groups, in whole eights
 
-// eight bytes in their order to the even ones, then the odd ones
-__device__ __forceinline__ uint2 evens_odds(uint2 v) {
-  return make_uint2(__builtin_amdgcn_perm(v.y, v.x, 0x06040200u), __builtin_amdgcn_perm(v.y, v.x, 0x07050301u));
-}
-
 // A wave makes the tiles of 16 rows and four groups.
 template <int BITS, int GROUP, bool WIDE>
 __global__ __launch_bounds__(256) void rows8_prepare_kernel(const signed char *x, int64_t M, int K, uint4 *tiles, void *sums) {  // WIDE: float32 scales

@@ -32,7 +32,8 @@ constexpr float rows8_time(const Rows8Cost &c, int64_t M, int N, int K) {
   const float x = blocks > 256.f ? blocks / 256.f : 1.f;
   return c.start + c.first * k + (x - 1.f) * (c.more * k + c.more0);
 }
-constexpr int kRows8NoTiles = 16;  // rows that no number of columns brings to the tiles
+constexpr int kRows8Dot = 4;       // rows that take no matrix instructions at all
+constexpr int kRows8NoTiles = 16;   // rows that no number of columns brings to the tiles
 // tiles: there is a workspace, and the columns' scales start where copies can
 constexpr Rows8Kind rows8_kind(int64_t M, int N, int K, bool tiles) {
   int best = 0;

@@ -155,6 +155,16 @@ def test_shapes_of_rows_and_no_rows():
     assert m.ops.quantized_linear_rows8(x[:0], sx[:0], w, s, b).shape == (0, 32)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bits,group", [(4, 32), (4, 64), (4, 128), (8, 32), (8, 64), (8, 128)])
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 5])
+def test_one_to_five_rows(M, bits, group, dtype):
+    """K of less than a wave's step and more, whole steps and not; one column, an odd number, more than a block's."""
+    for N, K in ((1, 128), (7, 256), (8, 2048), (33, 1920), (1001, 4096), (300, 8320)):
+        args = layer(M, N, K, bits, group, dtype, bias=N % 2 == 1)
+        check(run(args, group, bits), args, group, bits)
+
+
 @pytest.mark.parametrize("M,N,K,step", [(8192 + 70, 2 ** 20, 128, 8192), (2 ** 16 * 8 + 70, 512, 32, 2 ** 16 * 8)])
 def test_more_rows_than_a_launch_takes(M, N, K, step):
     """Rows on both sides of where a launch ends, results past 2^32 elements: the bits of a call of their own rows."""

@@ -66,9 +66,10 @@ int mi_moe_forward_routed(mi_moe_handle h, const uint16_t *x, const uint32_t *to
 
 /* ---- The linear layer on rows in eight bits (mi_moe_add_rms_norm_rows8 makes such rows): y = (row_scales x) . dequantize(w)^T + linear_bias, each result
  * rounded once.  x: signed bytes [M, K]; row_scales: f32 [M]; w [N, K*bits/32]; scales, biases [N, K/group_size], linear_bias [N]
- * (or NULL) and y [M, N] of element type dtype.  bits 4 or 8; group_size 32, 64 or 128; K a multiple of group_size.  Sums over a group are exact integers.
- * The fast kernels want K a multiple of 128, x and w 16-byte aligned and
- * workspace >= mi_moe_quantized_linear_rows8_workspace_size (16-byte aligned); without these the plain kernel runs. ---- */
+ * (or NULL) and y [M, N] of element type dtype.  bits 4 or 8; group_size 32, 64 or 128; K a multiple of group_size.  Products of rows and codes are summed exactly, as integers,
+ * over runs of a group; with many rows and 16-bit scales the factor of a group's sum of x (biases + the codes' centre times scales) keeps 2^-18 of its value.
+ * The fast kernels want K a multiple of 128 and x, w, scales and biases 16-byte aligned; those for many rows an even number of 16-bit scales a column and
+ * workspace >= mi_moe_quantized_linear_rows8_workspace_size (16-byte aligned; 0 for up to 16 rows), too.  Without these, slower kernels give the same product. ---- */
 int mi_moe_quantized_linear_rows8_workspace_size(int64_t M, int32_t K, size_t *bytes);
 int mi_moe_quantized_linear_rows8(const void *x, const float *row_scales, const uint32_t *w,
                                   const void *scales, const void *biases, const void *linear_bias,

@@ -351,13 +351,15 @@ struct NormGradArgs {
   float *parts;  // [blocks, H]: every block's sums over its rows
 };
 
-// A block has every blocks-th row (rows of up to 1024 values: a wave each, four at a time) and its columns' sums for dw in registers; the sums of the blocks meet in a second launch, in a
-// fixed order.  4096 x 4096, bf16, with the gradient along the residual: 31.8 us, 134 MB at 4.2 TB/s; bound by memory (those, and the blocks' sums written and read, 17 MB) and by the latency of
-// a row, whose loads, sums and barrier follow each other in a block.
-template <int DT, int TPR, int CH>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR, 4) void norm_grad_kernel(NormGradArgs a) {
-  constexpr int kRows = TPR < 256 ? 256 / TPR : 1, kWaves = TPR / kWave;
-  __shared__ double part[2][kWaves][2];
+constexpr int norm_grad_threads(int tpr, bool together) { return tpr == kWave ? 256 : together ? 1024 : tpr; }
+
+// A block has every blocks-th run of kRows rows (of up to 1024 values: a wave each) and their columns' sums for dw in registers; the sums of the blocks meet in a second launch, in a
+// fixed order.  4096 x 4096, bf16, with the gradient along the residual: 32.4 us, 134 MB at 4.1 TB/s; bound by memory (those, and the blocks' sums written and read, 8 MB) and by the latency of
+// a row, whose loads, sums and barrier follow each other.
+template <int DT, int TPR, int CH, bool TOGETHER>
+__global__ __launch_bounds__(norm_grad_threads(TPR, TOGETHER), 4) void norm_grad_kernel(NormGradArgs a) {
+  constexpr int kRows = norm_grad_threads(TPR, TOGETHER) / TPR, kWaves = TPR / kWave;
+  __shared__ double part[2][kRows][kWaves][2];
   const int t = threadIdx.x % TPR, which = threadIdx.x / TPR;
   const int64_t step = (int64_t)gridDim.x * kRows;
   Octet<DT> w[CH];
@@ -368,8 +370,10 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR, 4) void norm_grad_kernel(Nor
 #pragma unroll
     for (int i = 0; i < 8; ++i) dw[c][i] = 0.f;
   }
-  int64_t row = (int64_t)blockIdx.x * kRows + which;
-  for (int turn = 0; row < a.T; row += step, turn ^= 1) {  // (rows of several waves: the same for all of the block's)
+  int turn = 0;
+  for (int64_t base = (int64_t)blockIdx.x * kRows; base < a.T; base += step, turn ^= 1) {  // (the same turns for all of a block's)
+    const int64_t row = base + which < a.T ? base + which : a.T - 1;
+    const bool mine = base + which < a.T;  // (else the last row again, without a result)
     struct { Octet<DT> h[CH], dy[CH], dh[CH]; } R;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
@@ -396,7 +400,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR, 4) void norm_grad_kernel(Nor
       }
     ss = wave_sum_f64(ss);
     dot = wave_sum_f64(dot);
-    if constexpr (kWaves > 1) meet<kWaves>(part[turn], ss, dot, true);  // (one barrier a row: the next row's sums go to the other half)
+    if constexpr (kWaves > 1) meet<kWaves>(part[turn][which], ss, dot, true);  // (one barrier a row: the next row's sums go to the other half)
     const float rstd = rstd_of(ss, a.H, a.eps);
     const float mean = (float)(dot * (double)rstd / (double)a.H);
 #pragma unroll
@@ -408,13 +412,13 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR, 4) void norm_grad_kernel(Nor
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const float hat = R.h[c].at(i + k) * rstd, g = R.dy[c].at(i + k);
-          dw[c][i + k] = __builtin_fmaf(g, hat, dw[c][i + k]);
+          if (mine) dw[c][i + k] = __builtin_fmaf(g, hat, dw[c][i + k]);
           d[k] = rstd * __builtin_fmaf(-hat, mean, w[c].at(i + k) * g);
           if (a.dh) d[k] += R.dh[c].at(i + k);
         }
         R.h[c].put2(i, d[0], d[1]);
       }
-      store_octet<DT>(a.dx, row * a.H + j, a.H - j, R.h[c]);
+      if (mine) store_octet<DT>(a.dx, row * a.H + j, a.H - j, R.h[c]);
     }
   }
   float *const to = a.parts + (int64_t)blockIdx.x * a.H;
@@ -513,19 +517,25 @@ __global__ __launch_bounds__(1024) void norm_grad_weight_kernel(const float *par
   }
 }
 
-// Blocks of the backward pass: what the chip holds at once (of 1024 threads one a CU), and rows enough for each that its sums for dw are little beside them.  us, bf16, 256 / 512 / 768 / 1024
-// blocks: 1000 x 2048 11.3, 12.4, 15.1, 17.7; 4096 x 4096 34.0, 31.8, 35.9, 38.8; 16384 x 1024 34.0, 27.9, 28.4, 28.5; float32 2048 x 8192 51.5, 61.7, 70.4, 79.2.  (The next row's loads
-// ahead of a row's sums cost registers, and with them waves: 46.3, 39.1, 44.0, 45.7 where 4096 x 4096 took 42.8, 37.5, 41.0, 41.8; so does holding 64 registers, for twice the waves: 48.)
+// Rows of a block of 1024 threads are worked on at once, as many as it holds, where there are more rows than CUs: their sums for dw meet in LDS, and half or a quarter as many blocks' sums go through
+// memory.  us, together / a block a row and more blocks: 1000 x 2048 10.9 / 11.3, 1000 x 2045 12.0 / 13.1, 300 x 4096 10.9 / 12.1, 8192 x 4096 53.2 / 53.1; 32 x 2048 7.7 / 6.4.
+static bool norm_grad_together(int64_t T) { return T > 256; }
+// Blocks of the backward pass: one a CU, of rows up to 1024 values what the chip holds at once and rows enough for each that its sums for dw are little beside them.  us, bf16, 256 / 512 / 768 / 1024
+// blocks of 256 threads: 16384 x 1024 34.0, 27.9, 28.4, 28.5.  (The next row's loads ahead of a row's sums cost registers, and with them waves: 39.1 where 4096 x 4096 took 37.5; so does holding
+// 64 registers, for twice the waves: 48 for 32.)
 static int norm_grad_blocks(int64_t T, int H) {
-  const int64_t rows = H <= 1024 ? (T + 3) / 4 : T, most = H <= 1024 ? 768 : H <= 4096 ? 512 : 256;
-  const int64_t few = rows / 5 > 256 ? rows / 5 : 256, blocks = few < most ? few : most;
+  const int64_t each = H <= 1024 ? 4 : !norm_grad_together(T) ? 1 : H <= 2048 ? 4 : H <= 4096 ? 2 : 1, rows = (T + each - 1) / each;  // (turns of a block)
+  const int64_t few = rows / 5 > 256 ? rows / 5 : 256, most = H <= 1024 ? 768 : 256, blocks = few < most ? few : most;
   return (int)(rows < blocks ? rows : blocks);
 }
-size_t norm_grad_bytes(int64_t T, int H) { return (size_t)norm_grad_blocks(T, H) * H * sizeof(float); }
+// (of no fewer rows less: what a batch has reserved is enough for every smaller one)
+size_t norm_grad_bytes(int64_t T, int H) { return (size_t)(H > 1024 ? (T < 256 ? T : 256) : norm_grad_blocks(T, H)) * H * sizeof(float); }
 
 template <int DT, int TPR, int CH>
 static hipError_t start_norm_grad(const NormGradArgs &a, int blocks, hipStream_t st) {
-  norm_grad_kernel<DT, TPR, CH><<<(unsigned)blocks, TPR < 256 ? 256 : TPR, 0, st>>>(a);
+  constexpr bool able = TPR > kWave && TPR < 1024;
+  if (able && norm_grad_together(a.T)) norm_grad_kernel<DT, TPR, CH, able><<<(unsigned)blocks, norm_grad_threads(TPR, able), 0, st>>>(a);
+  else norm_grad_kernel<DT, TPR, CH, false><<<(unsigned)blocks, norm_grad_threads(TPR, false), 0, st>>>(a);
   return hipGetLastError();
 }
 

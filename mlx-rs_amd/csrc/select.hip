@@ -146,10 +146,11 @@ __device__ __forceinline__ void select_exact(const SelectKernelArgs &p, const Sl
   }
 }
 
-// The keys and the groups' ranks in float where that decides them: float scores are within kNear / 4 of the exact ones (exp and reciprocal to 2^-22 of their values, an
-// exponent off by 2^-24 of itself, of scores of one at most, a sum to 2^-22), biased keys within 2^-24 of their size more.  Where two keys that follow each other in the choice, or two groups' ranks, are nearer than
-// that allows, or something is an infinity above zero or no number, the token goes through select_exact (one in some hundred); without a bias the logits are exact keys.  Scores of the chosen
-// are in double, a lane each, of softmax scores that are renormalised from the chosen logits alone: they hold where a softmax over all would round to zero.
+// The keys and the groups' ranks in float where that decides them.  A float score is off by 2^-22 of itself for the exponential, 2^-23 for the reciprocal and, of a softmax, 14 * 2^-24 for
+// the sum, which is the same factor for all of a token's; scores are at most one, so two of them differ by what doubles say to within 1.9 * 2^-20, and biased keys to within 2^-23 of their size more.
+// Where two keys that follow each other in the choice, or two groups' ranks, are nearer than kNear and kNearOfSize of them allow, or something is an infinity above zero or no number, doubles decide
+// (for one token in some hundred); without a bias the logits are exact keys.  Scores of the chosen are in double, a lane each, of softmax scores that are renormalised from the chosen logits
+// alone: they hold where a softmax over all would round to zero.
 constexpr float kNear = 0x1p-19f, kNearOfSize = 0x1p-21f;
 
 // the key's part that a bias is, minus infinity for an expert that is masked, and whether floats can decide
@@ -218,13 +219,13 @@ __global__ __launch_bounds__(256) void select_experts_kernel(SelectKernelArgs p)
   if constexpr (KEYS) {
     float s[S];
     if (a.scoring == 0) {
-      float sum = 0.f;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < S; ++j) {
         s[j] = __expf(x.l[j] - most);
-        sum += s[j];
+        sum[j % 4] += s[j];
       }
-      const float inv = __builtin_amdgcn_rcpf((float)wave_sum_f64((double)sum));
+      const float inv = __builtin_amdgcn_rcpf((float)wave_sum_f64((double)(sum[0] + sum[1]) + (double)(sum[2] + sum[3])));
 #pragma unroll
       for (int j = 0; j < S; ++j) s[j] *= inv;
     } else {
@@ -440,13 +441,13 @@ __global__ __launch_bounds__(256) void select_rows_kernel(SelectKernelArgs p, Se
   if constexpr (KEYS) {
     if (a.bias || a.group_score == 1) {
       if (a.scoring == 0) {
-        float sum = 0.f;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};  // (of up to eight, so that no addend goes through more than 14 roundings)
 #pragma unroll
         for (int j = 0; j < S; ++j) {
           y[j] = __expf(l[j] - most);
-          sum += y[j];
+          sum[j % 4] += y[j];
         }
-        const float inv = __builtin_amdgcn_rcpf(row_join(sum, [](float u, float v) { return u + v; }));
+        const float inv = __builtin_amdgcn_rcpf(row_join((sum[0] + sum[1]) + (sum[2] + sum[3]), [](float u, float v) { return u + v; }));
 #pragma unroll
         for (int j = 0; j < S; ++j) y[j] = __builtin_fmaf(y[j], inv, b[j]);
       } else {

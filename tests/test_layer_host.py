@@ -128,3 +128,17 @@ def test_python_refuses_host_tensors():
                  lambda: m.ops.quantized_linear_rows8(x.to(torch.int8), torch.ones(2), torch.zeros(2, 1, dtype=torch.int32), w, w)):
         with pytest.raises(m.MoeError, match="device tensor"):
             call()
+
+
+@pytest.mark.parametrize("hidden", [1, 512, 1000, 1025, 2048, 4096, 8192, 32768])
+def test_a_workspace_is_enough_for_every_smaller_batch(lib, hidden):
+    def sizes(fn, rows):
+        need = C.c_size_t()
+        for t in rows:
+            assert getattr(lib, fn)(t, hidden, C.byref(need)) == 0
+            yield need.value
+
+    rows = list(range(0, 1400)) + [4096, 5000, 16384, 100000, 1 << 24]
+    for fn in ("mi_moe_add_rms_norm_grad_workspace_size", "mi_moe_quantized_linear_rows8_workspace_size"):
+        got = list(sizes(fn, rows))
+        assert got == sorted(got), fn

@@ -36,4 +36,4 @@ def test_tiles_only_with_a_workspace_and_enough_rows(kind):
 
 def test_the_gpu_tests_reach_every_kind(kind):
     import test_gpu_rows8 as t
-    assert {kind(*s) for s in t.SHAPES + t.TILED} == set(KINDS)
+    assert {kind(*s) for s in t.SHAPES + t.TILED if s[0] > 4} == set(KINDS)  # (up to four rows take no kind at all)

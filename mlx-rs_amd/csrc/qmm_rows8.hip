@@ -71,7 +71,7 @@ static hipError_t start_plain(const Rows8Args &a, hipStream_t st) {
   return a.M == 1 ? start(std::integral_constant<int, 1>{}) : start(std::integral_constant<int, 8>{});
 }
 
-// ---------------------------------------------------------------- up to four rows
+// ---------------------------------------------------------------- one row, two rows
 __device__ __forceinline__ float wave_sum_in_order(float v) {
   v += __uint_as_float(dpp_u32<kDppXor1>(__float_as_uint(v)));
   v += __uint_as_float(dpp_u32<kDppXor2>(__float_as_uint(v)));
@@ -82,8 +82,8 @@ __device__ __forceinline__ float wave_sum_in_order(float v) {
 }
 
 // A wave has two columns; a lane 16 bytes of each column's codes at a time, of one group, which it multiplies four at a time (v_dot4) and scales once; whole lines are loaded and nothing
-// is loaded twice.  What bounds it is memory, for a few thousand columns the latency of a wave's loads.  us, 4-bit, groups of 64, K = 4096 (the matrix instructions below: 6.9, 19.7, 20.3, 7.5, 21.1):
-//   1 x 4096 3.9, 1 x 14336 6.7 (4.9 TB/s), 4 x 14336 12.2, 8 rows would be 8.5 and 22.2; one column a wave 4.0, 7.7, 15.9, four 3.9, 6.8, 12.4 and more registers.
+// is loaded twice.  What bounds it is memory, for a few thousand columns the latency of a wave's loads.  us, 4-bit, groups of 64, K = 4096 (the matrix instructions below for five rows: 5.4, 11.6):
+//   1 x 4096 3.9, 1 x 14336 6.7 (4.9 TB/s), 2 rows 4.7 and 8.7; four would be 5.9 and 12.2; one column a wave 4.0 and 7.7 (one row), four 3.9 and 6.8 and more registers.
 template <int DT, int BITS, int GROUP, int ROWS>
 __global__ __launch_bounds__(256) void rows8_dot_kernel(Rows8Args a) {
   using T = Value<DT>;
@@ -185,78 +185,84 @@ static hipError_t start_dot(const Rows8Args &a, hipStream_t st) {
 }
 
 // ---------------------------------------------------------------- few rows
-// A block multiplies 16 MI rows by 16 NI columns; its eight waves share K, every eighth stage of 128 values each, and meet in LDS in a fixed order.  Nothing is prepared: a wave
+// A block multiplies 16 MI rows by 16 NI columns; its eight waves share K, a run of stages of 128 values each, and meet in LDS in a fixed order.  Nothing is prepared: a wave
 // loads its codes, scales and rows straight into registers (a stage ahead), unpacks the codes in the rows' own order, and forms the group sums beside the products
-// (a lane's part of them is an operand of the biases' product as it is).  What bounds it is the L1 cache's tags: the 16 rows of an operand are 16 lanes that follow each other, 8 bytes of 16 lines
-// each, 48 accesses a load on average (1 x 14336, 4096 values: 32000 accesses a CU in 46000 cycles).  Whole lines through LDS instead, passed to the lanes there: 10.1 us for 8.1 (16 x 4096),
-// 32.3 for 21.9 (16 x 14336).
+// (a lane's part of them is an operand of the biases' product as it is).
+// What bounds it is the L1 cache's tags: an operand's 16 rows are 16 lanes that follow each other, so a load is 64 accesses whatever its width.  So every load is 16 bytes a lane, also where a lane's
+// values are then not those that one product of a group wants of it, and scales come for several stages at once.  us, 4-bit, groups of 64, before (8 bytes of codes and a stage's scales a load) / so:
+//   8 x 4096, 4096 values 7.5 / 5.4   16 x 14336 21.9 / 12.7   32 x 4096 10.2 / 7.7   64 x 4096 14.3 / 11.0   128 x 4096 19.4 / 16.6   16 x 14336, groups of 32 35 / 16.3
+// (Whole lines through LDS, passed to the lanes there: 10.1 for 16 x 4096, 32 for 16 x 14336.)
 template <int DT, int BITS, int GROUP, int MI, int NI>
-__global__ __launch_bounds__(512, MI * NI <= 4 ? 4 : 2) void rows8_few_kernel(Rows8Args a, int wide) {
+__global__ __launch_bounds__(512, MI * NI < 4 && !(DT == 2 && NI == 2) ? 4 : 2) void rows8_few_kernel(Rows8Args a, int wide) {
   using T = Value<DT>;
   constexpr int kWaves = 8, GS = 128 / GROUP, ROWS = 16 * MI, COLS = 16 * NI;
+  constexpr int WSTAGES = GROUP == 32 ? 2 : 4, WINDOW = WSTAGES * GS;  // stages and groups whose scales are loaded at once
   __shared__ float parts[kWaves][ROWS][COLS];
   const int n0 = (int)(blockIdx.x % (uint32_t)wide) * COLS;
   const int64_t m0 = (int64_t)(blockIdx.x / (uint32_t)wide) * ROWS;
   const int lane = lane_id(), ln = lane & 15, kb = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int K = a.K, n_stages = K / 128, G = K / GROUP;
+  // A lane loads 16 bytes: of 4-bit codes 32 values that follow each other (and 32 of a row), both products' of a stage; of 8-bit codes 16, one product's.  They are of one group; where the other
+  // lanes' are of other groups (APART), a group's product takes zeros for the rows' values there.
+  constexpr bool PAIR = BITS == 4;
+  auto group_of = [&](int h) { return (PAIR ? kb * 32 : h * 64 + kb * 16) / GROUP; };
+  constexpr bool APART = PAIR ? GROUP < 128 : GROUP < 64;
+  const int K = a.K, n_stages = K / 128, G = K / GROUP, each = (n_stages + kWaves - 1) / kWaves;
+  const int first = wave * each, last = first + each < n_stages ? first + each : n_stages;
   const signed char *xp[MI];
 #pragma unroll
   for (int m = 0; m < MI; ++m) {  // rows and columns outside: the last ones again, not stored
     const int64_t row = m0 + 16 * m + ln;
-    xp[m] = a.x + (row < a.M ? row : a.M - 1) * K + (GROUP == 32 ? 8 : 16) * kb;
+    xp[m] = a.x + (row < a.M ? row : a.M - 1) * K + (PAIR ? 32 : 16) * kb;
   }
   const unsigned char *wp[NI];
   const T *sp[NI], *bp[NI];
 #pragma unroll
   for (int n = 0; n < NI; ++n) {
     const int64_t col = n0 + 16 * n + ln < a.N ? n0 + 16 * n + ln : a.N - 1;
-    wp[n] = reinterpret_cast<const unsigned char *>(a.w) + col * (K / 8 * BITS) + (GROUP == 32 ? BITS : 2 * BITS) * kb;
+    wp[n] = reinterpret_cast<const unsigned char *>(a.w) + col * (K / 8 * BITS) + 16 * kb;
     sp[n] = static_cast<const T *>(a.s) + col * G;
     bp[n] = static_cast<const T *>(a.b) + col * G;
   }
   struct Stage {
-    uint2 x[2][MI][2], w[2][NI][2];  // two halves of 64 values, two pieces of 8 of a lane's 16
-    T s[NI][GS], b[NI][GS];
+    uint4 x[2][MI], w[PAIR ? 1 : 2][NI];
+  };
+  constexpr int STEP = GS * (int)sizeof(T), DWORDS = WINDOW * (int)sizeof(T) / 4;  // bytes of a stage, words of a window
+  struct Window {
+    uint32_t s[NI][DWORDS], b[NI][DWORDS];
+  };
+  auto pass = [](uint32_t (&v)[DWORDS]) __attribute__((always_inline)) {  // the next stage's to the front
+#pragma unroll
+    for (int i = 0; i < DWORDS; ++i) {
+      if constexpr (STEP == 2) v[i] = v[i] >> 16 | (i + 1 < DWORDS ? v[i + 1] << 16 : 0u);
+      else if (i + STEP / 4 < DWORDS) v[i] = v[i + STEP / 4];
+    }
   };
   auto load = [&](int t, Stage &S) __attribute__((always_inline)) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int k = t * 128 + h * 64;
+    for (int h = 0; h < (PAIR ? 1 : 2); ++h)
 #pragma unroll
-      for (int n = 0; n < NI; ++n) {
-        const unsigned char *const p = wp[n] + k * BITS / 8;
-        if constexpr (GROUP == 32) {  // 8 codes of either group
-          __builtin_memcpy(&S.w[h][n][0], __builtin_assume_aligned(p, BITS), BITS);
-          __builtin_memcpy(&S.w[h][n][1], __builtin_assume_aligned(p + 4 * BITS, BITS), BITS);
-        } else if constexpr (BITS == 8) {
-          const uint4 v = *reinterpret_cast<const uint4 *>(p);
-          S.w[h][n][0] = make_uint2(v.x, v.y), S.w[h][n][1] = make_uint2(v.z, v.w);
-        } else {
-          const uint2 v = *reinterpret_cast<const uint2 *>(p);
-          S.w[h][n][0].x = v.x, S.w[h][n][1].x = v.y;
-        }
-      }
-    }
-#pragma unroll
-    for (int n = 0; n < NI; ++n) {
-      constexpr int size = GS * sizeof(T);
-      __builtin_memcpy(S.s[n], __builtin_assume_aligned(sp[n] + t * GS, size), size);
-      __builtin_memcpy(S.b[n], __builtin_assume_aligned(bp[n] + t * GS, size), size);
-    }
+      for (int n = 0; n < NI; ++n) S.w[h][n] = *reinterpret_cast<const uint4 *>(wp[n] + (t * 128 + h * 64) * BITS / 8);
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int m = 0; m < MI; ++m) {
-        const signed char *const p = xp[m] + t * 128 + h * 64;
-        if constexpr (GROUP == 32) {
-          S.x[h][m][0] = *reinterpret_cast<const uint2 *>(p);
-          S.x[h][m][1] = *reinterpret_cast<const uint2 *>(p + 32);
-        } else {
-          const uint4 v = *reinterpret_cast<const uint4 *>(p);
-          S.x[h][m][0] = make_uint2(v.x, v.y), S.x[h][m][1] = make_uint2(v.z, v.w);
-        }
+      for (int m = 0; m < MI; ++m) S.x[h][m] = *reinterpret_cast<const uint4 *>(xp[m] + t * 128 + h * (PAIR ? 16 : 64));
+  };
+  auto load_window = [&](int t, Window &V) __attribute__((always_inline)) {
+#pragma unroll
+    for (int n = 0; n < NI; ++n) {
+      if (t + WSTAGES <= n_stages) {
+        __builtin_memcpy(V.s[n], sp[n] + t * GS, sizeof V.s[n]);
+        __builtin_memcpy(V.b[n], bp[n] + t * GS, sizeof V.b[n]);
+      } else {  // what is left of the columns, a stage at a time
+#pragma unroll
+        for (int i = 0; i < WSTAGES; ++i)
+          if (t + i < n_stages) {
+            __builtin_memcpy(reinterpret_cast<char *>(V.s[n]) + i * STEP, sp[n] + (t + i) * GS, STEP);
+            __builtin_memcpy(reinterpret_cast<char *>(V.b[n]) + i * STEP, bp[n] + (t + i) * GS, STEP);
+          }
       }
+    }
   };
   i32x4_t whole = {kWholeBits, kWholeBits, kWholeBits, kWholeBits};
   asm("" : "+v"(whole));
@@ -266,69 +272,88 @@ __global__ __launch_bounds__(512, MI * NI <= 4 ? 4 : 2) void rows8_few_kernel(Ro
 #pragma unroll
     for (int n = 0; n < NI; ++n) acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   Stage next;
-  if (wave < n_stages) load(wave, next);
+  Window scales;
+  if (first < last) {
+    load_window(first, scales);
+    load(first, next);
+  }
 #pragma unroll 1
-  for (int t = wave; t < n_stages; t += kWaves) {
+  for (int t = first; t < last; ++t) {
     const Stage S = next;
-    if (t + kWaves < n_stages) load(t + kWaves, next);
+    if (t + 1 < last) load(t + 1, next);
     float s[NI][GS], beta[NI][GS];
 #pragma unroll
-    for (int n = 0; n < NI; ++n)
+    for (int n = 0; n < NI; ++n) {
+      T sv[GS], bv[GS];
+      __builtin_memcpy(sv, scales.s[n], sizeof sv);
+      __builtin_memcpy(bv, scales.b[n], sizeof bv);
 #pragma unroll
       for (int g = 0; g < GS; ++g) {
         constexpr float k = Centre<BITS>::of_codes;
-        s[n][g] = as_f32(S.s[n][g]);
-        beta[n][g] = __builtin_fmaf(k * Centre<BITS>::value, s[n][g], k * as_f32(S.b[n][g]));
+        s[n][g] = as_f32(sv[g]);
+        beta[n][g] = __builtin_fmaf(k * Centre<BITS>::value, s[n][g], k * as_f32(bv[g]));
       }
+      pass(scales.s[n]);
+      pass(scales.b[n]);
+    }
+    if ((t - first) % WSTAGES == WSTAGES - 1 && t + 1 < last) load_window(t + 1, scales);
     i32x4_t w[2][NI];
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int n = 0; n < NI; ++n) {
-        if constexpr (BITS == 4) {
+    for (int n = 0; n < NI; ++n) {
+      if constexpr (BITS == 4) {
+        auto codes = [](uint32_t u, uint32_t v) {
           int32_t lo[2], hi[2];
-          centred_bytes<4>(S.w[h][n][0].x, lo);
-          centred_bytes<4>(S.w[h][n][1].x, hi);
-          w[h][n] = i32x4_t{lo[0], lo[1], hi[0], hi[1]};
-        } else {
-          w[h][n] = operand_of<8>(S.w[h][n][0], S.w[h][n][1]);
-        }
+          centred_bytes<4>(u, lo);
+          centred_bytes<4>(v, hi);
+          return i32x4_t{lo[0], lo[1], hi[0], hi[1]};
+        };
+        w[0][n] = codes(S.w[0][n].x, S.w[0][n].y);
+        w[1][n] = codes(S.w[0][n].z, S.w[0][n].w);
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) w[h][n] = operand_of<8>(make_uint2(S.w[h][n].x, S.w[h][n].y), make_uint2(S.w[h][n].z, S.w[h][n].w));
       }
+    }
 #pragma unroll
     for (int m = 0; m < MI; ++m) {
       i32x4_t x[2];
-      float sum[GS];
-      int32_t part[4];  // a lane's part of the sums of the four runs of 32 values
+      int32_t sum[2];  // of a lane's values
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        x[h] = i32x4_t{(int32_t)S.x[h][m][0].x, (int32_t)S.x[h][m][0].y, (int32_t)S.x[h][m][1].x, (int32_t)S.x[h][m][1].y};
+        x[h] = __builtin_bit_cast(i32x4_t, S.x[h][m]);
+        sum[h] = 0;
 #pragma unroll
-        for (int p = 0; p < 2; ++p) part[2 * h + p] = byte_sum(S.x[h][m][p].y, byte_sum(S.x[h][m][p].x, 0));
+        for (int p = 0; p < 4; ++p) sum[h] = byte_sum((uint32_t)x[h][p], sum[h]);
       }
-#pragma unroll
-      for (int g = 0; g < GS; ++g) {
-        int32_t v = 0;
-#pragma unroll
-        for (int p = 0; p < 4 / GS; ++p) v += part[g * (4 / GS) + p];
-        sum[g] = (float)v;
-      }
+      constexpr int SUMS = PAIR || GROUP == 128 ? 1 : 2;  // products of sums and biases: one takes what a lane has of one group
+      if constexpr (SUMS == 1) sum[0] += sum[1];
 #pragma unroll
       for (int n = 0; n < NI; ++n)
 #pragma unroll
-        for (int g = 0; g < GS; ++g) {
-          i32x4_t d;
-          if constexpr (GROUP == 32) {
-            const int h = g / 2, p = g % 2;
-            const i32x2_t x2 = {x[h][2 * p], x[h][2 * p + 1]}, w2 = {w[h][n][2 * p], w[h][n][2 * p + 1]};
-            d = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, x2), __builtin_bit_cast(long, w2), whole, 0, 0, 0);
-          } else {
-            d = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[g], w[g][n], whole, 0, 0, 0);
-            if constexpr (GROUP == 128) d = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[1], w[1][n], d, 0, 0, 0);
-          }
-          acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(sum[g], beta[n][g], acc[m][n], 0, 0, 0);
+        for (int h = 0; h < SUMS; ++h) {
+          float mine = beta[n][0];
+#pragma unroll
+          for (int g = 1; g < GS; ++g) mine = group_of(h) == g ? beta[n][g] : mine;
+          acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)sum[h], mine, acc[m][n], 0, 0, 0);
+        }
+#pragma unroll
+      for (int g = 0; g < GS; ++g) {
+        constexpr int PER = PAIR || GROUP == 128 ? 2 : 1;  // products of a group
+        i32x4_t rows[PER];
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+          const int h = PER == 2 ? k : g * GROUP / 64;
+          rows[k] = !APART || group_of(h) == g ? x[h] : i32x4_t{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int n = 0; n < NI; ++n) {
+          i32x4_t d = whole;
+#pragma unroll
+          for (int k = 0; k < PER; ++k) d = __builtin_amdgcn_mfma_i32_16x16x64_i8(rows[k], w[PER == 2 ? k : g * GROUP / 64][n], d, 0, 0, 0);
 #pragma unroll
           for (int i = 0; i < 4; ++i) acc[m][n][i] = __builtin_fmaf(s[n][g], __int_as_float(d[i]) - kWhole, acc[m][n][i]);
         }
+      }
     }
   }
 #pragma unroll
@@ -390,7 +415,7 @@ hipError_t launch_qmm_rows8(const Rows8Args &a, int bits, int dt, void *workspac
   if (a.M <= kRows8Dot) {
     return rows8_with_types(dt, bits, a.group, [&](auto d, auto b, auto g) {
       constexpr int DT = decltype(d)::value, BITS = decltype(b)::value, GROUP = decltype(g)::value;
-      return a.M == 1 ? start_dot<DT, BITS, GROUP, 1>(a, st) : a.M == 2 ? start_dot<DT, BITS, GROUP, 2>(a, st) : start_dot<DT, BITS, GROUP, 4>(a, st);
+      return a.M == 1 ? start_dot<DT, BITS, GROUP, 1>(a, st) : start_dot<DT, BITS, GROUP, 2>(a, st);
     });
   }
   const bool words = a.K / a.group * (dt == 2 ? 4 : 2) % 4 == 0;  // (groups of 128, 16-bit scales: an odd number of them starts half of the columns off a word)
@@ -401,6 +426,7 @@ hipError_t launch_qmm_rows8(const Rows8Args &a, int bits, int dt, void *workspac
     constexpr int DT = decltype(d)::value, BITS = decltype(b)::value, GROUP = decltype(g)::value;
     switch (kind) {
       case Rows8Kind::kFew16x16: return start_few<DT, BITS, GROUP, 1, 1>(a, st);
+      case Rows8Kind::kFew16x32: return start_few<DT, BITS, GROUP, 1, 2>(a, st);
       case Rows8Kind::kFew32x16: return start_few<DT, BITS, GROUP, 2, 1>(a, st);
       case Rows8Kind::kFew32x32: return start_few<DT, BITS, GROUP, 2, 2>(a, st);
       default: return start_few<DT, BITS, GROUP, 4, 2>(a, st);

@@ -23,20 +23,29 @@ template <int BITS, int GROUP, bool WIDE>
 __global__ __launch_bounds__(256) void rows8_prepare_kernel(const signed char *x, int64_t M, int K, uint4 *tiles, void *sums) {  // WIDE: float32 scales
   constexpr int NT = GROUP * 4 / 64;  // tiles of four groups
   const int lane = lane_id(), kb = lane >> 4, quads = rows8_quads(K / GROUP), n_tiles = K / 64;
-  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), mt = unit / quads;
-  const int q = (int)(unit % quads);
+  const uint32_t unit = (uint32_t)__builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));  // (fewer than 2^25)
+  const int64_t mt = unit / (uint32_t)quads;
+  const int q = (int)(unit % (uint32_t)quads);
   if (mt >= row_tiles(M)) return;
   const int64_t row = mt * 16 + (lane & 15);
+  uint4 v[NT];  // all under way before the first is stored; outside: the last ones again
+  const signed char *const at = x + (row < M ? row : M - 1) * K;
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    const signed char *const p = at + (q * NT + i < n_tiles ? q * NT + i : n_tiles - 1) * 64;
+    if constexpr (GROUP == 32) {
+      const uint2 a = *reinterpret_cast<const uint2 *>(p + 8 * kb), b = *reinterpret_cast<const uint2 *>(p + 32 + 8 * kb);
+      v[i] = make_uint4(a.x, a.y, b.x, b.y);
+    } else {
+      v[i] = *reinterpret_cast<const uint4 *>(p + 16 * kb);
+    }
+  }
   int32_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
     const int kt = q * NT + i;
-    uint2 a = make_uint2(0, 0), b = a;
-    if (kt < n_tiles && row < M) {
-      const signed char *const p = x + row * K + kt * 64;
-      a = *reinterpret_cast<const uint2 *>(p + (GROUP == 32 ? 8 * kb : 16 * kb));
-      b = *reinterpret_cast<const uint2 *>(p + (GROUP == 32 ? 32 + 8 * kb : 16 * kb + 8));
-    }
+    const bool there = kt < n_tiles && row < M;
+    uint2 a = there ? make_uint2(v[i].x, v[i].y) : make_uint2(0, 0), b = there ? make_uint2(v[i].z, v[i].w) : make_uint2(0, 0);
     if constexpr (GROUP == 32) {
       sum[2 * i] = byte_sum(a.y, byte_sum(a.x, 0));
       sum[2 * i + 1] = byte_sum(b.y, byte_sum(b.x, 0));

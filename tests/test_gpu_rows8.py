@@ -73,7 +73,7 @@ def run(args, group, bits):
 
 # rows x columns x K: one row, one column, K of one group, of no whole 128, rows and columns on both sides of 16, 32, 64 and 128, more of them than a tile, K of an odd number of groups
 SHAPES = [(1, 1, 128), (1, 17, 256), (1, 1000, 2048), (2, 64, 384), (7, 33, 640), (15, 16, 128), (16, 48, 1152), (17, 100, 512), (31, 129, 896), (33, 64, 1024), (48, 200, 4096),
-          (64, 128, 256), (65, 127, 384), (100, 300, 2176), (128, 256, 640), (129, 513, 128), (200, 96, 1280), (257, 384, 768), (300, 1000, 1024), (520, 272, 512)]
+          (64, 128, 256), (65, 127, 384), (100, 300, 2176), (128, 256, 640), (129, 513, 128), (200, 96, 1280), (257, 384, 768), (300, 1000, 1024), (520, 272, 512), (13, 9001, 384), (6, 9000, 1152), (30, 4500, 2176)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)

@@ -260,6 +260,35 @@ def test_gradient_against_differences(scoring, renormalize):
     assert abs(float((got * d.double()).sum()) - along) <= 1e-6 * float((got * d.double()).abs().sum())
 
 
+@pytest.mark.parametrize("E,k", [(1, 1), (3, 2), (17, 16), (40, 17), (65, 9), (512, 16), (511, 3)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gradient_of_any_ids(dtype, E, k):
+    """Ids that no selection would give: repeated any number of times, outside, in every slot; 1 to 9 tokens, nothing written behind the last."""
+    import mlx_rs_amd as m
+    gen = torch.Generator().manual_seed(E + k)
+    for T in (1, 2, 3, 4, 5, 9):
+        logits = torch.randn(T, E, generator=gen).to(dtype).cuda()
+        inds = torch.randint(-1, min(E, 6) + 1, (T, k), generator=gen).to(torch.int32).cuda()  # (-1 and, of few experts, E: outside)
+        dw = torch.randn(T, k, generator=gen).cuda()
+        inside = (inds >= 0) & (inds < E)
+        for scoring in ("softmax", "sigmoid"):
+            for renormalize in (True, False):
+                room = torch.full((T * E + 64,), 7.0, dtype=dtype, device="cuda")
+                m.capi.check(m.load_library().mi_moe_select_experts_grad(dw.data_ptr(), 2, logits.data_ptr(), m.ops._DTYPES[dtype], inds.data_ptr(), T, E, k, int(scoring == "sigmoid"),
+                                                                         int(renormalize), 1.5, room.data_ptr(), m.ops._stream()))
+                assert bool((room[T * E:] == 7).all())
+                x = logits.double().cpu().requires_grad_()
+                s = torch.sigmoid(x) if scoring == "sigmoid" else torch.softmax(x, -1)
+                w = s.gather(1, inds.cpu().long().clamp(0, E - 1)) * inside.cpu()
+                if renormalize:
+                    total = w.sum(-1, keepdim=True)
+                    w = w / torch.where(total == 0, torch.ones_like(total), total)
+                (w * 1.5 * dw.double().cpu()).sum().backward()
+                # (as in test_gradient, the terms that meet in one id up to 32)
+                bound = (half_step(dtype) + 2.0 ** -24) * x.grad.abs() + 1e-12 * float(dw.abs().max()) + torch.finfo(dtype).smallest_normal * half_step(dtype) * 2
+                assert bool(((room[:T * E].reshape(T, E).double().cpu() - x.grad).abs() <= bound).all())
+
+
 def test_gradient_of_repeated_and_foreign_ids_and_masked_rows():
     import mlx_rs_amd as m
     logits = torch.randn(4, 16, generator=torch.Generator().manual_seed(2)).cuda()

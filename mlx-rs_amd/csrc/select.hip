@@ -148,10 +148,12 @@ __device__ __forceinline__ void select_exact(const SelectKernelArgs &p, const Sl
 
 // The keys and the groups' ranks in float where that decides them.  A float score is off by 2^-22 of itself for the exponential, 2^-23 for the reciprocal and, of a softmax, 14 * 2^-24 for
 // the sum, which is the same factor for all of a token's; scores are at most one, so two of them differ by what doubles say to within 1.9 * 2^-20, and biased keys to within 2^-23 of their size more.
-// Where two keys that follow each other in the choice, or two groups' ranks, are nearer than kNear and kNearOfSize of them allow, or something is an infinity above zero or no number, doubles decide
+// A sigmoid is 1 / (1 + e): a quarter of the exponential's error at most, a rounding and the reciprocal, together 3.9 * 2^-24.
+// Where two keys that follow each other in the choice, or two groups' ranks, are nearer than near_of and kNearOfSize of them allow, or something is an infinity above zero or no number, doubles decide
 // (for one token in some hundred); without a bias the logits are exact keys.  Scores of the chosen are in double, a lane each, of softmax scores that are renormalised from the chosen logits
 // alone: they hold where a softmax over all would round to zero.
-constexpr float kNear = 0x1p-19f, kNearOfSize = 0x1p-21f;
+constexpr float kNearOfSize = 0x1p-21f;
+__device__ __forceinline__ float near_of(const SelectArgs &a) { return a.scoring == 1 ? 0x1p-21f : 0x1p-19f; }
 
 // the key's part that a bias is, minus infinity for an expert that is masked, and whether floats can decide
 __device__ __forceinline__ float with_mask(float l, float bias) { return l == -INFINITY ? -INFINITY : bias; }
@@ -258,7 +260,7 @@ __global__ __launch_bounds__(256) void select_experts_kernel(SelectKernelArgs p)
       if (n > 5) merge_two(t1, t2, __shfl_xor(t1, 32), __shfl_xor(t2, 32));
       const bool two = a.group_score == 1 && p.size > 1;
       const float mine = two ? t1 + t2 : t1;
-      const float clear = 2 * kNear + kNearOfSize * wave_max_f32(g >= a.groups ? 0.f : rank_size(mine, t1, t2, two));
+      const float clear = 2 * near_of(a) + kNearOfSize * wave_max_f32(g >= a.groups ? 0.f : rank_size(mine, t1, t2, two));
       int before = 0, maybe = 0;  // groups that are better, and that could be
       for (int o = 0; o < a.groups; ++o) {
         const float its = f32_of((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(mine), o << n));
@@ -302,7 +304,7 @@ __global__ __launch_bounds__(256) void select_experts_kernel(SelectKernelArgs p)
       if (KEYS && a.bias) {
         if (top == 0) break;  // (no more than were chosen)
         const float now = f32_of((top >> 31) ? top & 0x7fffffffu : ~top);
-        near |= r > 0 && !(last - now > kNear + kNearOfSize * fabsf(last));
+        near |= r > 0 && !(last - now > near_of(a) + kNearOfSize * fabsf(last));
         last = now;
       }
       const int owner = __builtin_ctzll(__ballot(best == top));
@@ -479,7 +481,7 @@ __global__ __launch_bounds__(256) void select_rows_kernel(SelectKernelArgs p, Se
     const bool two = a.group_score == 1 && p.size > 1;
     const float mine = two ? t1 + t2 : t1;
     float clear = 0.f;
-    if constexpr (KEYS) clear = 2 * kNear + kNearOfSize * row_join(g >= a.groups ? 0.f : rank_size(mine, t1, t2, two), larger);
+    if constexpr (KEYS) clear = 2 * near_of(a) + kNearOfSize * row_join(g >= a.groups ? 0.f : rank_size(mine, t1, t2, two), larger);
     int before = 0, maybe = 0;  // lanes of groups that are better, and that could be
     each_other(mine, [&](int n_back, float its) __attribute__((always_inline)) {
       const int og = ((lane - n_back) & 15) >> n;
@@ -511,7 +513,7 @@ __global__ __launch_bounds__(256) void select_rows_kernel(SelectKernelArgs p, Se
     if (KEYS && a.bias) {
       const float now = f32_of((top >> 31) ? top & 0x7fffffffu : ~top);
       if (r == a.k - 1) kth = now;
-      const float clear = kNear + kNearOfSize * fabsf(r == candidates ? kth : last);
+      const float clear = near_of(a) + kNearOfSize * fabsf(r == candidates ? kth : last);
       if (r == candidates) odd |= top != 0 && !(kth - now > clear);
       else close |= r > 0 && top != 0 && !(last - now > clear);
       last = now;

@@ -175,6 +175,15 @@ def test_many_tokens(dtype, scoring, E, groups, k):
                 check_many(rows, k, scoring, b, groups, top, group_score, renormalize, 2.5)
 
 
+test_every_layout_of_many_tokens = test_many_tokens  # (collected by this name: a test further down has the other)
+
+
+@pytest.mark.parametrize("E,groups,k", MANY)
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_every_layout_of_many_float16_tokens(scoring, E, groups, k):
+    test_every_layout_of_many_tokens(torch.float16, scoring, E, groups, k)
+
+
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("k", [1, 2, 7, 8, 14, 15, 16])
 def test_many_tokens_with_keys_close_together(k, scoring):

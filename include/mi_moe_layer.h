@@ -39,9 +39,10 @@ int mi_moe_add_rms_norm_grad(const void *dy, const void *sum, const void *dsum, 
  * Scores s of a token's logits [n_experts] (element type dtype): softmax over the experts, or sigmoid.  Experts are ordered by s + bias
  * (f32 [n_experts], takes part in the choice alone), without a bias by the logits themselves; ties go to the lower id.  n_groups
  * (a divisor of n_experts, up to 64) runs of consecutive experts: only the best top_groups of them are open, by their largest key or by the sum of their two
- * largest s + bias (group_score; the largest alone in groups of one).  Weights: scale * s, divided by the sum of the chosen s with renormalize
+ * largest s + bias (group_score; the largest alone in groups of one; an expert whose logit is -inf or NaN has a part in such a sum with a score of zero, one
+ * whose bias is -inf or NaN none).  A group without an expert whose logit and bias are above -inf comes after all others.  Weights: scale * s, divided by the sum of the chosen s with renormalize
  * (a sum of zero gives zeros).  Scores are computed and compared in float64.  topk_idx [T, top_k], best first; topk_w of element type
- * w_dtype.  An expert whose logit is -inf is chosen only where no other is left, one whose logit is NaN after those; neither changes another's score.
+ * w_dtype.  An expert whose logit is -inf is chosen only where no other of the open groups is left, one whose logit is NaN after those; neither changes another's score.
  * n_experts 1..512, top_k 1..min(32, top_groups * n_experts / n_groups). ---- */
 typedef enum { MI_MOE_SCORING_SOFTMAX = 0, MI_MOE_SCORING_SIGMOID = 1 } mi_moe_scoring;
 typedef enum { MI_MOE_GROUP_SCORE_MAX = 0, MI_MOE_GROUP_SCORE_TOP2 = 1 } mi_moe_group_score;

@@ -3,6 +3,7 @@
 //
 //   s = softmax(l) over the experts, or 1 / (1 + exp(-l))           key = l without a bias, s + b with one
 //   a group's rank: its largest key, or the sum of its two largest s + b     the best `top_groups` groups are open
+//     (masked experts have a part in such a sum with a score of zero; a group of masked ones alone is the last)
 //   chosen: the k largest keys of the open groups, ties to the lower id      weight = scale s / (sum of the chosen s, or 1)
 //   backward, g = scale dw, share = s / sum of the chosen s:
 //     softmax, renormalised: dl = share (g - sum share g)       sigmoid: the same times 1 - s
@@ -74,6 +75,8 @@ __device__ __forceinline__ void merge_two(T &t1, T &t2, T o1, T o2) {
   t1 = fmax(t1, o1);
 }
 __device__ __forceinline__ float f32_of(uint32_t u) { return __uint_as_float(u); }
+// whether one of the group's lanes is among `lanes` (groups > 1: of half of the lanes at most)
+__device__ __forceinline__ bool group_has(uint64_t lanes, int g, int lanes_log2) { return (lanes >> (g << lanes_log2) & (((uint64_t)1 << (1 << lanes_log2)) - 1)) != 0; }
 
 // Everything in double, u64 keys: any logits and biases.  Lane r gets the r-th expert's id.
 template <int S>
@@ -107,10 +110,17 @@ __device__ __forceinline__ void select_exact(const SelectKernelArgs &p, const Sl
     key[j] = !x.on[j] ? 0 : a.bias ? key_of(v[j]) : key_of((double)x.l[j]);
   }
   if (a.groups > 1) {
+    const bool two = a.group_score == 1 && p.size > 1;
     double t1 = -INFINITY, t2 = -INFINITY;  // the two largest of the group
+    bool able = false;                      // this lane has an expert that is not masked
 #pragma unroll
     for (int j = 0; j < S; ++j) {
       double y = a.group_score == 0 && !a.bias ? (double)x.l[j] : v[j];
+      if (x.on[j]) {
+        const float b = a.bias ? a.bias[x.base + j] : 0.f;
+        able |= x.l[j] > -INFINITY && b > -INFINITY;
+        if (two && !(x.l[j] > -INFINITY)) y = b;  // (a score of zero)
+      }
       if (!x.on[j] || y != y) y = -INFINITY;
       t2 = fmax(t2, fmin(t1, y));
       t1 = fmax(t1, y);
@@ -119,7 +129,8 @@ __device__ __forceinline__ void select_exact(const SelectKernelArgs &p, const Sl
       const double o1 = __shfl_xor(t1, 1 << d), o2 = __shfl_xor(t2, 1 << d);
       merge_two(t1, t2, o1, o2);
     }
-    const uint64_t mine = key_of(a.group_score == 0 || p.size == 1 ? t1 : t1 + t2);
+    const bool has = group_has(__ballot(able), g, p.lanes_log2);
+    const uint64_t mine = key_of(!has ? -INFINITY : two && t2 > -INFINITY ? t1 + t2 : t1);
     int before = 0;
     for (int o = 0; o < a.groups; ++o) {
       const uint64_t other = readlane_key(mine, o << p.lanes_log2);
@@ -158,6 +169,8 @@ __device__ __forceinline__ float near_of(const SelectArgs &a) { return a.scoring
 // the key's part that a bias is, minus infinity for an expert that is masked, and whether floats can decide
 __device__ __forceinline__ float with_mask(float l, float bias) { return l == -INFINITY ? -INFINITY : bias; }
 __device__ __forceinline__ bool not_below(float l, float b) { return !(l < INFINITY && b < INFINITY); }
+// what an expert whose logit is -inf adds to the rank of its group
+__device__ __forceinline__ float score_of_zero(const SelectArgs &a, int id) { return a.bias ? fmaxf(a.bias[id], -INFINITY) : 0.f; }
 // what a group's rank may be off by, in kNearOfSize (a rank of minus infinity is that)
 __device__ __forceinline__ float rank_size(float rank, float t1, float t2, bool two) { return rank == -INFINITY ? 0.f : two ? fabsf(t1) + fabsf(t2) : fabsf(t1); }
 
@@ -240,10 +253,19 @@ __global__ __launch_bounds__(256) void select_experts_kernel(SelectKernelArgs p)
       if (a.bias && x.on[j]) key[j] = key_of(s[j]);
     }
     if (a.groups > 1) {
+      const bool two = a.group_score == 1 && p.size > 1;
       float t1 = -INFINITY, t2 = -INFINITY;
+      bool out = false, able = false;  // of this lane's experts one is masked, one is not
 #pragma unroll
       for (int j = 0; j < S; ++j) {
-        const float y = !x.on[j] ? -INFINITY : a.group_score == 0 && !a.bias ? x.l[j] : s[j];
+        out |= x.on[j] && b[j] == -INFINITY;
+        able |= x.on[j] && b[j] > -INFINITY;
+      }
+      const bool masks = two && __any(out);
+#pragma unroll
+      for (int j = 0; j < S; ++j) {
+        float y = !x.on[j] ? -INFINITY : a.group_score == 0 && !a.bias ? x.l[j] : s[j];
+        if (masks && x.on[j] && x.l[j] == -INFINITY) y = score_of_zero(a, x.base + j);
         t2 = fmaxf(t2, fminf(t1, y));
         t1 = fmaxf(t1, y);
       }
@@ -258,8 +280,9 @@ __global__ __launch_bounds__(256) void select_experts_kernel(SelectKernelArgs p)
       if (n > 3) other(std::integral_constant<int, kDppMirror>{});
       if (n > 4) merge_two(t1, t2, __shfl_xor(t1, 16), __shfl_xor(t2, 16));
       if (n > 5) merge_two(t1, t2, __shfl_xor(t1, 32), __shfl_xor(t2, 32));
-      const bool two = a.group_score == 1 && p.size > 1;
-      const float mine = two ? t1 + t2 : t1;
+      if (masks && t2 == -INFINITY) t2 = 0.f;
+      float mine = two ? t1 + t2 : t1;
+      if (masks && !group_has(__ballot(able), g, n)) mine = -INFINITY;
       const float clear = 2 * near_of(a) + kNearOfSize * wave_max_f32(g >= a.groups ? 0.f : rank_size(mine, t1, t2, two));
       int before = 0, maybe = 0;  // groups that are better, and that could be
       for (int o = 0; o < a.groups; ++o) {
@@ -463,6 +486,22 @@ __global__ __launch_bounds__(256) void select_rows_kernel(SelectKernelArgs p, Se
     }
   }
   if (a.groups > 1) {
+    const bool two = a.group_score == 1 && p.size > 1;
+    bool masks = false, able = false;  // of the wave's experts one is masked; of this lane's one is not
+    if constexpr (KEYS) {
+      bool out = false;
+#pragma unroll
+      for (int j = 0; j < S; ++j) {
+        out |= j < n_mine && b[j] == -INFINITY;
+        able |= j < n_mine && b[j] > -INFINITY;
+      }
+      masks = two && __any(out);
+      if (masks) {
+#pragma unroll
+        for (int j = 0; j < S; ++j)
+          if (j < n_mine && l[j] == -INFINITY) y[j] = score_of_zero(a, base + j);
+      }
+    }
     float t1 = -INFINITY, t2 = -INFINITY;
 #pragma unroll
     for (int j = 0; j < S; ++j) {
@@ -478,8 +517,9 @@ __global__ __launch_bounds__(256) void select_rows_kernel(SelectKernelArgs p, Se
     if (n > 0) other(std::integral_constant<int, kDppXor1>{});
     if (n > 1) other(std::integral_constant<int, kDppXor2>{});
     if (n > 2) other(std::integral_constant<int, kDppHalfMirror>{});
-    const bool two = a.group_score == 1 && p.size > 1;
-    const float mine = two ? t1 + t2 : t1;
+    if (masks && t2 == -INFINITY) t2 = 0.f;
+    float mine = two ? t1 + t2 : t1;
+    if (masks && !group_has(__ballot(able) >> (lane_id() & 48), g, n)) mine = -INFINITY;
     float clear = 0.f;
     if constexpr (KEYS) clear = 2 * near_of(a) + kNearOfSize * row_join(g >= a.groups ? 0.f : rank_size(mine, t1, t2, two), larger);
     int before = 0, maybe = 0;  // lanes of groups that are better, and that could be

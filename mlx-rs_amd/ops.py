@@ -464,7 +464,8 @@ def select_experts(logits, top_k, scoring="softmax", bias=None, n_groups=1, top_
     """Experts of every token from the router's logits, for routers that ``route`` does not cover: (inds int32 [..., k], best first, weights
     [..., k] of ``dtype``).  logits: [..., E] in bfloat16, float16 or float32.  Scores are ``scoring`` ("softmax" over the experts, or
     "sigmoid") of the logits; ``bias`` (float32 [E]) is added for the choice alone; of ``n_groups`` runs of experts the best ``top_groups`` are open, by
-    their largest key or by the sum of their two largest scores (``group_score`` "max" / "top2"); ties go to the lower id.  Weights: the chosen
+    their largest key or by the sum of their two largest scores (``group_score`` "max" / "top2"; what is masked counts as a score of zero, and groups of
+    masked experts alone come last); ties go to the lower id.  Weights: the chosen
     scores, divided by their sum with ``renormalize``, times ``scale``.  ``SparseMoeBlock.forward_routed`` takes the results."""
     out = _native("select_experts", logits, top_k, scoring, bias, n_groups, top_groups, group_score, renormalize, scale, dtype)
     if out is not None:

@@ -84,6 +84,9 @@ __device__ __forceinline__ void select_exact(const SelectKernelArgs &p, const Sl
   const SelectArgs &a = p.a;
   const int lane = lane_id();
   double v[S];
+  float b[S];
+#pragma unroll
+  for (int j = 0; j < S; ++j) b[j] = a.bias && x.on[j] ? a.bias[x.base + j] : 0.f;
   if (a.scoring == 0) {
     float most = -INFINITY;  // (fmaxf passes over what is no number)
 #pragma unroll
@@ -105,7 +108,7 @@ __device__ __forceinline__ void select_exact(const SelectKernelArgs &p, const Sl
   uint64_t key[S];
 #pragma unroll
   for (int j = 0; j < S; ++j) {
-    if (a.bias && x.on[j]) v[j] += (double)a.bias[x.base + j];
+    v[j] += (double)b[j];
     if (x.l[j] == -INFINITY) v[j] = -INFINITY;
     key[j] = !x.on[j] ? 0 : a.bias ? key_of(v[j]) : key_of((double)x.l[j]);
   }
@@ -116,11 +119,8 @@ __device__ __forceinline__ void select_exact(const SelectKernelArgs &p, const Sl
 #pragma unroll
     for (int j = 0; j < S; ++j) {
       double y = a.group_score == 0 && !a.bias ? (double)x.l[j] : v[j];
-      if (x.on[j]) {
-        const float b = a.bias ? a.bias[x.base + j] : 0.f;
-        able |= x.l[j] > -INFINITY && b > -INFINITY;
-        if (two && !(x.l[j] > -INFINITY)) y = b;  // (a score of zero)
-      }
+      able |= x.on[j] && x.l[j] > -INFINITY && b[j] > -INFINITY;
+      if (two && !(x.l[j] > -INFINITY)) y = b[j];  // (a score of zero)
       if (!x.on[j] || y != y) y = -INFINITY;
       t2 = fmax(t2, fmin(t1, y));
       t1 = fmax(t1, y);
@@ -166,11 +166,8 @@ __device__ __forceinline__ void select_exact(const SelectKernelArgs &p, const Sl
 constexpr float kNearOfSize = 0x1p-21f;
 __device__ __forceinline__ float near_of(const SelectArgs &a) { return a.scoring == 1 ? 0x1p-21f : 0x1p-19f; }
 
-// the key's part that a bias is, minus infinity for an expert that is masked, and whether floats can decide
-__device__ __forceinline__ float with_mask(float l, float bias) { return l == -INFINITY ? -INFINITY : bias; }
+// whether floats can decide
 __device__ __forceinline__ bool not_below(float l, float b) { return !(l < INFINITY && b < INFINITY); }
-// what an expert whose logit is -inf adds to the rank of its group
-__device__ __forceinline__ float score_of_zero(const SelectArgs &a, int id) { return a.bias ? fmaxf(a.bias[id], -INFINITY) : 0.f; }
 // what a group's rank may be off by, in kNearOfSize (a rank of minus infinity is that)
 __device__ __forceinline__ float rank_size(float rank, float t1, float t2, bool two) { return rank == -INFINITY ? 0.f : two ? fabsf(t1) + fabsf(t2) : fabsf(t1); }
 
@@ -205,13 +202,17 @@ __global__ __launch_bounds__(256) void select_experts_kernel(SelectKernelArgs p)
     x.l[j] = x.on[j] ? as_f32(row[x.base + j]) : -INFINITY;
   }
   float b[S];
-  bool odd = false;  // something that floats do not decide
+  bool odd = false;    // something that floats do not decide
+  bool masks = false;  // one of the token's logits is -inf
   if constexpr (KEYS) {
+    float least = INFINITY;
 #pragma unroll
     for (int j = 0; j < S; ++j) {
-      b[j] = with_mask(x.l[j], a.bias && x.on[j] ? a.bias[x.base + j] : 0.f);
+      b[j] = a.bias && x.on[j] ? a.bias[x.base + j] : 0.f;
       odd |= x.on[j] && not_below(x.l[j], b[j]);
+      if (x.on[j]) least = fminf(least, x.l[j]);
     }
+    masks = __any(least == -INFINITY);
   }
   float most = -INFINITY;
   if (SUM || (KEYS && a.scoring == 0)) {
@@ -252,20 +253,20 @@ __global__ __launch_bounds__(256) void select_experts_kernel(SelectKernelArgs p)
       s[j] += b[j];
       if (a.bias && x.on[j]) key[j] = key_of(s[j]);
     }
+    const bool two = a.groups > 1 && a.group_score == 1 && p.size > 1;
+    if (masks) {  // (ranked by two, they have a score of zero)
+#pragma unroll
+      for (int j = 0; j < S; ++j)
+        if (x.on[j] && x.l[j] == -INFINITY) {
+          key[j] = key_of(-INFINITY);
+          if (!two) s[j] = -INFINITY;
+        }
+    }
     if (a.groups > 1) {
-      const bool two = a.group_score == 1 && p.size > 1;
       float t1 = -INFINITY, t2 = -INFINITY;
-      bool out = false, able = false;  // of this lane's experts one is masked, one is not
 #pragma unroll
       for (int j = 0; j < S; ++j) {
-        out |= x.on[j] && b[j] == -INFINITY;
-        able |= x.on[j] && b[j] > -INFINITY;
-      }
-      const bool masks = two && __any(out);
-#pragma unroll
-      for (int j = 0; j < S; ++j) {
-        float y = !x.on[j] ? -INFINITY : a.group_score == 0 && !a.bias ? x.l[j] : s[j];
-        if (masks && x.on[j] && x.l[j] == -INFINITY) y = score_of_zero(a, x.base + j);
+        const float y = !x.on[j] ? -INFINITY : a.group_score == 0 && !a.bias ? x.l[j] : s[j];
         t2 = fmaxf(t2, fminf(t1, y));
         t1 = fmaxf(t1, y);
       }
@@ -280,9 +281,14 @@ __global__ __launch_bounds__(256) void select_experts_kernel(SelectKernelArgs p)
       if (n > 3) other(std::integral_constant<int, kDppMirror>{});
       if (n > 4) merge_two(t1, t2, __shfl_xor(t1, 16), __shfl_xor(t2, 16));
       if (n > 5) merge_two(t1, t2, __shfl_xor(t1, 32), __shfl_xor(t2, 32));
-      if (masks && t2 == -INFINITY) t2 = 0.f;
+      if (t2 == -INFINITY) t2 = 0.f;
       float mine = two ? t1 + t2 : t1;
-      if (masks && !group_has(__ballot(able), g, n)) mine = -INFINITY;
+      if (two && masks) {  // (where no logit is masked, a group of masked ones has nothing but biases of -inf)
+        bool able = false;
+#pragma unroll
+        for (int j = 0; j < S; ++j) able |= x.on[j] && x.l[j] > -INFINITY && b[j] > -INFINITY;
+        if (!group_has(__ballot(able), g, n)) mine = -INFINITY;
+      }
       const float clear = 2 * near_of(a) + kNearOfSize * wave_max_f32(g >= a.groups ? 0.f : rank_size(mine, t1, t2, two));
       int before = 0, maybe = 0;  // groups that are better, and that could be
       for (int o = 0; o < a.groups; ++o) {
@@ -425,7 +431,7 @@ __global__ __launch_bounds__(256) void select_rows_kernel(SelectKernelArgs p, Se
     for (int j = 0; j < S; ++j) l[j] = j < n_mine ? as_f32(row[base + j]) : -INFINITY;
   }
   float b[S];
-  bool odd = false;
+  bool odd = false, masks = false;  // masks: one of the four tokens' logits is -inf
   if constexpr (KEYS) {
     if (a.bias && p.slots == S && n_mine == S) {
       __builtin_memcpy(b, a.bias + base, sizeof b);
@@ -433,11 +439,18 @@ __global__ __launch_bounds__(256) void select_rows_kernel(SelectKernelArgs p, Se
 #pragma unroll
       for (int j = 0; j < S; ++j) b[j] = a.bias && j < n_mine ? a.bias[base + j] : 0.f;
     }
+    float least = INFINITY;
+    if (n_mine == S) {
 #pragma unroll
-    for (int j = 0; j < S; ++j) {
-      b[j] = with_mask(l[j], b[j]);
-      odd |= j < n_mine && not_below(l[j], b[j]);
+      for (int j = 0; j < S; ++j) least = fminf(least, l[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < S; ++j)
+        if (j < n_mine) least = fminf(least, l[j]);
     }
+    masks = __any(least == -INFINITY);
+#pragma unroll
+    for (int j = 0; j < S; ++j) odd |= j < n_mine && not_below(l[j], b[j]);
   }
   auto larger = [](float x, float y) { return fmaxf(x, y); };
   float most = -INFINITY;
@@ -460,6 +473,7 @@ __global__ __launch_bounds__(256) void select_rows_kernel(SelectKernelArgs p, Se
 #pragma unroll
     for (int j = 0; j < S; ++j) key[j] = j < n_mine ? key_of(l[j]) : 0;
   }
+  const bool two = a.groups > 1 && a.group_score == 1 && p.size > 1;
   float y[S];  // what groups are ranked by
 #pragma unroll
   for (int j = 0; j < S; ++j) y[j] = l[j] == l[j] ? l[j] : -INFINITY;  // (no numbers rank as -inf)
@@ -483,25 +497,17 @@ __global__ __launch_bounds__(256) void select_rows_kernel(SelectKernelArgs p, Se
 #pragma unroll
         for (int j = 0; j < S; ++j) key[j] = j < n_mine ? key_of(y[j]) : 0;
       }
+      if (masks) {  // (ranked by two, they have a score of zero)
+#pragma unroll
+        for (int j = 0; j < S; ++j)
+          if (j < n_mine && l[j] == -INFINITY) {
+            key[j] = key_of(-INFINITY);
+            if (!two) y[j] = -INFINITY;
+          }
+      }
     }
   }
   if (a.groups > 1) {
-    const bool two = a.group_score == 1 && p.size > 1;
-    bool masks = false, able = false;  // of the wave's experts one is masked; of this lane's one is not
-    if constexpr (KEYS) {
-      bool out = false;
-#pragma unroll
-      for (int j = 0; j < S; ++j) {
-        out |= j < n_mine && b[j] == -INFINITY;
-        able |= j < n_mine && b[j] > -INFINITY;
-      }
-      masks = two && __any(out);
-      if (masks) {
-#pragma unroll
-        for (int j = 0; j < S; ++j)
-          if (j < n_mine && l[j] == -INFINITY) y[j] = score_of_zero(a, base + j);
-      }
-    }
     float t1 = -INFINITY, t2 = -INFINITY;
 #pragma unroll
     for (int j = 0; j < S; ++j) {
@@ -517,9 +523,14 @@ __global__ __launch_bounds__(256) void select_rows_kernel(SelectKernelArgs p, Se
     if (n > 0) other(std::integral_constant<int, kDppXor1>{});
     if (n > 1) other(std::integral_constant<int, kDppXor2>{});
     if (n > 2) other(std::integral_constant<int, kDppHalfMirror>{});
-    if (masks && t2 == -INFINITY) t2 = 0.f;
+    if (t2 == -INFINITY) t2 = 0.f;
     float mine = two ? t1 + t2 : t1;
-    if (masks && !group_has(__ballot(able) >> (lane_id() & 48), g, n)) mine = -INFINITY;
+    if (two && masks) {  // (where no logit is masked, a group of masked ones has nothing but biases of -inf)
+      bool able = false;
+#pragma unroll
+      for (int j = 0; j < S; ++j) able |= j < n_mine && l[j] > -INFINITY && b[j] > -INFINITY;
+      if (!group_has(__ballot(able) >> (lane_id() & 48), g, n)) mine = -INFINITY;
+    }
     float clear = 0.f;
     if constexpr (KEYS) clear = 2 * near_of(a) + kNearOfSize * row_join(g >= a.groups ? 0.f : rank_size(mine, t1, t2, two), larger);
     int before = 0, maybe = 0;  // lanes of groups that are better, and that could be

@@ -60,7 +60,7 @@ int mi_moe_select_experts_grad(const void *dw, int32_t w_dtype, const void *logi
 /* The block with a routing of the caller's (mi_moe_select_experts, or any other): mi_moe_forward behind its router.
  * topk_idx [T, top_k], topk_w bf16 [T, top_k]; the handle's router is not used.  A token that names an expert twice gets it
  * once, with the sum of its weights (one rounding to bf16); an id outside the experts (a padded slot) contributes nothing.  dbg->topk_idx and topk_w
- * hold the routing as the kernels took it: another expert with a weight of zero in such slots.  Same workspace as mi_moe_forward. */
+ * hold the routing as the kernels took it: another expert with a weight of -0 in such slots, whose result is computed and left out (also where it is not finite).  Same workspace as mi_moe_forward. */
 int mi_moe_forward_routed(mi_moe_handle h, const uint16_t *x, const uint32_t *topk_idx,
                           const uint16_t *topk_w, int64_t T, uint16_t *out, void *workspace,
                           size_t workspace_bytes, const mi_moe_debug_out *dbg, void *stream);

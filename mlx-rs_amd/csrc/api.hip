@@ -891,7 +891,7 @@ static int forward_impl(mi_moe_handle h, const uint16_t *x_in, int64_t T, uint16
     MI_STAGE_DONE();
   }
   if (streams_guard.owns_lock()) streams_guard.unlock();
-  MI_HIP(launch_combine(f.y, f.topk_w, nullptr, T, c.top_k, c.hidden, norm_weight ? x_in : nullptr, out, st));
+  MI_HIP(launch_combine(f.y, f.topk_w, nullptr, T, c.top_k, c.hidden, norm_weight ? x_in : nullptr, out, st, given_idx != nullptr));
   MI_STAGE_DONE();
 #undef MI_STAGE_DONE
 

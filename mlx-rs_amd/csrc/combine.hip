@@ -12,7 +12,9 @@ namespace mi_moe {
 // several blocks: at decode sizes the launch is latency, and a block per token would leave most of
 // the chip idle).  The k rows of a token are fetched eight at a time, all loads of a batch in flight
 // before the first is used; the sum itself runs in slot order.
+// DROPS: a slot whose weight has the bits kNoSlot has no part in the sum, whatever its row holds.
 constexpr int kCombineThreads = 64;
+template <bool DROPS>
 __global__ __launch_bounds__(kCombineThreads) void combine_kernel(
     const uint16_t *__restrict__ y, const uint16_t *__restrict__ scores,
     const uint32_t *__restrict__ inv_perm, int64_t T, int k, int H,
@@ -28,8 +30,10 @@ __global__ __launch_bounds__(kCombineThreads) void combine_kernel(
     for (int j = 0; j < 8; ++j) {
       const int s = s0 + j < k ? s0 + j : k - 1;  // (clamped: loads without a condition stay in flight together)
       const int64_t r = inv_perm ? (int64_t)inv_perm[t * k + s] : t * k + s;
-      sc[j] = bf16_to_f32(scores[t * k + s]);
+      const uint16_t score = scores[t * k + s];
+      sc[j] = bf16_to_f32(score);
       v[j] = *reinterpret_cast<const uint4 *>(y + r * H + h);
+      if (DROPS && score == kNoSlot) v[j] = make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -62,10 +66,11 @@ __global__ __launch_bounds__(kCombineThreads) void combine_kernel(
 
 hipError_t launch_combine(const uint16_t *y, const uint16_t *scores, const uint32_t *inv_perm,
                           int64_t T, int k, int H, const uint16_t *residual, uint16_t *out,
-                          hipStream_t st) {
+                          hipStream_t st, bool drops) {
   if (T == 0) return hipSuccess;
   dim3 grid((unsigned)T, (unsigned)((H / 8 + kCombineThreads - 1) / kCombineThreads));
-  combine_kernel<<<grid, kCombineThreads, 0, st>>>(y, scores, inv_perm, T, k, H, residual, out);
+  if (drops) combine_kernel<true><<<grid, kCombineThreads, 0, st>>>(y, scores, inv_perm, T, k, H, residual, out);
+  else combine_kernel<false><<<grid, kCombineThreads, 0, st>>>(y, scores, inv_perm, T, k, H, residual, out);
   return hipGetLastError();
 }
 

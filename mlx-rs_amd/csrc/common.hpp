@@ -366,9 +366,11 @@ hipError_t launch_dense_records(int64_t M, int big_thr, bool one_list, uint32_t 
 hipError_t launch_swiglu(const uint16_t *g, const uint16_t *u, int64_t n, uint16_t *out,
                          hipStream_t st);
 hipError_t launch_stream_probe(const void *buf, size_t bytes, uint32_t *sink, hipStream_t st);
+// drops: slots of the weight kNoSlot (minus zero, which no named slot has there) are left out of the sum, not multiplied by zero.
+constexpr uint16_t kNoSlot = 0x8000;
 hipError_t launch_combine(const uint16_t *y, const uint16_t *scores, const uint32_t *inv_perm,
                           int64_t T, int k, int H, const uint16_t *residual, uint16_t *out,
-                          hipStream_t st);
+                          hipStream_t st, bool drops = false);
 hipError_t launch_rms_norm(const uint16_t *x, const uint16_t *weight, float eps, int64_t T, int H,
                            uint16_t *out, hipStream_t st);
 // plain products (any float type, group sizes 32 / 64 / 128, 2 / 4 / 8 bits, both weight layouts);

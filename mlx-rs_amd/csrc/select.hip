@@ -832,7 +832,7 @@ hipError_t launch_select_grad(const SelectGradArgs &a, int dt, hipStream_t st) {
 // ---------------------------------------------------------------- a routing that the caller brings
 // A wave a token copies the ids and weights into the workspace, and makes of them what the dispatch and the products rely on: k different experts.  A token's
 // second mention of an expert is added to the first (in slot order, one rounding), an id outside the experts is dropped; what then stands in the slot is an expert
-// that the token does not name, with a weight of zero.
+// that the token does not name, with a weight (kNoSlot, a zero) at which the sum over the slots passes over its result: zero times that would be no number where it is not finite.
 __global__ __launch_bounds__(256) void check_routing_kernel(const uint32_t *idx, const uint16_t *w, int64_t T, int E, int k, uint32_t *idx_out, uint16_t *w_out) {
   const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (t >= T) return;
@@ -857,12 +857,13 @@ __global__ __launch_bounds__(256) void check_routing_kernel(const uint32_t *idx,
       if (__ballot(lane < k && named == c)) continue;
       const int to = __builtin_ctzll(left);
       left &= left - 1;
-      if (lane == to) id = c, weight = 0.f;
+      if (lane == to) id = c;
     }
   }
   if (lane < k) {
     idx_out[t * k + lane] = id;
-    w_out[t * k + lane] = f32_to_bf16(weight);
+    const uint16_t w16 = f32_to_bf16(weight);
+    w_out[t * k + lane] = bad ? kNoSlot : w16 == kNoSlot ? (uint16_t)0 : w16;
   }
 }
 

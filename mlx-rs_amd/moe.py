@@ -121,7 +121,7 @@ class SparseMoeBlock:
     def forward_routed(self, x, inds, weights, debug=False, out=None):
         """forward() with a routing of the caller's in place of the block's router: inds int32 and weights bf16 [..., top_k] for x bf16
         [..., H] (``ops.select_experts``).  A token that names an expert twice gets it once, with the sum of its weights; an id outside the experts
-        contributes nothing."""
+        contributes nothing, whatever its token's row holds (though the slot takes the time of another)."""
         c = self.config
         _need(inds, torch.int32, "inds")
         _need(weights, torch.bfloat16, "weights")

@@ -35,6 +35,7 @@ __device__ __forceinline__ Value<DT> value_of(float v) {
 
 __device__ __forceinline__ int32_t byte_sum(uint32_t v, int32_t c) { return __builtin_amdgcn_sdot4((int32_t)v, 0x01010101, c, false); }
 typedef int32_t i32x2_t __attribute__((ext_vector_type(2)));
+typedef short i16x4_t __attribute__((ext_vector_type(4)));
 
 // Integer sums start at the bits of 1.5 * 2^23, where a float's step is one: below 2^22 (128 products of 2^14 at most are 2^21) they leave the bits of that number
 // and the sum, and a subtraction takes the place of a conversion.  Measured a tile of 16 x 16 (multiply, four of either, four multiply-adds), four waves a SIMD: 36 cycles, 43 with

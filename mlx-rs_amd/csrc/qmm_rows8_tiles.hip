@@ -80,8 +80,10 @@ __device__ __forceinline__ void copy_scalars_to_lds(i32x4_t rsrc, uint32_t voff,
 // A group is one matrix instruction a 16 x 16 tile (two for 128 values, one of half the depth for 32), whose integer sums are exact; then a subtraction and a
 // multiply-add a result.  What bounds it is those, a matrix unit and a vector unit that do not run at once (kWhole): 4096 x 4096 x 4096, 4-bit, groups of 64, 144 us with the rows' preparation
 // (956 TFLOP/s), groups of 128 1320 TFLOP/s, 32 730.  The biases' terms are a product over the groups as well, eight of them a bf16 instruction: the sums in two exact values, their factors
-// b + 8 s (b + 128 s) in two that leave 2^-18 of the factor, 2^-9 of the result's own rounding to bf16.  (Four groups of float32 a float32 instruction are 32 cycles for 16: 149, 1290 and 670;
-// with float32 scales, whose results keep 24 bits, they remain.)
+// b + 8 s (b + 128 s) in as many as hold all of it.  Of bf16 scales those are two: where the smaller of b and 8 s is below half a step of the larger, it is what the first piece leaves, and has
+// eight bits; where it is not, its last bit is 2^-15 or more of the larger's power of two, and what a piece of eight bits leaves, 2^-7 of that at most, has eight again.  Of f16 scales, of eleven bits, they are
+// three, the last in an instruction of half the depth (with two, a factor's error would be up to 2^-17 of it; 77 and 45 us for 75 and 44 with 2048 and 777 rows, 4096 x 4096, 8-bit).  (Four groups of
+// float32 a float32 instruction are 32 cycles for 16: 149, 1290 and 670; with float32 scales they remain.)
 template <int DT, int BITS, int GROUP, int MI, int NI, int WM, int WN, int KS, int NB>
 struct Rows8Tile {
   static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves * KS, ROWS = 16 * MI * WM, COLS = 16 * NI * WN;
@@ -247,12 +249,20 @@ __global__ __launch_bounds__(64 * WM * WN * KS, OCC) void rows8_tiles_kernel(Row
           float beta[2];
 #pragma unroll
           for (int i = 0; i < 2; ++i) beta[i] = there ? __builtin_fmaf(k * Centre<BITS>::value, as_f32(sv[i]), k * as_f32(bv[i])) : 0.f;
-          const uint32_t first = cvt_pk_bf16(beta[0], beta[1]);
-          const uint32_t rest = cvt_pk_bf16(beta[0] - __uint_as_float(first << 16), beta[1] - __uint_as_float(first & 0xffff0000u));
+          auto pieces = [&] {  // as bf16, and what they leave
+            const uint32_t p = cvt_pk_bf16(beta[0], beta[1]);
+            beta[0] -= __uint_as_float(p << 16), beta[1] -= __uint_as_float(p & 0xffff0000u);
+            return p;
+          };
+          const uint32_t first = pieces(), rest = pieces(), last = DT == 1 ? pieces() : 0;
           const i32x4_t b4 = {(int32_t)first, (int32_t)first, (int32_t)rest, (int32_t)rest};
 #pragma unroll
-          for (int m = 0; m < MI; ++m)
+          for (int m = 0; m < MI; ++m) {
             acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, sum[m]), __builtin_bit_cast(bf16x8_t, b4), acc[m][n], 0, 0, 0);
+            if constexpr (DT == 1)
+              acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(i16x4_t, i32x2_t{sum[m][0], sum[m][1]}), __builtin_bit_cast(i16x4_t, i32x2_t{(int32_t)last, (int32_t)last}),
+                                                                    acc[m][n], 0, 0, 0);
+          }
         }
       }
     }

@@ -67,7 +67,7 @@ int mi_moe_forward_routed(mi_moe_handle h, const uint16_t *x, const uint32_t *to
 
 /* ---- The linear layer on rows in eight bits (mi_moe_add_rms_norm_rows8 makes such rows): y = (row_scales x) . dequantize(w)^T + linear_bias, each result
  * rounded once.  x: signed bytes [M, K]; row_scales: f32 [M]; w [N, K*bits/32]; scales, biases [N, K/group_size], linear_bias [N]
- * (or NULL) and y [M, N] of element type dtype.  bits 4 or 8; group_size 32, 64 or 128; K a multiple of group_size.  Products of rows and codes are summed exactly, as integers,
+ * (or NULL) and y [M, N] of element type dtype.  bits 4 or 8; group_size 32, 64 or 128; K a multiple of group_size; N up to 2^26 - 4.  Products of rows and codes are summed exactly, as integers,
  * over runs of a group; everything else in float32.
  * The fast kernels want K a multiple of 128 and x, w, scales and biases 16-byte aligned; those for many rows an even number of 16-bit scales a column and
  * workspace >= mi_moe_quantized_linear_rows8_workspace_size (16-byte aligned; 0 for up to 16 rows), too.  Without these, slower kernels give the same product. ---- */

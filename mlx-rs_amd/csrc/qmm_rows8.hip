@@ -381,9 +381,22 @@ __global__ __launch_bounds__(512, MI * NI < 4 && !(DT == 2 && NI == 2) ? 4 : 2) 
 template <int DT, int BITS, int GROUP, int MI, int NI>
 static hipError_t start_few(const Rows8Args &a, hipStream_t st) {
   const int64_t wide = (a.N + 16 * NI - 1) / (16 * NI), grid = (a.M + 16 * MI - 1) / (16 * MI) * wide;
-  if (grid >= (int64_t)1 << 23) return hipErrorInvalidValue;  // (a launch has less than 2^32 threads)
+  if (grid > kRows8Blocks) return hipErrorInvalidValue;
   rows8_few_kernel<DT, BITS, GROUP, MI, NI><<<(unsigned)grid, 512, 0, st>>>(a, (int)wide);
   return hipGetLastError();
+}
+
+static hipError_t launch_few(const Rows8Args &a, Rows8Kind kind, int bits, int dt, hipStream_t st) {
+  return rows8_with_types(dt, bits, a.group, [&](auto d, auto b, auto g) {
+    constexpr int DT = decltype(d)::value, BITS = decltype(b)::value, GROUP = decltype(g)::value;
+    switch (kind) {
+      case Rows8Kind::kFew16x16: return start_few<DT, BITS, GROUP, 1, 1>(a, st);
+      case Rows8Kind::kFew16x32: return start_few<DT, BITS, GROUP, 1, 2>(a, st);
+      case Rows8Kind::kFew32x16: return start_few<DT, BITS, GROUP, 2, 1>(a, st);
+      case Rows8Kind::kFew32x32: return start_few<DT, BITS, GROUP, 2, 2>(a, st);
+      default: return start_few<DT, BITS, GROUP, 4, 2>(a, st);
+    }
+  });
 }
 
 // Operands that the fast kernels take: rows, codes and scales in pieces of up to 16 bytes, whole stages of 128 values.
@@ -396,19 +409,6 @@ size_t rows8_workspace_bytes(int64_t M, int K) { return M <= kRows8NoTiles || K 
 
 hipError_t launch_qmm_rows8(const Rows8Args &a, int bits, int dt, void *workspace, size_t workspace_bytes, hipStream_t st) {
   if (a.M == 0) return hipSuccess;
-  // rows of a launch: every kernel's has less than 2^32 threads with these
-  const int64_t by_k = ((int64_t)1 << 34) / a.K, by_n = ((int64_t)1 << 33) / a.N, fit = (by_k < by_n ? by_k : by_n) / 128 * 128, step = fit ? fit : 128;
-  if (a.M > step) {
-    Rows8Args some = a;
-    for (int64_t m = 0; m < a.M; m += step) {
-      some.x = a.x + m * a.K;
-      some.row_scales = a.row_scales + m;
-      some.y = static_cast<char *>(a.y) + m * a.N * (dt == 2 ? 4 : 2);
-      some.M = a.M - m < step ? a.M - m : step;
-      if (hipError_t e = launch_qmm_rows8(some, bits, dt, workspace, workspace_bytes, st); e != hipSuccess) return e;
-    }
-    return hipSuccess;
-  }
   if (!rows8_even(a)) {
     return rows8_with_types(dt, bits, a.group, [&](auto d, auto b, auto) { return start_plain<decltype(d)::value, decltype(b)::value>(a, st); });
   }
@@ -421,17 +421,18 @@ hipError_t launch_qmm_rows8(const Rows8Args &a, int bits, int dt, void *workspac
   const bool words = a.K / a.group * (dt == 2 ? 4 : 2) % 4 == 0;  // (groups of 128, 16-bit scales: an odd number of them starts half of the columns off a word)
   const bool tiles = words && workspace && (reinterpret_cast<uintptr_t>(workspace) & 15u) == 0 && workspace_bytes >= rows8_workspace_bytes(a.M, a.K);
   const Rows8Kind kind = rows8_kind(a.M, a.N, a.K, tiles);
-  if (kRows8Costs[(int)kind].tiles) return launch_rows8_tiles(a, kind, bits, dt, workspace, st);
-  return rows8_with_types(dt, bits, a.group, [&](auto d, auto b, auto g) {
-    constexpr int DT = decltype(d)::value, BITS = decltype(b)::value, GROUP = decltype(g)::value;
-    switch (kind) {
-      case Rows8Kind::kFew16x16: return start_few<DT, BITS, GROUP, 1, 1>(a, st);
-      case Rows8Kind::kFew16x32: return start_few<DT, BITS, GROUP, 1, 2>(a, st);
-      case Rows8Kind::kFew32x16: return start_few<DT, BITS, GROUP, 2, 1>(a, st);
-      case Rows8Kind::kFew32x32: return start_few<DT, BITS, GROUP, 2, 2>(a, st);
-      default: return start_few<DT, BITS, GROUP, 4, 2>(a, st);
-    }
-  });
+  const int64_t step = rows8_step(kind, a.N, a.K, a.group);
+  if (step == 0) return hipErrorInvalidValue;
+  for (int64_t m = 0; m < a.M; m += step) {
+    Rows8Args some = a;
+    some.x = a.x + m * a.K;
+    some.row_scales = a.row_scales + m;
+    some.y = static_cast<char *>(a.y) + m * a.N * (dt == 2 ? 4 : 2);
+    some.M = a.M - m < step ? a.M - m : step;
+    const hipError_t e = kRows8Costs[(int)kind].tiles ? launch_rows8_tiles(some, kind, bits, dt, workspace, st) : launch_few(some, kind, bits, dt, st);
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 }  // namespace mi_moe

@@ -16,8 +16,6 @@ __host__ __device__ constexpr int64_t row_tiles(int64_t M) { return (M + 15) / 1
 constexpr size_t rows8_tiles_bytes(int64_t M, int K) { return (size_t)row_tiles(M) * 16 * K; }
 constexpr size_t rows8_sums_bytes(int64_t M, int K, int group) { return (size_t)row_tiles(M) * ((K / group + 7) / 8) * 512; }
 
-__host__ __device__ constexpr int rows8_quads(int G) { return (G + 7) / 8 * 2; }  // fours of groups, in whole eights
-
 // A wave makes the tiles of 16 rows and four groups.
 template <int BITS, int GROUP, bool WIDE>
 __global__ __launch_bounds__(256) void rows8_prepare_kernel(const signed char *x, int64_t M, int K, uint4 *tiles, void *sums) {  // WIDE: float32 scales
@@ -359,7 +357,7 @@ hipError_t launch_rows8_tiles(const Rows8Args &a, Rows8Kind kind, int bits, int 
   uint4 *const tiles = static_cast<uint4 *>(workspace);
   char *const sums = static_cast<char *>(workspace) + rows8_tiles_bytes(a.M, a.K);
   const int64_t units = row_tiles(a.M) * rows8_quads(a.K / a.group);
-  if (units >= (int64_t)1 << 25) return hipErrorInvalidValue;  // (a launch has less than 2^32 threads)
+  if (units > kRows8Units) return hipErrorInvalidValue;
   return rows8_with_types(dt, bits, a.group, [&](auto d, auto b, auto g) {
     constexpr int DT = decltype(d)::value, BITS = decltype(b)::value, GROUP = decltype(g)::value;
     rows8_prepare_kernel<BITS, GROUP, DT == 2><<<(unsigned)((units + 3) / 4), 256, 0, st>>>(a.x, a.M, a.K, tiles, sums);

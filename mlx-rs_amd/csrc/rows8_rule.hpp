@@ -48,4 +48,19 @@ constexpr Rows8Kind rows8_kind(int64_t M, int N, int K, bool tiles) {
   return static_cast<Rows8Kind>(best);
 }
 
+// A launch has less than 2^32 threads: blocks of 512 for every kind, and waves of the rows' preparation, in blocks of 256, that take 16 rows and four groups each.
+constexpr int64_t kRows8Blocks = ((int64_t)1 << 23) - 1, kRows8Units = ((int64_t)1 << 25) - 1;
+constexpr int rows8_quads(int G) { return (G + 7) / 8 * 2; }  // fours of groups, in whole eights
+constexpr int64_t rows8_blocks(Rows8Kind kind, int64_t M, int N) {
+  const Rows8Cost &c = kRows8Costs[(int)kind];
+  const int64_t tall = (M + c.rows - 1) / c.rows, wide = ((int64_t)N + c.cols - 1) / c.cols;
+  return tall * (c.tiles ? (wide + 7) / 8 * 8 : wide);
+}
+// rows of a launch, in whole blocks; 0: one block of rows already has too many columns
+constexpr int64_t rows8_step(Rows8Kind kind, int N, int K, int group) {
+  const Rows8Cost &c = kRows8Costs[(int)kind];
+  const int64_t rows = kRows8Blocks / rows8_blocks(kind, 1, N) * c.rows, prepared = kRows8Units / rows8_quads(K / group) * 16 / c.rows * c.rows;
+  return c.tiles && prepared < rows ? prepared : rows;
+}
+
 }  // namespace mi_moe

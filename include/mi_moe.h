@@ -118,7 +118,7 @@ int mi_moe_create(const mi_moe_config *cfg, const mi_moe_weights *weights, mi_mo
 int mi_moe_destroy(mi_moe_handle h);
 /* the workspace with which a batch of max_tokens, and every smaller one, takes the kernels it is given in one of its own */
 int mi_moe_workspace_size(const mi_moe_config *cfg, int64_t max_tokens, size_t *bytes);
-/* x: bf16 [T, H] -> out: bf16 [T, H].  workspace: device memory of at least
+/* x: bf16 [T, H] -> out: bf16 [T, H], T up to 2^26 - 4 and T * top_k up to 2^30.  workspace: device memory of at least
  * mi_moe_workspace_size(cfg, T) bytes, 256-byte aligned, contents irrelevant. */
 int mi_moe_forward(mi_moe_handle h, const uint16_t *x, int64_t T, uint16_t *out,
                    void *workspace, size_t workspace_bytes, const mi_moe_debug_out *dbg,

@@ -571,6 +571,9 @@ static void grouped_args(const mi_moe_config &c, const mi_moe_weights &w, const 
   d.K = c.intermediate;
 }
 
+// A launch has less than 2^32 threads, and the norm, the check of a given routing (a wave a token, four a block) and the sum over the slots 64 a token.
+constexpr int64_t kForwardMostTokens = ((int64_t)1 << 26) - 4;
+
 // The launch sequence of one forward.  ev: nullptr, or kStages + 1 events recorded on the
 // stream before the first launch and after each stage.
 // kt: nullptr, or MI_MOE_N_KERNEL_TIMES timers for the grouped-product kernels (with ev).
@@ -591,6 +594,7 @@ static int forward_impl(mi_moe_handle h, const uint16_t *x_in, int64_t T, uint16
   const mi_moe_config &c = h->cfg;
   const int64_t P = T * c.top_k;
   if (P > (int64_t)1 << 30) return fail("forward: too many (token, expert) pairs");
+  if (T > kForwardMostTokens) return fail("forward: %lld tokens, a call takes up to %lld", (long long)T, (long long)kForwardMostTokens);
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u))
     return fail("forward: workspace must be non-NULL and 256-byte aligned");
   ForwardWs f = carve_forward(c, T, workspace, norm_weight != nullptr);

@@ -81,3 +81,19 @@ def test_a_weight_of_zero_is_no_empty_slot():
     for zero in (0.0, -0.0):
         out = blk.forward_routed(x, inds, torch.full((4, 2), zero, dtype=torch.bfloat16, device="cuda"))
         assert not out[:2].any() and torch.isnan(out[2:]).all()
+
+
+def test_more_tokens_than_a_launch_takes_are_refused():
+    """From 2^26 - 3 tokens on the launches of a wave a token would have 2^32 threads; nothing is launched, and nothing is read."""
+    import mlx_rs_amd as m
+    blk, _ = block(128, 2, 1, 128)
+    x = torch.zeros(4096, dtype=torch.bfloat16, device="cuda")
+    ids = torch.zeros(4096, dtype=torch.int32, device="cuda")
+    lib, p = m.load_library(), x.data_ptr()
+    for T in (2 ** 26 - 3, 2 ** 26, 2 ** 30):
+        for call in (lambda: lib.mi_moe_forward_routed(blk._handle, p, ids.data_ptr(), p, T, p, p, 4096, None, m.ops._stream()),
+                     lambda: lib.mi_moe_forward(blk._handle, p, T, p, p, 4096, None, m.ops._stream())):
+            assert call() != 0 and f"{T} tokens" in m.capi.last_error(), m.capi.last_error()
+    assert lib.mi_moe_forward(blk._handle, p, 2 ** 26 - 4, p, p, 4096, None, m.ops._stream()) != 0 and "workspace too small" in m.capi.last_error()
+    torch.cuda.synchronize()
+    assert not x.any()

@@ -761,7 +761,8 @@ __global__ __launch_bounds__(256) void select_grad_rows_kernel(SelectGradArgs a)
   if (t0 >= a.T) return;
   const int lane = lane_id() & 15, share_bytes = (4 * a.E * (int)sizeof(Raw) + 15) & ~15;
   unsigned char *const out = grad_raw + (threadIdx.x >> 6) * share_bytes;
-  for (int c = lane_id() * 16; c < share_bytes; c += kWave * 16) *reinterpret_cast<uint4 *>(out + c) = make_uint4(0, 0, 0, 0);
+  const uint4 zeros = make_uint4(0, 0, 0, 0);  // (LDS is bytes, which the accesses of either width copy)
+  for (int c = lane_id() * 16; c < share_bytes; c += kWave * 16) __builtin_memcpy(__builtin_assume_aligned(out + c, 16), &zeros, 16);
   const uint32_t id = lane < a.k && t < a.T ? a.idx[t * a.k + lane] : ~0u;
   const bool on = id < (uint32_t)a.E;
   const float l = on ? as_f32(static_cast<const Raw *>(a.logits)[t * a.E + id]) : -INFINITY;
@@ -786,16 +787,22 @@ __global__ __launch_bounds__(256) void select_grad_rows_kernel(SelectGradArgs a)
     if (same && other > tag) mine += its;
   });
   __builtin_amdgcn_wave_barrier();
-  if (first) put_value(out, (lane_id() >> 4) * a.E + (int)id, DT, mine);
+  if (first) {
+    Raw raw;
+    put_value(&raw, 0, DT, mine);
+    __builtin_memcpy(__builtin_assume_aligned(out + ((lane_id() >> 4) * a.E + (int)id) * (int)sizeof(Raw), sizeof(Raw)), &raw, sizeof(Raw));
+  }
   __builtin_amdgcn_wave_barrier();
   const int bytes = (int)(a.T - t0 < 4 ? a.T - t0 : 4) * a.E * (int)sizeof(Raw);
   unsigned char *const to = static_cast<unsigned char *>(a.dlogits) + t0 * a.E * (int64_t)sizeof(Raw);
   for (int c = lane_id() * 16; c < bytes; c += kWave * 16) {
     if (c + 16 <= bytes) {
-      const uint4 v = *reinterpret_cast<const uint4 *>(out + c);
+      uint4 v;
+      __builtin_memcpy(&v, __builtin_assume_aligned(out + c, 16), 16);
       __builtin_memcpy(__builtin_assume_aligned(to + c, sizeof(Raw)), &v, 16);
     } else {
-      for (int i = c; i < bytes; i += (int)sizeof(Raw)) *reinterpret_cast<Raw *>(to + i) = *reinterpret_cast<const Raw *>(out + i);
+      for (int i = c; i < bytes; i += (int)sizeof(Raw))
+        __builtin_memcpy(__builtin_assume_aligned(to + i, sizeof(Raw)), __builtin_assume_aligned(out + i, sizeof(Raw)), sizeof(Raw));
     }
   }
 }

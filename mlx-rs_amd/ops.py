@@ -9,6 +9,7 @@ patterns (torch has no arithmetic on uint32).
 import ctypes as C
 import functools
 import importlib.util
+import operator
 import os
 import warnings
 
@@ -160,10 +161,18 @@ def gather_qmm(x, w, scales, biases, lhs_indices=None, rhs_indices=None, transpo
     return y.reshape(*out_batch, M, N)
 
 
+def _int32(who, *args):
+    """(name, value), ...: whole numbers that go to the library in 32 bits, to which a larger one would be cut without a word."""
+    for name, value in args:
+        if not -2 ** 31 <= operator.index(value) < 2 ** 31:
+            raise capi.MoeError(f"{who}: {name} is out of range, got {value}")
+
+
 def _check_qmat(who, w, scales, biases, K, transpose, group_size, bits):
     """Shapes of one quantized matrix against x's K: returns N.  w [N, K*bits/32] and scales / biases
     [N, K/group_size] with transpose, w [K, N*bits/32] and scales / biases [K, N/group_size] without."""
     if bits not in (2, 4, 8) or group_size not in (32, 64, 128):
+        _int32(who, ("group_size", group_size), ("bits", bits))
         return None  # the library words the refusal
     per = 32 // bits
     if transpose:
@@ -294,6 +303,7 @@ def quantized_linear_rows8(x, row_scales, w, scales, biases, linear_bias=None, g
     if row_scales.shape != x.shape[:-1]:
         raise capi.MoeError(f"{who}: row_scales must be {tuple(x.shape[:-1])}, got {tuple(row_scales.shape)}")
     K, N = x.shape[-1], w.shape[0]
+    _int32(who, ("K", K), ("N", N))
     _check_qmat(who, w, scales, biases, K, True, group_size, bits)
     if linear_bias is not None:
         _need(linear_bias, scales.dtype, "linear_bias")
@@ -350,6 +360,7 @@ def _norm_operands(who, x, residual, weight):
             raise capi.MoeError(f"{who}: residual must be {tuple(x.shape)} as x, got {tuple(residual.shape)}")
     _together(who, x, residual, weight)
     H = x.shape[-1]
+    _int32(who, ("hidden", H))
     return dt, x.numel() // H if H else 0, H
 
 
@@ -482,8 +493,9 @@ def select_experts(logits, top_k, scoring="softmax", bias=None, n_groups=1, top_
         if bias.numel() != E:
             raise capi.MoeError(f"select_experts: bias must have {E} elements, got {bias.numel()}")
     _together("select_experts", logits, bias)
+    _int32("select_experts", ("n_experts", E), ("top_k", top_k), ("n_groups", n_groups), ("top_groups", top_groups))
     T = logits.numel() // E if E else 0
-    shape = logits.shape[:-1] + (max(int(top_k), 0),)
+    shape = logits.shape[:-1] + (min(max(int(top_k), 0), E),)  # (outside of that the library refuses the call)
     inds = torch.empty(shape, dtype=torch.int32, device=logits.device)
     weights = torch.empty(shape, dtype=dtype, device=logits.device)
     check(lib.mi_moe_select_experts(_ptr(logits), dt, _ptr(bias), T, E, top_k, _choice("select_experts", _SCORINGS, scoring, "scoring"), n_groups, top_groups,
@@ -505,6 +517,7 @@ def select_experts_grad(dweights, logits, inds, scoring="softmax", renormalize=T
         raise capi.MoeError(f"select_experts_grad: inds and dweights must be {tuple(logits.shape[:-1])} + (k,), got {tuple(inds.shape)} and {tuple(dweights.shape)}")
     _together("select_experts_grad", logits, dweights, inds)
     E = logits.shape[-1]
+    _int32("select_experts_grad", ("n_experts", E), ("top_k", inds.shape[-1]))
     dlogits = torch.empty_like(logits)
     check(lib.mi_moe_select_experts_grad(_ptr(dweights), wt, _ptr(logits), dt, _ptr(inds), logits.numel() // E if E else 0, E, inds.shape[-1],
                                          _choice("select_experts_grad", _SCORINGS, scoring, "scoring"), int(bool(renormalize)), float(scale), _ptr(dlogits),

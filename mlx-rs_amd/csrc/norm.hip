@@ -395,7 +395,7 @@ __global__ __launch_bounds__(norm_grad_threads(TPR, TOGETHER), 4) void norm_grad
       for (int i = 0; i < 8; ++i) {
         const double v = R.h[c].at(i);
         ss = __builtin_fma(v, v, ss);
-        const double g = DT == 2 ? (double)w[c].at(i) * (double)R.dy[c].at(i) : (double)(w[c].at(i) * R.dy[c].at(i));  // (exact either way)
+        const double g = DT == 2 ? (double)w[c].at(i) * (double)R.dy[c].at(i) : (double)(w[c].at(i) * R.dy[c].at(i));  // (exact of float16; of bfloat16 within the floats' range)
         dot = __builtin_fma(g, v, dot);
       }
     ss = wave_sum_f64(ss);

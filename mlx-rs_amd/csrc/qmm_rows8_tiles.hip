@@ -77,7 +77,7 @@ __device__ __forceinline__ void copy_scalars_to_lds(i32x4_t rsrc, uint32_t voff,
 // 149 in windows).  Codes: 64 or 128 bytes of a weight row a stage, its 16-byte pieces in an order turned by the row, so that the lanes' reads meet all banks.
 // A group is one matrix instruction a 16 x 16 tile (two for 128 values, one of half the depth for 32), whose integer sums are exact; then a subtraction and a
 // multiply-add a result.  What bounds it is those, a matrix unit and a vector unit that do not run at once (kWhole): 4096 x 4096 x 4096, 4-bit, groups of 64, 144 us with the rows' preparation
-// (956 TFLOP/s), groups of 128 1320 TFLOP/s, 32 730.  The biases' terms are a product over the groups as well, eight of them a bf16 instruction: the sums in two exact values, their factors
+// (956 TFLOP/s), groups of 128 1320 TFLOP/s, 32 710; counted, vector instructions are 0.86 of a SIMD's cycles and matrix units at work in 0.29.  The biases' terms are a product over the groups as well, eight of them a bf16 instruction: the sums in two exact values, their factors
 // b + 8 s (b + 128 s) in as many as hold all of it.  Of bf16 scales those are two: where the smaller of b and 8 s is below half a step of the larger, it is what the first piece leaves, and has
 // eight bits; where it is not, its last bit is 2^-15 or more of the larger's power of two, and what a piece of eight bits leaves, 2^-7 of that at most, has eight again.  Of f16 scales, of eleven bits, they are
 // three, the last in an instruction of half the depth (with two, a factor's error would be up to 2^-17 of it; 77 and 45 us for 75 and 44 with 2048 and 777 rows, 4096 x 4096, 8-bit).  (Four groups of

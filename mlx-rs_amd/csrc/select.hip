@@ -161,7 +161,7 @@ __device__ __forceinline__ void select_exact(const SelectKernelArgs &p, const Sl
 // the sum, which is the same factor for all of a token's; scores are at most one, so two of them differ by what doubles say to within 1.9 * 2^-20, and biased keys to within 2^-23 of their size more.
 // A sigmoid is 1 / (1 + e): a quarter of the exponential's error at most, a rounding and the reciprocal, together 3.9 * 2^-24.
 // Where two keys that follow each other in the choice, or two groups' ranks, are nearer than near_of and kNearOfSize of them allow, or something is an infinity above zero or no number, doubles decide
-// (for one token in some hundred); without a bias the logits are exact keys.  Scores of the chosen are in double, a lane each, of softmax scores that are renormalised from the chosen logits
+// (of random logits and small biases, 256 experts, for one token in 1700, 512 experts with 16 chosen one in 370); without a bias the logits are exact keys.  Scores of the chosen are in double, a lane each, of softmax scores that are renormalised from the chosen logits
 // alone: they hold where a softmax over all would round to zero.
 constexpr float kNearOfSize = 0x1p-21f;
 __device__ __forceinline__ float near_of(const SelectArgs &a) { return a.scoring == 1 ? 0x1p-21f : 0x1p-19f; }
@@ -363,16 +363,20 @@ __global__ __launch_bounds__(256) void select_experts_kernel(SelectKernelArgs p)
 }
 
 // ---------------------------------------------------------------- up to 16 groups and 16 choices: a row of 16 lanes a token
-// The same choice with four tokens in a wave and up to 32 experts a lane: what a round of the choice exchanges between lanes stays in a row, and a wave's instructions, which are
-// what bounds the selection, serve four tokens.  What floats do not decide is gone over by the whole wave, a token after the other.  It takes over where there is a wave for each SIMD.  us, a row / a wave a token, bf16 logits
-// but for the groups, 2048, 4096, 8192 tokens:
-//   128 experts, 8 chosen               4.6 / 4.5    4.7 / 5.5    5.3 / 7.7
-//   512, 10                             8.7 / 6.8    8.8 / 10.0   10.8 / 16.4
-//   256, 8, sigmoid, bias               9.2 / 9.3    9.4 / 10.3   10.1 / 15.2
-//   256, 8, sigmoid, bias, 8 groups    13.4 / 11.1  13.5 / 13.4   12.2 / 17.9
-//   512, 16, sigmoid, bias             24.1 / 19.5  25.2 / 25.1   29.2 / 36.6
-// At one token they are 4.6 and 4.0 in the first line, 8.5 and 6.0 in the fourth.  8192 tokens of 256 float32 logits are 8.4 MB, 1.7 us of a copy's traffic: what bounds the choice are its
-// instructions, some 20 for each chosen and two for each expert and chosen, and the double exponentials of the weights; where doubles decide, in half of the fourth line's waves, theirs too.
+// The same choice with four tokens in a wave and up to 32 experts a lane: what a round of the choice exchanges between lanes stays in a row, and a wave's instructions serve four
+// tokens.  Candidates whose order floats do not decide are ordered by their double scores; where they do not decide which those are, the whole wave goes over the token in double, a token
+// after the other.  It takes over where there is a wave for each SIMD.  us, a row / a wave a token, bf16 logits but for the groups, of 2048, 4096 and 8192 tokens that floats decide:
+//   128 experts, 8 chosen               4.6 / 4.5    4.7 / 5.5    5.3 / 7.5
+//   512, 10                             8.7 / 6.8    8.8 / 9.7   11.0 / 15.6
+//   256, 8, sigmoid, bias               9.2 / 6.9    9.4 / 8.8   10.8 / 12.7
+//   256, 8, sigmoid, bias, 8 groups    10.4 / 7.7   10.7 / 10.1  12.2 / 14.6
+//   512, 16, sigmoid, bias             16.5 / 12.2  16.9 / 17.8  21.6 / 27.8
+// and of random ones, some of which (0.006 % to be gone over by a row's wave in the fourth line, 0.05 % to be ordered; all of those to be gone over where a wave has a token) floats do not:
+//   256, 8, sigmoid, bias               9.5 / 9.0    9.5 / 10.9  10.7 / 13.3
+//   256, 8, sigmoid, bias, 8 groups    10.6 / 11.0  14.0 / 11.1  13.9 / 16.5
+//   512, 16, sigmoid, bias             23.7 / 18.5  23.7 / 23.7  28.4 / 33.6
+// 8192 tokens of 256 float32 logits are 8.4 MB, 1.7 us of a copy's traffic.  What bounds the choice is the length of a wave's chain, not what the chip issues: four times the tokens take 1.2
+// times as long (a round for each chosen, each over all of a lane's experts and then over the row; the weights' double exponentials), and a wave that goes over a token in double, 2 to 7 us longer, ends last.
 constexpr int64_t kSelectWaves = 1024;
 __device__ __forceinline__ uint32_t row_max(uint32_t v) {
   uint32_t o;

@@ -33,7 +33,7 @@ constexpr Rows8Cost kRows8Costs[] = {
     {64, 64, true, 8.7f, 14.5f, 10.3f, 1.7f},  {64, 128, true, 8.5f, 27.5f, 15.0f, 2.0f},  {128, 128, true, 10.5f, 43.0f, 28.0f, 2.0f},
 };
 constexpr float rows8_time(const Rows8Cost &c, int64_t M, int N, int K) {
-  const int64_t tall = (M + c.rows - 1) / c.rows, wide = (N + c.cols - 1) / c.cols;
+  const int64_t tall = (M + c.rows - 1) / c.rows, wide = ((int64_t)N + c.cols - 1) / c.cols;
   const float blocks = c.tiles ? 8.f * (float)((wide + 7) / 8 * tall) : (float)(wide * tall), k = (float)K / 4096.f;
   const float x = blocks > 256.f ? blocks / 256.f : 1.f;
   return c.start + c.first * k + (x - 1.f) * (c.more * k + c.more0);

@@ -55,3 +55,11 @@ def test_columns_beyond_a_launch(rule):
     for kind in range(8):
         assert rule.step(kind, 2 ** 31 - 1, 128, 64) >= 0
     assert rule.step(0, 2 ** 31 - 1, 128, 64) == 0
+
+
+@pytest.mark.parametrize("tiles", [False, True])
+def test_the_rule_at_the_most_columns(rule, tiles):
+    """A count of columns that ends just below 2^31 takes what one a block below takes."""
+    for m in (3, 17, 40, 300, 5000):
+        for k in (128, 4096):
+            assert rule.kind(m, 2 ** 31 - 1, k, tiles) == rule.kind(m, 2 ** 31 - 2 ** 12, k, tiles), (m, k)

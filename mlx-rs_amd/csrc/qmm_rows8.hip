@@ -188,7 +188,8 @@ static hipError_t start_dot(const Rows8Args &a, hipStream_t st) {
 // A block multiplies 16 MI rows by 16 NI columns; its eight waves share K, a run of stages of 128 values each, and meet in LDS in a fixed order.  Nothing is prepared: a wave
 // loads its codes, scales and rows straight into registers (a stage ahead), unpacks the codes in the rows' own order, and forms the group sums beside the products
 // (a lane's part of them is an operand of the biases' product as it is).
-// What bounds it is the L1 cache's tags: an operand's 16 rows are 16 lanes that follow each other, so a load is 64 accesses whatever its width.  So every load is 16 bytes a lane, also where a lane's
+// What bounds it is the L1 cache's tags: an operand's 16 rows are 16 lanes that follow each other, so a load is 64 accesses whatever its width (counted, 0.76 lookups a
+// cycle at 16 x 14336, 0.72 at 64 x 4096).  So every load is 16 bytes a lane, also where a lane's
 // values are then not those that one product of a group wants of it, and scales come for several stages at once.  us, 4-bit, groups of 64, before (8 bytes of codes and a stage's scales a load) / so:
 //   8 x 4096, 4096 values 7.5 / 5.4   16 x 14336 21.9 / 12.7   32 x 4096 10.2 / 7.7   64 x 4096 14.3 / 11.0   128 x 4096 19.4 / 16.6   16 x 14336, groups of 32 35 / 16.3
 // (Whole lines through LDS, passed to the lanes there: 10.1 for 16 x 4096, 32 for 16 x 14336.)

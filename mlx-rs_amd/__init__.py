@@ -10,8 +10,8 @@ There is no CPU fallback: every call fails loudly when the library is missing.
 from . import capi  # noqa: F401
 from .capi import MoeError, library_path, load_library  # noqa: F401
 from . import ops  # noqa: F401
-from .moe import MoeConfig, QuantizedSwitchLinear, SparseMoeBlock  # noqa: F401
+from .moe import F8SwitchLinear, MoeConfig, QuantizedSwitchLinear, SparseMoeBlock, SwitchGluF8  # noqa: F401
 from . import synth  # noqa: F401
 
 __all__ = ["capi", "ops", "synth", "MoeError", "MoeConfig", "QuantizedSwitchLinear",
-           "SparseMoeBlock", "load_library", "library_path"]
+           "SparseMoeBlock", "F8SwitchLinear", "SwitchGluF8", "load_library", "library_path"]

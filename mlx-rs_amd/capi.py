@@ -1,4 +1,4 @@
-"""ctypes binding of include/mi_moe.h and include/mi_moe_layer.h (one function per exported symbol)."""
+"""ctypes binding of include/mi_moe.h, include/mi_moe_layer.h and include/mi_moe_f8.h (one function per exported symbol)."""
 import ctypes as C
 import os
 
@@ -40,6 +40,12 @@ LAYER_EXPORTS = (
     "mi_moe_forward_routed", "mi_moe_select_experts", "mi_moe_select_experts_grad",
     "mi_moe_quantized_linear_rows8_workspace_size", "mi_moe_quantized_linear_rows8",
 )
+# and include/mi_moe_f8.h
+F8_EXPORTS = (
+    "mi_moe_sort_tokens_workspace_size", "mi_moe_sort_tokens", "mi_moe_sort_tokens_grad", "mi_moe_unsort_tokens", "mi_moe_unsort_tokens_grad",
+    "mi_moe_quantize_f8", "mi_moe_dequantize_f8", "mi_moe_linear_f8_workspace_size", "mi_moe_linear_f8", "mi_moe_grouped_linear_f8",
+    "mi_moe_switch_glu_f8_workspace_size", "mi_moe_switch_glu_f8", "mi_moe_switch_glu_f8_grad",
+)
 
 
 class MoeError(RuntimeError):
@@ -63,6 +69,10 @@ class QMat(C.Structure):
 class Weights(C.Structure):
     _fields_ = [("router_w", C.c_void_p), ("router_bias", C.c_void_p),
                 ("gate", QMat), ("up", QMat), ("down", QMat)]
+
+
+class F8Experts(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("gate", "up", "down", "gate_scales", "up_scales", "down_scales")]
 
 
 class DebugOut(C.Structure):
@@ -138,6 +148,19 @@ def load_library():
         "mi_moe_select_experts_grad": [vp, i32, vp, i32, vp, i64, i32, i32, i32, i32, C.c_float, vp, vp],
         "mi_moe_quantized_linear_rows8_workspace_size": [i64, i32, C.POINTER(sz)],
         "mi_moe_quantized_linear_rows8": [vp, vp, vp, vp, vp, vp, i64, i32, i32, i32, i32, i32, vp, vp, sz, vp],
+        "mi_moe_sort_tokens_workspace_size": [i64, i32, i32, C.POINTER(sz)],
+        "mi_moe_sort_tokens": [vp, vp, i64, i32, i32, i32, i32, vp, vp, vp, vp, vp, sz, vp],
+        "mi_moe_sort_tokens_grad": [vp, vp, i64, i32, i32, i32, vp, vp],
+        "mi_moe_unsort_tokens": [vp, vp, i32, vp, i64, i32, i32, i32, vp, vp],
+        "mi_moe_unsort_tokens_grad": [vp, vp, vp, i32, vp, i64, i32, i32, i32, vp, vp, vp],
+        "mi_moe_quantize_f8": [vp, i32, i64, i64, i32, vp, vp, vp],
+        "mi_moe_dequantize_f8": [vp, vp, i64, i64, i32, i32, vp, vp],
+        "mi_moe_linear_f8_workspace_size": [i64, i32, C.POINTER(sz)],
+        "mi_moe_linear_f8": [vp, vp, vp, vp, i64, i32, i32, i32, i32, vp, vp, sz, vp],
+        "mi_moe_grouped_linear_f8": [vp, vp, vp, vp, i64, i32, i32, i32, i32, i32, vp, vp, sz, vp],
+        "mi_moe_switch_glu_f8_workspace_size": [i64, i32, i32, i32, i32, i32, C.POINTER(sz)],
+        "mi_moe_switch_glu_f8": [vp, vp, vp, i32, C.POINTER(F8Experts), i64, i32, i32, i32, i32, i32, vp, vp, sz, vp],
+        "mi_moe_switch_glu_f8_grad": [vp, vp, vp, vp, i32, C.POINTER(F8Experts), i64, i32, i32, i32, i32, i32, vp, vp, vp, sz, vp],
         "mi_moe_debug_plan_forward": [C.POINTER(Config), i64, C.c_char_p, sz],
         "mi_moe_debug_tile_rule": [C.POINTER(Config), i64, C.POINTER(i32), C.POINTER(i32)],
         "mi_moe_debug_plan_grouped": [i32, i32, i32, i32, i64, i32, i64, i64, i32, i32, C.c_char_p, sz],

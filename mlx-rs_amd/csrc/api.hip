@@ -6,12 +6,11 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
-#include <exception>
 #include <memory>
 #include <mutex>
 #include <new>
 
-#include "common.hpp"
+#include "entries.hpp"
 
 using namespace mi_moe;
 
@@ -34,7 +33,9 @@ struct Handler {
 std::mutex g_handler_lock;
 std::shared_ptr<Handler> g_handler;
 
-int fail(const char *fmt, ...) __attribute__((format(printf, 1, 2)));
+}  // namespace
+
+namespace mi_moe {
 int fail(const char *fmt, ...) {
   va_list ap;
   va_start(ap, fmt);
@@ -48,25 +49,9 @@ int fail(const char *fmt, ...) {
   if (h && h->fn) h->fn(g_last_error, h->data);
   return 1;
 }
+}  // namespace mi_moe
 
-// No exception leaves an entry point: every extern "C" body is a function-try-block that ends in this.
-#define MI_CATCH(name)                                                                  \
-  catch (const std::exception &ex_) { return fail(name ": %s", ex_.what()); }           \
-  catch (...) { return fail(name ": unknown C++ exception"); }
-
-int hip_fail(const char *what, hipError_t e) {
-  return fail("%s: %s", what, hipGetErrorString(e));
-}
-
-#define MI_HIP(call)                                   \
-  do {                                                 \
-    hipError_t e_ = (call);                            \
-    if (e_ != hipSuccess) return hip_fail(#call, e_);  \
-  } while (0)
-
-bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
-size_t align_up(size_t v, size_t a = 256) { return (v + a - 1) / a * a; }
+namespace {
 
 // the block runs on the tuned kernels with 4- or 8-bit codes in groups of 64; other group sizes take the
 // products on raw codes where those serve the shape (ForwardWs::raw), the rest and 2-bit codes the plain products
@@ -99,21 +84,6 @@ int check_qmat(const mi_moe_qmat &m, const char *name) {
     return fail("%s: pointers must be 16-byte aligned", name);
   return 0;
 }
-
-// carve consecutive 256-byte aligned regions out of a workspace; the first one starts at the next
-// 256-byte boundary (every *_workspace_size reserves 256 bytes for that)
-struct Carver {
-  char *base;
-  size_t off = 0;
-  explicit Carver(void *p)
-      : base(reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(p) + 255u) & ~(uintptr_t)255u)) {}
-  template <typename T>
-  T *take(size_t n) {
-    T *p = reinterpret_cast<T *>(base + off);
-    off += align_up(n * sizeof(T));
-    return p;
-  }
-};
 
 struct ForwardWs {
   uint16_t *logits;

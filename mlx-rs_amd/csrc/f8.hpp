@@ -1,0 +1,235 @@
+// Linear layers and experts on e4m3 weights with a scale for each block of 128 x 128, and rows in e4m3 with a scale for each run of 128 values:
+// launchers, and what their kernels share.
+//
+//   W[n][k] = scale[n / 128][k / 128] * code[n][k]        x[r][k] = scale[r][k / 128] * code[r][k]
+//   y[r][n] = sum over runs j of  sx[r][j] * sw[n / 128][j] * (sum over the run's 128 products of codes)
+//
+// A run's products are summed by the matrix instructions on codes; scales come in once a run, in float32.
+//
+// The f8 matrix instructions line a sum's products up with the largest of them and keep some thirteen bits below it (measured: a result is off by up to 2^-11 of its
+// largest product, 1.4e-5 of the results' length with normally distributed rows and weights, with 16x16x128, 16x16x32 and 32x32x64 alike).  A result of 16 bits does not
+// show that (a rounding to bfloat16 is off by 1.7e-3 of the length, to float16 by 2.1e-4); results in float32 are computed with the bf16 instructions instead, on codes
+// taken to bf16, where every product is exact and sums are float32.
+#pragma once
+#include "common.hpp"
+
+namespace mi_moe {
+
+constexpr int kF8Run = 128;
+__host__ __device__ constexpr int f8_runs(int n) { return (n + kF8Run - 1) / kF8Run; }
+__host__ __device__ inline int64_t f8_row_bytes(int k) { return (int64_t)f8_runs(k) * kF8Run; }  // of a row of codes in a workspace: whole runs, zeros behind the last value
+
+// rows in e4m3 as the products read them: codes [rows][whole runs], scales [runs][rows]
+struct F8Rows {
+  const uint8_t *codes;
+  const float *scales;
+  int64_t rows;
+};
+struct F8Mat {
+  const uint8_t *w;
+  const float *s;
+};
+struct F8Product {
+  F8Rows x;
+  const uint32_t *order;    // sorted row r reads x row order[r] / k_div; nullptr: r
+  int k_div;
+  const uint32_t *offsets;  // matrix e has the rows from offsets[e] to offsets[e + 1]; rows behind the last are zeros of y.  nullptr: one matrix, all rows
+  int n_mats;
+  int64_t rows;             // of y
+  F8Mat m[2];               // the second one: of a gate/up pair (y1 or h), or of a second half of the summed axis (pair_sum)
+  bool transpose;           // matrices [N][K], else [K][N]
+  bool pair_sum;
+  int N, K;
+  const void *bias;
+  void *y, *y1;
+  int dt;
+  uint8_t *h;  // gate/up pairs: silu(gate) * up in e4m3, as F8Rows
+  float *hs;
+};
+bool f8_few_rows(const F8Product &p);                     // which of the two the product takes
+hipError_t launch_f8_few(const F8Product &p, hipStream_t st);    // a few rows a matrix (f8_few.hip); transposed only
+hipError_t launch_f8_tiles(const F8Product &p, hipStream_t st);  // tiles (f8_tiles.hip)
+inline hipError_t launch_f8_product(const F8Product &p, hipStream_t st) { return f8_few_rows(p) ? launch_f8_few(p, st) : launch_f8_tiles(p, st); }
+
+// f8_rows.hip.  Codes go to `codes` + row * code_stride, the scale of a row's run j to scales[row * row_stride + j * run_stride].
+struct F8Out {
+  uint8_t *codes;
+  int64_t code_stride;
+  float *scales;
+  int64_t row_stride, run_stride;
+  bool pad;  // zeros up to the end of the last run
+};
+inline F8Out f8_workspace_rows(uint8_t *codes, float *scales, int64_t rows, int cols) { return {codes, f8_row_bytes(cols), scales, 1, rows, true}; }
+hipError_t launch_quantize_f8_rows(const void *x, int dt, int64_t rows, int cols, const F8Out &to, hipStream_t st);
+hipError_t launch_quantize_f8_blocks(const void *x, int dt, int64_t rows, int cols, uint8_t *codes, float *scales, hipStream_t st);
+hipError_t launch_dequantize_f8(const uint8_t *codes, const float *scales, int64_t rows, int cols, int block_rows, int dt, void *out, hipStream_t st);
+// h = silu(gate) * up of float32 rows, in e4m3
+hipError_t launch_swiglu_f8(const float *g, const float *u, int64_t rows, int cols, const F8Out &to, hipStream_t st);
+// Its gradient for sorted rows: dh (but for the slot's weight) float32; dg and du in e4m3, one row of both (dg's runs first), and the weights' gradient
+struct F8SwigluGrad {
+  const float *g, *u, *dh;
+  const void *weights;
+  int w_dtype;
+  const uint32_t *order, *offsets;  // offsets[n_experts]: where the named rows end
+  int n_experts;
+  int64_t rows;
+  int cols;
+  uint8_t *codes;
+  float *scales;
+  void *dweights;
+};
+hipError_t launch_swiglu_f8_grad(const F8SwigluGrad &a, hipStream_t st);
+
+// Tokens sorted by expert (sort_tokens.hip).  inverse: a slot's row, or -1 - row where it names no expert (those rows lie behind the others').
+struct SortTokens {
+  const uint32_t *ids;
+  int64_t T;
+  int k, E;
+  uint32_t *order;
+  int32_t *inverse;
+  uint32_t *offsets;  // [E + 1]
+};
+size_t sort_tokens_bytes(int64_t T, int k, int E);
+// rows != nullptr: the sorted rows of x, those that no slot names zeros
+hipError_t launch_sort_tokens(const SortTokens &a, const void *x, int dt, int H, void *rows, void *scratch, hipStream_t st);
+// weights nullptr: sums without weights (the sorting's gradient)
+hipError_t launch_unsort_tokens(const void *rows, const void *weights, int w_dtype, const int32_t *inverse, int64_t T, int k, int H, int dt, void *out,
+                                hipStream_t st);
+hipError_t launch_unsort_tokens_grad(const void *dout, const void *rows, const void *weights, int w_dtype, const int32_t *inverse, int64_t T, int k, int H, int dt,
+                                     void *drows, void *dweights, hipStream_t st);
+
+#ifdef __HIPCC__
+// ---------------------------------------------------------------- codes
+constexpr float kF8Most = 448.f;
+
+// scale = largest / 448, what it makes of the values (quotient and code as the definition rounds them), and whether they have codes at all: a run of zeros has a scale and
+// codes of zero, one that holds an infinity or a NaN codes of zero and a scale that is NaN, so that what is made of it is, too.
+struct F8Scale {
+  float scale, inv;
+  bool coded, plain;
+  __device__ __forceinline__ explicit F8Scale(uint32_t largest_bits) {
+    const float most = __uint_as_float(largest_bits);
+    coded = largest_bits < 0x7f800000u;
+    scale = coded ? most / kF8Most : NAN;
+    coded = coded && scale > 0.f;
+    // reciprocal and residual: with inv = round(1 / scale), q0 = round(v inv) is off by at most an ulp, and round(q0 + (v - q0 scale) inv) is the correctly rounded
+    // quotient, if the residual is exact: with scale above 2^-93 it is no smaller than the least float for every quotient that has a code (2^-10 and more).
+    plain = largest_bits < 0x17800000u;  // 2^-80
+    inv = coded ? 1.f / scale : 0.f;
+  }
+  __device__ __forceinline__ float quotient(float v) const {
+    float q;
+    if (plain) {
+      q = coded ? v / scale : 0.f;
+    } else {
+      const float q0 = v * inv;
+      q = __builtin_fmaf(__builtin_fmaf(-q0, scale, v), inv, q0);
+    }
+    return __builtin_amdgcn_fmed3f(q, -kF8Most, kF8Most);  // (beyond it where the scale itself is a few of the least floats)
+  }
+  // four codes, the first value's in the low byte
+  __device__ __forceinline__ uint32_t codes(float a, float b, float c, float d) const {
+    if (!coded) return 0u;
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(quotient(a), quotient(b), 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(quotient(c), quotient(d), w, true);
+  }
+};
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }  // ordered as the magnitudes, NaN behind infinity
+__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
+__device__ __forceinline__ uint32_t max_of_16_lanes(uint32_t m) {
+  m = umax(m, dpp_u32<kDppXor1>(m));
+  m = umax(m, dpp_u32<kDppXor2>(m));
+  m = umax(m, dpp_u32<kDppHalfMirror>(m));
+  return umax(m, dpp_u32<kDppMirror>(m));
+}
+__device__ __forceinline__ float silu(float g) { return g / (1.f + __expf(-g)); }
+
+// ---------------------------------------------------------------- segments
+// Tile m of the segments that offsets[n_mats + 1] cut the rows into, in pieces of `tile` rows: matrix, first row and number of rows.  Behind the segments' tiles come those of the
+// rows that belong to none (matrix n_mats), behind those nothing (rows 0).  By one wave; offsets out of order or range only make pieces that overlap or are missing.
+struct F8Piece {
+  int mat;
+  uint32_t row, rows;
+};
+__device__ __forceinline__ F8Piece f8_piece(const uint32_t *__restrict__ offsets, int n_mats, uint32_t total, uint32_t tile, uint32_t m) {
+  if (!offsets) {
+    const uint32_t row = m * tile;
+    return {0, row, row >= total ? 0u : total - row < tile ? total - row : tile};
+  }
+  const int lane = lane_id();
+  uint32_t before = 0;
+  for (int e0 = 0; e0 <= n_mats; e0 += kWave) {
+    const int e = e0 + lane;
+    uint32_t lo = 0, hi = 0;
+    if (e <= n_mats) {
+      lo = offsets[e];
+      hi = e < n_mats ? offsets[e + 1] : total;
+      lo = lo < total ? lo : total;
+      hi = hi < lo ? lo : hi < total ? hi : total;
+    }
+    const uint32_t tiles = (hi - lo + tile - 1) / tile;
+    uint32_t upto = tiles;
+    for (int d = 1; d < kWave; d <<= 1) {
+      const uint32_t v = __shfl_up(upto, d, kWave);
+      if (lane >= d) upto += v;
+    }
+    const uint64_t found = __ballot(m < before + upto);
+    if (found) {
+      const int at = __builtin_amdgcn_readfirstlane((int)__builtin_ctzll(found));
+      const uint32_t first = m - before - (uint32_t)(__builtin_amdgcn_readlane((int)upto, at) - __builtin_amdgcn_readlane((int)tiles, at));
+      const uint32_t slo = (uint32_t)__builtin_amdgcn_readlane((int)lo, at), shi = (uint32_t)__builtin_amdgcn_readlane((int)hi, at);
+      const uint32_t row = slo + first * tile;
+      return {e0 + at, row, shi - row < tile ? shi - row : tile};
+    }
+    before += (uint32_t)__builtin_amdgcn_readlane((int)upto, kWave - 1);
+  }
+  return {0, 0, 0};
+}
+inline int64_t f8_most_pieces(const F8Product &p, int tile) {
+  if (!p.offsets) return (p.rows + tile - 1) / tile;
+  return p.rows / tile + (p.n_mats + 1 < p.rows ? p.n_mats + 1 : p.rows) ;
+}
+
+// ---------------------------------------------------------------- products
+typedef int32_t i32x8_t __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4_f8 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ f32x16_t mfma_f8_32(i32x8_t a, i32x8_t b, f32x16_t c) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4_t mfma_f8_16(i32x8_t a, i32x8_t b, f32x4_t c) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
+}
+// eight codes as bf16 (exact)
+__device__ __forceinline__ bf16x8_t codes_to_bf16(uint32_t lo, uint32_t hi) {
+  typedef __bf16 pair_t __attribute__((ext_vector_type(2)));
+  struct { pair_t p[4]; } v = {{__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false), __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true),
+                                __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false), __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true)}};
+  return __builtin_bit_cast(bf16x8_t, v);
+}
+__device__ __forceinline__ void store4(void *base, int64_t at, int n, int dt, const float v[4]) {  // n of four values, rounded
+  if (dt == 2) {
+    float *p = static_cast<float *>(base) + at;
+    if (n >= 4) __builtin_memcpy(p, v, 16);
+    else
+      for (int i = 0; i < n; ++i) p[i] = v[i];
+    return;
+  }
+  uint16_t *p = static_cast<uint16_t *>(base) + at;
+  uint16_t o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = dt == 0 ? f32_to_bf16(v[i]) : __builtin_bit_cast(uint16_t, (_Float16)v[i]);
+  if (n >= 4) __builtin_memcpy(p, o, 8);
+  else
+    for (int i = 0; i < n; ++i) p[i] = o[i];
+}
+__device__ __forceinline__ float value_of(const void *base, int64_t at, int dt) {
+  return dt == 0 ? bf16_to_f32(static_cast<const uint16_t *>(base)[at]) : dt == 1 ? (float)static_cast<const _Float16 *>(base)[at] : static_cast<const float *>(base)[at];
+}
+__device__ __forceinline__ void put_value(void *base, int64_t at, int dt, float v) {
+  if (dt == 0) static_cast<uint16_t *>(base)[at] = f32_to_bf16(v);
+  else if (dt == 1) static_cast<_Float16 *>(base)[at] = (_Float16)v;
+  else static_cast<float *>(base)[at] = v;
+}
+#endif
+
+}  // namespace mi_moe

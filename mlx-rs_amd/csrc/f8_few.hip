@@ -1,0 +1,112 @@
+// Product of a few rows a matrix with e4m3 weights: one token's or a decode batch's linear layers and experts.  Memory bound: a matrix's codes are read once for up to
+// 16 TG rows.
+//
+// A block of four waves computes 16 weight rows (the rows of a 16x16x128 matrix instruction) for up to 16 TG token rows (its columns).  The waves share the summed
+// axis, every fourth run of 128 values each; a lane's 32 bytes of a run are two pieces of 16, at 16 (l / 16) and 64 bytes on, for codes and rows alike (which values a lane
+// multiplies is free as long as both sides agree), so that one load takes 64 consecutive bytes of a weight row.  Codes go from memory into the instruction's
+// registers, nothing is unpacked; token rows come the same way out of L2.  A run's sums are scaled in float32; the waves' sums meet in LDS in a fixed order.
+#include "f8.hpp"
+
+namespace mi_moe {
+
+constexpr int kFewWaves = 4;
+
+template <int TG, bool F32>  // F32: on the bf16 instructions
+__global__ __launch_bounds__(kFewWaves *kWave) void f8_few_kernel(F8Product a) {
+  constexpr int AHEAD = TG == 1 ? 4 : 2;  // runs whose loads are in flight at once
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ln = lane & 15, part = lane >> 4;
+  const int tiles = (a.N + 15) / 16, which = (int)blockIdx.x / tiles, n0 = ((int)blockIdx.x - which * tiles) * 16;
+  const F8Piece piece = f8_piece(a.offsets, a.n_mats, (uint32_t)a.rows, 16 * TG, blockIdx.y);
+  if (piece.rows == 0) return;
+  void *const y = which ? a.y1 : a.y;
+  if (piece.mat == a.n_mats) {  // rows of no matrix
+    const float none[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int r = threadIdx.x / 4; r < (int)piece.rows; r += kFewWaves * kWave / 4) {
+      const int n = n0 + (threadIdx.x % 4) * 4;
+      store4(y, (int64_t)(piece.row + r) * a.N + n, a.N - n, a.dt, none);
+    }
+    return;
+  }
+  const int runs = f8_runs(a.K), wide = f8_runs(a.K) * kF8Run;
+  const F8Mat m = which ? a.m[1] : a.m[0];
+  const uint8_t *const w = m.w + (int64_t)piece.mat * a.N * a.K + (int64_t)(n0 + ln < a.N ? n0 + ln : a.N - 1) * a.K;
+  const float *const ws = m.s + ((int64_t)piece.mat * f8_runs(a.N) + n0 / kF8Run) * runs;
+  const uint8_t *x[TG];
+  const float *xs[TG];
+#pragma unroll
+  for (int t = 0; t < TG; ++t) {
+    const uint32_t r = t * 16 + ln < (int)piece.rows ? piece.row + t * 16 + ln : piece.row;
+    int64_t at = a.order ? a.order[r] / (uint32_t)a.k_div : r;
+    if (at >= a.x.rows) at = 0;  // (an order of the caller's: never followed out of the rows)
+    x[t] = a.x.codes + at * wide;
+    xs[t] = a.x.scales + at;
+  }
+  f32x4_t acc[TG] = {};
+  for (int j0 = wave; j0 < runs; j0 += kFewWaves * AHEAD) {
+    u32x4_f8 wv[AHEAD][2], xv[AHEAD][TG][2];
+    float s[AHEAD], sx[AHEAD][TG];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int j = j0 + i * kFewWaves < runs ? j0 + i * kFewWaves : runs - 1;  // (past the end the last run again, with a scale of zero)
+      s[i] = j0 + i * kFewWaves < runs ? ws[j] : 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k = j * kF8Run + h * 64 + part * 16;
+        wv[i][h] = *reinterpret_cast<const u32x4_f8 *>(w + (k < a.K ? k : 0));
+        if (k >= a.K) wv[i][h] = u32x4_f8{0, 0, 0, 0};
+#pragma unroll
+        for (int t = 0; t < TG; ++t) xv[i][t][h] = *reinterpret_cast<const u32x4_f8 *>(x[t] + k);
+      }
+#pragma unroll
+      for (int t = 0; t < TG; ++t) sx[i][t] = xs[t][(int64_t)j * a.x.rows];
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+#pragma unroll
+      for (int t = 0; t < TG; ++t) {
+        f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+        if constexpr (F32) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+              sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes_to_bf16(wv[i][h][2 * p], wv[i][h][2 * p + 1]), codes_to_bf16(xv[i][t][h][2 * p], xv[i][t][h][2 * p + 1]),
+                                                            sum, 0, 0, 0);
+        } else {
+          sum = mfma_f8_16(__builtin_bit_cast(i32x8_t, wv[i]), __builtin_bit_cast(i32x8_t, xv[i][t]), sum);
+        }
+        const float f = s[i] * sx[i][t];
+#pragma unroll
+        for (int v = 0; v < 4; ++v) acc[t][v] = __builtin_fmaf(sum[v], f, acc[t][v]);
+      }
+  }
+  __shared__ f32x4_t sums[kFewWaves][TG][kWave];
+#pragma unroll
+  for (int t = 0; t < TG; ++t) sums[wave][t][lane] = acc[t];
+  __syncthreads();
+  for (int t = wave; t < TG; t += kFewWaves) {
+    const f32x4_t v = (sums[0][t][lane] + sums[1][t][lane]) + (sums[2][t][lane] + sums[3][t][lane]);
+    const int r = t * 16 + ln, n = n0 + part * 4;  // lane: token row ln of the group, four weight rows
+    if (r >= (int)piece.rows || n >= a.N) continue;
+    float o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = v[i] + (a.bias && n + i < a.N ? value_of(a.bias, n + i, a.dt) : 0.f);
+    store4(y, (int64_t)(piece.row + r) * a.N + n, a.N - n, a.dt, o);
+  }
+}
+
+bool f8_few_rows(const F8Product &p) { return p.transpose && !p.h && !p.pair_sum && p.rows <= (int64_t)16 * (p.offsets ? p.n_mats : 1); }
+
+hipError_t launch_f8_few(const F8Product &p, hipStream_t st) {
+  if (p.rows == 0) return hipSuccess;
+  const unsigned tiles = (unsigned)((p.N + 15) / 16) * (p.y1 ? 2 : 1);
+  const int64_t avg = p.rows / (p.offsets ? p.n_mats : 1);
+  auto launch = [&](auto *kernel, int tg) {
+    kernel<<<dim3(tiles, (unsigned)f8_most_pieces(p, 16 * tg)), kFewWaves * kWave, 0, st>>>(p);
+    return hipGetLastError();
+  };
+  if (p.dt == 2) return avg > 4 ? launch(&f8_few_kernel<2, true>, 2) : launch(&f8_few_kernel<1, true>, 1);
+  return avg > 4 ? launch(&f8_few_kernel<2, false>, 2) : launch(&f8_few_kernel<1, false>, 1);
+}
+
+}  // namespace mi_moe

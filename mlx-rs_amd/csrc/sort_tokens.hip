@@ -1,0 +1,211 @@
+// Tokens to rows sorted by expert and back, with the weights applied, and the gradients of both.
+//
+//   sort      row[place(t, s)] = x[t]                       its gradient  dx[t] = sum over s of drow[place(t, s)]
+//   unsort    out[t] = sum over s of w[t][s] row[place(t, s)]             drow[place(t, s)] = w[t][s] dout[t],  dw[t][s] = dout[t] . row[place(t, s)]
+//
+// place: the stable sort of the (token, slot) pairs by expert (dispatch.hip).  Slots that name no expert have the places behind all others: their rows are zeros and have
+// no part in any sum.  Sums are float32, over the slots in their order, over a row's values in a fixed tree.  All four move bytes: a token's row is read (or written) once
+// and its k rows written (or read) once.
+#include "dispatch_dev.hpp"
+#include "f8.hpp"
+#include "octets.hpp"
+
+namespace mi_moe {
+
+constexpr int kSortThreads = 256, kSortMostSlots = 32;
+constexpr int64_t kSortSmall = 2048;  // pairs up to which every token's block finds its own places
+
+// a token's row to its places: 16 bytes a thread and step, with no more alignment than the elements' own
+__device__ __forceinline__ void spread_row(const char *from, char *rows, int64_t bytes, const int32_t *at, int k) {
+  for (int64_t b = (int64_t)threadIdx.x * 16; b < bytes; b += kSortThreads * 16) {
+    const int n = bytes - b < 16 ? (int)(bytes - b) / 2 : 8;
+    uint16_t v[8] = {};
+    if (n == 8) __builtin_memcpy(v, from + b, 16);
+    else
+      for (int i = 0; i < n; ++i) __builtin_memcpy(&v[i], from + b + 2 * i, 2);
+    for (int s = 0; s < k; ++s) {
+      const int32_t to = at[s];
+      const bool named = to >= 0;
+      char *const p = rows + (int64_t)(named ? to : ~to) * bytes + b;
+      uint16_t o[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] = named ? v[i] : 0;
+      if (n == 8) __builtin_memcpy(p, o, 16);
+      else
+        for (int i = 0; i < n; ++i) __builtin_memcpy(p + 2 * i, &o[i], 2);
+    }
+  }
+}
+
+// Few pairs: block t finds the places of token t's pairs by counting the pairs before each (a smaller expert, or the same and an earlier pair), and writes its rows; the last block
+// counts the experts' rows.  One launch, no block waits for another.
+__global__ __launch_bounds__(kSortThreads) void sort_few_kernel(SortTokens a, const char *__restrict__ x, int64_t row_bytes, char *__restrict__ rows) {
+  __shared__ uint32_t ids[kSortSmall];
+  __shared__ int32_t at[kSortMostSlots];
+  __shared__ uint32_t count[513];
+  const int P = (int)a.T * a.k, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t E = (uint32_t)a.E;
+  for (int i = threadIdx.x; i < P; i += kSortThreads) ids[i] = a.ids[i] < E ? a.ids[i] : E;
+  if ((int64_t)blockIdx.x == a.T) {
+    for (int e = threadIdx.x; e <= a.E; e += kSortThreads) count[e] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < P; i += kSortThreads) atomicAdd(&count[ids[i]], 1u);
+    __syncthreads();
+    if (wave == 0) {
+      uint32_t before = 0;
+      for (int e0 = 0; e0 <= a.E; e0 += kWave) {
+        const uint32_t own = e0 + lane <= a.E ? count[e0 + lane] : 0u;
+        uint32_t upto = own;
+        for (int d = 1; d < kWave; d <<= 1) {
+          const uint32_t v = __shfl_up(upto, d, kWave);
+          if (lane >= d) upto += v;
+        }
+        if (e0 + lane <= a.E) a.offsets[e0 + lane] = before + upto - own;
+        before += __shfl(upto, kWave - 1, kWave);
+      }
+    }
+    return;
+  }
+  __syncthreads();
+  const int first = (int)blockIdx.x * a.k;
+  for (int s = wave; s < a.k; s += kSortThreads / kWave) {
+    const int p = first + s;
+    const uint32_t e = ids[p];
+    int n = 0;
+    for (int q = lane; q < P; q += kWave) n += ids[q] < e || (ids[q] == e && q < p);
+    for (int d = 1; d < kWave; d <<= 1) n += __shfl_xor(n, d, kWave);
+    if (lane == 0) {
+      at[s] = e < E ? n : ~n;
+      a.order[n] = (uint32_t)p;
+      a.inverse[p] = e < E ? n : ~n;
+    }
+  }
+  if (!rows) return;
+  __syncthreads();
+  spread_row(x + blockIdx.x * row_bytes, rows, row_bytes, at, a.k);
+}
+
+// Behind the dispatch of more pairs, with one expert more for those that name none: `inverse` gets its form (a place that has it already stays what it is), rows are written.
+__global__ __launch_bounds__(kSortThreads) void sort_rows_kernel(SortTokens a, const uint32_t *__restrict__ offsets, const char *__restrict__ x, int64_t row_bytes,
+                                                                 char *__restrict__ rows) {
+  __shared__ int32_t at[kSortMostSlots];
+  const int64_t first = (int64_t)blockIdx.x * a.k;
+  if ((int)threadIdx.x < a.k) {
+    const int32_t n = a.inverse[first + threadIdx.x];
+    at[threadIdx.x] = a.ids[first + threadIdx.x] < (uint32_t)a.E ? n : ~n;
+    a.inverse[first + threadIdx.x] = at[threadIdx.x];
+  }
+  if (blockIdx.x == 0)
+    for (int e = threadIdx.x; e <= a.E; e += kSortThreads) a.offsets[e] = offsets[e];
+  if (!rows) return;
+  __syncthreads();
+  spread_row(x + blockIdx.x * row_bytes, rows, row_bytes, at, a.k);
+}
+
+size_t sort_tokens_bytes(int64_t T, int k, int E) {
+  return T * k <= kSortSmall ? 0 : ((size_t)(E + 2) * 4 + 255) / 256 * 256 + dispatch_workspace_bytes(E + 1, T * k);
+}
+
+hipError_t launch_sort_tokens(const SortTokens &a, const void *x, int dt, int H, void *rows, void *scratch, hipStream_t st) {
+  const int64_t P = a.T * a.k, row_bytes = (int64_t)H * (dt == 2 ? 4 : 2);
+  if (P <= kSortSmall) {  // (no tokens: the offsets alone)
+    sort_few_kernel<<<(unsigned)a.T + 1, kSortThreads, 0, st>>>(a, static_cast<const char *>(x), row_bytes, static_cast<char *>(rows));
+    return hipGetLastError();
+  }
+  uint32_t *const offsets = static_cast<uint32_t *>(scratch);
+  if (hipError_t e = launch_dispatch(a.ids, P, a.E + 1, a.k, nullptr, offsets, a.order, reinterpret_cast<uint32_t *>(a.inverse), nullptr, Records(), nullptr, 0, 0, ShortTiles(),
+                                     PrepareArgs(), static_cast<char *>(scratch) + ((size_t)(a.E + 2) * 4 + 255) / 256 * 256, st);
+      e != hipSuccess)
+    return e;
+  sort_rows_kernel<<<(unsigned)a.T, kSortThreads, 0, st>>>(a, offsets, static_cast<const char *>(x), row_bytes, static_cast<char *>(rows));
+  return hipGetLastError();
+}
+
+// A thread eight columns of a token; its slots' rows eight at a time, all their loads in flight together.
+template <int DT>
+__global__ __launch_bounds__(64) void unsort_kernel(const void *__restrict__ rows, const void *__restrict__ weights, int w_dtype, const int32_t *__restrict__ inverse, int64_t T,
+                                                    int k, int H, void *__restrict__ out) {
+  const int64_t t = blockIdx.x;
+  const int h = (blockIdx.y * 64 + threadIdx.x) * 8, n = H - h;
+  if (n <= 0) return;
+  float acc[8] = {};
+  for (int s0 = 0; s0 < k; s0 += 8) {
+    Octet<DT> v[8];
+    float w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int64_t s = t * k + (s0 + j < k ? s0 + j : k - 1);
+      const int32_t at = inverse[s];
+      const bool named = s0 + j < k && at >= 0 && at < T * k;
+      w[j] = weights ? value_of(weights, s, w_dtype) : 1.f;
+      v[j] = load_octet<DT>(rows, (named ? (int64_t)at : 0) * H + h, n);
+      if (!named) {  // (not multiplied by zero: its row, or its weight, may be infinite)
+        w[j] = 0.f;
+        v[j] = Octet<DT>{};
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] = __builtin_fmaf(w[j], v[j].at(i), acc[i]);
+  }
+  Octet<DT> o;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) o.put(i, acc[i]);
+  store_octet<DT>(out, t * H + h, n, o);
+}
+
+hipError_t launch_unsort_tokens(const void *rows, const void *weights, int w_dtype, const int32_t *inverse, int64_t T, int k, int H, int dt, void *out, hipStream_t st) {
+  if (T == 0) return hipSuccess;
+  auto *const kernel = dt == 0 ? &unsort_kernel<0> : dt == 1 ? &unsort_kernel<1> : &unsort_kernel<2>;
+  kernel<<<dim3((unsigned)T, (unsigned)((H + 511) / 512)), 64, 0, st>>>(rows, weights, w_dtype, inverse, T, k, H, out);
+  return hipGetLastError();
+}
+
+template <int DT>
+__global__ __launch_bounds__(kSortThreads) void unsort_grad_kernel(const void *__restrict__ dout, const void *__restrict__ rows, const void *__restrict__ weights, int w_dtype,
+                                                                   const int32_t *__restrict__ inverse, int64_t T, int k, int H, void *__restrict__ drows,
+                                                                   void *__restrict__ dweights) {
+  __shared__ float sums[kSortMostSlots][kSortThreads / kWave];
+  const int64_t t = blockIdx.x;
+  for (int s = 0; s < k; ++s) {
+    const int32_t at = inverse[t * k + s];
+    const bool named = at >= 0;
+    const int64_t row = named ? at : ~at;
+    if (row >= T * k) {  // (no place at all: a slot of nobody's)
+      if (threadIdx.x < kSortThreads / kWave) sums[s][threadIdx.x] = 0.f;
+      continue;
+    }
+    const float w = value_of(weights, t * k + s, w_dtype);
+    float dot = 0.f;
+    for (int h = threadIdx.x * 8; h < H; h += kSortThreads * 8) {
+      Octet<DT> o{};
+      if (named) {
+        const Octet<DT> g = load_octet<DT>(dout, t * H + h, H - h), v = load_octet<DT>(rows, row * H + h, H - h);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          dot = __builtin_fmaf(g.at(i), v.at(i), dot);
+          o.put(i, w * g.at(i));
+        }
+      }
+      store_octet<DT>(drows, row * H + h, H - h, o);
+    }
+    for (int d = 1; d < kWave; d <<= 1) dot += __shfl_xor(dot, d, kWave);
+    if (threadIdx.x % kWave == 0) sums[s][threadIdx.x / kWave] = dot;
+  }
+  __syncthreads();
+  if ((int)threadIdx.x < k) {
+    const float *const p = sums[threadIdx.x];
+    put_value(dweights, t * k + threadIdx.x, w_dtype, (p[0] + p[1]) + (p[2] + p[3]));
+  }
+}
+
+hipError_t launch_unsort_tokens_grad(const void *dout, const void *rows, const void *weights, int w_dtype, const int32_t *inverse, int64_t T, int k, int H, int dt,
+                                     void *drows, void *dweights, hipStream_t st) {
+  if (T == 0) return hipSuccess;
+  auto *const kernel = dt == 0 ? &unsort_grad_kernel<0> : dt == 1 ? &unsort_grad_kernel<1> : &unsort_grad_kernel<2>;
+  kernel<<<(unsigned)T, kSortThreads, 0, st>>>(dout, rows, weights, w_dtype, inverse, T, k, H, drows, dweights);
+  return hipGetLastError();
+}
+
+}  // namespace mi_moe

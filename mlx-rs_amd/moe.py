@@ -13,6 +13,7 @@ import torch
 
 from . import capi
 from .capi import check, load_library
+from . import ops
 from .ops import _need, _ptr, _stream, _together
 
 
@@ -190,3 +191,39 @@ class SparseMoeBlock:
         if kernels:
             return out.reshape(x.shape), list(ms), list(kms)
         return out.reshape(x.shape), list(ms)
+
+
+@dataclass
+class F8SwitchLinear:
+    """A bank of E matrices in e4m3 with a scale for each block of 128 x 128 (a checkpoint's ``weight`` and ``weight_scale_inv``)."""
+    weight: torch.Tensor  # float8_e4m3fn [E, N, K]
+    scales: torch.Tensor  # float32 [E, ceil(N / 128), ceil(K / 128)]
+
+    @classmethod
+    def quantize(cls, w):
+        """From a bank in bfloat16, float16 or float32 [E, N, K]."""
+        return cls(*ops.quantize_f8(w))
+
+
+class SwitchGluF8:
+    """SwiGLU experts on e4m3 weights, behind a router of the caller's: the f8 form of what SparseMoeBlock.forward_routed computes.  The weights are frozen: ``gradient``
+    gives what fine-tuning through the experts needs, the gradients of the tokens and of the routing weights."""
+
+    def __init__(self, gate_proj, up_proj, down_proj):
+        self.gate_proj, self.up_proj, self.down_proj = gate_proj, up_proj, down_proj
+        self._banks = tuple((p.weight, p.scales) for p in (gate_proj, up_proj, down_proj))
+        self.training = False
+
+    def training_mode(self, mode):
+        """The experts compute the same in training (module.rs:44-50)."""
+        self.training = bool(mode)
+
+    def forward(self, x, inds, weights):
+        """x: bfloat16 or float16 [..., H]; inds int32 and weights [..., top_k] (``ops.select_experts``, ``ops.route``) -> [..., H]."""
+        return ops.switch_glu_f8(x, inds, weights, *self._banks)
+
+    __call__ = forward
+
+    def gradient(self, dout, x, inds, weights):
+        """(dx, dweights) for the gradient dout that arrives at forward's result."""
+        return ops.switch_glu_f8_grad(dout, x, inds, weights, *self._banks)

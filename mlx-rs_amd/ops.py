@@ -568,3 +568,303 @@ def combine(y, scores, inv_perm=None):
                              _ptr(None if inv_perm is None else _need(inv_perm, torch.int32, "inv_perm")),
                              T, k, H, _ptr(out), _stream()))
     return out
+
+
+# ---------------------------------------------------------------- tokens sorted by expert
+def _slots(who, t, inverse):
+    """T, top_k and hidden of a token tensor t [T, H] with its slots' rows."""
+    _need(inverse, torch.int32, "inverse")
+    if inverse.dim() != 2:
+        raise capi.MoeError(f"{who}: inverse must be [T, top_k], got {tuple(inverse.shape)}")
+    if t.dim() != 2:
+        raise capi.MoeError(f"{who}: expected a matrix, got {tuple(t.shape)}")
+    _int32(who, ("top_k", inverse.shape[1]), ("hidden", t.shape[1]))
+    return inverse.shape[0], inverse.shape[1], t.shape[1]
+
+
+def _rows_of(who, name, t, T, k):
+    if t.shape[0] != T * k:
+        raise capi.MoeError(f"{who}: {name} must have {T * k} rows, got {t.shape[0]}")
+
+
+def sort_tokens(x, inds, n_experts):
+    """Tokens to rows sorted by expert: (rows [T * k, H], order int32 [T * k], inverse int32 [T, k], offsets int32 [n_experts + 1]).
+    x: [T, H] in bfloat16, float16 or float32; inds: int32 [T, k] (``route``, ``select_experts``).  Row r is token ``order[r] // k``; the pairs
+    ``t * k + s`` are sorted stably; expert e has the rows from ``offsets[e]`` to ``offsets[e + 1]``; ``inverse`` has every slot's row.  Slots whose id is
+    outside the experts (padding) come last: their rows are zeros and ``inverse`` is -1 - row there, which the functions below leave out."""
+    out = _native("sort_tokens", x, inds, n_experts)
+    if out is not None:
+        return out
+    lib = load_library()
+    who = "sort_tokens"
+    dt = _float_dtype(x, "x")
+    _need(inds, torch.int32, "inds")
+    if x.dim() != 2 or inds.dim() != 2 or inds.shape[0] != x.shape[0]:
+        raise capi.MoeError(f"{who}: x must be [T, H] and inds [T, top_k], got {tuple(x.shape)} and {tuple(inds.shape)}")
+    _together(who, x, inds)
+    (T, k), H, dev = inds.shape, x.shape[1], x.device
+    _int32(who, ("top_k", k), ("hidden", H), ("n_experts", n_experts))
+    need = C.c_size_t()
+    check(lib.mi_moe_sort_tokens_workspace_size(T, k, n_experts, C.byref(need)))
+    rows = torch.empty((T * k, H), dtype=x.dtype, device=dev)
+    order = torch.empty(T * k, dtype=torch.int32, device=dev)
+    inverse = torch.empty((T, k), dtype=torch.int32, device=dev)
+    offsets = torch.empty(n_experts + 1, dtype=torch.int32, device=dev)
+    ws = torch.empty(need.value, dtype=torch.uint8, device=dev) if need.value else None
+    check(lib.mi_moe_sort_tokens(_ptr(x), _ptr(inds), T, k, n_experts, H, dt, _ptr(rows), _ptr(order), _ptr(inverse), _ptr(offsets), _ptr(ws), need.value, _stream()))
+    return rows, order, inverse, offsets
+
+
+def sort_tokens_grad(drows, inverse):
+    """The gradient of sort_tokens' rows with respect to x: dx [T, H], the sum over each token's named slots (float32, in the slots' order)."""
+    out = _native("sort_tokens_grad", drows, inverse)
+    if out is not None:
+        return out
+    lib = load_library()
+    who = "sort_tokens_grad"
+    dt = _float_dtype(drows, "drows")
+    T, k, H = _slots(who, drows, inverse)
+    _rows_of(who, "drows", drows, T, k)
+    _together(who, drows, inverse)
+    dx = torch.empty((T, H), dtype=drows.dtype, device=drows.device)
+    check(lib.mi_moe_sort_tokens_grad(_ptr(drows), _ptr(inverse), T, k, H, dt, _ptr(dx), _stream()))
+    return dx
+
+
+def unsort_tokens(rows, weights, inverse):
+    """Rows sorted by expert back to tokens: out[t] = sum over the named slots of weights[t, s] * rows[inverse[t, s]], [T, H] of rows' type, summed in float32.
+    rows: [T * k, H] in bfloat16, float16 or float32; weights: [T, k] in any of these; inverse: from ``sort_tokens``."""
+    out = _native("unsort_tokens", rows, weights, inverse)
+    if out is not None:
+        return out
+    lib = load_library()
+    who = "unsort_tokens"
+    dt, wt = _float_dtype(rows, "rows"), _float_dtype(weights, "weights")
+    T, k, H = _slots(who, rows, inverse)
+    _rows_of(who, "rows", rows, T, k)
+    if weights.shape != inverse.shape:
+        raise capi.MoeError(f"{who}: weights must be {tuple(inverse.shape)}, got {tuple(weights.shape)}")
+    _together(who, rows, weights, inverse)
+    y = torch.empty((T, H), dtype=rows.dtype, device=rows.device)
+    check(lib.mi_moe_unsort_tokens(_ptr(rows), _ptr(weights), wt, _ptr(inverse), T, k, H, dt, _ptr(y), _stream()))
+    return y
+
+
+def unsort_tokens_grad(dout, rows, weights, inverse):
+    """The gradients of unsort_tokens: (drows, dweights), of rows' and weights' shapes and types; zeros where a slot names no expert."""
+    out = _native("unsort_tokens_grad", dout, rows, weights, inverse)
+    if out is not None:
+        return out
+    lib = load_library()
+    who = "unsort_tokens_grad"
+    dt, wt = _float_dtype(rows, "rows"), _float_dtype(weights, "weights")
+    _need(dout, rows.dtype, "dout")
+    T, k, H = _slots(who, rows, inverse)
+    _rows_of(who, "rows", rows, T, k)
+    if weights.shape != inverse.shape or dout.shape != (T, H):
+        raise capi.MoeError(f"{who}: weights must be {tuple(inverse.shape)} and dout {(T, H)}, got {tuple(weights.shape)} and {tuple(dout.shape)}")
+    _together(who, dout, rows, weights, inverse)
+    drows, dweights = torch.empty_like(rows), torch.empty_like(weights)
+    check(lib.mi_moe_unsort_tokens_grad(_ptr(dout), _ptr(rows), _ptr(weights), wt, _ptr(inverse), T, k, H, dt, _ptr(drows), _ptr(dweights), _stream()))
+    return drows, dweights
+
+
+# ---------------------------------------------------------------- e4m3 weights with a scale for each block of 128 x 128
+_F8 = torch.float8_e4m3fn
+
+
+def _blocks(n):
+    return -(-n // 128)
+
+
+def _f8_rows(block_rows, shape):
+    if block_rows not in (1, 128):
+        raise capi.MoeError(f"quantize_f8: block_rows must be 1 or 128, got {block_rows!r}")
+    return shape[:-2] + (shape[-2] if block_rows == 1 else _blocks(shape[-2]), _blocks(shape[-1]))
+
+
+def quantize_f8(w, block_rows=128):
+    """Matrices in e4m3 with float32 scales: (codes float8_e4m3fn of w's shape, scales).  w: [..., N, K] in bfloat16, float16 or float32.  ``block_rows`` 128: a scale
+    for each block of 128 x 128, [..., ceil(N / 128), ceil(K / 128)], as ``linear_f8`` takes weights; 1: for each run of 128 values of a row, [..., N, ceil(K / 128)].
+    scale = max |w| / 448, a code is the e4m3 value nearest to w / scale (ties to even), scale and quotient rounded to float32."""
+    lib = load_library()
+    dt = _float_dtype(w, "w")
+    if w.dim() < 2:
+        raise capi.MoeError(f"quantize_f8: w must be [..., N, K], got {tuple(w.shape)}")
+    shape = _f8_rows(block_rows, tuple(w.shape))
+    _together("quantize_f8", w)
+    N, K = w.shape[-2:]
+    codes = torch.empty(w.shape, dtype=_F8, device=w.device)
+    scales = torch.empty(shape, dtype=torch.float32, device=w.device)
+    if w.numel() == 0:
+        return codes, scales
+    whole = block_rows == 1 or N % 128 == 0  # (blocks of a bank end with its matrices)
+    for i in range(1 if whole else w.numel() // (N * K)):
+        size = w.element_size()
+        check(lib.mi_moe_quantize_f8(w.data_ptr() + i * N * K * size, dt, w.numel() // K if whole else N, K, block_rows, codes.data_ptr() + i * N * K,
+                                     scales.data_ptr() + i * 4 * shape[-2] * shape[-1], _stream()))
+    return codes, scales
+
+
+def dequantize_f8(codes, scales, dtype=torch.bfloat16):
+    """The values that quantize_f8's results stand for (code times scale, rounded once), of ``dtype``; which of the two forms they have is told by the scales' shape (a matrix of
+    one row has a scale for each run either way)."""
+    lib = load_library()
+    _need(codes, _F8, "codes")
+    _need(scales, torch.float32, "scales")
+    if dtype not in _DTYPES:
+        raise capi.MoeError(f"dequantize_f8: dtype must be bfloat16, float16 or float32, got {dtype}")
+    if codes.dim() < 2 or tuple(scales.shape) not in (_f8_rows(1, tuple(codes.shape)), _f8_rows(128, tuple(codes.shape))):
+        raise capi.MoeError(f"dequantize_f8: scales {tuple(scales.shape)} do not go with codes {tuple(codes.shape)}")
+    _together("dequantize_f8", codes, scales)
+    N, K = codes.shape[-2:]
+    block_rows = 1 if scales.shape[-2] == N else 128
+    out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
+    if out.numel() == 0:
+        return out
+    whole = block_rows == 1 or N % 128 == 0
+    for i in range(1 if whole else codes.numel() // (N * K)):
+        check(lib.mi_moe_dequantize_f8(codes.data_ptr() + i * N * K, scales.data_ptr() + i * 4 * scales.shape[-2] * scales.shape[-1], codes.numel() // K if whole else N, K,
+                                       block_rows, _DTYPES[dtype], out.data_ptr() + i * N * K * out.element_size(), _stream()))
+    return out
+
+
+def _f8_bank(who, name, w, scales, lead, N=None, K=None):
+    """Checks weights [*lead, N, K] and the scales of their blocks."""
+    _need(w, _F8, name)
+    _need(scales, torch.float32, f"{name}'s scales")
+    if w.dim() != lead + 2 or scales.dim() != lead + 2 or (N is not None and tuple(w.shape[-2:]) != (N, K)):
+        raise capi.MoeError(f"{who}: {name} must be [{'n_experts, ' if lead else ''}{N or 'N'}, {K or 'K'}], got {tuple(w.shape)}")
+    want = tuple(w.shape[:lead]) + (_blocks(w.shape[-2]), _blocks(w.shape[-1]))
+    if tuple(scales.shape) != want:
+        raise capi.MoeError(f"{who}: {name}'s scales must be {want}, got {tuple(scales.shape)}")
+
+
+@functools.lru_cache(maxsize=1024)
+def _linear_f8_workspace_bytes(M, K):
+    need = C.c_size_t()
+    check(load_library().mi_moe_linear_f8_workspace_size(M, K, C.byref(need)))
+    return need.value
+
+
+def linear_f8(x, w, scales, linear_bias=None, transpose=True):
+    """A linear layer on e4m3 weights with a scale for each block of 128 x 128: y = q(x) . W^T + linear_bias, where q rounds rows to e4m3 with a scale for each run of 128
+    values (``quantize_f8`` with block_rows 1).  x: [..., K] in bfloat16, float16 or float32, which is y's type; w: float8_e4m3fn [N, K], scales: float32
+    [ceil(N / 128), ceil(K / 128)] (``quantize_f8``); K a multiple of 16.  Returns [..., N].
+    transpose = False: q(x) . W for x [..., N], the gradient with respect to the layer's input; returns [..., K]."""
+    out = _native("linear_f8", x, w, scales, linear_bias, transpose)
+    if out is not None:
+        return out
+    lib = load_library()
+    who = "linear_f8"
+    dt = _float_dtype(x, "x")
+    _f8_bank(who, "w", w, scales, 0)
+    inner, outer = (w.shape[1], w.shape[0]) if transpose else (w.shape[0], w.shape[1])
+    if x.dim() < 1 or x.shape[-1] != inner:
+        raise capi.MoeError(f"{who}: x must be [..., {inner}], got {tuple(x.shape)}")
+    if linear_bias is not None:
+        if not transpose:
+            raise capi.MoeError(f"{who}: a linear bias goes with transpose = True")
+        _need(linear_bias, x.dtype, "linear_bias")
+        if linear_bias.numel() != outer:
+            raise capi.MoeError(f"{who}: linear_bias must have {outer} elements, got {linear_bias.numel()}")
+    _together(who, x, w, scales, linear_bias)
+    _int32(who, ("N", outer), ("K", inner))
+    M = x.numel() // inner if inner else 0
+    y = torch.empty(x.shape[:-1] + (outer,), dtype=x.dtype, device=x.device)
+    need = _linear_f8_workspace_bytes(M, inner) if M else 0
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+    check(lib.mi_moe_linear_f8(_ptr(x), _ptr(w), _ptr(scales), _ptr(linear_bias), M, outer, inner, 1 if transpose else 0, dt, _ptr(y), _ptr(ws), need, _stream()))
+    return y
+
+
+def grouped_linear_f8(rows, w, scales, offsets, transpose=True):
+    """linear_f8 for rows sorted by expert (``sort_tokens``): rows from offsets[e] to offsets[e + 1] with matrix e.  rows: [R, K] in bfloat16, float16 or float32; w: float8_e4m3fn
+    [E, N, K], scales: float32 [E, ceil(N / 128), ceil(K / 128)]; offsets: int32 [E + 1].  Returns [R, N]; rows behind the last expert's are zeros.
+    transpose = False: the gradient with respect to the rows, [R, N] to [R, K]."""
+    out = _native("grouped_linear_f8", rows, w, scales, offsets, transpose)
+    if out is not None:
+        return out
+    lib = load_library()
+    who = "grouped_linear_f8"
+    dt = _float_dtype(rows, "rows")
+    _f8_bank(who, "w", w, scales, 1)
+    E = w.shape[0]
+    inner, outer = (w.shape[2], w.shape[1]) if transpose else (w.shape[1], w.shape[2])
+    if rows.dim() != 2 or rows.shape[1] != inner:
+        raise capi.MoeError(f"{who}: rows must be [R, {inner}], got {tuple(rows.shape)}")
+    _need(offsets, torch.int32, "offsets")
+    if tuple(offsets.shape) != (E + 1,):
+        raise capi.MoeError(f"{who}: offsets must be [{E + 1}], got {tuple(offsets.shape)}")
+    _together(who, rows, w, scales, offsets)
+    _int32(who, ("N", outer), ("K", inner), ("n_experts", E))
+    R = rows.shape[0]
+    y = torch.empty((R, outer), dtype=rows.dtype, device=rows.device)
+    need = _linear_f8_workspace_bytes(R, inner) if R and inner else 0
+    ws = torch.empty(need, dtype=torch.uint8, device=rows.device)
+    check(lib.mi_moe_grouped_linear_f8(_ptr(rows), _ptr(w), _ptr(scales), _ptr(offsets), R, E, outer, inner, 1 if transpose else 0, dt, _ptr(y), _ptr(ws), need, _stream()))
+    return y
+
+
+@functools.lru_cache(maxsize=1024)
+def _switch_glu_f8_workspace_bytes(T, hidden, intermediate, n_experts, top_k, grad):
+    need = C.c_size_t()
+    check(load_library().mi_moe_switch_glu_f8_workspace_size(T, hidden, intermediate, n_experts, top_k, grad, C.byref(need)))
+    return need.value
+
+
+def _f8_experts(who, x, inds, weights, gate, up, down):
+    """Checks the operands of the experts: their types' codes, the C struct of the banks, and T, hidden, intermediate, n_experts, top_k."""
+    dt, wt = _float_dtype(x, "x"), _float_dtype(weights, "weights")
+    _need(inds, torch.int32, "inds")
+    _f8_bank(who, "gate", *gate, 1)
+    E, inter, hidden = gate[0].shape
+    _f8_bank(who, "up", *up, 1, inter, hidden)
+    _f8_bank(who, "down", *down, 1, hidden, inter)
+    if up[0].shape[0] != E or down[0].shape[0] != E:
+        raise capi.MoeError(f"{who}: gate, up and down must have as many experts, got {E}, {up[0].shape[0]}, {down[0].shape[0]}")
+    if x.dim() < 1 or x.shape[-1] != hidden:
+        raise capi.MoeError(f"{who}: x must be [..., {hidden}], got {tuple(x.shape)}")
+    if inds.dim() != x.dim() or inds.shape[:-1] != x.shape[:-1] or weights.shape != inds.shape:
+        raise capi.MoeError(f"{who}: inds and weights must be {tuple(x.shape[:-1])} + (top_k,), got {tuple(inds.shape)} and {tuple(weights.shape)}")
+    _together(who, x, inds, weights, *gate, *up, *down)
+    k = inds.shape[-1]
+    _int32(who, ("hidden", hidden), ("intermediate", inter), ("n_experts", E), ("top_k", k))
+    banks = capi.F8Experts(gate[0].data_ptr(), up[0].data_ptr(), down[0].data_ptr(), gate[1].data_ptr(), up[1].data_ptr(), down[1].data_ptr())
+    return dt, wt, banks, (x.numel() // hidden if hidden else 0, hidden, inter, E, k)
+
+
+def switch_glu_f8(x, inds, weights, gate, up, down):
+    """SwiGLU experts on e4m3 weights, on a routing of the caller's (``select_experts``, ``route``): out[t] = sum over s of weights[t, s] *
+    q(silu(q(x[t]) . gate_e^T) * (q(x[t]) . up_e^T)) . down_e^T with e = inds[t, s] and q as in ``linear_f8``.  x: [..., H] in bfloat16 or float16; inds int32 and weights
+    (bfloat16, float16 or float32) [..., k]; gate, up, down: (codes, scales) of [E, I, H], [E, I, H] and [E, H, I] (``quantize_f8``).  Slots whose id is outside the experts
+    contribute nothing.  Returns [..., H] of x's type."""
+    out = _native("switch_glu_f8", x, inds, weights, *gate, *up, *down)
+    if out is not None:
+        return out
+    lib = load_library()
+    dt, wt, banks, sizes = _f8_experts("switch_glu_f8", x, inds, weights, gate, up, down)
+    y = torch.empty_like(x)
+    need = _switch_glu_f8_workspace_bytes(*sizes, 0)
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+    check(lib.mi_moe_switch_glu_f8(_ptr(x), _ptr(inds), _ptr(weights), wt, C.byref(banks), *sizes, dt, _ptr(y), _ptr(ws), need, _stream()))
+    return y
+
+
+def switch_glu_f8_grad(dout, x, inds, weights, gate, up, down):
+    """The gradients of switch_glu_f8 with respect to x and the routing weights: (dx, dweights), of x's and weights' shapes and types.  Roundings to e4m3 pass a gradient on as
+    it is; nothing of the forward call is needed."""
+    out = _native("switch_glu_f8_grad", dout, x, inds, weights, *gate, *up, *down)
+    if out is not None:
+        return out
+    lib = load_library()
+    dt, wt, banks, sizes = _f8_experts("switch_glu_f8_grad", x, inds, weights, gate, up, down)
+    _need(dout, x.dtype, "dout")
+    if dout.shape != x.shape:
+        raise capi.MoeError(f"switch_glu_f8_grad: dout must be {tuple(x.shape)} as x, got {tuple(dout.shape)}")
+    _together("switch_glu_f8_grad", dout)
+    dx, dweights = torch.empty_like(x), torch.empty_like(weights)
+    need = _switch_glu_f8_workspace_bytes(*sizes, 1)
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+    check(lib.mi_moe_switch_glu_f8_grad(_ptr(dout), _ptr(x), _ptr(inds), _ptr(weights), wt, C.byref(banks), *sizes, dt, _ptr(dx), _ptr(dweights), _ptr(ws), need, _stream()))
+    return dx, dweights

@@ -4,6 +4,7 @@
 
 use std::os::raw::{c_char, c_int, c_void};
 
+pub mod f8;
 pub mod layer;
 
 #[repr(C)]

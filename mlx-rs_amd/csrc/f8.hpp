@@ -211,7 +211,9 @@ __device__ __forceinline__ void store4(void *base, int64_t at, int n, int dt, co
     float *p = static_cast<float *>(base) + at;
     if (n >= 4) __builtin_memcpy(p, v, 16);
     else
-      for (int i = 0; i < n; ++i) p[i] = v[i];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i < n) p[i] = v[i];
     return;
   }
   uint16_t *p = static_cast<uint16_t *>(base) + at;
@@ -220,7 +222,9 @@ __device__ __forceinline__ void store4(void *base, int64_t at, int n, int dt, co
   for (int i = 0; i < 4; ++i) o[i] = dt == 0 ? f32_to_bf16(v[i]) : __builtin_bit_cast(uint16_t, (_Float16)v[i]);
   if (n >= 4) __builtin_memcpy(p, o, 8);
   else
-    for (int i = 0; i < n; ++i) p[i] = o[i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < n) p[i] = o[i];
 }
 __device__ __forceinline__ float value_of(const void *base, int64_t at, int dt) {
   return dt == 0 ? bf16_to_f32(static_cast<const uint16_t *>(base)[at]) : dt == 1 ? (float)static_cast<const _Float16 *>(base)[at] : static_cast<const float *>(base)[at];

@@ -4,6 +4,7 @@
 // rows).  Its stage is one run of 128 values: the weight rows are the 32x32x64 instruction's rows and token rows its columns, so that a lane has one token row's scale
 // and sixteen sums of it.  A run's two instructions start from zero, their sums are scaled and added in float32 while the next ones run.
 #include <atomic>
+#include <type_traits>
 
 #include "f8.hpp"
 #include "lds_copies.hpp"
@@ -23,14 +24,23 @@ __device__ __forceinline__ i32x4_t uniform(i32x4_t v) {
 }
 __device__ __forceinline__ uint32_t at_most_4g(int64_t bytes) { return bytes > 0xffffff00ll ? 0xffffff00u : (uint32_t)bytes; }
 
-// The sixteen-byte pieces of a tile's row of 128 lie turned by a number of the row's: eight rows one after the other, and eight rows four apart, have a piece in different banks
-// (the reads of eight lanes; the writes of eight lanes whose columns are four apart).
-__device__ __forceinline__ constexpr int f8_turn(int row) { return (row & 7) ^ (row >> 3 & 3); }
+// The sixteen-byte pieces of a tile's row of 128 lie turned by the row's number, so that sixteen rows one after the other, which a read takes at once, have a piece in
+// different banks.
+__device__ __forceinline__ constexpr int f8_turn(int row) { return row >> 1 & 7; }
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)lo) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)hi) << 16;
+}
 
 template <int TM>
 struct F8Stage {
-  static constexpr int X = TM * 128, W = kF8TileN * 128, S = TM * 4, BYTES = X + W + S;
+  // token rows, weight rows, a scale a token row, and 256 bytes each of the scale of the tile's first and second 128 weight rows
+  static constexpr int X = TM * 128, W = kF8TileN * 128, S = TM * 4, BYTES = X + W + S + 512;
 };
+
+constexpr size_t f8_tiles_lds(int tm) {  // two stages, and what a thread copies
+  return 2 * (size_t)(tm * 128 + kF8TileN * 128 + tm * 4 + 512) + kF8Threads * 4 * (tm / 64) + tm * 4;
+}
 
 template <int TM, F8Mode MODE, bool F32>
 __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, int n_tiles, int m_tiles) {
@@ -77,78 +87,77 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, int n
   };
   const int64_t x_first = a.order ? 0 : row0, x_rows = a.order ? a.x.rows : rows;
   const i32x4_t xr = uniform(words_of(a.x.codes + x_first * wide, at_most_4g(x_rows * wide)));
-  uint32_t x_off[XC];
+  // (in LDS between a stage and the next: the registers are for the sums)
+  uint32_t *const x_offs = reinterpret_cast<uint32_t *>(lds + 2 * L::BYTES), *const s_offs = reinterpret_cast<uint32_t *>(lds + 2 * L::BYTES) + kF8Threads * XC;
 #pragma unroll
   for (int c = 0; c < XC; ++c) {
     const int r = (wave * XC + c) * 8 + lane / 8;
-    x_off[c] = source(r) * (uint32_t)wide + (uint32_t)((lane % 8) ^ f8_turn(r)) * 16;
+    x_offs[threadIdx.x * XC + c] = source(r) * (uint32_t)wide + (uint32_t)((lane % 8) ^ f8_turn(r)) * 16;
   }
-  const uint32_t s_off = wave < TM / 64 ? source(wave * 64 + lane) * 4 : 0;
+  if (threadIdx.x < TM) s_offs[threadIdx.x] = source(threadIdx.x) * 4;
   const int64_t matrix = (int64_t)mat * N * K;
-  uint32_t w_off[4], w_k[4];
   i32x4_t wr{};
-  uint32_t w_reg[16];
   if constexpr (MODE != kColsOfWeights) {
     const int which = MODE == kPair ? wave >> 2 : 0;  // waves 4 to 7 copy the up rows
     wr = uniform(words_of(a.m[which].w + matrix + (int64_t)n0 * K, at_most_4g((int64_t)(N - n0) * K)));
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const int r = (wave * 4 + c) * 8 + lane / 8;
-      w_k[c] = (uint32_t)((lane % 8) ^ f8_turn(r)) * 16;
-      w_off[c] = (uint32_t)(MODE == kPair ? r & 127 : r) * (uint32_t)K + w_k[c];
-    }
   }
-  const bool w_inside = n0 + 4 * lane < N;
-  auto fetch = [&](int j, int place) __attribute__((always_inline)) {
-    const uint32_t at = lds_at + place * L::BYTES;
+  // where the scales of the wave's half of the weight rows are (past the last block its own again, of rows that are never stored)
+  const float *w_scale[2];
+  {
+    const int second = wave & 1, block = MODE == kPair ? nt : n0 / kF8Run + second < n_blocks ? n0 / kF8Run + second : n_blocks - 1;
 #pragma unroll
-    for (int c = 0; c < XC; ++c) copy_to_lds(xr, x_off[c], (uint32_t)(j * kF8Run), at + (wave * XC + c) * 1024);
-    if (wave < TM / 64) copy4_to_lds(uniform(words_of(a.x.scales + (int64_t)j * a.x.rows + x_first, at_most_4g(x_rows * 4))), s_off, at + L::X + L::W + wave * 256);
-    if constexpr (MODE != kColsOfWeights) {
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        copy_to_lds(wr, (uint32_t)(j * kF8Run) + w_k[c] < (uint32_t)K ? w_off[c] : kF8Outside, (uint32_t)(j * kF8Run), at + L::X + (wave * 4 + c) * 1024);
-    } else {
-      const bool second = j >= runs;
-      const int k0 = (second ? j - runs : j) * kF8Run + wave * 16;
-      // (what lies past the matrix's last row is past the descriptor's end)
-      const int64_t left = ((int64_t)K - k0) * N - n0;
-      const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(a.m[second].w + matrix + (int64_t)k0 * N + n0), 0,
-                                                                             (int)(left > 0 ? at_most_4g(left) : 0u), 0x00020000);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) w_reg[i] = __builtin_amdgcn_raw_buffer_load_b32(from, w_inside ? lane * 4 : (int)kF8Outside, i * N, 0);
-    }
+    for (int i = 0; i < 2; ++i)
+      w_scale[i] = MODE == kPair ? a.m[second].s + ((int64_t)mat * n_blocks + block) * runs : MODE == kRowsOfWeights ? a.m[0].s + ((int64_t)mat * n_blocks + block) * runs
+                                                                                                                     : a.m[i].s + (int64_t)mat * runs * n_blocks + block;
+  }
+  // Token rows and all scales, XC + 2 copies.  (Every wave copies scales, several the same: with a branch around them the compiler puts the sums' arithmetic off past it.)
+  struct Offsets {
+    uint32_t x[XC], s;
   };
-  auto put_columns = [&](int place) __attribute__((always_inline)) {  // sixteen weight rows of four columns: 16 bytes of each column
-    if constexpr (MODE == kColsOfWeights) {
-      uint32_t o[4][4];
+  auto offsets = [&]() __attribute__((always_inline)) {
+    Offsets o;
+    uint32_t thread = threadIdx.x;
+    asm volatile("" : "+v"(thread));  // (addresses are made where they are used: there are no registers to keep them)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t *const d = w_reg + 4 * i;
-        const uint32_t t0 = __builtin_amdgcn_perm(d[1], d[0], 0x05010400u), t1 = __builtin_amdgcn_perm(d[1], d[0], 0x07030602u);
-        const uint32_t t2 = __builtin_amdgcn_perm(d[3], d[2], 0x05010400u), t3 = __builtin_amdgcn_perm(d[3], d[2], 0x07030602u);
-        o[0][i] = __builtin_amdgcn_perm(t2, t0, 0x05040100u), o[1][i] = __builtin_amdgcn_perm(t2, t0, 0x07060302u);
-        o[2][i] = __builtin_amdgcn_perm(t3, t1, 0x05040100u), o[3][i] = __builtin_amdgcn_perm(t3, t1, 0x07060302u);
-      }
+    for (int c = 0; c < XC; ++c) o.x[c] = x_offs[thread * XC + c];
+    o.s = s_offs[wave % (TM / 64) * 64 + thread % 64];
+    return o;
+  };
+  auto fetch_rows = [&](int j, const Offsets &o) __attribute__((always_inline)) {
+    const uint32_t at = lds_at + (j & 1) * L::BYTES;
+#pragma unroll
+    for (int c = 0; c < XC; ++c) copy_to_lds(xr, o.x[c], (uint32_t)(j * kF8Run), at + (wave * XC + c) * 1024);
+    copy4_to_lds(uniform(words_of(a.x.scales + (int64_t)j * a.x.rows + x_first, at_most_4g(x_rows * 4))), o.s, at + L::X + L::W + wave % (TM / 64) * 256);
+    const float *const from = MODE != kColsOfWeights ? w_scale[0] + j : j < runs ? w_scale[0] + (int64_t)j * n_blocks : w_scale[1] + (int64_t)(j - runs) * n_blocks;
+    copy4_to_lds(uniform(words_of(from, 4)), 0, at + L::X + L::W + L::S + (wave & 1) * 256);
+  };
+  auto fetch_weights = [&](int j) __attribute__((always_inline)) {  // four copies
+    const uint32_t at = lds_at + (j & 1) * L::BYTES;
+    uint32_t l = threadIdx.x & 63;
+    asm volatile("" : "+v"(l));
+    if constexpr (MODE != kColsOfWeights) {
+      // rows c * 8 + l / 8 of the wave's 32, whose pieces are turned by half the row's number
+      const bool whole = (j + 1) * kF8Run <= K;
+      const uint32_t row = (uint32_t)((MODE == kPair ? wave & 3 : wave) * 32 + l / 8) * (uint32_t)K, piece = ((l % 8) ^ (l / 16)) * 16;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const int r = 4 * lane + c;
-        *reinterpret_cast<u32x4_f8 *>(lds + place * L::BYTES + L::X + r * 128 + (wave ^ f8_turn(r)) * 16) = u32x4_f8{o[c][0], o[c][1], o[c][2], o[c][3]};
+        // (the scalar offset stays within a row: past the descriptor's end it would not be checked)
+        const uint32_t k = piece ^ ((c & 1) * 64), off = row + (uint32_t)(c * 8 * K) + k;
+        copy_to_lds(wr, whole || j * kF8Run + (int)k < K ? off : kF8Outside, (uint32_t)(j * kF8Run), at + L::X + (wave * 4 + c) * 1024);
+      }
+    } else {
+      // matrices [K][N]: rows c * 4 + l / 16 of the wave's sixteen, 256 columns each, whose pieces of sixteen are turned by twice the row's number (mod 8)
+      const bool second = j >= runs;
+      const int k0 = (second ? j - runs : j) * kF8Run;
+      // (rows past the matrix's last one are past the descriptor's end)
+      const i32x4_t from = uniform(words_of(a.m[second].w + matrix + (int64_t)k0 * N + n0, at_most_4g(((int64_t)K - k0) * N - n0)));
+      const uint32_t row = (uint32_t)(wave * 16 + l / 16) * (uint32_t)N, piece = ((l % 16) ^ (l / 16 * 2)) * 16;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const uint32_t col = piece ^ ((c & 1) * 128);
+        copy_to_lds(from, n0 + (int)col < N ? row + (uint32_t)(c * 4 * N) + col : kF8Outside, 0, at + L::X + (wave * 4 + c) * 1024);
       }
     }
-  };
-  const float *ws[2];
-  if constexpr (MODE == kPair) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) ws[i] = a.m[i].s + ((int64_t)mat * n_blocks + nt) * runs;
-  } else {
-    const int block = (n0 + wn * 64) / kF8Run < n_blocks ? (n0 + wn * 64) / kF8Run : n_blocks - 1;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) ws[i] = MODE == kRowsOfWeights ? a.m[0].s + ((int64_t)mat * n_blocks + block) * runs : a.m[i].s + (int64_t)mat * runs * n_blocks + block;
-  }
-  auto weight_scale = [&](int j, int i) __attribute__((always_inline)) {
-    if constexpr (MODE == kColsOfWeights) return j < runs ? ws[0][(int64_t)j * n_blocks] : ws[1][(int64_t)(j - runs) * n_blocks];
-    return ws[i][j];
   };
 
   f32x16_t acc[MT][2];
@@ -159,115 +168,200 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, int n
 #pragma unroll
       for (int v = 0; v < 16; ++v) acc[t][i][v] = 0.f;
   const int x_at = (wm * 32 * MT + ln) * 128, w_at0 = (MODE == kPair ? wn * 32 + ln : wn * 64 + ln) * 128, w_at1 = w_at0 + (MODE == kPair ? 128 : 32) * 128;
+  // matrices [K][N]: a lane's place for the transposing reads, which give each of sixteen lanes eight values of its column out of eight rows of sixteen columns
+  const int c_k = (lane & 15) >> 1, c_at = (half * 32 + c_k) * 256 + (((wn * 4 + (lane >> 4 & 1)) ^ (2 * c_k)) * 16) + (lane & 1) * 8;
   const int turn = f8_turn(ln);  // (rows 32 apart are turned alike)
   auto operand = [&](const unsigned char *row, int q) __attribute__((always_inline)) {  // values 64 q + 32 half to 64 q + 32 half + 31
     const u32x4_f8 lo = *reinterpret_cast<const u32x4_f8 *>(row + ((4 * q + 2 * half) ^ turn) * 16), hi = *reinterpret_cast<const u32x4_f8 *>(row + ((4 * q + 2 * half + 1) ^ turn) * 16);
     return i32x8_t{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
   };
-  auto multiply = [&](const i32x8_t *w, const i32x8_t *x) __attribute__((always_inline)) {
-    f32x16_t sum{};
+  auto weights = [&](const unsigned char *tile, int i, int q) __attribute__((always_inline)) {
+    if constexpr (MODE != kColsOfWeights) return operand(tile + (i ? w_at1 : w_at0), q);
+    typedef int pair_t __attribute__((ext_vector_type(2)));
+    typedef __attribute__((address_space(3))) pair_t lds_pair_t;
+    i32x8_t v;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const pair_t r = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_pair_t *)(tile + (c_at ^ (i * 32)) + (64 * q + 8 * p) * 256));
+      v[2 * p] = r.x, v[2 * p + 1] = r.y;
+    }
+    return v;
+  };
+  auto multiply = [&](const i32x8_t &w, const i32x8_t &x, f32x16_t sum) __attribute__((always_inline)) {
     if constexpr (F32) {
 #pragma unroll
-      for (int q = 0; q < 2; ++q)
-#pragma unroll
-        for (int p = 0; p < 4; ++p)
-          sum = __builtin_amdgcn_mfma_f32_32x32x16_bf16(codes_to_bf16((uint32_t)w[q][2 * p], (uint32_t)w[q][2 * p + 1]), codes_to_bf16((uint32_t)x[q][2 * p], (uint32_t)x[q][2 * p + 1]),
-                                                        sum, 0, 0, 0);
+      for (int p = 0; p < 4; ++p)
+        sum = __builtin_amdgcn_mfma_f32_32x32x16_bf16(codes_to_bf16((uint32_t)w[2 * p], (uint32_t)w[2 * p + 1]), codes_to_bf16((uint32_t)x[2 * p], (uint32_t)x[2 * p + 1]), sum, 0, 0, 0);
+      return sum;
     } else {
-      sum = mfma_f8_32(w[0], x[0], sum);
-      sum = mfma_f8_32(w[1], x[1], sum);
+      return mfma_f8_32(w, x, sum);
     }
-    return sum;
   };
 
-  fetch(0, 0);
-  wait_copies<0>();
-  put_columns(0);
-  wait_reads();
-  block_barrier();
-  for (int j = 0; j < steps; ++j) {
-    const int place = j & 1;
-    if (j + 1 < steps) fetch(j + 1, place ^ 1);
-    const unsigned char *const at = lds + place * L::BYTES;
-    const float *const sx = reinterpret_cast<const float *>(at + L::X + L::W) + wm * 32 * MT + ln;
-    const float s0 = weight_scale(j, 0), s1 = MODE == kPair ? weight_scale(j, 1) : s0;
-    i32x8_t w[2][2];
+  // The stages of a wave with LIVE sub-tiles of token rows.  An operand's registers take the next one's values as soon as its last multiply has been issued: those of the
+  // next sub-tile, and in the last sub-tile's time those of the next stage.  So a stage has one barrier, amid its multiplies, ahead of the last sub-tile: all waves have read what
+  // they read of the stage by then, whose place the copies of the stage after the next may take, and the next stage's copies have arrived.
+  auto add = [&](f32x16_t &to, const f32x16_t &sum, float f) __attribute__((always_inline)) {
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      w[0][q] = operand(at + L::X + w_at0, q);
-      w[1][q] = operand(at + L::X + w_at1, q);
-    }
+    for (int v = 0; v < 16; ++v) to[v] = __builtin_fmaf(sum[v], f, to[v]);
+  };
+  auto all_stages = [&](auto live_of) __attribute__((always_inline)) {
+    constexpr int LIVE = decltype(live_of)::value, LAST = LIVE - 1;
+    i32x8_t w[2][2], x[2];  // [weight sub-tile][half of the run]
+    auto stage = [&](int j, bool more) __attribute__((always_inline)) {
+      if constexpr (LIVE == 0) {
+        wait_copies<0>();
+        block_barrier();
+        if (more) {
+          fetch_rows(j + 2, offsets());
+          fetch_weights(j + 2);
+        }
+      } else {
+        const unsigned char *const at = lds + (j & 1) * L::BYTES, *const next = lds + ((j + 1) & 1) * L::BYTES;  // (behind the last stage: a place that nothing waits for)
+        const float *const sx = reinterpret_cast<const float *>(at + L::X + L::W) + wm * 32 * MT + ln, *const sw = reinterpret_cast<const float *>(at + L::X + L::W + L::S);
+        const float s0 = sw[MODE == kPair ? 0 : (wn >> 1) * 64], s1 = MODE == kPair ? sw[64] : s0;
+        float s = sx[0];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      if (wm * 32 * MT + t * 32 < rows) {
-        i32x8_t x[2];
+        for (int t = 0; t < LIVE; ++t) {
+          Offsets o{};
+          if (t == LAST) {
+            wait_copies<0>();
+            block_barrier();
+            if (more) o = offsets();
+          }
+          f32x16_t sum[2] = {};
+          const float now = s;
 #pragma unroll
-        for (int q = 0; q < 2; ++q) x[q] = operand(at + x_at + t * 32 * 128, q);
-        const float s = sx[t * 32];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const f32x16_t sum = multiply(w[i], x);
-          const float f = s * (i ? s1 : s0);
-#pragma unroll
-          for (int v = 0; v < 16; ++v) acc[t][i][v] = __builtin_fmaf(sum[v], f, acc[t][i][v]);
+          for (int q = 0; q < 2; ++q) {
+            sum[0] = multiply(w[0][q], x[q], sum[0]);
+            sum[1] = multiply(w[1][q], x[q], sum[1]);
+            __builtin_amdgcn_sched_barrier(0);  // (no operand earlier: there are no registers for more)
+            if (t == LAST) {
+              if (more && q == 0) fetch_rows(j + 2, o);
+              if (more && q == 1) fetch_weights(j + 2);
+              w[0][q] = weights(next + L::X, 0, q);
+              w[1][q] = weights(next + L::X, 1, q);
+              x[q] = operand(next + x_at, q);
+            } else {
+              x[q] = operand(at + x_at + (t + 1) * 32 * 128, q);
+              if (q == 0) s = sx[(t + 1) * 32];
+            }
+          }
+          add(acc[t][0], sum[0], now * s0);
+          add(acc[t][1], sum[1], now * s1);
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
+    };
+    if constexpr (LIVE > 0) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        w[0][q] = weights(lds + L::X, 0, q);
+        w[1][q] = weights(lds + L::X, 1, q);
+        x[q] = operand(lds + x_at, q);
+      }
     }
+    int j = 0;
+    for (; j + 2 < steps; ++j) stage(j, true);
+    for (; j < steps; ++j) stage(j, false);
+  };
+  __syncthreads();  // (offsets of scales come from other threads)
+  fetch_rows(0, offsets());
+  fetch_weights(0);
+  if (steps > 1) {
+    fetch_rows(1, offsets());
+    fetch_weights(1);
+    wait_copies<XC + 6>();
+  } else {
     wait_copies<0>();
-    if (j + 1 < steps) put_columns(place ^ 1);
-    wait_reads();
-    block_barrier();
   }
+  block_barrier();
+  const int live = (rows - wm * 32 * MT + 31) / 32;  // sub-tiles of this wave's that hold rows
+  if (live >= MT) all_stages(std::integral_constant<int, MT>());
+  else if (MT > 3 && live == 3) all_stages(std::integral_constant<int, (MT > 3 ? 3 : 0)>());
+  else if (MT > 2 && live == 2) all_stages(std::integral_constant<int, (MT > 2 ? 2 : 0)>());
+  else if (MT > 1 && live == 1) all_stages(std::integral_constant<int, (MT > 1 ? 1 : 0)>());
+  else all_stages(std::integral_constant<int, 0>());
 
-  // lane: token row ln of each sub-tile; of weight rows 8 g + 4 half + 0..3 the sums 4 g + 0..3
+  // Results: a lane has token row ln of each sub-tile, and of weight rows 8 g + 4 half + 0..3 the sums 4 g + 0..3.  They go through LDS, rows of 128 bytes whose pieces of
+  // sixteen are turned as the operands', and out of it in whole lines: stored as they lie, 8 bytes a lane and 32 rows an instruction, a 4096 x 4096 bf16 result took 16 us.
+  __syncthreads();  // (all waves have read their last operands)
+  const int row_of_wave = wm * 32 * MT;
   if constexpr (MODE == kPair) {
-    float *const most = reinterpret_cast<float *>(lds);  // [4][TM]
-    uint32_t m[MT];
+    float *const most = reinterpret_cast<float *>(lds + TM * 128);  // [4][TM]
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-      m[t] = 0;
+      uint32_t m = 0;
 #pragma unroll
       for (int v = 0; v < 16; ++v) {
         acc[t][0][v] = silu(acc[t][0][v]) * acc[t][1][v];
-        m[t] = umax(m[t], abs_bits(acc[t][0][v]));
+        m = umax(m, abs_bits(acc[t][0][v]));
       }
-      m[t] = umax(m[t], (uint32_t)__shfl_xor((int)m[t], 32, kWave));
-      if (half == 0) most[wn * TM + wm * 32 * MT + t * 32 + ln] = __uint_as_float(m[t]);
+      m = umax(m, (uint32_t)__shfl_xor((int)m, 32, kWave));
+      if (half == 0) most[wn * TM + row_of_wave + t * 32 + ln] = __uint_as_float(m);
     }
     __syncthreads();
-    const int64_t h_wide = (int64_t)n_blocks * kF8Run;
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-      const int r = wm * 32 * MT + t * 32 + ln;
+      const int r = row_of_wave + t * 32 + ln;
       uint32_t all = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) all = umax(all, __float_as_uint(most[i * TM + r]));
       const F8Scale s(all);
-      if (r < rows) {
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
-          *reinterpret_cast<uint32_t *>(a.h + (int64_t)(row0 + r) * h_wide + n0 + wn * 32 + 8 * g + 4 * half) =
-              s.codes(acc[t][0][4 * g], acc[t][0][4 * g + 1], acc[t][0][4 * g + 2], acc[t][0][4 * g + 3]);
-        if (wn == 0 && half == 0) a.hs[(int64_t)nt * a.rows + row0 + r] = s.scale;
-      }
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<uint32_t *>(lds + r * 128 + ((wn * 2 + (g >> 1)) ^ f8_turn(r)) * 16 + (g & 1) * 8 + half * 4) =
+            s.codes(acc[t][0][4 * g], acc[t][0][4 * g + 1], acc[t][0][4 * g + 2], acc[t][0][4 * g + 3]);
+      if (wn == 0 && half == 0 && r < rows) a.hs[(int64_t)nt * a.rows + row0 + r] = s.scale;
     }
+    __syncthreads();
+    const int64_t h_wide = (int64_t)n_blocks * kF8Run;
+    for (int r = threadIdx.x / 8; r < rows; r += kF8Threads / 8)
+      *reinterpret_cast<u32x4_f8 *>(a.h + (int64_t)(row0 + r) * h_wide + n0 + ((threadIdx.x % 8) ^ f8_turn(r)) * 16) =
+          *reinterpret_cast<const u32x4_f8 *>(lds + r * 128 + threadIdx.x % 8 * 16);
   } else {
+    constexpr int SIZE = F32 ? 4 : 2, EACH = 16 / SIZE, PASSES = F32 ? 2 : 1;  // bytes of a value, values of a piece; 64 weight rows at once, or 32
+    unsigned char *const own = lds + wave * (32 * MT * 128);
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      const int r = wm * 32 * MT + t * 32 + ln;
-      if (r < rows) {
+    for (int pass = 0; pass < PASSES; ++pass) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+      for (int i = pass; i < (F32 ? pass + 1 : 2); ++i)
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const int n = n0 + wn * 64 + i * 32 + 8 * g + 4 * half;
-            if (n < N) {
-              float o[4];
+        for (int g = 0; g < 4; ++g) {
+          float bias[4] = {0.f, 0.f, 0.f, 0.f};
+          if (a.bias)
 #pragma unroll
-              for (int v = 0; v < 4; ++v) o[v] = acc[t][i][4 * g + v] + (a.bias && n + v < N ? value_of(a.bias, n + v, a.dt) : 0.f);
-              store4(a.y, (int64_t)(row0 + r) * N + n, N - n, a.dt, o);
+            for (int v = 0; v < 4; ++v) {
+              const int n = n0 + wn * 64 + i * 32 + 8 * g + 4 * half + v;
+              bias[v] = n < N ? value_of(a.bias, n, a.dt) : 0.f;
             }
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            const int r = t * 32 + ln;
+            float o[4];
+#pragma unroll
+            for (int v = 0; v < 4; ++v) o[v] = acc[t][i][4 * g + v] + bias[v];
+            const int piece = F32 ? 2 * g + half : i * 4 + g;
+            unsigned char *const to = own + r * 128 + (piece ^ f8_turn(r)) * 16 + (F32 ? 0 : half * 8);
+            if constexpr (F32) *reinterpret_cast<f32x4_t *>(to) = f32x4_t{o[0], o[1], o[2], o[3]};
+            else if (a.dt == 0) *reinterpret_cast<uint2 *>(to) = make_uint2(cvt_pk_bf16(o[0], o[1]), cvt_pk_bf16(o[2], o[3]));
+            else *reinterpret_cast<uint2 *>(to) = make_uint2(pack_f16(o[0], o[1]), pack_f16(o[2], o[3]));
           }
+        }
+#pragma unroll
+      for (int r0 = 0; r0 < 32 * MT; r0 += 8) {
+        const int r = r0 + lane / 8, n = n0 + wn * 64 + pass * 32 + ((lane % 8) ^ f8_turn(r)) * EACH;
+        const u32x4_f8 v = *reinterpret_cast<const u32x4_f8 *>(own + r * 128 + lane % 8 * 16);
+        if (row_of_wave + r < rows && n < N) {
+          unsigned char *const to = static_cast<unsigned char *>(a.y) + ((int64_t)(row0 + row_of_wave + r) * N + n) * SIZE;
+          if (n + EACH <= N) {
+            __builtin_memcpy(to, &v, 16);
+          } else {
+#pragma unroll
+            for (int e = 0; e < EACH; ++e)
+              if (n + e < N) __builtin_memcpy(to + e * SIZE, reinterpret_cast<const unsigned char *>(&v) + e * SIZE, SIZE);
+          }
+        }
       }
     }
   }
@@ -275,7 +369,7 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, int n
 
 template <int TM, F8Mode MODE, bool F32>
 static hipError_t launch_tiles(const F8Product &p, hipStream_t st) {
-  constexpr size_t lds = 2 * F8Stage<TM>::BYTES;
+  constexpr size_t lds = f8_tiles_lds(TM);
   constexpr int kMaxDevices = 64;
   static std::atomic<bool> raised[kMaxDevices];  // more LDS than a kernel gets without asking
   int dev = 0;

@@ -145,8 +145,11 @@ __device__ __forceinline__ uint32_t max_of_16_lanes(uint32_t m) {
 __device__ __forceinline__ float silu(float g) { return g / (1.f + __expf(-g)); }
 
 // ---------------------------------------------------------------- segments
-// Tile m of the segments that offsets[n_mats + 1] cut the rows into, in pieces of `tile` rows: matrix, first row and number of rows.  Behind the segments' tiles come those of the
-// rows that belong to none (matrix n_mats), behind those nothing (rows 0).  By one wave; offsets out of order or range only make pieces that overlap or are missing.
+// Piece m of the segments that offsets[n_mats + 1] cut the rows into: matrix, first row and number of rows.  A segment is cut into as few pieces of at most `tile` rows as
+// it can be, of about one size (multiples of 32 rows).  Behind the segments' pieces come those of the rows that belong to none (matrix n_mats), behind those nothing (rows 0).
+// By one wave; offsets out of order or range only make pieces that overlap or are missing.
+// In the experts' order: with whole pieces first and the rest of the segments behind them, the longest first, the launch ends more evenly, but its first half multiplies and its
+// second one waits for weights (4096 tokens, skewed routing over 128 experts of 2048 x 768: down 138 us, 156 so).
 struct F8Piece {
   int mat;
   uint32_t row, rows;
@@ -167,8 +170,8 @@ __device__ __forceinline__ F8Piece f8_piece(const uint32_t *__restrict__ offsets
       lo = lo < total ? lo : total;
       hi = hi < lo ? lo : hi < total ? hi : total;
     }
-    const uint32_t tiles = (hi - lo + tile - 1) / tile;
-    uint32_t upto = tiles;
+    const uint32_t pieces = (hi - lo + tile - 1) / tile;
+    uint32_t upto = pieces;
     for (int d = 1; d < kWave; d <<= 1) {
       const uint32_t v = __shfl_up(upto, d, kWave);
       if (lane >= d) upto += v;
@@ -176,10 +179,10 @@ __device__ __forceinline__ F8Piece f8_piece(const uint32_t *__restrict__ offsets
     const uint64_t found = __ballot(m < before + upto);
     if (found) {
       const int at = __builtin_amdgcn_readfirstlane((int)__builtin_ctzll(found));
-      const uint32_t first = m - before - (uint32_t)(__builtin_amdgcn_readlane((int)upto, at) - __builtin_amdgcn_readlane((int)tiles, at));
+      const uint32_t p = (uint32_t)__builtin_amdgcn_readlane((int)pieces, at), i = m - before - ((uint32_t)__builtin_amdgcn_readlane((int)upto, at) - p);
       const uint32_t slo = (uint32_t)__builtin_amdgcn_readlane((int)lo, at), shi = (uint32_t)__builtin_amdgcn_readlane((int)hi, at);
-      const uint32_t row = slo + first * tile;
-      return {e0 + at, row, shi - row < tile ? shi - row : tile};
+      const uint32_t even = p == 1 ? tile : ((shi - slo + p - 1) / p + 31) / 32 * 32, size = even < tile ? even : tile, row = slo + i * size;
+      return {e0 + at, row, shi - row < size ? shi - row : size};
     }
     before += (uint32_t)__builtin_amdgcn_readlane((int)upto, kWave - 1);
   }
@@ -187,7 +190,7 @@ __device__ __forceinline__ F8Piece f8_piece(const uint32_t *__restrict__ offsets
 }
 inline int64_t f8_most_pieces(const F8Product &p, int tile) {
   if (!p.offsets) return (p.rows + tile - 1) / tile;
-  return p.rows / tile + (p.n_mats + 1 < p.rows ? p.n_mats + 1 : p.rows) ;
+  return p.rows / tile + (p.n_mats + 1 < p.rows ? p.n_mats + 1 : p.rows);
 }
 
 // ---------------------------------------------------------------- products

@@ -79,10 +79,9 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, int n
   }
   // ---- what a lane copies of a stage
   const int64_t wide = (int64_t)steps * kF8Run;
-  auto source = [&](int r) __attribute__((always_inline)) {  // x row of the piece's row r, as the descriptors below count; rows past the end repeat the last one (never stored)
-    const uint32_t tr = (uint32_t)(r < rows ? r : rows - 1);
-    if (!a.order) return tr;
-    const uint32_t at = a.order[row0 + tr] / (uint32_t)a.k_div;
+  auto source = [&](int r) __attribute__((always_inline)) {  // x row of the piece's row r, as the descriptors below count (rows past the end are zeros)
+    if (!a.order) return (uint32_t)r;
+    const uint32_t at = a.order[row0 + r] / (uint32_t)a.k_div;
     return at < (uint32_t)a.x.rows ? at : 0u;
   };
   const int64_t x_first = a.order ? 0 : row0, x_rows = a.order ? a.x.rows : rows;
@@ -92,9 +91,9 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, int n
 #pragma unroll
   for (int c = 0; c < XC; ++c) {
     const int r = (wave * XC + c) * 8 + lane / 8;
-    x_offs[threadIdx.x * XC + c] = source(r) * (uint32_t)wide + (uint32_t)((lane % 8) ^ f8_turn(r)) * 16;
+    x_offs[threadIdx.x * XC + c] = r < rows ? source(r) * (uint32_t)wide + (uint32_t)((lane % 8) ^ f8_turn(r)) * 16 : kF8Outside;
   }
-  if (threadIdx.x < TM) s_offs[threadIdx.x] = source(threadIdx.x) * 4;
+  if (threadIdx.x < TM) s_offs[threadIdx.x] = (int)threadIdx.x < rows ? source(threadIdx.x) * 4 : kF8Outside;
   const int64_t matrix = (int64_t)mat * N * K;
   i32x4_t wr{};
   if constexpr (MODE != kColsOfWeights) {
@@ -167,7 +166,7 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, int n
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int v = 0; v < 16; ++v) acc[t][i][v] = 0.f;
-  const int x_at = (wm * 32 * MT + ln) * 128, w_at0 = (MODE == kPair ? wn * 32 + ln : wn * 64 + ln) * 128, w_at1 = w_at0 + (MODE == kPair ? 128 : 32) * 128;
+  const int x_at = (wm * 32 + ln) * 128, w_at0 = (MODE == kPair ? wn * 32 + ln : wn * 64 + ln) * 128, w_at1 = w_at0 + (MODE == kPair ? 128 : 32) * 128;
   // matrices [K][N]: a lane's place for the transposing reads, which give each of sixteen lanes eight values of its column out of eight rows of sixteen columns
   const int c_k = (lane & 15) >> 1, c_at = (half * 32 + c_k) * 256 + (((wn * 4 + (lane >> 4 & 1)) ^ (2 * c_k)) * 16) + (lane & 1) * 8;
   const int turn = f8_turn(ln);  // (rows 32 apart are turned alike)
@@ -218,7 +217,7 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, int n
         }
       } else {
         const unsigned char *const at = lds + (j & 1) * L::BYTES, *const next = lds + ((j + 1) & 1) * L::BYTES;  // (behind the last stage: a place that nothing waits for)
-        const float *const sx = reinterpret_cast<const float *>(at + L::X + L::W) + wm * 32 * MT + ln, *const sw = reinterpret_cast<const float *>(at + L::X + L::W + L::S);
+        const float *const sx = reinterpret_cast<const float *>(at + L::X + L::W) + wm * 32 + ln, *const sw = reinterpret_cast<const float *>(at + L::X + L::W + L::S);
         const float s0 = sw[MODE == kPair ? 0 : (wn >> 1) * 64], s1 = MODE == kPair ? sw[64] : s0;
         float s = sx[0];
 #pragma unroll
@@ -243,8 +242,8 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, int n
               w[1][q] = weights(next + L::X, 1, q);
               x[q] = operand(next + x_at, q);
             } else {
-              x[q] = operand(at + x_at + (t + 1) * 32 * 128, q);
-              if (q == 0) s = sx[(t + 1) * 32];
+              x[q] = operand(at + x_at + (t + 1) * 64 * 128, q);
+              if (q == 0) s = sx[(t + 1) * 64];
             }
           }
           add(acc[t][0], sum[0], now * s0);
@@ -276,7 +275,7 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, int n
     wait_copies<0>();
   }
   block_barrier();
-  const int live = (rows - wm * 32 * MT + 31) / 32;  // sub-tiles of this wave's that hold rows
+  const int live = (rows - wm * 32 + 63) / 64;  // sub-tiles of this wave's (every other one of the block's) that hold rows
   if (live >= MT) all_stages(std::integral_constant<int, MT>());
   else if (MT > 3 && live == 3) all_stages(std::integral_constant<int, (MT > 3 ? 3 : 0)>());
   else if (MT > 2 && live == 2) all_stages(std::integral_constant<int, (MT > 2 ? 2 : 0)>());
@@ -286,7 +285,6 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, int n
   // Results: a lane has token row ln of each sub-tile, and of weight rows 8 g + 4 half + 0..3 the sums 4 g + 0..3.  They go through LDS, rows of 128 bytes whose pieces of
   // sixteen are turned as the operands', and out of it in whole lines: stored as they lie, 8 bytes a lane and 32 rows an instruction, a 4096 x 4096 bf16 result took 16 us.
   __syncthreads();  // (all waves have read their last operands)
-  const int row_of_wave = wm * 32 * MT;
   if constexpr (MODE == kPair) {
     float *const most = reinterpret_cast<float *>(lds + TM * 128);  // [4][TM]
 #pragma unroll
@@ -298,12 +296,12 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, int n
         m = umax(m, abs_bits(acc[t][0][v]));
       }
       m = umax(m, (uint32_t)__shfl_xor((int)m, 32, kWave));
-      if (half == 0) most[wn * TM + row_of_wave + t * 32 + ln] = __uint_as_float(m);
+      if (half == 0) most[wn * TM + (2 * t + wm) * 32 + ln] = __uint_as_float(m);
     }
     __syncthreads();
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-      const int r = row_of_wave + t * 32 + ln;
+      const int r = (2 * t + wm) * 32 + ln;
       uint32_t all = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) all = umax(all, __float_as_uint(most[i * TM + r]));
@@ -352,8 +350,9 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, int n
       for (int r0 = 0; r0 < 32 * MT; r0 += 8) {
         const int r = r0 + lane / 8, n = n0 + wn * 64 + pass * 32 + ((lane % 8) ^ f8_turn(r)) * EACH;
         const u32x4_f8 v = *reinterpret_cast<const u32x4_f8 *>(own + r * 128 + lane % 8 * 16);
-        if (row_of_wave + r < rows && n < N) {
-          unsigned char *const to = static_cast<unsigned char *>(a.y) + ((int64_t)(row0 + row_of_wave + r) * N + n) * SIZE;
+        const int row = (r0 / 32 * 2 + wm) * 32 + r % 32;
+        if (row < rows && n < N) {
+          unsigned char *const to = static_cast<unsigned char *>(a.y) + ((int64_t)(row0 + row) * N + n) * SIZE;
           if (n + EACH <= N) {
             __builtin_memcpy(to, &v, 16);
           } else {

@@ -9,7 +9,7 @@ using namespace mi_moe;
 namespace {
 
 constexpr int64_t kMostPairs = ((int64_t)1 << 24) - 1;  // a block a token or row, in launches of less than 2^32 threads
-constexpr int32_t kMostExtent = 1 << 22;
+constexpr int32_t kMostExtent = 1 << 22, kMostExperts = 512;
 
 int check_types(const char *who, int32_t dtype, int32_t w_dtype = MI_MOE_DTYPE_BF16) {
   for (int32_t d : {dtype, w_dtype})
@@ -53,7 +53,15 @@ int check_linear(const char *who, const void *x, const void *w, const float *sca
 size_t linear_bytes(int64_t M, int K) {
   Carver c(nullptr);
   RowsIn(c, M, K);
+  c.take<uint4>((size_t)f8_list_places(M, kMostExperts));
   return c.off + 256;
+}
+// A list for a product, or none for one matrix.
+void list_for(F8Product &p, F8Lists &lists, int i, uint4 *at) {
+  p.list = at;
+  lists.list[i] = at;
+  lists.tile[i] = f8_tile_rows(p);
+  lists.places[i] = (int)f8_most_pieces(p.rows, p.n_mats, lists.tile[i]);
 }
 
 int linear(const char *who, const void *x, const void *w, const float *scales, const void *bias, const uint32_t *offsets, int64_t M, int E, int32_t N, int32_t K, int32_t transpose,
@@ -61,10 +69,9 @@ int linear(const char *who, const void *x, const void *w, const float *scales, c
   if (check_workspace(who, workspace, workspace_bytes, linear_bytes(M, K))) return 1;
   Carver c(workspace);
   const RowsIn q(c, M, K);
-  MI_HIP(launch_quantize_f8_rows(x, dtype, M, K, q.out(M, K), st));
+  uint4 *const list = c.take<uint4>((size_t)f8_list_places(M, kMostExperts));
   F8Product p{};
   p.x = q.as(M);
-  p.offsets = offsets;
   p.n_mats = E;
   p.rows = M;
   p.m[0] = p.m[1] = {static_cast<const uint8_t *>(w), scales};
@@ -74,6 +81,12 @@ int linear(const char *who, const void *x, const void *w, const float *scales, c
   p.bias = bias;
   p.y = y;
   p.dt = dtype;
+  F8Lists lists;
+  lists.offsets = offsets;
+  lists.n_mats = E;
+  lists.rows = M;
+  if (offsets) list_for(p, lists, 0, list);
+  MI_HIP(launch_quantize_f8_rows(x, dtype, M, K, q.out(M, K), st, lists));
   MI_HIP(launch_f8_product(p, st));
   return 0;
 }
@@ -82,6 +95,7 @@ int linear(const char *who, const void *x, const void *w, const float *scales, c
 struct ExpertsWs {
   uint32_t *order, *offsets;
   int32_t *inverse;
+  uint4 *list[3];
   void *sort;
   RowsIn x, dout;   // rows of tokens
   float *g, *u, *dh;  // float32 rows of pairs: gradients, and batches of a few rows an expert
@@ -92,7 +106,8 @@ struct ExpertsWs {
 
  private:
   ExpertsWs(Carver c, int64_t T, int64_t P, int H, int I, int E, int k, bool grad)
-      : order(c.take<uint32_t>((size_t)P)), offsets(c.take<uint32_t>((size_t)E + 1)), inverse(c.take<int32_t>((size_t)P)), sort(c.take<char>(sort_tokens_bytes(T, k, E))),
+      : order(c.take<uint32_t>((size_t)P)), offsets(c.take<uint32_t>((size_t)E + 1)), inverse(c.take<int32_t>((size_t)P)),
+        list{c.take<uint4>((size_t)f8_list_places(P, E)), c.take<uint4>((size_t)f8_list_places(P, E)), c.take<uint4>((size_t)f8_list_places(P, E))}, sort(c.take<char>(sort_tokens_bytes(T, k, E))),
         x(c, T, H), dout(c, grad ? T : 0, H), g(c.take<float>(float_rows(P, E, grad) * I)), u(c.take<float>(float_rows(P, E, grad) * I)), dh(c.take<float>(grad ? (size_t)P * I : 0)),
         h(c, P, I, grad ? 2 : 1), y(c.take<uint16_t>((size_t)P * H)), bytes(c.off + 256) {}
   static size_t float_rows(int64_t P, int E, bool grad) { return (size_t)(grad || P <= (int64_t)16 * E ? P : (int64_t)16 * E); }  // (never less for more tokens)
@@ -230,34 +245,30 @@ int mi_moe_switch_glu_f8(const void *x, const uint32_t *topk_idx, const void *to
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const int64_t P = T * top_k;
   MI_HIP(launch_sort_tokens({topk_idx, T, top_k, n_experts, ws.order, ws.inverse, ws.offsets}, nullptr, dtype, hidden, nullptr, ws.sort, st));
-  MI_HIP(launch_quantize_f8_rows(x, dtype, T, hidden, ws.x.out(T, hidden), st));
   F8Product p{};
   p.x = ws.x.as(T);
   p.order = ws.order;
   p.k_div = top_k;
-  p.offsets = ws.offsets;
   p.n_mats = n_experts;
   p.rows = P;
+  p.list = ws.list[0];
   p.m[0] = mat(experts->gate, experts->gate_scales);
   p.m[1] = mat(experts->up, experts->up_scales);
   p.transpose = true;
   p.N = intermediate;
   p.K = hidden;
   p.dt = MI_MOE_DTYPE_F32;
-  if (f8_few_rows(p)) {
+  const bool few = f8_few_rows(p);
+  if (few) {
     p.y = ws.g;
     p.y1 = ws.u;
-    MI_HIP(launch_f8_product(p, st));
-    MI_HIP(launch_swiglu_f8(ws.g, ws.u, P, intermediate, ws.h.out(P, intermediate), st));
   } else {
     p.dt = dtype;
     p.h = ws.h.codes;
     p.hs = ws.h.scales;
-    MI_HIP(launch_f8_product(p, st));
   }
   F8Product d{};
   d.x = ws.h.as(P);
-  d.offsets = ws.offsets;
   d.n_mats = n_experts;
   d.rows = P;
   d.m[0] = d.m[1] = mat(experts->down, experts->down_scales);
@@ -266,6 +277,15 @@ int mi_moe_switch_glu_f8(const void *x, const uint32_t *topk_idx, const void *to
   d.K = intermediate;
   d.y = ws.y;
   d.dt = dtype;
+  F8Lists lists;
+  lists.offsets = ws.offsets;
+  lists.n_mats = n_experts;
+  lists.rows = P;
+  list_for(p, lists, 0, ws.list[0]);
+  list_for(d, lists, 1, ws.list[1]);
+  MI_HIP(launch_quantize_f8_rows(x, dtype, T, hidden, ws.x.out(T, hidden), st, lists));
+  MI_HIP(launch_f8_product(p, st));
+  if (few) MI_HIP(launch_swiglu_f8(ws.g, ws.u, P, intermediate, ws.h.out(P, intermediate), st));
   MI_HIP(launch_f8_product(d, st));
   MI_HIP(launch_unsort_tokens(ws.y, topk_w, w_dtype, ws.inverse, T, top_k, hidden, dtype, out, st));
   return 0;
@@ -282,16 +302,14 @@ int mi_moe_switch_glu_f8_grad(const void *dout, const void *x, const uint32_t *t
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const int64_t P = T * top_k;
   MI_HIP(launch_sort_tokens({topk_idx, T, top_k, n_experts, ws.order, ws.inverse, ws.offsets}, nullptr, dtype, hidden, nullptr, ws.sort, st));
-  MI_HIP(launch_quantize_f8_rows(x, dtype, T, hidden, ws.x.out(T, hidden), st));
-  MI_HIP(launch_quantize_f8_rows(dout, dtype, T, hidden, ws.dout.out(T, hidden), st));
   // gate, up and the gradient at h (but for the slot's weight), in float32: the weights' gradient is made of them
   F8Product p{};
   p.x = ws.x.as(T);
   p.order = ws.order;
   p.k_div = top_k;
-  p.offsets = ws.offsets;
   p.n_mats = n_experts;
   p.rows = P;
+  p.list = ws.list[0];
   p.m[0] = mat(experts->gate, experts->gate_scales);
   p.m[1] = mat(experts->up, experts->up_scales);
   p.transpose = true;
@@ -300,19 +318,17 @@ int mi_moe_switch_glu_f8_grad(const void *dout, const void *x, const uint32_t *t
   p.y = ws.g;
   p.y1 = ws.u;
   p.dt = MI_MOE_DTYPE_F32;
-  MI_HIP(launch_f8_product(p, st));
-  p.x = ws.dout.as(T);
-  p.m[0] = p.m[1] = mat(experts->down, experts->down_scales);
-  p.transpose = false;
-  p.y = ws.dh;
-  p.y1 = nullptr;
-  MI_HIP(launch_f8_product(p, st));
-  MI_HIP(launch_swiglu_f8_grad({ws.g, ws.u, ws.dh, topk_w, w_dtype, ws.order, ws.offsets, n_experts, P, intermediate, ws.h.codes, ws.h.scales, dweights}, st));
+  F8Product b = p;
+  b.x = ws.dout.as(T);
+  b.m[0] = b.m[1] = mat(experts->down, experts->down_scales);
+  b.transpose = false;
+  b.y = ws.dh;
+  b.y1 = nullptr;
   F8Product d{};
   d.x = ws.h.as(P);
-  d.offsets = ws.offsets;
   d.n_mats = n_experts;
   d.rows = P;
+  d.list = ws.list[1];
   d.m[0] = mat(experts->gate, experts->gate_scales);
   d.m[1] = mat(experts->up, experts->up_scales);
   d.pair_sum = true;
@@ -320,6 +336,19 @@ int mi_moe_switch_glu_f8_grad(const void *dout, const void *x, const uint32_t *t
   d.K = intermediate;
   d.y = ws.y;
   d.dt = dtype;
+  // three lists, the forward products' beside the rounding of x, the others' beside that of dout
+  F8Lists lists, back;
+  lists.offsets = back.offsets = ws.offsets;
+  lists.n_mats = back.n_mats = n_experts;
+  lists.rows = back.rows = P;
+  list_for(p, lists, 0, ws.list[0]);
+  list_for(b, back, 0, ws.list[2]);
+  list_for(d, back, 1, ws.list[1]);
+  MI_HIP(launch_quantize_f8_rows(x, dtype, T, hidden, ws.x.out(T, hidden), st, lists));
+  MI_HIP(launch_quantize_f8_rows(dout, dtype, T, hidden, ws.dout.out(T, hidden), st, back));
+  MI_HIP(launch_f8_product(p, st));
+  MI_HIP(launch_f8_product(b, st));
+  MI_HIP(launch_swiglu_f8_grad({ws.g, ws.u, ws.dh, topk_w, w_dtype, ws.order, ws.offsets, n_experts, P, intermediate, ws.h.codes, ws.h.scales, dweights}, st));
   MI_HIP(launch_f8_product(d, st));
   MI_HIP(launch_unsort_tokens(ws.y, nullptr, 0, ws.inverse, T, top_k, hidden, dtype, dx, st));
   return 0;

@@ -33,8 +33,8 @@ struct F8Product {
   F8Rows x;
   const uint32_t *order;    // sorted row r reads x row order[r] / k_div; nullptr: r
   int k_div;
-  const uint32_t *offsets;  // matrix e has the rows from offsets[e] to offsets[e + 1]; rows behind the last are zeros of y.  nullptr: one matrix, all rows
-  int n_mats;
+  const uint4 *list;        // the pieces of at most f8_tile_rows rows that the matrices' rows are cut into, and rows of no matrix, which are zeros of y (f8_list).  nullptr: one
+  int n_mats;               // matrix, all rows
   int64_t rows;             // of y
   F8Mat m[2];               // the second one: of a gate/up pair (y1 or h), or of a second half of the summed axis (pair_sum)
   bool transpose;           // matrices [N][K], else [K][N]
@@ -46,7 +46,20 @@ struct F8Product {
   uint8_t *h;  // gate/up pairs: silu(gate) * up in e4m3, as F8Rows
   float *hs;
 };
-bool f8_few_rows(const F8Product &p);                     // which of the two the product takes
+// Rows of a piece: what the product's kernel takes at once (16 or 32: the one for a few rows).
+int f8_tile_rows(const F8Product &p);
+inline bool f8_few_rows(const F8Product &p) { return f8_tile_rows(p) < 64; }
+inline int64_t f8_most_pieces(int64_t rows, int n_mats, int tile) { return rows / tile + (n_mats + 1 < rows ? n_mats + 1 : rows); }
+inline int64_t f8_list_places(int64_t rows, int n_mats) { return f8_most_pieces(rows, n_mats, 16); }
+// What is to be listed, beside the rounding of rows (launch_quantize_f8_rows): up to two lists.
+struct F8Lists {
+  const uint32_t *offsets = nullptr;  // [n_mats + 1]
+  int n_mats = 0;
+  int64_t rows = 0;
+  uint4 *list[2] = {nullptr, nullptr};
+  int tile[2] = {0, 0};
+  int places[2] = {0, 0};
+};
 hipError_t launch_f8_few(const F8Product &p, hipStream_t st);    // a few rows a matrix (f8_few.hip); transposed only
 hipError_t launch_f8_tiles(const F8Product &p, hipStream_t st);  // tiles (f8_tiles.hip)
 inline hipError_t launch_f8_product(const F8Product &p, hipStream_t st) { return f8_few_rows(p) ? launch_f8_few(p, st) : launch_f8_tiles(p, st); }
@@ -60,7 +73,7 @@ struct F8Out {
   bool pad;  // zeros up to the end of the last run
 };
 inline F8Out f8_workspace_rows(uint8_t *codes, float *scales, int64_t rows, int cols) { return {codes, f8_row_bytes(cols), scales, 1, rows, true}; }
-hipError_t launch_quantize_f8_rows(const void *x, int dt, int64_t rows, int cols, const F8Out &to, hipStream_t st);
+hipError_t launch_quantize_f8_rows(const void *x, int dt, int64_t rows, int cols, const F8Out &to, hipStream_t st, const F8Lists &lists = F8Lists());
 hipError_t launch_quantize_f8_blocks(const void *x, int dt, int64_t rows, int cols, uint8_t *codes, float *scales, hipStream_t st);
 hipError_t launch_dequantize_f8(const uint8_t *codes, const float *scales, int64_t rows, int cols, int block_rows, int dt, void *out, hipStream_t st);
 // h = silu(gate) * up of float32 rows, in e4m3
@@ -145,20 +158,25 @@ __device__ __forceinline__ uint32_t max_of_16_lanes(uint32_t m) {
 __device__ __forceinline__ float silu(float g) { return g / (1.f + __expf(-g)); }
 
 // ---------------------------------------------------------------- segments
-// Piece m of the segments that offsets[n_mats + 1] cut the rows into: matrix, first row and number of rows.  A segment is cut into as few pieces of at most `tile` rows as
-// it can be, of about one size (multiples of 32 rows).  Behind the segments' pieces come those of the rows that belong to none (matrix n_mats), behind those nothing (rows 0).
-// By one wave; offsets out of order or range only make pieces that overlap or are missing.
-// In the experts' order: with whole pieces first and the rest of the segments behind them, the longest first, the launch ends more evenly, but its first half multiplies and its
-// second one waits for weights (4096 tokens, skewed routing over 128 experts of 2048 x 768: down 138 us, 156 so).
+// A piece of at most `tile` rows of one matrix (n_mats: of none); rows 0: nothing.
 struct F8Piece {
   int mat;
   uint32_t row, rows;
 };
-__device__ __forceinline__ F8Piece f8_piece(const uint32_t *__restrict__ offsets, int n_mats, uint32_t total, uint32_t tile, uint32_t m) {
-  if (!offsets) {
-    const uint32_t row = m * tile;
+__device__ __forceinline__ F8Piece f8_piece(const F8Product &p, uint32_t tile, uint32_t m) {
+  if (!p.list) {
+    const uint32_t row = m * tile, total = (uint32_t)p.rows;
     return {0, row, row >= total ? 0u : total - row < tile ? total - row : tile};
   }
+  const uint4 v = p.list[m];
+  return {__builtin_amdgcn_readfirstlane((int)v.x), (uint32_t)__builtin_amdgcn_readfirstlane((int)v.y), (uint32_t)__builtin_amdgcn_readfirstlane((int)v.z)};
+}
+// The list of pieces of the segments that offsets[n_mats + 1] cut the rows into, by one wave.  A segment is cut into as few pieces of at most `tile` rows as it can be, of about one
+// size (multiples of 32 rows).  Behind the segments' pieces come those of the rows that belong to none, then empty ones.  Offsets out of order or range only make pieces
+// that overlap or are missing.
+// In the experts' order: with whole pieces first and the rest of the segments behind them, the longest first, the launch ends more evenly, but its first half multiplies and its
+// second one waits for weights (4096 tokens, skewed routing over 128 experts of 2048 x 768: down 138 us, 156 so).
+__device__ __forceinline__ void f8_list(const uint32_t *__restrict__ offsets, int n_mats, uint32_t total, uint32_t tile, uint4 *__restrict__ list, uint32_t places) {
   const int lane = lane_id();
   uint32_t before = 0;
   for (int e0 = 0; e0 <= n_mats; e0 += kWave) {
@@ -176,21 +194,15 @@ __device__ __forceinline__ F8Piece f8_piece(const uint32_t *__restrict__ offsets
       const uint32_t v = __shfl_up(upto, d, kWave);
       if (lane >= d) upto += v;
     }
-    const uint64_t found = __ballot(m < before + upto);
-    if (found) {
-      const int at = __builtin_amdgcn_readfirstlane((int)__builtin_ctzll(found));
-      const uint32_t p = (uint32_t)__builtin_amdgcn_readlane((int)pieces, at), i = m - before - ((uint32_t)__builtin_amdgcn_readlane((int)upto, at) - p);
-      const uint32_t slo = (uint32_t)__builtin_amdgcn_readlane((int)lo, at), shi = (uint32_t)__builtin_amdgcn_readlane((int)hi, at);
-      const uint32_t even = p == 1 ? tile : ((shi - slo + p - 1) / p + 31) / 32 * 32, size = even < tile ? even : tile, row = slo + i * size;
-      return {e0 + at, row, shi - row < size ? shi - row : size};
+    const uint32_t even = pieces <= 1 ? tile : ((hi - lo + pieces - 1) / pieces + 31) / 32 * 32, size = even < tile ? even : tile;
+    const uint32_t first = before + upto - pieces;
+    for (uint32_t i = 0; i < pieces && first + i < places; ++i) {
+      const uint32_t row = lo + i * size;
+      list[first + i] = make_uint4((uint32_t)e, row, hi - row < size ? hi - row : size, 0u);
     }
     before += (uint32_t)__builtin_amdgcn_readlane((int)upto, kWave - 1);
   }
-  return {0, 0, 0};
-}
-inline int64_t f8_most_pieces(const F8Product &p, int tile) {
-  if (!p.offsets) return (p.rows + tile - 1) / tile;
-  return p.rows / tile + (p.n_mats + 1 < p.rows ? p.n_mats + 1 : p.rows);
+  for (uint32_t i = before + lane; i < places; i += kWave) list[i] = make_uint4(0, 0, 0, 0);
 }
 
 // ---------------------------------------------------------------- products

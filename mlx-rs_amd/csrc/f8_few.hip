@@ -16,7 +16,7 @@ __global__ __launch_bounds__(kFewWaves *kWave) void f8_few_kernel(F8Product a) {
   constexpr int AHEAD = TG == 1 ? 4 : 2;  // runs whose loads are in flight at once
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ln = lane & 15, part = lane >> 4;
   const int tiles = (a.N + 15) / 16, which = (int)blockIdx.x / tiles, n0 = ((int)blockIdx.x - which * tiles) * 16;
-  const F8Piece piece = f8_piece(a.offsets, a.n_mats, (uint32_t)a.rows, 16 * TG, blockIdx.y);
+  const F8Piece piece = f8_piece(a, 16 * TG, blockIdx.y);
   if (piece.rows == 0) return;
   void *const y = which ? a.y1 : a.y;
   if (piece.mat == a.n_mats) {  // rows of no matrix
@@ -95,18 +95,24 @@ __global__ __launch_bounds__(kFewWaves *kWave) void f8_few_kernel(F8Product a) {
   }
 }
 
-bool f8_few_rows(const F8Product &p) { return p.transpose && !p.h && !p.pair_sum && p.rows <= (int64_t)16 * (p.offsets ? p.n_mats : 1); }
+int f8_tile_rows(const F8Product &p) {
+  const int64_t mats = p.list ? p.n_mats : 1, avg = p.rows / mats;
+  if (p.transpose && !p.h && !p.pair_sum && p.rows <= 16 * mats) return avg > 4 ? 32 : 16;
+  if (p.dt == 2) return avg > 128 ? 128 : 64;
+  return avg > 192 ? 256 : avg > 64 ? 128 : 64;
+}
 
 hipError_t launch_f8_few(const F8Product &p, hipStream_t st) {
   if (p.rows == 0) return hipSuccess;
   const unsigned tiles = (unsigned)((p.N + 15) / 16) * (p.y1 ? 2 : 1);
-  const int64_t avg = p.rows / (p.offsets ? p.n_mats : 1);
   auto launch = [&](auto *kernel, int tg) {
-    kernel<<<dim3(tiles, (unsigned)f8_most_pieces(p, 16 * tg)), kFewWaves * kWave, 0, st>>>(p);
+    const int64_t pieces = p.list ? f8_most_pieces(p.rows, p.n_mats, 16 * tg) : (p.rows + 16 * tg - 1) / (16 * tg);
+    kernel<<<dim3(tiles, (unsigned)pieces), kFewWaves * kWave, 0, st>>>(p);
     return hipGetLastError();
   };
-  if (p.dt == 2) return avg > 4 ? launch(&f8_few_kernel<2, true>, 2) : launch(&f8_few_kernel<1, true>, 1);
-  return avg > 4 ? launch(&f8_few_kernel<2, false>, 2) : launch(&f8_few_kernel<1, false>, 1);
+  const bool two = f8_tile_rows(p) == 32;
+  if (p.dt == 2) return two ? launch(&f8_few_kernel<2, true>, 2) : launch(&f8_few_kernel<1, true>, 1);
+  return two ? launch(&f8_few_kernel<2, false>, 2) : launch(&f8_few_kernel<1, false>, 1);
 }
 
 }  // namespace mi_moe

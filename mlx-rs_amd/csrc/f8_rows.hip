@@ -29,10 +29,15 @@ __device__ __forceinline__ void write_run(const float v[8], const F8Out &to, int
   if (l == 0) to.scales[row * to.row_stride + run * to.run_stride] = s.scale;
 }
 
+// lists: blocks of their own, ahead of the rows', list the pieces of the product that follows, which else were a launch or a search at the start of every block of it.
 template <int DT>
-__global__ __launch_bounds__(kRowThreads) void quantize_rows_kernel(const void *__restrict__ x, int64_t rows, int cols, F8Out to) {
+__global__ __launch_bounds__(kRowThreads) void quantize_rows_kernel(const void *__restrict__ x, int64_t rows, int cols, F8Out to, F8Lists lists, int n_lists) {
+  if ((int)blockIdx.x < n_lists) {
+    if (threadIdx.x < kWave) f8_list(lists.offsets, lists.n_mats, (uint32_t)lists.rows, (uint32_t)lists.tile[blockIdx.x], lists.list[blockIdx.x], (uint32_t)lists.places[blockIdx.x]);
+    return;
+  }
   const int runs = f8_runs(cols);
-  const int64_t at = (int64_t)blockIdx.x * kRowRuns + threadIdx.x / 16;
+  const int64_t at = (int64_t)(blockIdx.x - n_lists) * kRowRuns + threadIdx.x / 16;
   if (at >= rows * runs) return;  // (whole rows of lanes)
   const int64_t row = at / runs;
   const int run = (int)(at - row * runs), k = run * kF8Run + (threadIdx.x % 16) * 8, n = cols - k;
@@ -63,10 +68,14 @@ static F8Out rows_from(F8Out to, int64_t row) {
 }
 static const char *value_at(const void *x, int dt, int64_t at) { return static_cast<const char *>(x) + at * (dt == 2 ? 4 : 2); }
 
-hipError_t launch_quantize_f8_rows(const void *x, int dt, int64_t rows, int cols, const F8Out &to, hipStream_t st) {
+hipError_t launch_quantize_f8_rows(const void *x, int dt, int64_t rows, int cols, const F8Out &to, hipStream_t st, const F8Lists &lists) {
   if (rows == 0 || cols == 0) return hipSuccess;
+  const int n_lists = lists.list[1] ? 2 : lists.list[0] ? 1 : 0;
   auto *const kernel = dt == 0 ? &quantize_rows_kernel<0> : dt == 1 ? &quantize_rows_kernel<1> : &quantize_rows_kernel<2>;
-  return in_launches(rows, cols, [&](int64_t r, int64_t n) { kernel<<<run_blocks(n, cols), kRowThreads, 0, st>>>(value_at(x, dt, r * cols), n, cols, rows_from(to, r)); });
+  return in_launches(rows, cols, [&](int64_t r, int64_t n) {
+    const int also = r == 0 ? n_lists : 0;
+    kernel<<<run_blocks(n, cols) + also, kRowThreads, 0, st>>>(value_at(x, dt, r * cols), n, cols, rows_from(to, r), lists, also);
+  });
 }
 
 // A block of 128 x 128 values, a thread eight columns of eight rows sixteen apart.

@@ -61,9 +61,9 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, int n
     nt = (int)blockIdx.x % n_tiles;
   }
   if (mt >= m_tiles) return;
-  const F8Piece piece = f8_piece(a.offsets, a.n_mats, (uint32_t)a.rows, TM, (uint32_t)mt);
-  const int rows = __builtin_amdgcn_readfirstlane((int)piece.rows), mat = __builtin_amdgcn_readfirstlane(piece.mat);
-  const uint32_t row0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)piece.row);
+  const F8Piece piece = f8_piece(a, TM, (uint32_t)mt);
+  const int rows = (int)piece.rows, mat = piece.mat;
+  const uint32_t row0 = piece.row;
   if (rows == 0) return;
   const int N = a.N, K = a.K, runs = f8_runs(K), n_blocks = f8_runs(N), steps = a.pair_sum ? 2 * runs : runs;
   const int n0 = nt * (MODE == kPair ? 128 : kF8TileN);
@@ -377,7 +377,7 @@ static hipError_t launch_tiles(const F8Product &p, hipStream_t st) {
     if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&f8_tiles_kernel<TM, MODE, F32>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds); e != hipSuccess) return e;
     if (dev >= 0 && dev < kMaxDevices) raised[dev].store(true, std::memory_order_release);
   }
-  const int64_t n_tiles = (p.N + (MODE == kPair ? 127 : kF8TileN - 1)) / (MODE == kPair ? 128 : kF8TileN), m_tiles = f8_most_pieces(p, TM);
+  const int64_t n_tiles = (p.N + (MODE == kPair ? 127 : kF8TileN - 1)) / (MODE == kPair ? 128 : kF8TileN), m_tiles = p.list ? f8_most_pieces(p.rows, p.n_mats, TM) : (p.rows + TM - 1) / TM;
   const int64_t grid = n_tiles * (m_tiles >= 16 ? (m_tiles + 7) / 8 * 8 : m_tiles);
   if (grid > (int64_t)1 << 22) return hipErrorInvalidValue;  // (a launch has less than 2^32 threads)
   f8_tiles_kernel<TM, MODE, F32><<<(unsigned)grid, kF8Threads, lds, st>>>(p, (int)n_tiles, (int)m_tiles);
@@ -386,9 +386,9 @@ static hipError_t launch_tiles(const F8Product &p, hipStream_t st) {
 
 template <F8Mode MODE>
 static hipError_t launch_mode(const F8Product &p, hipStream_t st) {
-  const int64_t avg = p.rows / (p.offsets ? p.n_mats : 1);
-  if (p.dt == 2) return avg > 128 ? launch_tiles<128, MODE, true>(p, st) : launch_tiles<64, MODE, true>(p, st);
-  return avg > 192 ? launch_tiles<256, MODE, false>(p, st) : avg > 64 ? launch_tiles<128, MODE, false>(p, st) : launch_tiles<64, MODE, false>(p, st);
+  const int tile = f8_tile_rows(p);
+  if (p.dt == 2) return tile == 128 ? launch_tiles<128, MODE, true>(p, st) : launch_tiles<64, MODE, true>(p, st);
+  return tile == 256 ? launch_tiles<256, MODE, false>(p, st) : tile == 128 ? launch_tiles<128, MODE, false>(p, st) : launch_tiles<64, MODE, false>(p, st);
 }
 
 hipError_t launch_f8_tiles(const F8Product &p, hipStream_t st) {

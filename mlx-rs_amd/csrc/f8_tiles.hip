@@ -42,26 +42,37 @@ constexpr size_t f8_tiles_lds(int tm) {  // two stages, and what a thread copies
   return 2 * (size_t)(tm * 128 + kF8TileN * 128 + tm * 4 + 512) + kF8Threads * 4 * (tm / 64) + tm * 4;
 }
 
+struct F8Grid {
+  int m_tiles, n_tiles, xcds_m, m_each, n_each;  // one matrix: xcds_m XCDs along the token rows, rectangles of m_each x n_each tiles
+};
+
 template <int TM, F8Mode MODE, bool F32>
-__global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, int n_tiles, int m_tiles) {
+__global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, F8Grid g) {
   typedef F8Stage<TM> L;
   constexpr int XC = TM / 64, MT = TM / 64;  // copies of token rows a wave; sub-tiles of 32 token rows a wave
   extern __shared__ __align__(16) unsigned char lds[];
   const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)lds;
   const int lane = threadIdx.x & 63, ln = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 2, wn = wave & 3;
-  // blocks go round the eight XCDs: with many pieces all tiles of a piece go to one, whose L2 then serves its rows
-  int mt, nt;
-  if (m_tiles >= 16) {
-    const int q = (int)blockIdx.x >> 3;
-    mt = q / n_tiles * 8 + ((int)blockIdx.x & 7);
-    nt = q % n_tiles;
+  // Blocks go round the eight XCDs, each of which has an L2 of its own.  One matrix: an XCD takes a rectangle of tiles.  Several: it takes a run of pieces (f8_list), those
+  // of a matrix beside each other for each 256 of its rows.
+  const uint32_t xcd = blockIdx.x & 7, q = blockIdx.x >> 3;
+  uint32_t mt, nt;
+  F8Piece piece;
+  if (!a.list) {
+    mt = (xcd % (uint32_t)g.xcds_m) * (uint32_t)g.m_each + q % (uint32_t)g.m_each;
+    nt = (xcd / (uint32_t)g.xcds_m) * (uint32_t)g.n_each + q / (uint32_t)g.m_each;
+    if (mt >= (uint32_t)g.m_tiles || nt >= (uint32_t)g.n_tiles) return;
+    piece = f8_piece(a, TM, mt);
   } else {
-    mt = (int)blockIdx.x / n_tiles;
-    nt = (int)blockIdx.x % n_tiles;
+    const uint32_t *const start = reinterpret_cast<const uint32_t *>(a.list) + xcd;
+    const uint32_t tiles = (uint32_t)g.n_tiles, s = start[0] * tiles + q;
+    if (s >= start[1] * tiles) return;
+    piece = f8_piece(a, TM, s / tiles);
+    const uint32_t first = s / tiles - piece.at, in = s - first * tiles;
+    nt = in / piece.of;
+    if (piece.of > 1) piece = f8_piece(a, TM, first + in % piece.of);
   }
-  if (mt >= m_tiles) return;
-  const F8Piece piece = f8_piece(a, TM, (uint32_t)mt);
   const int rows = (int)piece.rows, mat = piece.mat;
   const uint32_t row0 = piece.row;
   if (rows == 0) return;
@@ -377,10 +388,22 @@ static hipError_t launch_tiles(const F8Product &p, hipStream_t st) {
     if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&f8_tiles_kernel<TM, MODE, F32>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds); e != hipSuccess) return e;
     if (dev >= 0 && dev < kMaxDevices) raised[dev].store(true, std::memory_order_release);
   }
-  const int64_t n_tiles = (p.N + (MODE == kPair ? 127 : kF8TileN - 1)) / (MODE == kPair ? 128 : kF8TileN), m_tiles = p.list ? f8_most_pieces(p.rows, p.n_mats, TM) : (p.rows + TM - 1) / TM;
-  const int64_t grid = n_tiles * (m_tiles >= 16 ? (m_tiles + 7) / 8 * 8 : m_tiles);
-  if (grid > (int64_t)1 << 22) return hipErrorInvalidValue;  // (a launch has less than 2^32 threads)
-  f8_tiles_kernel<TM, MODE, F32><<<(unsigned)grid, kF8Threads, lds, st>>>(p, (int)n_tiles, (int)m_tiles);
+  const int64_t n_tiles = (p.N + (MODE == kPair ? 127 : kF8TileN - 1)) / (MODE == kPair ? 128 : kF8TileN), m_tiles = p.list ? 0 : (p.rows + TM - 1) / TM;
+  F8Grid g{(int)m_tiles, (int)n_tiles, 1, (int)m_tiles, (int)((n_tiles + 7) / 8)};
+  int64_t each;  // blocks of an XCD
+  if (p.list) {
+    // (runs of one time hold up to kPieceMost / kPieceBase of their share of the pieces)
+    each = ((f8_most_pieces(p.rows, p.n_mats, TM) * kPieceMost + kPieceBase * 8 - 1) / (kPieceBase * 8) + 1) * n_tiles;
+  } else {
+    for (int xm = 2; xm <= 8; xm *= 2) {
+      const int m_each = (int)((m_tiles + xm - 1) / xm), n_each = (int)((n_tiles + 8 / xm - 1) / (8 / xm));
+      const int64_t now = (int64_t)g.m_each * g.n_each, then = (int64_t)m_each * n_each;
+      if (then < now || (then == now && m_each * TM + n_each * kF8TileN < g.m_each * TM + g.n_each * kF8TileN)) g.xcds_m = xm, g.m_each = m_each, g.n_each = n_each;
+    }
+    each = (int64_t)g.m_each * g.n_each;
+  }
+  if (each > (int64_t)1 << 19) return hipErrorInvalidValue;  // (a launch has less than 2^32 threads)
+  f8_tiles_kernel<TM, MODE, F32><<<(unsigned)(each * 8), kF8Threads, lds, st>>>(p, g);
   return hipGetLastError();
 }
 

@@ -9,7 +9,8 @@
 //
 // So with the operators around a layer, in ops' argument order: add_rms_norm, add_rms_norm_rows8, add_rms_norm_grad, quantized_linear_rows8, select_experts
 // and select_experts_grad, whose kernels take 4 us for a few tokens and whose calls took 9 in Python and
-// take 5 with this.
+// take 5 with this.  And with those on e4m3 weights and sorted tokens: sort_tokens, unsort_tokens and their _grad, linear_f8, grouped_linear_f8, switch_glu_f8 and its _grad (the
+// banks' codes and scales one after the other), a token's layer of which took 15 us in Python for 7 of kernels.
 #include <ATen/ATen.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
@@ -20,6 +21,7 @@
 #include <torch/csrc/api/include/torch/version.h>
 
 #include "../../include/mi_moe.h"
+#include "../../include/mi_moe_f8.h"
 #include "../../include/mi_moe_layer.h"
 
 namespace {
@@ -37,6 +39,19 @@ struct {
   decltype(&mi_moe_select_experts) select;
   decltype(&mi_moe_select_experts_grad) select_grad;
 } g_layer;
+struct {
+  decltype(&mi_moe_sort_tokens_workspace_size) sort_workspace;
+  decltype(&mi_moe_sort_tokens) sort;
+  decltype(&mi_moe_sort_tokens_grad) sort_grad;
+  decltype(&mi_moe_unsort_tokens) unsort;
+  decltype(&mi_moe_unsort_tokens_grad) unsort_grad;
+  decltype(&mi_moe_linear_f8_workspace_size) linear_workspace;
+  decltype(&mi_moe_linear_f8) linear;
+  decltype(&mi_moe_grouped_linear_f8) grouped;
+  decltype(&mi_moe_switch_glu_f8_workspace_size) experts_workspace;
+  decltype(&mi_moe_switch_glu_f8) experts;
+  decltype(&mi_moe_switch_glu_f8_grad) experts_grad;
+} g_f8;
 
 // a tensor itself (no subclass), dense, on a GPU, contiguous, seen through no transform (vmap, functionalisation, a Python key)
 const at::Tensor *plain(PyObject *o, at::ScalarType type) {
@@ -119,7 +134,7 @@ int dtype_code(at::ScalarType type) {
 
 // The operands of a call, kept alive across it (another thread may drop the caller's references while the interpreter is let go): plain tensors on the current device.
 struct Operands {
-  at::Tensor t[6];
+  at::Tensor t[10];
   int n = 0;
   bool good = true;
   const at::Tensor &add(PyObject *o, at::ScalarType type) {
@@ -347,6 +362,223 @@ PyObject *select_experts_grad(PyObject *, PyObject *const *args, Py_ssize_t n) {
   });
 }
 
+// ---------------------------------------------------------------- e4m3 weights, sorted tokens
+constexpr at::ScalarType kF8 = at::kFloat8_e4m3fn;
+int64_t blocks(int64_t n) { return (n + 127) / 128; }
+at::Tensor bytes_like(const at::Tensor &t, size_t n) { return n ? at::empty({(int64_t)n}, t.options().dtype(at::kByte)) : at::Tensor(); }
+void *ptr_of(const at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+// x, inds, n_experts
+PyObject *sort_tokens(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  if (!count_is(n, 3, "sort_tokens")) return nullptr;
+  Numbers num;
+  Operands in;
+  const int64_t E = num.whole(args[2]);
+  const at::ScalarType type = type_of(args[0]);
+  const int dt = dtype_code(type);
+  if (dt < 0 || !num.good) Py_RETURN_NONE;
+  const at::Tensor &x = in.add(args[0], type), &ids = in.add(args[1], at::kInt);
+  if (!in.good || x.dim() != 2 || ids.dim() != 2 || ids.size(0) != x.size(0) || x.numel() == 0 || ids.numel() == 0 || x.size(1) > INT32_MAX || ids.size(1) > INT32_MAX) Py_RETURN_NONE;
+  return call<4>([&](at::Tensor *out) {
+    const int64_t T = x.size(0), k = ids.size(1), H = x.size(1);
+    size_t need = 0;
+    if (g_f8.sort_workspace(T, (int32_t)k, (int32_t)E, &need)) return -1;
+    out[0] = at::empty({T * k, H}, x.options());
+    out[1] = at::empty({T * k}, ids.options());
+    out[2] = at::empty({T, k}, ids.options());
+    out[3] = at::empty({E + 1}, ids.options());
+    const at::Tensor ws = bytes_like(x, need);
+    return g_f8.sort(data_of(x), static_cast<const uint32_t *>(data_of(ids)), T, (int32_t)k, (int32_t)E, (int32_t)H, dt, out[0].data_ptr(), static_cast<uint32_t *>(out[1].data_ptr()),
+                     static_cast<int32_t *>(out[2].data_ptr()), static_cast<uint32_t *>(out[3].data_ptr()), ptr_of(ws), need, stream_here());
+  });
+}
+
+// rows [T * k, H] and inverse [T, k]
+bool rows_fit(const at::Tensor &rows, const at::Tensor &inverse) {
+  return rows.dim() == 2 && inverse.dim() == 2 && rows.numel() && inverse.numel() && rows.size(0) == inverse.numel() && rows.size(1) <= INT32_MAX && inverse.size(1) <= INT32_MAX;
+}
+
+// drows, inverse
+PyObject *sort_tokens_grad(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  if (!count_is(n, 2, "sort_tokens_grad")) return nullptr;
+  Operands in;
+  const at::ScalarType type = type_of(args[0]);
+  const int dt = dtype_code(type);
+  if (dt < 0) Py_RETURN_NONE;
+  const at::Tensor &rows = in.add(args[0], type), &inv = in.add(args[1], at::kInt);
+  if (!in.good || !rows_fit(rows, inv)) Py_RETURN_NONE;
+  return call<1>([&](at::Tensor *out) {
+    out[0] = at::empty({inv.size(0), rows.size(1)}, rows.options());
+    return g_f8.sort_grad(data_of(rows), static_cast<const int32_t *>(data_of(inv)), inv.size(0), (int32_t)inv.size(1), (int32_t)rows.size(1), dt, out[0].data_ptr(), stream_here());
+  });
+}
+
+// rows, weights, inverse
+PyObject *unsort_tokens(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  if (!count_is(n, 3, "unsort_tokens")) return nullptr;
+  Operands in;
+  const at::ScalarType type = type_of(args[0]), w_type = type_of(args[1]);
+  const int dt = dtype_code(type), wt = dtype_code(w_type);
+  if (dt < 0 || wt < 0) Py_RETURN_NONE;
+  const at::Tensor &rows = in.add(args[0], type), &w = in.add(args[1], w_type), &inv = in.add(args[2], at::kInt);
+  if (!in.good || !rows_fit(rows, inv) || w.sizes() != inv.sizes()) Py_RETURN_NONE;
+  return call<1>([&](at::Tensor *out) {
+    out[0] = at::empty({inv.size(0), rows.size(1)}, rows.options());
+    return g_f8.unsort(data_of(rows), data_of(w), wt, static_cast<const int32_t *>(data_of(inv)), inv.size(0), (int32_t)inv.size(1), (int32_t)rows.size(1), dt, out[0].data_ptr(),
+                       stream_here());
+  });
+}
+
+// dout, rows, weights, inverse
+PyObject *unsort_tokens_grad(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  if (!count_is(n, 4, "unsort_tokens_grad")) return nullptr;
+  Operands in;
+  const at::ScalarType type = type_of(args[1]), w_type = type_of(args[2]);
+  const int dt = dtype_code(type), wt = dtype_code(w_type);
+  if (dt < 0 || wt < 0) Py_RETURN_NONE;
+  const at::Tensor &dout = in.add(args[0], type), &rows = in.add(args[1], type), &w = in.add(args[2], w_type), &inv = in.add(args[3], at::kInt);
+  if (!in.good || !rows_fit(rows, inv) || w.sizes() != inv.sizes() || dout.dim() != 2 || dout.size(0) != inv.size(0) || dout.size(1) != rows.size(1)) Py_RETURN_NONE;
+  return call<2>([&](at::Tensor *out) {
+    out[0] = at::empty(rows.sizes(), rows.options());
+    out[1] = at::empty(w.sizes(), w.options());
+    return g_f8.unsort_grad(data_of(dout), data_of(rows), data_of(w), wt, static_cast<const int32_t *>(data_of(inv)), inv.size(0), (int32_t)inv.size(1), (int32_t)rows.size(1), dt,
+                            out[0].data_ptr(), out[1].data_ptr(), stream_here());
+  });
+}
+
+bool scales_fit(const at::Tensor &w, const at::Tensor &s, int64_t lead) {
+  const int64_t d = w.dim();
+  return d == lead + 2 && s.dim() == d && w.numel() && (!lead || s.size(0) == w.size(0)) && s.size(d - 2) == blocks(w.size(d - 2)) && s.size(d - 1) == blocks(w.size(d - 1)) &&
+         w.size(d - 2) <= INT32_MAX && w.size(d - 1) <= INT32_MAX;
+}
+
+// x, w, scales, linear_bias, transpose
+PyObject *linear_f8(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  if (!count_is(n, 5, "linear_f8")) return nullptr;
+  Numbers num;
+  Operands in;
+  const bool transpose = num.truth(args[4]);
+  const at::ScalarType type = type_of(args[0]);
+  const int dt = dtype_code(type);
+  if (dt < 0 || !num.good) Py_RETURN_NONE;
+  const at::Tensor &x = in.add(args[0], type), &w = in.add(args[1], kF8), &s = in.add(args[2], at::kFloat), &b = in.add_or_none(args[3], type);
+  if (!in.good || x.dim() < 1 || x.numel() == 0 || !scales_fit(w, s, 0) || x.size(-1) != w.size(transpose) || (b.defined() && (!transpose || b.numel() != w.size(0)))) Py_RETURN_NONE;
+  return call<1>([&](at::Tensor *out) {
+    const int64_t K = x.size(-1), N = w.size(!transpose), M = x.numel() / K;
+    size_t need = 0;
+    if (g_f8.linear_workspace(M, (int32_t)K, &need)) return -1;
+    at::DimVector shape(x.sizes().begin(), x.sizes().end());
+    shape.back() = N;
+    out[0] = at::empty(shape, x.options());
+    const at::Tensor ws = bytes_like(x, need);
+    return g_f8.linear(data_of(x), data_of(w), static_cast<const float *>(data_of(s)), data_of(b), M, (int32_t)N, (int32_t)K, transpose, dt, out[0].data_ptr(), ptr_of(ws), need,
+                       stream_here());
+  });
+}
+
+// rows, w, scales, offsets, transpose
+PyObject *grouped_linear_f8(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  if (!count_is(n, 5, "grouped_linear_f8")) return nullptr;
+  Numbers num;
+  Operands in;
+  const bool transpose = num.truth(args[4]);
+  const at::ScalarType type = type_of(args[0]);
+  const int dt = dtype_code(type);
+  if (dt < 0 || !num.good) Py_RETURN_NONE;
+  const at::Tensor &x = in.add(args[0], type), &w = in.add(args[1], kF8), &s = in.add(args[2], at::kFloat), &off = in.add(args[3], at::kInt);
+  if (!in.good || x.dim() != 2 || x.numel() == 0 || !scales_fit(w, s, 1) || w.size(0) > INT32_MAX - 1 || x.size(1) != w.size(1 + transpose) || off.dim() != 1 || off.size(0) != w.size(0) + 1)
+    Py_RETURN_NONE;
+  return call<1>([&](at::Tensor *out) {
+    const int64_t M = x.size(0), K = x.size(1), N = w.size(1 + !transpose);
+    size_t need = 0;
+    if (g_f8.linear_workspace(M, (int32_t)K, &need)) return -1;
+    out[0] = at::empty({M, N}, x.options());
+    const at::Tensor ws = bytes_like(x, need);
+    return g_f8.grouped(data_of(x), data_of(w), static_cast<const float *>(data_of(s)), static_cast<const uint32_t *>(data_of(off)), M, (int32_t)w.size(0), (int32_t)N, (int32_t)K, transpose,
+                        dt, out[0].data_ptr(), ptr_of(ws), need, stream_here());
+  });
+}
+
+// what the two calls of the experts share: x, inds, weights, and codes and scales of gate, up and down
+struct ExpertsCall {
+  Operands in;
+  int dt, wt;
+  bool good = false;
+  int64_t T = 0, H = 0, I = 0, E = 0, k = 0;
+  mi_moe_f8_experts banks{};
+  explicit ExpertsCall(PyObject *const *args) {
+    const at::ScalarType type = type_of(args[0]), w_type = type_of(args[2]);
+    dt = dtype_code(type);
+    wt = dtype_code(w_type);
+    if (dt < 0 || wt < 0) return;
+    const at::Tensor &x = in.add(args[0], type), &ids = in.add(args[1], at::kInt), &w = in.add(args[2], w_type);
+    for (int i = 0; i < 3; ++i) {
+      in.add(args[3 + 2 * i], kF8);
+      in.add(args[4 + 2 * i], at::kFloat);
+    }
+    const at::Tensor *const b = in.t + 3;
+    if (!in.good || x.dim() < 1 || x.numel() == 0 || ids.dim() != x.dim() || ids.numel() == 0 || ids.sizes().slice(0, ids.dim() - 1) != x.sizes().slice(0, x.dim() - 1) ||
+        w.sizes() != ids.sizes() || ids.size(-1) > INT32_MAX)
+      return;
+    for (int i = 0; i < 3; ++i)
+      if (!scales_fit(b[2 * i], b[2 * i + 1], 1)) return;
+    E = b[0].size(0);
+    I = b[0].size(1);
+    H = b[0].size(2);
+    k = ids.size(-1);
+    if (x.size(-1) != H || E > INT32_MAX || b[2].sizes() != b[0].sizes() || b[4].size(0) != E || b[4].size(1) != H || b[4].size(2) != I) return;
+    T = x.numel() / H;
+    banks = {data_of(b[0]), data_of(b[2]), data_of(b[4]), static_cast<const float *>(data_of(b[1])), static_cast<const float *>(data_of(b[3])), static_cast<const float *>(data_of(b[5]))};
+    good = true;
+  }
+  int workspace(int grad, size_t *need) const { return g_f8.experts_workspace(T, (int32_t)H, (int32_t)I, (int32_t)E, (int32_t)k, grad, need); }
+};
+
+PyObject *switch_glu_f8(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  if (!count_is(n, 9, "switch_glu_f8")) return nullptr;
+  const ExpertsCall c(args);
+  if (!c.good) Py_RETURN_NONE;
+  return call<1>([&](at::Tensor *out) {
+    const at::Tensor &x = c.in.t[0];
+    size_t need = 0;
+    if (c.workspace(0, &need)) return -1;
+    out[0] = at::empty(x.sizes(), x.options());
+    const at::Tensor ws = bytes_like(x, need);
+    return g_f8.experts(data_of(x), static_cast<const uint32_t *>(data_of(c.in.t[1])), data_of(c.in.t[2]), c.wt, &c.banks, c.T, (int32_t)c.H, (int32_t)c.I, (int32_t)c.E, (int32_t)c.k, c.dt,
+                        out[0].data_ptr(), ptr_of(ws), need, stream_here());
+  });
+}
+
+// dout, then switch_glu_f8's
+PyObject *switch_glu_f8_grad(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  if (!count_is(n, 10, "switch_glu_f8_grad")) return nullptr;
+  ExpertsCall c(args + 1);
+  if (!c.good) Py_RETURN_NONE;
+  const at::Tensor &dout = c.in.add(args[0], c.in.t[0].scalar_type());
+  if (!c.in.good || dout.sizes() != c.in.t[0].sizes()) Py_RETURN_NONE;
+  return call<2>([&](at::Tensor *out) {
+    const at::Tensor &x = c.in.t[0], &w = c.in.t[2];
+    size_t need = 0;
+    if (c.workspace(1, &need)) return -1;
+    out[0] = at::empty(x.sizes(), x.options());
+    out[1] = at::empty(w.sizes(), w.options());
+    const at::Tensor ws = bytes_like(x, need);
+    return g_f8.experts_grad(data_of(dout), data_of(x), static_cast<const uint32_t *>(data_of(c.in.t[1])), data_of(w), c.wt, &c.banks, c.T, (int32_t)c.H, (int32_t)c.I, (int32_t)c.E,
+                             (int32_t)c.k, c.dt, out[0].data_ptr(), out[1].data_ptr(), ptr_of(ws), need, stream_here());
+  });
+}
+
+// bind_f8(addresses of the functions of g_f8, in its order)
+PyObject *bind_f8(PyObject *, PyObject *args) {
+  unsigned long long a[11];
+  if (!PyArg_ParseTuple(args, "KKKKKKKKKKK", a, a + 1, a + 2, a + 3, a + 4, a + 5, a + 6, a + 7, a + 8, a + 9, a + 10)) return nullptr;
+  g_f8 = {reinterpret_cast<decltype(g_f8.sort_workspace)>(a[0]), reinterpret_cast<decltype(g_f8.sort)>(a[1]), reinterpret_cast<decltype(g_f8.sort_grad)>(a[2]),
+          reinterpret_cast<decltype(g_f8.unsort)>(a[3]), reinterpret_cast<decltype(g_f8.unsort_grad)>(a[4]), reinterpret_cast<decltype(g_f8.linear_workspace)>(a[5]),
+          reinterpret_cast<decltype(g_f8.linear)>(a[6]), reinterpret_cast<decltype(g_f8.grouped)>(a[7]), reinterpret_cast<decltype(g_f8.experts_workspace)>(a[8]),
+          reinterpret_cast<decltype(g_f8.experts)>(a[9]), reinterpret_cast<decltype(g_f8.experts_grad)>(a[10])};
+  Py_RETURN_NONE;
+}
+
 // bind_layer(addresses of the eight functions of g_layer, in its order)
 PyObject *bind_layer(PyObject *, PyObject *args) {
   unsigned long long a[8];
@@ -394,7 +626,16 @@ PyMethodDef methods[] = {
     {"quantized_linear_rows8", fast(caught<quantized_linear_rows8>), METH_FASTCALL, nullptr},
     {"select_experts", fast(caught<select_experts>), METH_FASTCALL, nullptr},
     {"select_experts_grad", fast(caught<select_experts_grad>), METH_FASTCALL, nullptr},
+    {"sort_tokens", fast(caught<sort_tokens>), METH_FASTCALL, nullptr},
+    {"sort_tokens_grad", fast(caught<sort_tokens_grad>), METH_FASTCALL, nullptr},
+    {"unsort_tokens", fast(caught<unsort_tokens>), METH_FASTCALL, nullptr},
+    {"unsort_tokens_grad", fast(caught<unsort_tokens_grad>), METH_FASTCALL, nullptr},
+    {"linear_f8", fast(caught<linear_f8>), METH_FASTCALL, nullptr},
+    {"grouped_linear_f8", fast(caught<grouped_linear_f8>), METH_FASTCALL, nullptr},
+    {"switch_glu_f8", fast(caught<switch_glu_f8>), METH_FASTCALL, nullptr},
+    {"switch_glu_f8_grad", fast(caught<switch_glu_f8_grad>), METH_FASTCALL, nullptr},
     {"bind", bind, METH_VARARGS, nullptr},
+    {"bind_f8", bind_f8, METH_VARARGS, nullptr},
     {"bind_layer", bind_layer, METH_VARARGS, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_linear_call", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -218,6 +218,9 @@ def _linear_call():
     mod.bind_layer(*(C.cast(getattr(lib, "mi_moe_" + n), C.c_void_p).value for n in
                      ("add_rms_norm", "add_rms_norm_rows8", "add_rms_norm_grad_workspace_size", "add_rms_norm_grad", "quantized_linear_rows8_workspace_size",
                       "quantized_linear_rows8", "select_experts", "select_experts_grad")))
+    mod.bind_f8(*(C.cast(getattr(lib, "mi_moe_" + n), C.c_void_p).value for n in
+                  ("sort_tokens_workspace_size", "sort_tokens", "sort_tokens_grad", "unsort_tokens", "unsort_tokens_grad", "linear_f8_workspace_size", "linear_f8",
+                   "grouped_linear_f8", "switch_glu_f8_workspace_size", "switch_glu_f8", "switch_glu_f8_grad")))
     return mod.quantized_linear
 
 

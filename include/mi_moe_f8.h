@@ -50,7 +50,7 @@ int mi_moe_dequantize_f8(const void *codes, const float *scales, int64_t rows, i
  * type dtype, sums in float32, each result rounded once.  W [N, K] (transpose; K a multiple of 16) or [K, N] (N a multiple of 16), 16-byte aligned; scales of its blocks.
  * M N and M K up to 2^35, N and K up to 2^22.  16-bit results are summed on the f8 matrix instructions, whose sums over a run are off by up to 2^-11 of its largest
  * product; float32 results are not.  workspace >= mi_moe_linear_f8_workspace_size, 16-byte aligned. ---- */
-int mi_moe_linear_f8_workspace_size(int64_t M, int32_t K, size_t *bytes);
+int mi_moe_linear_f8_workspace_size(int64_t M, int32_t N, int32_t K, size_t *bytes);
 int mi_moe_linear_f8(const void *x, const void *w, const float *scales, const void *linear_bias, int64_t M,
                      int32_t N, int32_t K, int32_t transpose, int32_t dtype, void *y, void *workspace,
                      size_t workspace_bytes, void *stream);

@@ -155,7 +155,7 @@ def load_library():
         "mi_moe_unsort_tokens_grad": [vp, vp, vp, i32, vp, i64, i32, i32, i32, vp, vp, vp],
         "mi_moe_quantize_f8": [vp, i32, i64, i64, i32, vp, vp, vp],
         "mi_moe_dequantize_f8": [vp, vp, i64, i64, i32, i32, vp, vp],
-        "mi_moe_linear_f8_workspace_size": [i64, i32, C.POINTER(sz)],
+        "mi_moe_linear_f8_workspace_size": [i64, i32, i32, C.POINTER(sz)],
         "mi_moe_linear_f8": [vp, vp, vp, vp, i64, i32, i32, i32, i32, vp, vp, sz, vp],
         "mi_moe_grouped_linear_f8": [vp, vp, vp, vp, i64, i32, i32, i32, i32, i32, vp, vp, sz, vp],
         "mi_moe_switch_glu_f8_workspace_size": [i64, i32, i32, i32, i32, i32, C.POINTER(sz)],

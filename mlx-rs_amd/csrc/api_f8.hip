@@ -50,10 +50,11 @@ int check_linear(const char *who, const void *x, const void *w, const float *sca
   if (!aligned16(w)) return fail("%s: w must be 16-byte aligned", who);
   return 0;
 }
-size_t linear_bytes(int64_t M, int K) {
+size_t linear_bytes(int64_t M, int N, int K) {
   Carver c(nullptr);
   RowsIn(c, M, K);
   c.take<uint4>((size_t)f8_list_places(M, kMostExperts));
+  c.take<char>(f8_parts_bytes(M, N));
   return c.off + 256;
 }
 // A list for a product, or none for one matrix.
@@ -66,7 +67,7 @@ void list_for(F8Product &p, F8Lists &lists, int i, uint4 *at) {
 
 int linear(const char *who, const void *x, const void *w, const float *scales, const void *bias, const uint32_t *offsets, int64_t M, int E, int32_t N, int32_t K, int32_t transpose,
            int32_t dtype, void *y, void *workspace, size_t workspace_bytes, hipStream_t st) {
-  if (check_workspace(who, workspace, workspace_bytes, linear_bytes(M, K))) return 1;
+  if (check_workspace(who, workspace, workspace_bytes, linear_bytes(M, N, K))) return 1;
   Carver c(workspace);
   const RowsIn q(c, M, K);
   uint4 *const list = c.take<uint4>((size_t)f8_list_places(M, kMostExperts));
@@ -86,6 +87,7 @@ int linear(const char *who, const void *x, const void *w, const float *scales, c
   lists.n_mats = E;
   lists.rows = M;
   if (offsets) list_for(p, lists, 0, list);
+  else p.parts = reinterpret_cast<float *>(c.take<char>(f8_parts_bytes(M, N)));
   MI_HIP(launch_quantize_f8_rows(x, dtype, M, K, q.out(M, K), st, lists));
   MI_HIP(launch_f8_product(p, st));
   return 0;
@@ -204,10 +206,10 @@ int mi_moe_dequantize_f8(const void *codes, const float *scales, int64_t rows, i
   return 0;
 } MI_CATCH("dequantize_f8")
 
-int mi_moe_linear_f8_workspace_size(int64_t M, int32_t K, size_t *bytes) try {
+int mi_moe_linear_f8_workspace_size(int64_t M, int32_t N, int32_t K, size_t *bytes) try {
   if (!bytes) return fail("linear_f8_workspace_size: bytes is NULL");
-  if (M < 0 || M > (int64_t)1 << 30 || K < 1 || K > kMostExtent || M > ((int64_t)1 << 35) / K) return fail("linear_f8_workspace_size: bad sizes");
-  *bytes = linear_bytes(M, K);
+  if (M < 0 || M > (int64_t)1 << 30 || N < 1 || N > kMostExtent || K < 1 || K > kMostExtent || M > ((int64_t)1 << 35) / K || M > ((int64_t)1 << 35) / N) return fail("linear_f8_workspace_size: bad sizes");
+  *bytes = linear_bytes(M, N, K);
   return 0;
 } MI_CATCH("linear_f8_workspace_size")
 

@@ -43,9 +43,16 @@ struct F8Product {
   const void *bias;
   void *y, *y1;
   int dt;
+  float *parts;  // one matrix: room for the sums of blocks that share a tile's summed axis (f8_parts_bytes), or nullptr
   uint8_t *h;  // gate/up pairs: silu(gate) * up in e4m3, as F8Rows
   float *hs;
 };
+// Parts are made where tiles of 64 x 256 and more are fewer than the chip's CUs: kF8MostParts of a product at most, 256 tiles of all of them.
+constexpr int kF8MostParts = 16;
+inline size_t f8_parts_bytes(int64_t M, int N) {
+  const size_t all = (size_t)M * N * 4 * kF8MostParts, most = (size_t)256 * 256 * 256 * 4;
+  return all < most ? all : most;
+}
 // Rows of a piece: what the product's kernel takes at once (16 or 32: the one for a few rows).
 int f8_tile_rows(const F8Product &p);
 inline bool f8_few_rows(const F8Product &p) { return f8_tile_rows(p) < 64; }

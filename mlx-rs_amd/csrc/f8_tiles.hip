@@ -44,7 +44,30 @@ constexpr size_t f8_tiles_lds(int tm) {  // two stages, and what a thread copies
 
 struct F8Grid {
   int m_tiles, n_tiles, xcds_m, m_each, n_each;  // one matrix: xcds_m XCDs along the token rows, rectangles of m_each x n_each tiles
+  int part_steps;                                // stages of a block: fewer than all where blocks share a tile, whose sums then go to a.parts
 };
+
+// Sums of parts, in their order, a bias added, rounded.
+__global__ __launch_bounds__(256) void f8_parts_kernel(const float *__restrict__ parts, int n_parts, int64_t rows, int N, const void *__restrict__ bias, int dt, void *__restrict__ y) {
+  const int n = ((int)blockIdx.x * 256 + (int)threadIdx.x) * 4;
+  const int64_t row = blockIdx.y;
+  if (n >= N) return;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int p = 0; p < n_parts; ++p) {
+    const float *const from = parts + ((int64_t)p * rows + row) * N + n;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (n + 4 <= N) __builtin_memcpy(v, from, 16);
+    else
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = n + i < N ? from[i] : 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[i] += v[i];
+  }
+  if (bias)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[i] += n + i < N ? value_of(bias, n + i, dt) : 0.f;
+  store4(y, row * N + n, N - n, dt, sum);
+}
 
 template <int TM, F8Mode MODE, bool F32>
 __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, F8Grid g) {
@@ -77,6 +100,7 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, F8Gri
   const uint32_t row0 = piece.row;
   if (rows == 0) return;
   const int N = a.N, K = a.K, runs = f8_runs(K), n_blocks = f8_runs(N), steps = a.pair_sum ? 2 * runs : runs;
+  const int begin = (int)blockIdx.y * g.part_steps, end = begin + g.part_steps < steps ? begin + g.part_steps : steps;
   const int n0 = nt * (MODE == kPair ? 128 : kF8TileN);
   if (mat == a.n_mats) {  // rows of no matrix
     if constexpr (MODE != kPair) {
@@ -266,21 +290,22 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, F8Gri
     if constexpr (LIVE > 0) {
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        w[0][q] = weights(lds + L::X, 0, q);
-        w[1][q] = weights(lds + L::X, 1, q);
-        x[q] = operand(lds + x_at, q);
+        const unsigned char *const at = lds + (begin & 1) * L::BYTES;
+        w[0][q] = weights(at + L::X, 0, q);
+        w[1][q] = weights(at + L::X, 1, q);
+        x[q] = operand(at + x_at, q);
       }
     }
-    int j = 0;
-    for (; j + 2 < steps; ++j) stage(j, true);
-    for (; j < steps; ++j) stage(j, false);
+    int j = begin;
+    for (; j + 2 < end; ++j) stage(j, true);
+    for (; j < end; ++j) stage(j, false);
   };
   __syncthreads();  // (offsets of scales come from other threads)
-  fetch_rows(0, offsets());
-  fetch_weights(0);
-  if (steps > 1) {
-    fetch_rows(1, offsets());
-    fetch_weights(1);
+  fetch_rows(begin, offsets());
+  fetch_weights(begin);
+  if (begin + 1 < end) {
+    fetch_rows(begin + 1, offsets());
+    fetch_weights(begin + 1);
     wait_copies<XC + 6>();
   } else {
     wait_copies<0>();
@@ -328,6 +353,20 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, F8Gri
     for (int r = threadIdx.x / 8; r < rows; r += kF8Threads / 8)
       *reinterpret_cast<u32x4_f8 *>(a.h + (int64_t)(row0 + r) * h_wide + n0 + ((threadIdx.x % 8) ^ f8_turn(r)) * 16) =
           *reinterpret_cast<const u32x4_f8 *>(lds + r * 128 + threadIdx.x % 8 * 16);
+  } else if (g.part_steps < steps) {
+    float *const to = a.parts + (int64_t)blockIdx.y * a.rows * N;
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      const int r = (2 * t + wm) * 32 + ln;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const int n = n0 + wn * 64 + i * 32 + 8 * v + 4 * half;
+          const float o[4] = {acc[t][i][4 * v], acc[t][i][4 * v + 1], acc[t][i][4 * v + 2], acc[t][i][4 * v + 3]};
+          if (r < rows && n < N) store4(to, (int64_t)(row0 + r) * N + n, N - n, 2, o);
+        }
+    }
   } else {
     constexpr int SIZE = F32 ? 4 : 2, EACH = 16 / SIZE, PASSES = F32 ? 2 : 1;  // bytes of a value, values of a piece; 64 weight rows at once, or 32
     unsigned char *const own = lds + wave * (32 * MT * 128);
@@ -377,6 +416,28 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, F8Gri
   }
 }
 
+// One matrix: the tile, and how many blocks share a tile's summed axis where the tiles alone leave CUs idle, by the time they take.  Us, measured: a launch 6; a stage 0.65 with a few
+// blocks and 1.1 with one on every CU (64 token rows), 1.0 and 1.45 (128), 1.7 and 2.2 (256); a join of parts 3, their bytes out and back 2.5 MB each.
+struct F8Plan {
+  int tile, parts;
+};
+static F8Plan f8_dense_plan(const F8Product &p) {
+  F8Plan best{64, 1};
+  double least = 1e30;
+  const int steps = f8_runs(p.K);
+  for (int tile : {64, 128, 256}) {
+    if (tile == 256 && p.dt == 2) continue;
+    const int64_t tiles = ((p.rows + tile - 1) / tile) * ((p.N + kF8TileN - 1) / kF8TileN);
+    for (int parts = 1; parts <= (p.parts ? kF8MostParts : 1); parts *= 2) {
+      if (parts > 1 && (steps < 2 * parts || tiles * parts > 256)) break;
+      const double full = (double)(tiles * parts < 256 ? tiles * parts : 256) / 256, few = tile == 64 ? 0.65 : tile == 128 ? 1.0 : 1.7;
+      const double t = (double)((tiles * parts + 255) / 256) * ((steps + parts - 1) / parts) * (few + 0.45 * full) + (parts > 1 ? 3.0 + (double)parts * p.rows * p.N * 8 / 2.5e6 : 0.0);
+      if (t < least) least = t, best = {tile, parts};
+    }
+  }
+  return best;
+}
+
 template <int TM, F8Mode MODE, bool F32>
 static hipError_t launch_tiles(const F8Product &p, hipStream_t st) {
   constexpr size_t lds = f8_tiles_lds(TM);
@@ -389,7 +450,8 @@ static hipError_t launch_tiles(const F8Product &p, hipStream_t st) {
     if (dev >= 0 && dev < kMaxDevices) raised[dev].store(true, std::memory_order_release);
   }
   const int64_t n_tiles = (p.N + (MODE == kPair ? 127 : kF8TileN - 1)) / (MODE == kPair ? 128 : kF8TileN), m_tiles = p.list ? 0 : (p.rows + TM - 1) / TM;
-  F8Grid g{(int)m_tiles, (int)n_tiles, 1, (int)m_tiles, (int)((n_tiles + 7) / 8)};
+  const int steps = f8_runs(p.K) * (p.pair_sum ? 2 : 1), parts = p.list ? 1 : f8_dense_plan(p).parts;
+  F8Grid g{(int)m_tiles, (int)n_tiles, 1, (int)m_tiles, (int)((n_tiles + 7) / 8), (steps + parts - 1) / parts};
   int64_t each;  // blocks of an XCD
   if (p.list) {
     // (runs of one time hold up to kPieceMost / kPieceBase of their share of the pieces)
@@ -403,13 +465,15 @@ static hipError_t launch_tiles(const F8Product &p, hipStream_t st) {
     each = (int64_t)g.m_each * g.n_each;
   }
   if (each > (int64_t)1 << 19) return hipErrorInvalidValue;  // (a launch has less than 2^32 threads)
-  f8_tiles_kernel<TM, MODE, F32><<<(unsigned)(each * 8), kF8Threads, lds, st>>>(p, g);
+  const unsigned used = (unsigned)((steps + g.part_steps - 1) / g.part_steps);
+  f8_tiles_kernel<TM, MODE, F32><<<dim3((unsigned)(each * 8), used), kF8Threads, lds, st>>>(p, g);
+  if (used > 1) f8_parts_kernel<<<dim3((unsigned)((p.N + 1023) / 1024), (unsigned)p.rows), 256, 0, st>>>(p.parts, (int)used, p.rows, p.N, p.bias, p.dt, p.y);
   return hipGetLastError();
 }
 
 template <F8Mode MODE>
 static hipError_t launch_mode(const F8Product &p, hipStream_t st) {
-  const int tile = f8_tile_rows(p);
+  const int tile = p.list ? f8_tile_rows(p) : f8_dense_plan(p).tile;
   if (p.dt == 2) return tile == 128 ? launch_tiles<128, MODE, true>(p, st) : launch_tiles<64, MODE, true>(p, st);
   return tile == 256 ? launch_tiles<256, MODE, false>(p, st) : tile == 128 ? launch_tiles<128, MODE, false>(p, st) : launch_tiles<64, MODE, false>(p, st);
 }

@@ -466,7 +466,7 @@ PyObject *linear_f8(PyObject *, PyObject *const *args, Py_ssize_t n) {
   return call<1>([&](at::Tensor *out) {
     const int64_t K = x.size(-1), N = w.size(!transpose), M = x.numel() / K;
     size_t need = 0;
-    if (g_f8.linear_workspace(M, (int32_t)K, &need)) return -1;
+    if (g_f8.linear_workspace(M, (int32_t)N, (int32_t)K, &need)) return -1;
     at::DimVector shape(x.sizes().begin(), x.sizes().end());
     shape.back() = N;
     out[0] = at::empty(shape, x.options());
@@ -491,7 +491,7 @@ PyObject *grouped_linear_f8(PyObject *, PyObject *const *args, Py_ssize_t n) {
   return call<1>([&](at::Tensor *out) {
     const int64_t M = x.size(0), K = x.size(1), N = w.size(1 + !transpose);
     size_t need = 0;
-    if (g_f8.linear_workspace(M, (int32_t)K, &need)) return -1;
+    if (g_f8.linear_workspace(M, (int32_t)N, (int32_t)K, &need)) return -1;
     out[0] = at::empty({M, N}, x.options());
     const at::Tensor ws = bytes_like(x, need);
     return g_f8.grouped(data_of(x), data_of(w), static_cast<const float *>(data_of(s)), static_cast<const uint32_t *>(data_of(off)), M, (int32_t)w.size(0), (int32_t)N, (int32_t)K, transpose,

@@ -97,9 +97,14 @@ __global__ __launch_bounds__(kSortThreads) void sort_rows_kernel(SortTokens a, c
   }
   if (blockIdx.x == 0)
     for (int e = threadIdx.x; e <= a.E; e += kSortThreads) a.offsets[e] = offsets[e];
-  if (!rows) return;
   __syncthreads();
   spread_row(x + blockIdx.x * row_bytes, rows, row_bytes, at, a.k);
+}
+
+__global__ __launch_bounds__(kSortThreads) void sort_places_kernel(SortTokens a, const uint32_t *__restrict__ offsets, int64_t P) {
+  const int64_t p = (int64_t)blockIdx.x * kSortThreads + threadIdx.x;
+  if (p < P && a.ids[p] >= (uint32_t)a.E) a.inverse[p] = ~a.inverse[p];
+  if (p <= a.E) a.offsets[p] = offsets[p];
 }
 
 size_t sort_tokens_bytes(int64_t T, int k, int E) {
@@ -117,81 +122,129 @@ hipError_t launch_sort_tokens(const SortTokens &a, const void *x, int dt, int H,
                                      PrepareArgs(), static_cast<char *>(scratch) + ((size_t)(a.E + 2) * 4 + 255) / 256 * 256, st);
       e != hipSuccess)
     return e;
+  if (!rows) {
+    sort_places_kernel<<<(unsigned)((P + kSortThreads - 1) / kSortThreads), kSortThreads, 0, st>>>(a, offsets, P);
+    return hipGetLastError();
+  }
   sort_rows_kernel<<<(unsigned)a.T, kSortThreads, 0, st>>>(a, offsets, static_cast<const char *>(x), row_bytes, static_cast<char *>(rows));
   return hipGetLastError();
 }
 
-// A thread eight columns of a token; its slots' rows eight at a time, all their loads in flight together.
+// How a block's threads lie over tokens and columns of eight: whole tokens a block where rows are short.
+struct TokenGrid {
+  int lanes, tokens, columns;  // threads of a token (a power of two), tokens of a block, blocks of a token
+  TokenGrid(int H, int most) {
+    const int octets = (H + 7) / 8;
+    lanes = most;
+    while (lanes > 16 && lanes / 2 >= octets) lanes /= 2;
+    tokens = most / lanes;
+    columns = (octets + lanes - 1) / lanes;
+  }
+};
+
+// Eight columns from h on of several rows (-1: of the first, for nobody).  The whole octets' loads stand together: with a condition around each, they were waited for one by one.
+template <int DT, int N>
+__device__ __forceinline__ void load_octets(Octet<DT> (&v)[N], const void *rows, const int64_t (&row)[N], int H, int h, int n) {
+  if (n >= 8) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = load_octet<DT>(rows, (row[j] < 0 ? 0 : row[j]) * H + h, 8);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = load_octet<DT>(rows, (row[j] < 0 ? 0 : row[j]) * H + (n > 0 ? h : 0), n > 0 ? n : 0);
+  }
+}
+
+// A thread eight columns of a token; its slots' rows eight at a time, all their loads in flight together.  Blocks of 256 threads: of 64, the launch of blocks is what it waits
+// for (8192 tokens of 2048 bf16 and eight slots: 80 us).
 template <int DT>
-__global__ __launch_bounds__(64) void unsort_kernel(const void *__restrict__ rows, const void *__restrict__ weights, int w_dtype, const int32_t *__restrict__ inverse, int64_t T,
-                                                    int k, int H, void *__restrict__ out) {
-  const int64_t t = blockIdx.x;
-  const int h = (blockIdx.y * 64 + threadIdx.x) * 8, n = H - h;
-  if (n <= 0) return;
+__global__ __launch_bounds__(kSortThreads) void unsort_kernel(const void *__restrict__ rows, const void *__restrict__ weights, int w_dtype, const int32_t *__restrict__ inverse,
+                                                              int64_t T, int k, int H, int lanes_log2, void *__restrict__ out) {
+  const int lanes = 1 << lanes_log2;
+  const int64_t t = (int64_t)blockIdx.x * (kSortThreads >> lanes_log2) + (threadIdx.x >> lanes_log2);
+  const int h = (int)(blockIdx.y * lanes + (threadIdx.x & (lanes - 1))) * 8, n = H - h;
+  if (n <= 0 || t >= T) return;
   float acc[8] = {};
   for (int s0 = 0; s0 < k; s0 += 8) {
     Octet<DT> v[8];
     float w[8];
+    int64_t row[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int64_t s = t * k + (s0 + j < k ? s0 + j : k - 1);
       const int32_t at = inverse[s];
-      const bool named = s0 + j < k && at >= 0 && at < T * k;
+      row[j] = s0 + j < k && at >= 0 && at < T * k ? at : -1;
       w[j] = weights ? value_of(weights, s, w_dtype) : 1.f;
-      v[j] = load_octet<DT>(rows, (named ? (int64_t)at : 0) * H + h, n);
-      if (!named) {  // (not multiplied by zero: its row, or its weight, may be infinite)
-        w[j] = 0.f;
-        v[j] = Octet<DT>{};
-      }
     }
+    load_octets(v, rows, row, H, h, n);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) acc[i] = __builtin_fmaf(w[j], v[j].at(i), acc[i]);
+      for (int i = 0; i < 8; ++i) acc[i] = row[j] >= 0 ? __builtin_fmaf(w[j], v[j].at(i), acc[i]) : acc[i];  // (not multiplied by zero: row or weight may be infinite)
   }
   Octet<DT> o;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) o.put(i, acc[i]);
+  for (int i = 0; i < 8; i += 2) o.put2(i, acc[i], acc[i + 1]);
   store_octet<DT>(out, t * H + h, n, o);
 }
 
 hipError_t launch_unsort_tokens(const void *rows, const void *weights, int w_dtype, const int32_t *inverse, int64_t T, int k, int H, int dt, void *out, hipStream_t st) {
   if (T == 0) return hipSuccess;
+  const TokenGrid g(H, kSortThreads);
   auto *const kernel = dt == 0 ? &unsort_kernel<0> : dt == 1 ? &unsort_kernel<1> : &unsort_kernel<2>;
-  kernel<<<dim3((unsigned)T, (unsigned)((H + 511) / 512)), 64, 0, st>>>(rows, weights, w_dtype, inverse, T, k, H, out);
+  kernel<<<dim3((unsigned)((T + g.tokens - 1) / g.tokens), (unsigned)g.columns), kSortThreads, 0, st>>>(rows, weights, w_dtype, inverse, T, k, H, __builtin_ctz((unsigned)g.lanes), out);
   return hipGetLastError();
 }
 
+__device__ __forceinline__ float wave_sum_f32(float v) {  // in a fixed order
+  auto moved = [](float u, auto ctrl) __attribute__((always_inline)) { return __uint_as_float(dpp_u32<decltype(ctrl)::value>(__float_as_uint(u))); };
+  v += moved(v, std::integral_constant<int, kDppXor1>());
+  v += moved(v, std::integral_constant<int, kDppXor2>());
+  v += moved(v, std::integral_constant<int, kDppHalfMirror>());
+  v += moved(v, std::integral_constant<int, kDppMirror>());
+  auto lane = [&](int l) __attribute__((always_inline)) { return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), l)); };
+  return (lane(0) + lane(16)) + (lane(32) + lane(48));
+}
+
+// A block a token; four slots' rows in flight at once.  A wave's share of a slot's dot product is kept in LDS from one pass over the columns to the next.
 template <int DT>
 __global__ __launch_bounds__(kSortThreads) void unsort_grad_kernel(const void *__restrict__ dout, const void *__restrict__ rows, const void *__restrict__ weights, int w_dtype,
                                                                    const int32_t *__restrict__ inverse, int64_t T, int k, int H, void *__restrict__ drows,
                                                                    void *__restrict__ dweights) {
   __shared__ float sums[kSortMostSlots][kSortThreads / kWave];
   const int64_t t = blockIdx.x;
-  for (int s = 0; s < k; ++s) {
-    const int32_t at = inverse[t * k + s];
-    const bool named = at >= 0;
-    const int64_t row = named ? at : ~at;
-    if (row >= T * k) {  // (no place at all: a slot of nobody's)
-      if (threadIdx.x < kSortThreads / kWave) sums[s][threadIdx.x] = 0.f;
-      continue;
-    }
-    const float w = value_of(weights, t * k + s, w_dtype);
-    float dot = 0.f;
-    for (int h = threadIdx.x * 8; h < H; h += kSortThreads * 8) {
-      Octet<DT> o{};
-      if (named) {
-        const Octet<DT> g = load_octet<DT>(dout, t * H + h, H - h), v = load_octet<DT>(rows, row * H + h, H - h);
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  for (int h0 = 0; h0 < H; h0 += kSortThreads * 8) {
+    const int h = h0 + (int)threadIdx.x * 8, n = H - h;
+    const Octet<DT> g = load_octet<DT>(dout, t * H + (n > 0 ? h : 0), n > 0 ? n : 0);
+    for (int s0 = 0; s0 < k; s0 += 4) {
+      Octet<DT> v[4];
+      int64_t row[4], read[4];
+      float w[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          dot = __builtin_fmaf(g.at(i), v.at(i), dot);
-          o.put(i, w * g.at(i));
-        }
+      for (int j = 0; j < 4; ++j) {
+        const int s = s0 + j < k ? s0 + j : k - 1;
+        const int32_t at = inverse[t * k + s];
+        row[j] = at >= 0 ? at : ~at;
+        if (s0 + j >= k || row[j] >= T * k) row[j] = -1;  // (no place at all: nothing is written)
+        read[j] = at >= 0 ? row[j] : -1;
+        w[j] = value_of(weights, t * k + s, w_dtype);
       }
-      store_octet<DT>(drows, row * H + h, H - h, o);
+      load_octets(v, rows, read, H, h, n);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        Octet<DT> o{};
+        float dot = 0.f;
+        if (read[j] >= 0) {
+#pragma unroll
+          for (int i = 0; i < 8; i += 2) o.put2(i, w[j] * g.at(i), w[j] * g.at(i + 1));
+#pragma unroll
+          for (int i = 0; i < 8; ++i) dot = __builtin_fmaf(g.at(i), v[j].at(i), dot);
+        }
+        if (n > 0 && row[j] >= 0) store_octet<DT>(drows, row[j] * H + h, n, o);
+        dot = wave_sum_f32(dot);
+        if (lane == 0 && s0 + j < k) sums[s0 + j][wave] = h0 ? sums[s0 + j][wave] + dot : dot;
+      }
     }
-    for (int d = 1; d < kWave; d <<= 1) dot += __shfl_xor(dot, d, kWave);
-    if (threadIdx.x % kWave == 0) sums[s][threadIdx.x / kWave] = dot;
   }
   __syncthreads();
   if ((int)threadIdx.x < k) {

@@ -744,9 +744,9 @@ def _f8_bank(who, name, w, scales, lead, N=None, K=None):
 
 
 @functools.lru_cache(maxsize=1024)
-def _linear_f8_workspace_bytes(M, K):
+def _linear_f8_workspace_bytes(M, N, K):
     need = C.c_size_t()
-    check(load_library().mi_moe_linear_f8_workspace_size(M, K, C.byref(need)))
+    check(load_library().mi_moe_linear_f8_workspace_size(M, N, K, C.byref(need)))
     return need.value
 
 
@@ -775,7 +775,7 @@ def linear_f8(x, w, scales, linear_bias=None, transpose=True):
     _int32(who, ("N", outer), ("K", inner))
     M = x.numel() // inner if inner else 0
     y = torch.empty(x.shape[:-1] + (outer,), dtype=x.dtype, device=x.device)
-    need = _linear_f8_workspace_bytes(M, inner) if M else 0
+    need = _linear_f8_workspace_bytes(M, outer, inner) if M else 0
     ws = torch.empty(need, dtype=torch.uint8, device=x.device)
     check(lib.mi_moe_linear_f8(_ptr(x), _ptr(w), _ptr(scales), _ptr(linear_bias), M, outer, inner, 1 if transpose else 0, dt, _ptr(y), _ptr(ws), need, _stream()))
     return y
@@ -803,7 +803,7 @@ def grouped_linear_f8(rows, w, scales, offsets, transpose=True):
     _int32(who, ("N", outer), ("K", inner), ("n_experts", E))
     R = rows.shape[0]
     y = torch.empty((R, outer), dtype=rows.dtype, device=rows.device)
-    need = _linear_f8_workspace_bytes(R, inner) if R and inner else 0
+    need = _linear_f8_workspace_bytes(R, outer, inner) if R and inner and outer else 0
     ws = torch.empty(need, dtype=torch.uint8, device=rows.device)
     check(lib.mi_moe_grouped_linear_f8(_ptr(rows), _ptr(w), _ptr(scales), _ptr(offsets), R, E, outer, inner, 1 if transpose else 0, dt, _ptr(y), _ptr(ws), need, _stream()))
     return y

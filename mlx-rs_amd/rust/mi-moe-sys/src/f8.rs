@@ -22,7 +22,7 @@ extern "C" {
     pub fn mi_moe_unsort_tokens_grad(dout: *const c_void, rows: *const c_void, topk_w: *const c_void, w_dtype: i32, inverse: *const i32, T: i64, top_k: i32, hidden: i32, dtype: i32, drows: *mut c_void, dweights: *mut c_void, stream: *mut c_void) -> c_int;
     pub fn mi_moe_quantize_f8(x: *const c_void, dtype: i32, rows: i64, cols: i64, block_rows: i32, codes: *mut c_void, scales: *mut f32, stream: *mut c_void) -> c_int;
     pub fn mi_moe_dequantize_f8(codes: *const c_void, scales: *const f32, rows: i64, cols: i64, block_rows: i32, dtype: i32, out: *mut c_void, stream: *mut c_void) -> c_int;
-    pub fn mi_moe_linear_f8_workspace_size(M: i64, K: i32, bytes: *mut usize) -> c_int;
+    pub fn mi_moe_linear_f8_workspace_size(M: i64, N: i32, K: i32, bytes: *mut usize) -> c_int;
     pub fn mi_moe_linear_f8(x: *const c_void, w: *const c_void, scales: *const f32, linear_bias: *const c_void, M: i64, N: i32, K: i32, transpose: i32, dtype: i32, y: *mut c_void, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
     pub fn mi_moe_grouped_linear_f8(x: *const c_void, w: *const c_void, scales: *const f32, offsets: *const u32, rows: i64, n_experts: i32, N: i32, K: i32, transpose: i32, dtype: i32, y: *mut c_void, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
     pub fn mi_moe_switch_glu_f8_workspace_size(T: i64, hidden: i32, intermediate: i32, n_experts: i32, top_k: i32, grad: i32, bytes: *mut usize) -> c_int;

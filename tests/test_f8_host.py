@@ -89,7 +89,7 @@ def test_linear_refusals(lib, needle, change):  # noqa: F811
     a = dict(x=P, w=P, s=P, M=5, N=48, K=128, t=1, dt=0, y=P, ws=P, short=0)
     a.update(change)
     n = C.c_size_t()
-    assert lib.mi_moe_linear_f8_workspace_size(5, 128, C.byref(n)) == 0
+    assert lib.mi_moe_linear_f8_workspace_size(5, max(a["N"], 1) % (1 << 22), 128, C.byref(n)) == 0
     size = n.value - a["short"]
     refused(lib, needle, "mi_moe_linear_f8", a["x"], a["w"], a["s"], None, a["M"], a["N"], a["K"], a["t"], a["dt"], a["y"], a["ws"], size, None)
     refused(lib, needle, "mi_moe_grouped_linear_f8", a["x"], a["w"], a["s"], P, a["M"], 2, a["N"], a["K"], a["t"], a["dt"], a["y"], a["ws"], size, None)
@@ -100,8 +100,8 @@ def test_more_linear_refusals(lib):  # noqa: F811
     refused(lib, "offsets", "mi_moe_grouped_linear_f8", P, P, P, None, 5, 2, 48, 128, 1, 0, P, P, 1 << 20, None)
     for E in (0, 513):
         refused(lib, "n_experts", "mi_moe_grouped_linear_f8", P, P, P, P, 5, E, 48, 128, 1, 0, P, P, 1 << 20, None)
-    refused(lib, "bytes", "mi_moe_linear_f8_workspace_size", 1, 16, None)
-    refused(lib, "bad sizes", "mi_moe_linear_f8_workspace_size", -1, 16, C.byref(C.c_size_t()))
+    refused(lib, "bytes", "mi_moe_linear_f8_workspace_size", 1, 16, 16, None)
+    refused(lib, "bad sizes", "mi_moe_linear_f8_workspace_size", -1, 16, 16, C.byref(C.c_size_t()))
     assert lib.mi_moe_linear_f8(None, None, None, None, 0, 48, 128, 1, 0, None, None, 0, None) == 0
     assert lib.mi_moe_grouped_linear_f8(None, None, None, None, 0, 3, 48, 128, 1, 0, None, None, 0, None) == 0
     assert lib.mi_moe_quantize_f8(None, 0, 0, 8, 1, None, None, None) == 0 and lib.mi_moe_dequantize_f8(None, None, 0, 8, 1, 0, None, None) == 0
@@ -139,7 +139,7 @@ def test_workspaces_grow_with_the_batch(lib):  # noqa: F811
             assert getattr(lib, fn)(t, *rest, C.byref(n)) == 0
             yield n.value
 
-    for fn, rest in (("mi_moe_sort_tokens_workspace_size", (8, 128)), ("mi_moe_linear_f8_workspace_size", (2048,)), ("mi_moe_linear_f8_workspace_size", (16,)),
+    for fn, rest in (("mi_moe_sort_tokens_workspace_size", (8, 128)), ("mi_moe_linear_f8_workspace_size", (4096, 2048)), ("mi_moe_linear_f8_workspace_size", (1, 16)),
                      ("mi_moe_switch_glu_f8_workspace_size", (2048, 768, 128, 8, 0)), ("mi_moe_switch_glu_f8_workspace_size", (2048, 768, 128, 8, 1)),
                      ("mi_moe_switch_glu_f8_workspace_size", (272, 400, 2, 1, 0))):
         got = list(sizes(fn, *rest))

@@ -88,6 +88,12 @@ int linear(const char *who, const void *x, const void *w, const float *scales, c
   lists.rows = M;
   if (offsets) list_for(p, lists, 0, list);
   else p.parts = reinterpret_cast<float *>(c.take<char>(f8_parts_bytes(M, N)));
+  if (!offsets && f8_in_blocks(p, M)) {
+    p.raw = x;
+    p.raw_dt = dtype;
+    MI_HIP(launch_f8_product(p, st));
+    return 0;
+  }
   MI_HIP(launch_quantize_f8_rows(x, dtype, M, K, q.out(M, K), st, lists));
   MI_HIP(launch_f8_product(p, st));
   return 0;
@@ -246,7 +252,6 @@ int mi_moe_switch_glu_f8(const void *x, const uint32_t *topk_idx, const void *to
   if (check_workspace("switch_glu_f8", workspace, workspace_bytes, ws.bytes)) return 1;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const int64_t P = T * top_k;
-  MI_HIP(launch_sort_tokens({topk_idx, T, top_k, n_experts, ws.order, ws.inverse, ws.offsets}, nullptr, dtype, hidden, nullptr, ws.sort, st));
   F8Product p{};
   p.x = ws.x.as(T);
   p.order = ws.order;
@@ -285,9 +290,19 @@ int mi_moe_switch_glu_f8(const void *x, const uint32_t *topk_idx, const void *to
   lists.rows = P;
   list_for(p, lists, 0, ws.list[0]);
   list_for(d, lists, 1, ws.list[1]);
-  MI_HIP(launch_quantize_f8_rows(x, dtype, T, hidden, ws.x.out(T, hidden), st, lists));
+  // A token or a few: the lists come beside the sorting, rows are rounded where they are multiplied.
+  const bool in_blocks = P <= kSortSmall && f8_in_blocks(p, T) && f8_in_blocks(d, T);
+  MI_HIP(launch_sort_tokens({topk_idx, T, top_k, n_experts, ws.order, ws.inverse, ws.offsets}, nullptr, dtype, hidden, nullptr, ws.sort, st, in_blocks ? lists : F8Lists()));
+  if (in_blocks) {
+    p.raw = x;
+    p.raw_dt = dtype;
+    d.raw = ws.g;
+    d.raw_up = ws.u;
+  } else {
+    MI_HIP(launch_quantize_f8_rows(x, dtype, T, hidden, ws.x.out(T, hidden), st, lists));
+  }
   MI_HIP(launch_f8_product(p, st));
-  if (few) MI_HIP(launch_swiglu_f8(ws.g, ws.u, P, intermediate, ws.h.out(P, intermediate), st));
+  if (few && !in_blocks) MI_HIP(launch_swiglu_f8(ws.g, ws.u, P, intermediate, ws.h.out(P, intermediate), st));
   MI_HIP(launch_f8_product(d, st));
   MI_HIP(launch_unsort_tokens(ws.y, topk_w, w_dtype, ws.inverse, T, top_k, hidden, dtype, out, st));
   return 0;

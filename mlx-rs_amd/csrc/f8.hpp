@@ -31,6 +31,9 @@ struct F8Mat {
 };
 struct F8Product {
   F8Rows x;
+  // instead of codes, for a few rows (f8_in_blocks), rows that every block of the product rounds for itself: of element type raw_dt, or silu(raw) * raw_up in float32
+  const void *raw, *raw_up;
+  int raw_dt;
   const uint32_t *order;    // sorted row r reads x row order[r] / k_div; nullptr: r
   int k_div;
   const uint4 *list;        // the pieces of at most f8_tile_rows rows that the matrices' rows are cut into, and rows of no matrix, which are zeros of y (f8_list).  nullptr: one
@@ -56,6 +59,13 @@ inline size_t f8_parts_bytes(int64_t M, int N) {
 // Rows of a piece: what the product's kernel takes at once (16 or 32: the one for a few rows).
 int f8_tile_rows(const F8Product &p);
 inline bool f8_few_rows(const F8Product &p) { return f8_tile_rows(p) < 64; }
+// Whether the blocks of a product for a few rows round them by themselves, where a matrix has `most` rows as a rule.  (A piece may hold as many as its kernel takes, of tokens that
+// name an expert more than once: there is room for them.)
+inline size_t f8_own_bytes(const F8Product &p) {
+  const int tile = f8_tile_rows(p);
+  return (size_t)(p.rows < tile ? p.rows : tile) * (size_t)(f8_row_bytes(p.K) + 16 + 4 * f8_runs(p.K));
+}
+inline bool f8_in_blocks(const F8Product &p, int64_t most) { return f8_few_rows(p) && most * f8_runs(p.K) <= 64 && f8_own_bytes(p) <= 48 * 1024; }
 inline int64_t f8_most_pieces(int64_t rows, int n_mats, int tile) { return rows / tile + (n_mats + 1 < rows ? n_mats + 1 : rows); }
 // A list: kF8ListHead words of where the pieces of each of the eight XCDs begin (and end), then the pieces.
 constexpr int kF8ListHead = 3;  // (uint4s)
@@ -112,8 +122,10 @@ struct SortTokens {
   uint32_t *offsets;  // [E + 1]
 };
 size_t sort_tokens_bytes(int64_t T, int k, int E);
+constexpr int64_t kSortSmall = 2048;  // pairs up to which one launch sorts, and lists
 // rows != nullptr: the sorted rows of x, those that no slot names zeros
-hipError_t launch_sort_tokens(const SortTokens &a, const void *x, int dt, int H, void *rows, void *scratch, hipStream_t st);
+// lists (up to kSortSmall pairs): made beside it
+hipError_t launch_sort_tokens(const SortTokens &a, const void *x, int dt, int H, void *rows, void *scratch, hipStream_t st, const F8Lists &lists = F8Lists());
 // weights nullptr: sums without weights (the sorting's gradient)
 hipError_t launch_unsort_tokens(const void *rows, const void *weights, int w_dtype, const int32_t *inverse, int64_t T, int k, int H, int dt, void *out,
                                 hipStream_t st);
@@ -214,7 +226,9 @@ __device__ __forceinline__ void f8_list(const uint32_t *__restrict__ offsets, in
     }
     return v;
   };
-  uint32_t before = 0;
+  // (a segment's pieces are of about one time)
+  auto time_of = [&](uint32_t rows, uint32_t pieces) __attribute__((always_inline)) { return pieces * kPieceBase + (rows + 31) / 32; };
+  uint32_t before = 0, time = 0;
   for_segments([&](uint32_t e, uint32_t lo, uint32_t hi, uint32_t pieces, uint32_t size) __attribute__((always_inline)) {
     const uint32_t upto = sum_up_to(pieces), first = before + upto - pieces;
     for (uint32_t i = 0; i < pieces && first + i < places; ++i) {
@@ -222,25 +236,30 @@ __device__ __forceinline__ void f8_list(const uint32_t *__restrict__ offsets, in
       pieces_at[first + i] = make_uint4(e, row, (hi - row < size ? hi - row : size) | i << 16, i >> 16 | pieces << 8);
     }
     before += (uint32_t)__builtin_amdgcn_readlane((int)upto, kWave - 1);
+    time += time_of(hi - lo, pieces);
   });
   const uint32_t n = before < places ? before : places;
   for (uint32_t i = n + lane; i < places; i += kWave) pieces_at[i] = make_uint4(0, 0, 0, 0);
   if (tile < 64) return;  // (the kernel for a few rows takes a piece a block)
-  __threadfence_block();
-  uint32_t time = 0;
-  auto time_of = [&](uint32_t i) __attribute__((always_inline)) { return i < n ? kPieceBase + ((pieces_at[i].z & 0xffffu) + 31) / 32 : 0u; };
-  for (uint32_t i = lane; i < (n + kWave - 1) / kWave * kWave; i += kWave) time += (uint32_t)__builtin_amdgcn_readlane((int)sum_up_to(time_of(i)), kWave - 1);
-  uint32_t done = 0, start = lane == 8 ? n : 0u;  // lane k: where XCD k's begin
-  for (uint32_t i = lane; i < (n + kWave - 1) / kWave * kWave; i += kWave) {
-    const uint32_t own = time_of(i), upto = sum_up_to(own);
-    const uint32_t xcd = i < n ? (uint32_t)((uint64_t)(done + upto - own) * 8 / time) : 8u;
+  const uint64_t whole = (uint32_t)__builtin_amdgcn_readlane((int)sum_up_to(time), kWave - 1);
+  uint32_t done = 0, start[8] = {};  // how many pieces begin ahead of each XCD's share of the time
+  for_segments([&](uint32_t, uint32_t lo, uint32_t hi, uint32_t pieces, uint32_t) __attribute__((always_inline)) {
+    const uint32_t own = time_of(hi - lo, pieces), upto = sum_up_to(own), from = done + upto - own;
+#pragma unroll
     for (uint32_t k = 1; k < 8; ++k) {
-      const uint32_t c = (uint32_t)__popcll(__ballot(xcd < k));
-      if ((uint32_t)lane == k) start += c;
+      const uint32_t line = (uint32_t)(whole * k / 8);
+      const uint64_t ahead = pieces && line > from ? ((uint64_t)(line - from) * pieces + own - 1) / own : 0u;
+      start[k] += ahead < pieces ? (uint32_t)ahead : pieces;
     }
     done += (uint32_t)__builtin_amdgcn_readlane((int)upto, kWave - 1);
+  });
+  uint32_t mine = lane == 8 ? n : 0u;
+#pragma unroll
+  for (uint32_t k = 1; k < 8; ++k) {
+    const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)sum_up_to(start[k]), kWave - 1);
+    if ((uint32_t)lane == k) mine = all < n ? all : n;
   }
-  if (lane <= 8) reinterpret_cast<uint32_t *>(list)[lane] = start;
+  if (lane <= 8) reinterpret_cast<uint32_t *>(list)[lane] = mine;
 }
 
 // ---------------------------------------------------------------- products

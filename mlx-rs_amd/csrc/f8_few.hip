@@ -6,14 +6,19 @@
 // multiplies is free as long as both sides agree), so that one load takes 64 consecutive bytes of a weight row.  Codes go from memory into the instruction's
 // registers, nothing is unpacked; token rows come the same way out of L2.  A run's sums are scaled in float32; the waves' sums meet in LDS in a fixed order.
 #include "f8.hpp"
+#include "octets.hpp"
 
 namespace mi_moe {
 
 constexpr int kFewWaves = 4;
 
-template <int TG, bool F32>  // F32: on the bf16 instructions
+// IN: rows as codes; as they are, or a gate and an up product of them, both rounded to e4m3 by the block itself, into LDS, while its first weights are on their way.  A launch
+// less (2 us) for a few microseconds of work.
+enum F8In { kCodes, kRaw, kGateUp };
+template <int TG, bool F32, F8In IN>  // F32: on the bf16 instructions
 __global__ __launch_bounds__(kFewWaves *kWave) void f8_few_kernel(F8Product a) {
   constexpr int AHEAD = TG == 1 ? 4 : 2;  // runs whose loads are in flight at once
+  extern __shared__ __align__(16) uint8_t own_rows[];  // [rows][whole runs + 16], then scales [rows][runs]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ln = lane & 15, part = lane >> 4;
   const int tiles = (a.N + 15) / 16, which = (int)blockIdx.x / tiles, n0 = ((int)blockIdx.x - which * tiles) * 16;
   const F8Piece piece = f8_piece(a, 16 * TG, blockIdx.y);
@@ -31,20 +36,13 @@ __global__ __launch_bounds__(kFewWaves *kWave) void f8_few_kernel(F8Product a) {
   const F8Mat m = which ? a.m[1] : a.m[0];
   const uint8_t *const w = m.w + (int64_t)piece.mat * a.N * a.K + (int64_t)(n0 + ln < a.N ? n0 + ln : a.N - 1) * a.K;
   const float *const ws = m.s + ((int64_t)piece.mat * f8_runs(a.N) + n0 / kF8Run) * runs;
-  const uint8_t *x[TG];
-  const float *xs[TG];
-#pragma unroll
-  for (int t = 0; t < TG; ++t) {
-    const uint32_t r = t * 16 + ln < (int)piece.rows ? piece.row + t * 16 + ln : piece.row;
-    int64_t at = a.order ? a.order[r] / (uint32_t)a.k_div : r;
-    if (at >= a.x.rows) at = 0;  // (an order of the caller's: never followed out of the rows)
-    x[t] = a.x.codes + at * wide;
-    xs[t] = a.x.scales + at;
-  }
-  f32x4_t acc[TG] = {};
-  for (int j0 = wave; j0 < runs; j0 += kFewWaves * AHEAD) {
-    u32x4_f8 wv[AHEAD][2], xv[AHEAD][TG][2];
-    float s[AHEAD], sx[AHEAD][TG];
+  auto source = [&](uint32_t r) __attribute__((always_inline)) {
+    const int64_t at = a.order ? a.order[r] / (uint32_t)a.k_div : r;
+    return at < a.x.rows ? at : 0;  // (never followed out of the rows)
+  };
+  u32x4_f8 wv[AHEAD][2];
+  float s[AHEAD];
+  auto fetch = [&](int j0) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
       const int j = j0 + i * kFewWaves < runs ? j0 + i * kFewWaves : runs - 1;  // (past the end the last run again, with a scale of zero)
@@ -54,11 +52,72 @@ __global__ __launch_bounds__(kFewWaves *kWave) void f8_few_kernel(F8Product a) {
         const int k = j * kF8Run + h * 64 + part * 16;
         wv[i][h] = *reinterpret_cast<const u32x4_f8 *>(w + (k < a.K ? k : 0));
         if (k >= a.K) wv[i][h] = u32x4_f8{0, 0, 0, 0};
-#pragma unroll
-        for (int t = 0; t < TG; ++t) xv[i][t][h] = *reinterpret_cast<const u32x4_f8 *>(x[t] + k);
       }
+    }
+  };
+  fetch(wave);
+  const uint8_t *x[TG];
+  const float *xs[TG];
+  if constexpr (IN == kCodes) {
 #pragma unroll
-      for (int t = 0; t < TG; ++t) sx[i][t] = xs[t][(int64_t)j * a.x.rows];
+    for (int t = 0; t < TG; ++t) {
+      const int64_t at = source(t * 16 + ln < (int)piece.rows ? piece.row + t * 16 + ln : piece.row);
+      x[t] = a.x.codes + at * wide;
+      xs[t] = a.x.scales + at;
+    }
+  } else {
+    float *const own_scales = reinterpret_cast<float *>(own_rows + piece.rows * (wide + 16));
+    for (int at = threadIdx.x / 16; at < (int)piece.rows * runs; at += kFewWaves * kWave / 16) {
+      const int r = at / runs, run = at - r * runs, k = run * kF8Run + (threadIdx.x % 16) * 8, n = a.K - k;
+      const int64_t from = (IN == kGateUp ? (int64_t)(piece.row + r) : source(piece.row + r)) * a.K + (n > 0 ? k : 0);
+      float v[8];
+      auto load = [&](auto dt_of) __attribute__((always_inline)) {
+        constexpr int DT = decltype(dt_of)::value;
+        const Octet<DT> o = load_octet<DT>(a.raw, from, n > 0 ? n : 0);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = o.at(i);
+      };
+      if constexpr (IN == kGateUp) {
+        load(std::integral_constant<int, 2>());
+        const Octet<2> up = load_octet<2>(a.raw_up, from, n > 0 ? n : 0);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = silu(v[i]) * up.v[i];
+      } else if (a.raw_dt == 0) {
+        load(std::integral_constant<int, 0>());
+      } else if (a.raw_dt == 1) {
+        load(std::integral_constant<int, 1>());
+      } else {
+        load(std::integral_constant<int, 2>());
+      }
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = umax(m, abs_bits(v[i]));
+      const F8Scale q(max_of_16_lanes(m));
+      *reinterpret_cast<uint2 *>(own_rows + r * (wide + 16) + k) = make_uint2(q.codes(v[0], v[1], v[2], v[3]), q.codes(v[4], v[5], v[6], v[7]));
+      if (threadIdx.x % 16 == 0) own_scales[r * runs + run] = q.scale;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < TG; ++t) {
+      const int r = t * 16 + ln < (int)piece.rows ? t * 16 + ln : 0;
+      x[t] = own_rows + r * (wide + 16);
+      xs[t] = own_scales + r * runs;
+    }
+  }
+  f32x4_t acc[TG] = {};
+  for (int j0 = wave; j0 < runs; j0 += kFewWaves * AHEAD) {
+    if (j0 != wave) fetch(j0);
+    u32x4_f8 xv[AHEAD][TG][2];
+    float sx[AHEAD][TG];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int j = j0 + i * kFewWaves < runs ? j0 + i * kFewWaves : runs - 1;
+#pragma unroll
+      for (int t = 0; t < TG; ++t) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) xv[i][t][h] = *reinterpret_cast<const u32x4_f8 *>(x[t] + j * kF8Run + h * 64 + part * 16);
+        sx[i][t] = IN == kCodes ? xs[t][(int64_t)j * a.x.rows] : xs[t][j];
+      }
     }
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i)
@@ -106,14 +165,19 @@ int f8_tile_rows(const F8Product &p) {
 hipError_t launch_f8_few(const F8Product &p, hipStream_t st) {
   if (p.rows == 0) return hipSuccess;
   const unsigned tiles = (unsigned)((p.N + 15) / 16) * (p.y1 ? 2 : 1);
-  auto launch = [&](auto *kernel, int tg) {
-    const int64_t pieces = p.list ? f8_most_pieces(p.rows, p.n_mats, 16 * tg) : (p.rows + 16 * tg - 1) / (16 * tg);
-    kernel<<<dim3(tiles, (unsigned)pieces), kFewWaves * kWave, 0, st>>>(p);
+  const int tile = f8_tile_rows(p);
+  const int64_t pieces = p.list ? f8_most_pieces(p.rows, p.n_mats, tile) : (p.rows + tile - 1) / tile;
+  const size_t own = p.raw ? f8_own_bytes(p) : 0;
+  auto launch = [&](auto *kernel) {
+    kernel<<<dim3(tiles, (unsigned)pieces), kFewWaves * kWave, own, st>>>(p);
     return hipGetLastError();
   };
-  const bool two = f8_tile_rows(p) == 32;
-  if (p.dt == 2) return two ? launch(&f8_few_kernel<2, true>, 2) : launch(&f8_few_kernel<1, true>, 1);
-  return two ? launch(&f8_few_kernel<2, false>, 2) : launch(&f8_few_kernel<1, false>, 1);
+  auto kind = [&](auto in_of) {
+    constexpr F8In IN = decltype(in_of)::value;
+    if (p.dt == 2) return tile == 32 ? launch(&f8_few_kernel<2, true, IN>) : launch(&f8_few_kernel<1, true, IN>);
+    return tile == 32 ? launch(&f8_few_kernel<2, false, IN>) : launch(&f8_few_kernel<1, false, IN>);
+  };
+  return !p.raw ? kind(std::integral_constant<F8In, kCodes>()) : !p.raw_up ? kind(std::integral_constant<F8In, kRaw>()) : kind(std::integral_constant<F8In, kGateUp>());
 }
 
 }  // namespace mi_moe

@@ -37,19 +37,29 @@ __global__ __launch_bounds__(kRowThreads) void quantize_rows_kernel(const void *
     return;
   }
   const int runs = f8_runs(cols);
-  const int64_t at = (int64_t)(blockIdx.x - n_lists) * kRowRuns + threadIdx.x / 16;
-  if (at >= rows * runs) return;  // (whole rows of lanes)
-  const int64_t row = at / runs;
-  const int run = (int)(at - row * runs), k = run * kF8Run + (threadIdx.x % 16) * 8, n = cols - k;
-  float v[8] = {};
-  if (n > 0) {
-    const Octet<DT> o = load_octet<DT>(x, row * cols + k, n);
+  const uint32_t first = (blockIdx.x - n_lists) * (2 * kRowRuns) + threadIdx.x / 16, all = (uint32_t)rows * (uint32_t)runs;  // (in 32 bits: in_launches)
+  Octet<DT> o[2];
+  int64_t row[2];
+  int run[2], n[2];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = o.at(i);
+  for (int i = 0; i < 2; ++i) {  // (two loads in flight: one took 14 us for 4096 x 4096 bf16)
+    const uint32_t at = first + i * kRowRuns < all ? first + i * kRowRuns : all - 1, r = at / (uint32_t)runs;
+    row[i] = r;
+    run[i] = (int)(at - r * (uint32_t)runs);
+    const int k = run[i] * kF8Run + (threadIdx.x % 16) * 8;
+    n[i] = cols - k;
+    o[i] = load_octet<DT>(x, row[i] * cols + (n[i] > 0 ? k : 0), n[i] > 0 ? n[i] : 0);
   }
-  write_run(v, to, row, run, n);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = o[i].at(j);
+    if (first + i * kRowRuns < all) write_run(v, to, row[i], run[i], n[i]);  // (whole rows of lanes)
+  }
 }
 
+static unsigned quantize_blocks(int64_t rows, int cols) { return (unsigned)((rows * f8_runs(cols) + 2 * kRowRuns - 1) / (2 * kRowRuns)); }
 static unsigned run_blocks(int64_t rows, int cols) { return (unsigned)((rows * f8_runs(cols) + kRowRuns - 1) / kRowRuns); }
 // f(first row, rows) for parts of the rows that a launch holds: less than 2^32 threads
 template <class F>
@@ -74,7 +84,7 @@ hipError_t launch_quantize_f8_rows(const void *x, int dt, int64_t rows, int cols
   auto *const kernel = dt == 0 ? &quantize_rows_kernel<0> : dt == 1 ? &quantize_rows_kernel<1> : &quantize_rows_kernel<2>;
   return in_launches(rows, cols, [&](int64_t r, int64_t n) {
     const int also = r == 0 ? n_lists : 0;
-    kernel<<<run_blocks(n, cols) + also, kRowThreads, 0, st>>>(value_at(x, dt, r * cols), n, cols, rows_from(to, r), lists, also);
+    kernel<<<quantize_blocks(n, cols) + also, kRowThreads, 0, st>>>(value_at(x, dt, r * cols), n, cols, rows_from(to, r), lists, also);
   });
 }
 
@@ -121,9 +131,9 @@ template <int DT>
 __global__ __launch_bounds__(kRowThreads) void dequantize_f8_kernel(const uint8_t *__restrict__ codes, const float *__restrict__ scales, int64_t rows, int cols, int block_rows,
                                                                     void *__restrict__ out) {
   const int runs = f8_runs(cols);
-  const int64_t at = (int64_t)blockIdx.x * kRowRuns + threadIdx.x / 16;
-  if (at >= rows * runs) return;
-  const int64_t row = at / runs;
+  const uint32_t at = blockIdx.x * kRowRuns + threadIdx.x / 16;
+  if (at >= (uint32_t)rows * (uint32_t)runs) return;
+  const int64_t row = at / (uint32_t)runs;
   const int run = (int)(at - row * runs), k = run * kF8Run + (threadIdx.x % 16) * 8, n = cols - k;
   if (n <= 0) return;
   const float s = scales[row / block_rows * runs + run];
@@ -154,9 +164,9 @@ hipError_t launch_dequantize_f8(const uint8_t *codes, const float *scales, int64
 // ---------------------------------------------------------------- silu(gate) * up
 __global__ __launch_bounds__(kRowThreads) void swiglu_f8_kernel(const float *__restrict__ g, const float *__restrict__ u, int64_t rows, int cols, F8Out to) {
   const int runs = f8_runs(cols);
-  const int64_t at = (int64_t)blockIdx.x * kRowRuns + threadIdx.x / 16;
-  if (at >= rows * runs) return;
-  const int64_t row = at / runs;
+  const uint32_t at = blockIdx.x * kRowRuns + threadIdx.x / 16;
+  if (at >= (uint32_t)rows * (uint32_t)runs) return;
+  const int64_t row = at / (uint32_t)runs;
   const int run = (int)(at - row * runs), k = run * kF8Run + (threadIdx.x % 16) * 8, n = cols - k;
   float v[8] = {};
   if (n > 0) {

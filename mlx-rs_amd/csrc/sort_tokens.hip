@@ -13,7 +13,6 @@
 namespace mi_moe {
 
 constexpr int kSortThreads = 256, kSortMostSlots = 32;
-constexpr int64_t kSortSmall = 2048;  // pairs up to which every token's block finds its own places
 
 // a token's row to its places: 16 bytes a thread and step, with no more alignment than the elements' own
 __device__ __forceinline__ void spread_row(const char *from, char *rows, int64_t bytes, const int32_t *at, int k) {
@@ -39,7 +38,8 @@ __device__ __forceinline__ void spread_row(const char *from, char *rows, int64_t
 
 // Few pairs: block t finds the places of token t's pairs by counting the pairs before each (a smaller expert, or the same and an earlier pair), and writes its rows; the last block
 // counts the experts' rows.  One launch, no block waits for another.
-__global__ __launch_bounds__(kSortThreads) void sort_few_kernel(SortTokens a, const char *__restrict__ x, int64_t row_bytes, char *__restrict__ rows) {
+__global__ __launch_bounds__(kSortThreads) void sort_few_kernel(SortTokens a, const char *__restrict__ x, int64_t row_bytes, char *__restrict__ rows,
+                                                                F8Lists lists) {
   __shared__ uint32_t ids[kSortSmall];
   __shared__ int32_t at[kSortMostSlots];
   __shared__ uint32_t count[513];
@@ -60,10 +60,15 @@ __global__ __launch_bounds__(kSortThreads) void sort_few_kernel(SortTokens a, co
           const uint32_t v = __shfl_up(upto, d, kWave);
           if (lane >= d) upto += v;
         }
-        if (e0 + lane <= a.E) a.offsets[e0 + lane] = before + upto - own;
+        if (e0 + lane <= a.E) {
+          a.offsets[e0 + lane] = before + upto - own;
+          count[e0 + lane] = before + upto - own;
+        }
         before += __shfl(upto, kWave - 1, kWave);
       }
     }
+    __syncthreads();
+    if (wave < 2 && lists.list[wave]) f8_list(count, a.E, (uint32_t)P, (uint32_t)lists.tile[wave], lists.list[wave], (uint32_t)lists.places[wave]);
     return;
   }
   __syncthreads();
@@ -111,10 +116,10 @@ size_t sort_tokens_bytes(int64_t T, int k, int E) {
   return T * k <= kSortSmall ? 0 : ((size_t)(E + 2) * 4 + 255) / 256 * 256 + dispatch_workspace_bytes(E + 1, T * k);
 }
 
-hipError_t launch_sort_tokens(const SortTokens &a, const void *x, int dt, int H, void *rows, void *scratch, hipStream_t st) {
+hipError_t launch_sort_tokens(const SortTokens &a, const void *x, int dt, int H, void *rows, void *scratch, hipStream_t st, const F8Lists &lists) {
   const int64_t P = a.T * a.k, row_bytes = (int64_t)H * (dt == 2 ? 4 : 2);
   if (P <= kSortSmall) {  // (no tokens: the offsets alone)
-    sort_few_kernel<<<(unsigned)a.T + 1, kSortThreads, 0, st>>>(a, static_cast<const char *>(x), row_bytes, static_cast<char *>(rows));
+    sort_few_kernel<<<(unsigned)a.T + 1, kSortThreads, 0, st>>>(a, static_cast<const char *>(x), row_bytes, static_cast<char *>(rows), lists);
     return hipGetLastError();
   }
   uint32_t *const offsets = static_cast<uint32_t *>(scratch);

@@ -108,7 +108,8 @@ struct ExpertsWs {
   RowsIn x, dout;   // rows of tokens
   float *g, *u, *dh;  // float32 rows of pairs: gradients, and batches of a few rows an expert
   RowsIn h;         // rows of pairs: h, or dg and du side by side
-  void *y;
+  void *y;          // of pairs, for the sum over slots: float32, or scaled float16
+  float *y_scales;
   size_t bytes;
   ExpertsWs(void *at, int64_t T, int H, int I, int E, int k, bool grad) : ExpertsWs(Carver(at), T, T * k, H, I, E, k, grad) {}
 
@@ -117,7 +118,11 @@ struct ExpertsWs {
       : order(c.take<uint32_t>((size_t)P)), offsets(c.take<uint32_t>((size_t)E + 1)), inverse(c.take<int32_t>((size_t)P)),
         list{c.take<uint4>((size_t)f8_list_places(P, E)), c.take<uint4>((size_t)f8_list_places(P, E)), c.take<uint4>((size_t)f8_list_places(P, E))}, sort(c.take<char>(sort_tokens_bytes(T, k, E))),
         x(c, T, H), dout(c, grad ? T : 0, H), g(c.take<float>(float_rows(P, E, grad) * I)), u(c.take<float>(float_rows(P, E, grad) * I)), dh(c.take<float>(grad ? (size_t)P * I : 0)),
-        h(c, P, I, grad ? 2 : 1), y(c.take<uint16_t>((size_t)P * H)), bytes(c.off + 256) {}
+        h(c, P, I, grad ? 2 : 1), y(c.take<char>(y_bytes(P, H, E))), y_scales(c.take<float>((size_t)P * ((H + 63) / 64))), bytes(c.off + 256) {}
+  static size_t y_bytes(int64_t P, int H, int E) {
+    const size_t halves = (size_t)P * H * 2, floats = (size_t)(P < (int64_t)16 * E ? P : (int64_t)16 * E) * H * 4;  // (few rows an expert: floats)
+    return halves > floats ? halves : floats;
+  }
   static size_t float_rows(int64_t P, int E, bool grad) { return (size_t)(grad || P <= (int64_t)16 * E ? P : (int64_t)16 * E); }  // (never less for more tokens)
 };
 
@@ -270,7 +275,8 @@ int mi_moe_switch_glu_f8(const void *x, const uint32_t *topk_idx, const void *to
     p.y = ws.g;
     p.y1 = ws.u;
   } else {
-    p.dt = dtype;
+    // (results of float16 would show what the f8 instructions lose of gate and up, in the codes that it changes)
+    p.dt = dtype == MI_MOE_DTYPE_F16 ? MI_MOE_DTYPE_F32 : dtype;
     p.h = ws.h.codes;
     p.hs = ws.h.scales;
   }
@@ -283,7 +289,10 @@ int mi_moe_switch_glu_f8(const void *x, const uint32_t *topk_idx, const void *to
   d.N = hidden;
   d.K = intermediate;
   d.y = ws.y;
+  d.list = ws.list[1];
   d.dt = dtype;
+  if (f8_few_rows(d)) d.dt = MI_MOE_DTYPE_F32;
+  else d.y_scales = ws.y_scales;
   F8Lists lists;
   lists.offsets = ws.offsets;
   lists.n_mats = n_experts;
@@ -304,7 +313,7 @@ int mi_moe_switch_glu_f8(const void *x, const uint32_t *topk_idx, const void *to
   MI_HIP(launch_f8_product(p, st));
   if (few && !in_blocks) MI_HIP(launch_swiglu_f8(ws.g, ws.u, P, intermediate, ws.h.out(P, intermediate), st));
   MI_HIP(launch_f8_product(d, st));
-  MI_HIP(launch_unsort_tokens(ws.y, topk_w, w_dtype, ws.inverse, T, top_k, hidden, dtype, out, st));
+  MI_HIP(launch_unsort_made(ws.y, d.y_scales, topk_w, w_dtype, ws.inverse, T, top_k, hidden, dtype, out, st));
   return 0;
 } MI_CATCH("switch_glu_f8")
 
@@ -352,6 +361,7 @@ int mi_moe_switch_glu_f8_grad(const void *dout, const void *x, const uint32_t *t
   d.N = hidden;
   d.K = intermediate;
   d.y = ws.y;
+  d.y_scales = ws.y_scales;
   d.dt = dtype;
   // three lists, the forward products' beside the rounding of x, the others' beside that of dout
   F8Lists lists, back;
@@ -367,7 +377,7 @@ int mi_moe_switch_glu_f8_grad(const void *dout, const void *x, const uint32_t *t
   MI_HIP(launch_f8_product(b, st));
   MI_HIP(launch_swiglu_f8_grad({ws.g, ws.u, ws.dh, topk_w, w_dtype, ws.order, ws.offsets, n_experts, P, intermediate, ws.h.codes, ws.h.scales, dweights}, st));
   MI_HIP(launch_f8_product(d, st));
-  MI_HIP(launch_unsort_tokens(ws.y, nullptr, 0, ws.inverse, T, top_k, hidden, dtype, dx, st));
+  MI_HIP(launch_unsort_made(ws.y, ws.y_scales, nullptr, 0, ws.inverse, T, top_k, hidden, dtype, dx, st));
   return 0;
 } MI_CATCH("switch_glu_f8_grad")
 

@@ -46,6 +46,8 @@ struct F8Product {
   const void *bias;
   void *y, *y1;
   int dt;
+  float *y_scales;  // tiles: y is float16 whatever dt, a row's values of 64 columns times a power of two of their own, [columns / 64][rows].  Rows that are summed over
+                    // slots afterwards: rounded to bfloat16 here and once more behind the sum, the experts' results were 1.5 times as far off as with one rounding.
   float *parts;  // one matrix: room for the sums of blocks that share a tile's summed axis (f8_parts_bytes), or nullptr
   uint8_t *h;  // gate/up pairs: silu(gate) * up in e4m3, as F8Rows
   float *hs;
@@ -126,7 +128,9 @@ constexpr int64_t kSortSmall = 2048;  // pairs up to which one launch sorts, and
 // rows != nullptr: the sorted rows of x, those that no slot names zeros
 // lists (up to kSortSmall pairs): made beside it
 hipError_t launch_sort_tokens(const SortTokens &a, const void *x, int dt, int H, void *rows, void *scratch, hipStream_t st, const F8Lists &lists = F8Lists());
-// weights nullptr: sums without weights (the sorting's gradient)
+// weights nullptr: sums without weights (the sorting's gradient).  out of type dt; rows of type dt, or scaled float16 (y_scales), or float32 for fewer bits of dt
+hipError_t launch_unsort_made(const void *rows, const float *y_scales, const void *weights, int w_dtype, const int32_t *inverse, int64_t T, int k, int H, int dt, void *out,
+                              hipStream_t st);
 hipError_t launch_unsort_tokens(const void *rows, const void *weights, int w_dtype, const int32_t *inverse, int64_t T, int k, int H, int dt, void *out,
                                 hipStream_t st);
 hipError_t launch_unsort_tokens_grad(const void *dout, const void *rows, const void *weights, int w_dtype, const int32_t *inverse, int64_t T, int k, int H, int dt,

@@ -102,7 +102,7 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, F8Gri
   const int N = a.N, K = a.K, runs = f8_runs(K), n_blocks = f8_runs(N), steps = a.pair_sum ? 2 * runs : runs;
   const int begin = (int)blockIdx.y * g.part_steps, end = begin + g.part_steps < steps ? begin + g.part_steps : steps;
   const int n0 = nt * (MODE == kPair ? 128 : kF8TileN);
-  if (mat == a.n_mats) {  // rows of no matrix
+  if (mat == a.n_mats) {  // rows of no matrix (scaled ones are read by nobody)
     if constexpr (MODE != kPair) {
       const float none[4] = {0.f, 0.f, 0.f, 0.f};
       for (int i = threadIdx.x; i < rows * (kF8TileN / 4); i += kF8Threads) {
@@ -370,6 +370,28 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, F8Gri
   } else {
     constexpr int SIZE = F32 ? 4 : 2, EACH = 16 / SIZE, PASSES = F32 ? 2 : 1;  // bytes of a value, values of a piece; 64 weight rows at once, or 32
     unsigned char *const own = lds + wave * (32 * MT * 128);
+    float down[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) down[t] = 1.f;
+    if constexpr (!F32) {
+      if (a.y_scales) {
+        // to within 2^15, by the exponent of the largest of a row's 64 values
+        const int column = n0 / 64 + wn;
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          uint32_t m = 0;
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) m = umax(m, abs_bits(acc[t][i][v]));
+          m = umax(m, (uint32_t)__shfl_xor((int)m, 32, kWave));
+          const int r = (2 * t + wm) * 32 + ln, exponent = (int)(m >> 23);
+          const int by = m >= 0x7f800000u ? 0 : exponent < 27 ? -114 : exponent - 141;  // (infinities and NaN as they are; the least values a little less exactly)
+          down[t] = __uint_as_float((uint32_t)(127 - by) << 23);
+          if (half == 0 && r < rows && column * 64 < N) a.y_scales[(int64_t)column * a.rows + row0 + r] = __uint_as_float((uint32_t)(127 + by) << 23);
+        }
+      }
+    }
 #pragma unroll
     for (int pass = 0; pass < PASSES; ++pass) {
 #pragma unroll
@@ -388,11 +410,11 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, F8Gri
             const int r = t * 32 + ln;
             float o[4];
 #pragma unroll
-            for (int v = 0; v < 4; ++v) o[v] = acc[t][i][4 * g + v] + bias[v];
+            for (int v = 0; v < 4; ++v) o[v] = __builtin_fmaf(acc[t][i][4 * g + v], down[t], bias[v]);
             const int piece = F32 ? 2 * g + half : i * 4 + g;
             unsigned char *const to = own + r * 128 + (piece ^ f8_turn(r)) * 16 + (F32 ? 0 : half * 8);
             if constexpr (F32) *reinterpret_cast<f32x4_t *>(to) = f32x4_t{o[0], o[1], o[2], o[3]};
-            else if (a.dt == 0) *reinterpret_cast<uint2 *>(to) = make_uint2(cvt_pk_bf16(o[0], o[1]), cvt_pk_bf16(o[2], o[3]));
+            else if (a.dt == 0 && !a.y_scales) *reinterpret_cast<uint2 *>(to) = make_uint2(cvt_pk_bf16(o[0], o[1]), cvt_pk_bf16(o[2], o[3]));
             else *reinterpret_cast<uint2 *>(to) = make_uint2(pack_f16(o[0], o[1]), pack_f16(o[2], o[3]));
           }
         }

@@ -161,8 +161,9 @@ __device__ __forceinline__ void load_octets(Octet<DT> (&v)[N], const void *rows,
 
 // A thread eight columns of a token; its slots' rows eight at a time, all their loads in flight together.  Blocks of 256 threads: of 64, the launch of blocks is what it waits
 // for (8192 tokens of 2048 bf16 and eight slots: 80 us).
-template <int DT>
-__global__ __launch_bounds__(kSortThreads) void unsort_kernel(const void *__restrict__ rows, const void *__restrict__ weights, int w_dtype, const int32_t *__restrict__ inverse,
+// IN, DT: types of the rows and of the result.  SCALED: the rows' values are times scales[column / 64][row].
+template <int IN, int DT, bool SCALED>
+__global__ __launch_bounds__(kSortThreads) void unsort_kernel(const void *__restrict__ rows, const float *__restrict__ scales, const void *__restrict__ weights, int w_dtype, const int32_t *__restrict__ inverse,
                                                               int64_t T, int k, int H, int lanes_log2, void *__restrict__ out) {
   const int lanes = 1 << lanes_log2;
   const int64_t t = (int64_t)blockIdx.x * (kSortThreads >> lanes_log2) + (threadIdx.x >> lanes_log2);
@@ -170,7 +171,7 @@ __global__ __launch_bounds__(kSortThreads) void unsort_kernel(const void *__rest
   if (n <= 0 || t >= T) return;
   float acc[8] = {};
   for (int s0 = 0; s0 < k; s0 += 8) {
-    Octet<DT> v[8];
+    Octet<IN> v[8];
     float w[8];
     int64_t row[8];
 #pragma unroll
@@ -181,6 +182,9 @@ __global__ __launch_bounds__(kSortThreads) void unsort_kernel(const void *__rest
       w[j] = weights ? value_of(weights, s, w_dtype) : 1.f;
     }
     load_octets(v, rows, row, H, h, n);
+    if constexpr (SCALED)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] *= scales[h / 64 * (T * k) + (row[j] < 0 ? 0 : row[j])];
 #pragma unroll
     for (int j = 0; j < 8; ++j)
 #pragma unroll
@@ -192,12 +196,22 @@ __global__ __launch_bounds__(kSortThreads) void unsort_kernel(const void *__rest
   store_octet<DT>(out, t * H + h, n, o);
 }
 
-hipError_t launch_unsort_tokens(const void *rows, const void *weights, int w_dtype, const int32_t *inverse, int64_t T, int k, int H, int dt, void *out, hipStream_t st) {
+template <int IN, int DT, bool SCALED = false>
+static hipError_t launch_unsort(const void *rows, const float *scales, const void *weights, int w_dtype, const int32_t *inverse, int64_t T, int k, int H, void *out, hipStream_t st) {
   if (T == 0) return hipSuccess;
   const TokenGrid g(H, kSortThreads);
-  auto *const kernel = dt == 0 ? &unsort_kernel<0> : dt == 1 ? &unsort_kernel<1> : &unsort_kernel<2>;
-  kernel<<<dim3((unsigned)((T + g.tokens - 1) / g.tokens), (unsigned)g.columns), kSortThreads, 0, st>>>(rows, weights, w_dtype, inverse, T, k, H, __builtin_ctz((unsigned)g.lanes), out);
+  unsort_kernel<IN, DT, SCALED><<<dim3((unsigned)((T + g.tokens - 1) / g.tokens), (unsigned)g.columns), kSortThreads, 0, st>>>(rows, scales, weights, w_dtype, inverse, T, k, H,
+                                                                                                                              __builtin_ctz((unsigned)g.lanes), out);
   return hipGetLastError();
+}
+hipError_t launch_unsort_tokens(const void *rows, const void *weights, int w_dtype, const int32_t *inverse, int64_t T, int k, int H, int dt, void *out, hipStream_t st) {
+  auto *const launch = dt == 0 ? &launch_unsort<0, 0> : dt == 1 ? &launch_unsort<1, 1> : &launch_unsort<2, 2>;
+  return launch(rows, nullptr, weights, w_dtype, inverse, T, k, H, out, st);
+}
+hipError_t launch_unsort_made(const void *rows, const float *y_scales, const void *weights, int w_dtype, const int32_t *inverse, int64_t T, int k, int H, int dt, void *out,
+                              hipStream_t st) {
+  auto *const launch = y_scales ? (dt == 0 ? &launch_unsort<1, 0, true> : &launch_unsort<1, 1, true>) : dt == 0 ? &launch_unsort<2, 0> : &launch_unsort<2, 1>;
+  return launch(rows, y_scales, weights, w_dtype, inverse, T, k, H, out, st);
 }
 
 __device__ __forceinline__ float wave_sum_f32(float v) {  // in a fixed order

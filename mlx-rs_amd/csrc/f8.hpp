@@ -69,9 +69,7 @@ inline size_t f8_own_bytes(const F8Product &p) {
 }
 inline bool f8_in_blocks(const F8Product &p, int64_t most) { return f8_few_rows(p) && most * f8_runs(p.K) <= 64 && f8_own_bytes(p) <= 48 * 1024; }
 inline int64_t f8_most_pieces(int64_t rows, int n_mats, int tile) { return rows / tile + (n_mats + 1 < rows ? n_mats + 1 : rows); }
-// A list: kF8ListHead words of where the pieces of each of the eight XCDs begin (and end), then the pieces.
-constexpr int kF8ListHead = 3;  // (uint4s)
-inline int64_t f8_list_places(int64_t rows, int n_mats) { return kF8ListHead + f8_most_pieces(rows, n_mats, 16); }
+inline int64_t f8_list_places(int64_t rows, int n_mats) { return f8_most_pieces(rows, n_mats, 16); }
 // What is to be listed, beside the rounding of rows (launch_quantize_f8_rows): up to two lists.
 struct F8Lists {
   const uint32_t *offsets = nullptr;  // [n_mats + 1]
@@ -180,90 +178,55 @@ __device__ __forceinline__ uint32_t max_of_16_lanes(uint32_t m) {
   m = umax(m, dpp_u32<kDppHalfMirror>(m));
   return umax(m, dpp_u32<kDppMirror>(m));
 }
-__device__ __forceinline__ float silu(float g) { return g / (1.f + __expf(-g)); }
+// (v_rcp_f32 is within an ulp; where exp(-g) is infinite it gives zero, and g times it the limit's own)
+__device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.f + __expf(-g)); }
+__device__ __forceinline__ float silu(float g) { return g * sigmoid(g); }
 
 // ---------------------------------------------------------------- segments
-// A piece of at most `tile` rows of one matrix (n_mats: of none); rows 0: nothing.  at, of: which of its matrix's pieces it is, and how many these are.
+// A piece of at most `tile` rows of one matrix (n_mats: of none); rows 0: nothing.
 struct F8Piece {
   int mat;
-  uint32_t row, rows, at, of;
+  uint32_t row, rows;
 };
 __device__ __forceinline__ F8Piece f8_piece(const F8Product &p, uint32_t tile, uint32_t m) {
   if (!p.list) {
     const uint32_t row = m * tile, total = (uint32_t)p.rows;
-    return {0, row, row >= total ? 0u : total - row < tile ? total - row : tile, 0, 1};
+    return {0, row, row >= total ? 0u : total - row < tile ? total - row : tile};
   }
-  const uint4 v = p.list[kF8ListHead + m];
-  const uint32_t w = (uint32_t)__builtin_amdgcn_readfirstlane((int)v.w), z = (uint32_t)__builtin_amdgcn_readfirstlane((int)v.z);
-  return {__builtin_amdgcn_readfirstlane((int)v.x), (uint32_t)__builtin_amdgcn_readfirstlane((int)v.y), z & 0xffffu, z >> 16 | (w & 0xffu) << 16, w >> 8};
+  const uint4 v = p.list[m];
+  return {__builtin_amdgcn_readfirstlane((int)v.x), (uint32_t)__builtin_amdgcn_readfirstlane((int)v.y), (uint32_t)__builtin_amdgcn_readfirstlane((int)v.z)};
 }
 // The list of pieces of the segments that offsets[n_mats + 1] cut the rows into, by one wave.  A segment is cut into as few pieces of at most `tile` rows as it can be, of about one
 // size (multiples of 32 rows).  Behind the segments' pieces come those of the rows that belong to none, then empty ones.  Offsets out of order or range only make pieces
 // that overlap or are missing.
 // In the experts' order: with whole pieces first and the rest of the segments behind them, the longest first, the launch ends more evenly, but its first half multiplies and its
 // second one waits for weights (4096 tokens, skewed routing over 128 experts of 2048 x 768: down 138 us, 156 so).
-// The pieces go to the XCDs in runs of about as much time, so that a matrix's lie together, where one L2 serves the weights to all of them: a piece's time is taken as
-// that of its sub-tiles of 32 rows and of four more for its weights.
-constexpr uint32_t kPieceBase = 4, kPieceMost = kPieceBase + 8;
 __device__ __forceinline__ void f8_list(const uint32_t *__restrict__ offsets, int n_mats, uint32_t total, uint32_t tile, uint4 *__restrict__ list, uint32_t places) {
   const int lane = lane_id();
-  uint4 *const pieces_at = list + kF8ListHead;
-  auto for_segments = [&](auto f) __attribute__((always_inline)) {
-    for (int e0 = 0; e0 <= n_mats; e0 += kWave) {
-      const int e = e0 + lane;
-      uint32_t lo = 0, hi = 0;
-      if (e <= n_mats) {
-        lo = offsets[e];
-        hi = e < n_mats ? offsets[e + 1] : total;
-        lo = lo < total ? lo : total;
-        hi = hi < lo ? lo : hi < total ? hi : total;
-      }
-      const uint32_t pieces = (hi - lo + tile - 1) / tile;
-      const uint32_t even = pieces <= 1 ? tile : ((hi - lo + pieces - 1) / pieces + 31) / 32 * 32;
-      f((uint32_t)e, lo, hi, pieces, even < tile ? even : tile);
+  uint32_t before = 0;
+  for (int e0 = 0; e0 <= n_mats; e0 += kWave) {
+    const int e = e0 + lane;
+    uint32_t lo = 0, hi = 0;
+    if (e <= n_mats) {
+      lo = offsets[e];
+      hi = e < n_mats ? offsets[e + 1] : total;
+      lo = lo < total ? lo : total;
+      hi = hi < lo ? lo : hi < total ? hi : total;
     }
-  };
-  auto sum_up_to = [&](uint32_t v) __attribute__((always_inline)) {
+    const uint32_t pieces = (hi - lo + tile - 1) / tile;
+    uint32_t upto = pieces;
     for (int d = 1; d < kWave; d <<= 1) {
-      const uint32_t up = __shfl_up(v, d, kWave);
-      if (lane >= d) v += up;
+      const uint32_t up = __shfl_up(upto, d, kWave);
+      if (lane >= d) upto += up;
     }
-    return v;
-  };
-  // (a segment's pieces are of about one time)
-  auto time_of = [&](uint32_t rows, uint32_t pieces) __attribute__((always_inline)) { return pieces * kPieceBase + (rows + 31) / 32; };
-  uint32_t before = 0, time = 0;
-  for_segments([&](uint32_t e, uint32_t lo, uint32_t hi, uint32_t pieces, uint32_t size) __attribute__((always_inline)) {
-    const uint32_t upto = sum_up_to(pieces), first = before + upto - pieces;
+    const uint32_t even = pieces <= 1 ? tile : ((hi - lo + pieces - 1) / pieces + 31) / 32 * 32, size = even < tile ? even : tile, first = before + upto - pieces;
     for (uint32_t i = 0; i < pieces && first + i < places; ++i) {
       const uint32_t row = lo + i * size;
-      pieces_at[first + i] = make_uint4(e, row, (hi - row < size ? hi - row : size) | i << 16, i >> 16 | pieces << 8);
+      list[first + i] = make_uint4((uint32_t)e, row, hi - row < size ? hi - row : size, 0u);
     }
     before += (uint32_t)__builtin_amdgcn_readlane((int)upto, kWave - 1);
-    time += time_of(hi - lo, pieces);
-  });
-  const uint32_t n = before < places ? before : places;
-  for (uint32_t i = n + lane; i < places; i += kWave) pieces_at[i] = make_uint4(0, 0, 0, 0);
-  if (tile < 64) return;  // (the kernel for a few rows takes a piece a block)
-  const uint64_t whole = (uint32_t)__builtin_amdgcn_readlane((int)sum_up_to(time), kWave - 1);
-  uint32_t done = 0, start[8] = {};  // how many pieces begin ahead of each XCD's share of the time
-  for_segments([&](uint32_t, uint32_t lo, uint32_t hi, uint32_t pieces, uint32_t) __attribute__((always_inline)) {
-    const uint32_t own = time_of(hi - lo, pieces), upto = sum_up_to(own), from = done + upto - own;
-#pragma unroll
-    for (uint32_t k = 1; k < 8; ++k) {
-      const uint32_t line = (uint32_t)(whole * k / 8);
-      const uint64_t ahead = pieces && line > from ? ((uint64_t)(line - from) * pieces + own - 1) / own : 0u;
-      start[k] += ahead < pieces ? (uint32_t)ahead : pieces;
-    }
-    done += (uint32_t)__builtin_amdgcn_readlane((int)upto, kWave - 1);
-  });
-  uint32_t mine = lane == 8 ? n : 0u;
-#pragma unroll
-  for (uint32_t k = 1; k < 8; ++k) {
-    const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)sum_up_to(start[k]), kWave - 1);
-    if ((uint32_t)lane == k) mine = all < n ? all : n;
   }
-  if (lane <= 8) reinterpret_cast<uint32_t *>(list)[lane] = mine;
+  for (uint32_t i = before + lane; i < places; i += kWave) list[i] = make_uint4(0, 0, 0, 0);
 }
 
 // ---------------------------------------------------------------- products

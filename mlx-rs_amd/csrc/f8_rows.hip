@@ -206,7 +206,7 @@ __global__ __launch_bounds__(kRowThreads) void swiglu_f8_grad_kernel(F8SwigluGra
       const Octet<2> g = load_octet<2>(a.g, row * a.cols + k, n), u = load_octet<2>(a.u, row * a.cols + k, n), dh = load_octet<2>(a.dh, row * a.cols + k, n);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float s = 1.f / (1.f + __expf(-g.v[i])), gs = g.v[i] * s, d = w * dh.v[i];
+        const float s = sigmoid(g.v[i]), gs = g.v[i] * s, d = w * dh.v[i];
         dw += dh.v[i] * (gs * u.v[i]);
         dg[i] = d * u.v[i] * s * (1.f + g.v[i] * (1.f - s));
         du[i] = d * gs;

@@ -75,32 +75,26 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, F8Gri
   constexpr int XC = TM / 64, MT = TM / 64;  // copies of token rows a wave; sub-tiles of 32 token rows a wave
   extern __shared__ __align__(16) unsigned char lds[];
   const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)lds;
-  const int lane = threadIdx.x & 63, ln = lane & 31, half = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 2, wn = wave & 3;
-  // Blocks go round the eight XCDs, each of which has an L2 of its own.  One matrix: an XCD takes a rectangle of tiles.  Several: it takes a run of pieces (f8_list), those
-  // of a matrix beside each other for each 256 of its rows.
+  const int N = a.N, K = a.K, runs = f8_runs(K), n_blocks = f8_runs(N), steps = a.pair_sum ? 2 * runs : runs;
+  const int begin = (int)blockIdx.y * g.part_steps, end = begin + g.part_steps < steps ? begin + g.part_steps : steps;
+  // Blocks go round the eight XCDs, each of which has an L2 of its own.  One matrix: an XCD takes a rectangle of tiles.  Several: all tiles of a piece go to one XCD.  (A matrix's
+  // pieces beside each other on one XCD, and blocks that take tile after tile, were tried: fewer misses of L2, and no faster, or slower by what the shares differ in time.)
   const uint32_t xcd = blockIdx.x & 7, q = blockIdx.x >> 3;
   uint32_t mt, nt;
-  F8Piece piece;
   if (!a.list) {
     mt = (xcd % (uint32_t)g.xcds_m) * (uint32_t)g.m_each + q % (uint32_t)g.m_each;
     nt = (xcd / (uint32_t)g.xcds_m) * (uint32_t)g.n_each + q / (uint32_t)g.m_each;
-    if (mt >= (uint32_t)g.m_tiles || nt >= (uint32_t)g.n_tiles) return;
-    piece = f8_piece(a, TM, mt);
   } else {
-    const uint32_t *const start = reinterpret_cast<const uint32_t *>(a.list) + xcd;
-    const uint32_t tiles = (uint32_t)g.n_tiles, s = start[0] * tiles + q;
-    if (s >= start[1] * tiles) return;
-    piece = f8_piece(a, TM, s / tiles);
-    const uint32_t first = s / tiles - piece.at, in = s - first * tiles;
-    nt = in / piece.of;
-    if (piece.of > 1) piece = f8_piece(a, TM, first + in % piece.of);
+    mt = q / (uint32_t)g.n_tiles * 8 + xcd;
+    nt = q % (uint32_t)g.n_tiles;
   }
+  if (mt >= (uint32_t)g.m_tiles || nt >= (uint32_t)g.n_tiles) return;
+  const F8Piece piece = f8_piece(a, TM, mt);
   const int rows = (int)piece.rows, mat = piece.mat;
   const uint32_t row0 = piece.row;
   if (rows == 0) return;
-  const int N = a.N, K = a.K, runs = f8_runs(K), n_blocks = f8_runs(N), steps = a.pair_sum ? 2 * runs : runs;
-  const int begin = (int)blockIdx.y * g.part_steps, end = begin + g.part_steps < steps ? begin + g.part_steps : steps;
+  const int lane = threadIdx.x & 63, ln = lane & 31, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 2, wn = wave & 3;
   const int n0 = nt * (MODE == kPair ? 128 : kF8TileN);
   if (mat == a.n_mats) {  // rows of no matrix (scaled ones are read by nobody)
     if constexpr (MODE != kPair) {
@@ -150,11 +144,11 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, F8Gri
   };
   auto offsets = [&]() __attribute__((always_inline)) {
     Offsets o;
-    uint32_t thread = threadIdx.x;
-    asm volatile("" : "+v"(thread));  // (addresses are made where they are used: there are no registers to keep them)
+    uint32_t own = threadIdx.x;
+    asm volatile("" : "+v"(own));  // (addresses are made where they are used: there are no registers to keep them)
 #pragma unroll
-    for (int c = 0; c < XC; ++c) o.x[c] = x_offs[thread * XC + c];
-    o.s = s_offs[wave % (TM / 64) * 64 + thread % 64];
+    for (int c = 0; c < XC; ++c) o.x[c] = x_offs[own * XC + c];
+    o.s = s_offs[wave % (TM / 64) * 64 + own % 64];
     return o;
   };
   auto fetch_rows = [&](int j, const Offsets &o) __attribute__((always_inline)) {
@@ -325,28 +319,32 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, F8Gri
     float *const most = reinterpret_cast<float *>(lds + TM * 128);  // [4][TM]
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-      uint32_t m = 0;
+      if (t < live) {
+        uint32_t m = 0;
 #pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        acc[t][0][v] = silu(acc[t][0][v]) * acc[t][1][v];
-        m = umax(m, abs_bits(acc[t][0][v]));
+        for (int v = 0; v < 16; ++v) {
+          acc[t][0][v] = silu(acc[t][0][v]) * acc[t][1][v];
+          m = umax(m, abs_bits(acc[t][0][v]));
+        }
+        m = umax(m, (uint32_t)__shfl_xor((int)m, 32, kWave));
+        if (half == 0) most[wn * TM + (2 * t + wm) * 32 + ln] = __uint_as_float(m);
       }
-      m = umax(m, (uint32_t)__shfl_xor((int)m, 32, kWave));
-      if (half == 0) most[wn * TM + (2 * t + wm) * 32 + ln] = __uint_as_float(m);
     }
     __syncthreads();
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-      const int r = (2 * t + wm) * 32 + ln;
-      uint32_t all = 0;
+      if (t < live) {
+        const int r = (2 * t + wm) * 32 + ln;
+        uint32_t all = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) all = umax(all, __float_as_uint(most[i * TM + r]));
-      const F8Scale s(all);
+        for (int i = 0; i < 4; ++i) all = umax(all, __float_as_uint(most[i * TM + r]));
+        const F8Scale s(all);
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<uint32_t *>(lds + r * 128 + ((wn * 2 + (g >> 1)) ^ f8_turn(r)) * 16 + (g & 1) * 8 + half * 4) =
-            s.codes(acc[t][0][4 * g], acc[t][0][4 * g + 1], acc[t][0][4 * g + 2], acc[t][0][4 * g + 3]);
-      if (wn == 0 && half == 0 && r < rows) a.hs[(int64_t)nt * a.rows + row0 + r] = s.scale;
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<uint32_t *>(lds + r * 128 + ((wn * 2 + (g >> 1)) ^ f8_turn(r)) * 16 + (g & 1) * 8 + half * 4) =
+              s.codes(acc[t][0][4 * g], acc[t][0][4 * g + 1], acc[t][0][4 * g + 2], acc[t][0][4 * g + 3]);
+        if (wn == 0 && half == 0 && r < rows) a.hs[(int64_t)nt * a.rows + row0 + r] = s.scale;
+      }
     }
     __syncthreads();
     const int64_t h_wide = (int64_t)n_blocks * kF8Run;
@@ -379,14 +377,24 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, F8Gri
         const int column = n0 / 64 + wn;
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
-          uint32_t m = 0;
+          if (t >= live) continue;
+          float most = 0.f;  // (of the numbers among them)
 #pragma unroll
           for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int v = 0; v < 16; ++v) m = umax(m, abs_bits(acc[t][i][v]));
-          m = umax(m, (uint32_t)__shfl_xor((int)m, 32, kWave));
-          const int r = (2 * t + wm) * 32 + ln, exponent = (int)(m >> 23);
-          const int by = m >= 0x7f800000u ? 0 : exponent < 27 ? -114 : exponent - 141;  // (infinities and NaN as they are; the least values a little less exactly)
+            for (int v = 0; v < 16; ++v) most = fmaxf(most, fabsf(acc[t][i][v]));
+          most = fmaxf(most, __shfl_xor(most, 32, kWave));
+          if (most == __builtin_inff()) {  // (rare: the scale is that of the finite ones)
+            most = 0.f;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int v = 0; v < 16; ++v)
+                if (const float one = fabsf(acc[t][i][v]); one < __builtin_inff()) most = fmaxf(most, one);
+            most = fmaxf(most, __shfl_xor(most, 32, kWave));
+          }
+          const int r = (2 * t + wm) * 32 + ln, exponent = (int)(__float_as_uint(most) >> 23);
+          const int by = exponent < 27 ? -114 : exponent - 141;  // (the least values a little less exactly)
           down[t] = __uint_as_float((uint32_t)(127 - by) << 23);
           if (half == 0 && r < rows && column * 64 < N) a.y_scales[(int64_t)column * a.rows + row0 + r] = __uint_as_float((uint32_t)(127 + by) << 23);
         }
@@ -407,6 +415,7 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, F8Gri
             }
 #pragma unroll
           for (int t = 0; t < MT; ++t) {
+            if (t >= live) continue;
             const int r = t * 32 + ln;
             float o[4];
 #pragma unroll
@@ -420,6 +429,7 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, F8Gri
         }
 #pragma unroll
       for (int r0 = 0; r0 < 32 * MT; r0 += 8) {
+        if (r0 >= 32 * live) continue;
         const int r = r0 + lane / 8, n = n0 + wn * 64 + pass * 32 + ((lane % 8) ^ f8_turn(r)) * EACH;
         const u32x4_f8 v = *reinterpret_cast<const u32x4_f8 *>(own + r * 128 + lane % 8 * 16);
         const int row = (r0 / 32 * 2 + wm) * 32 + r % 32;
@@ -471,13 +481,12 @@ static hipError_t launch_tiles(const F8Product &p, hipStream_t st) {
     if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&f8_tiles_kernel<TM, MODE, F32>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds); e != hipSuccess) return e;
     if (dev >= 0 && dev < kMaxDevices) raised[dev].store(true, std::memory_order_release);
   }
-  const int64_t n_tiles = (p.N + (MODE == kPair ? 127 : kF8TileN - 1)) / (MODE == kPair ? 128 : kF8TileN), m_tiles = p.list ? 0 : (p.rows + TM - 1) / TM;
+  const int64_t n_tiles = (p.N + (MODE == kPair ? 127 : kF8TileN - 1)) / (MODE == kPair ? 128 : kF8TileN), m_tiles = p.list ? f8_most_pieces(p.rows, p.n_mats, TM) : (p.rows + TM - 1) / TM;
   const int steps = f8_runs(p.K) * (p.pair_sum ? 2 : 1), parts = p.list ? 1 : f8_dense_plan(p).parts;
   F8Grid g{(int)m_tiles, (int)n_tiles, 1, (int)m_tiles, (int)((n_tiles + 7) / 8), (steps + parts - 1) / parts};
   int64_t each;  // blocks of an XCD
   if (p.list) {
-    // (runs of one time hold up to kPieceMost / kPieceBase of their share of the pieces)
-    each = ((f8_most_pieces(p.rows, p.n_mats, TM) * kPieceMost + kPieceBase * 8 - 1) / (kPieceBase * 8) + 1) * n_tiles;
+    each = (m_tiles + 7) / 8 * n_tiles;
   } else {
     for (int xm = 2; xm <= 8; xm *= 2) {
       const int m_each = (int)((m_tiles + xm - 1) / xm), n_each = (int)((n_tiles + 8 / xm - 1) / (8 / xm));

@@ -312,6 +312,24 @@ def test_few_tokens_all_at_one_expert(T, k, H):
     o.within(ops.switch_glu_f8(x, inds, w, gate, up, down), want, off)
 
 
+@pytest.mark.parametrize("T", [3, 300])
+def test_a_result_past_float32_leaves_those_beside_it(T):
+    """Down's product is infinite in one column and near the end of float32 in the others.  h is 128 equal values, all codes 448, and every product of a power of two: what is
+    left are silu(16) * 16 = 256 (1 - 2^-23), the roundings of the scales (2^-24 each), of a result held in 11 bits and of the sum to bfloat16."""
+    from mlx_rs_amd import ops
+    codes = torch.ones((2, 128, 128), device="cuda")
+    flat = (codes.to(o.F8), torch.full((2, 1, 1), 0.125, device="cuda"))
+    codes[:, 5] = 448.0
+    codes[:, 6] = -448.0
+    down = (codes.to(o.F8), torch.full((2, 1, 1), 2.0 ** 105, device="cuda"))
+    x = torch.ones((T, 128), device="cuda", dtype=torch.bfloat16)
+    inds = torch.tensor([0, 1], device="cuda", dtype=torch.int32).expand(T, 2).contiguous()
+    y = ops.switch_glu_f8(x, inds, torch.full((T, 2), 0.25, device="cuda"), flat, flat, down).double()
+    assert (y[:, 5] == float("inf")).all() and (y[:, 6] == -float("inf")).all()
+    rest = torch.cat((y[:, :5], y[:, 7:]), 1) * 2.0 ** -119
+    assert (rest - 1.0).abs().max() <= 2.0 ** -8 + 2.0 ** -11 + 2.0 ** -20
+
+
 @pytest.mark.parametrize("T", [3, 200])
 def test_experts_by_differences(T):
     """dweights is the change of sum(out * dout) with a weight, in the forward's own numbers but for their roundings: out is linear in the weights."""

@@ -158,8 +158,12 @@ int f8_tile_rows(const F8Product &p) {
   const int64_t mats = p.list ? p.n_mats : 1, avg = p.rows / mats;
   // One matrix: 4096 x 4096, 16 / 32 / 48 / 64 rows in pieces of 32 take 10 / 12 / 16 / 17 us.
   if (p.transpose && !p.h && !p.pair_sum && p.rows <= (p.list ? 16 * mats : 48)) return avg > 4 ? 32 : 16;
-  if (p.dt == 2) return avg > 128 ? 128 : 64;
-  return avg > 192 ? 256 : avg > 64 ? 128 : 64;
+  // Tiles of 64 / 128 rows to float32, us: 16 matrices of 1792 x 2048 at 56, 72, 100, 160 rows each 29 / 31, 31 / 37, 45 / 39, 51 / 42; 128 of 768 x 2048 72 / 77, 94 / 87, 127 / 99,
+  // 171 / 142.  To bfloat16, of 64 / 128 / 256 rows: the 128 at 40, 72, 100, 128, 200 rows 50 / 51 / 53, 81 / 63 / 67, 105 / 73 / 79, 117 / 96 / 90, 168 / 133 / 107; the 16, which have
+  // fewer tiles than there are CUs, at 56, 100, 200, 260 rows 24 / 24 / 26, 41 / 26 / 29, 48 / 32 / 41, 54 / 50 / 43.
+  if (p.dt == 2) return avg > 64 ? 128 : 64;
+  const int64_t tiles = (p.N + (p.h ? 127 : 255)) / (p.h ? 128 : 256) * mats;
+  return avg > (tiles >= 256 ? 112 : 208) ? 256 : avg > 48 ? 128 : 64;
 }
 
 hipError_t launch_f8_few(const F8Product &p, hipStream_t st) {

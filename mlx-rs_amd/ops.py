@@ -783,7 +783,7 @@ def linear_f8(x, w, scales, linear_bias=None, transpose=True):
 
 def grouped_linear_f8(rows, w, scales, offsets, transpose=True):
     """linear_f8 for rows sorted by expert (``sort_tokens``): rows from offsets[e] to offsets[e + 1] with matrix e.  rows: [R, K] in bfloat16, float16 or float32; w: float8_e4m3fn
-    [E, N, K], scales: float32 [E, ceil(N / 128), ceil(K / 128)]; offsets: int32 [E + 1].  Returns [R, N]; rows behind the last expert's are zeros.
+    [E, N, K], scales: float32 [E, ceil(N / 128), ceil(K / 128)]; offsets: int32 [E + 1], ascending from 0.  Returns [R, N]; rows behind the last expert's are zeros.
     transpose = False: the gradient with respect to the rows, [R, N] to [R, K]."""
     out = _native("grouped_linear_f8", rows, w, scales, offsets, transpose)
     if out is not None:

@@ -96,12 +96,14 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, F8Gri
   const int lane = threadIdx.x & 63, ln = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 2, wn = wave & 3;
   const int n0 = nt * (MODE == kPair ? 128 : kF8TileN);
+  const int product = MODE == kRowsOfWeights ? (int)blockIdx.z : 0;  // (two at most, of the same rows)
+  void *const y = product ? a.y1 : a.y;
   if (mat == a.n_mats) {  // rows of no matrix (scaled ones are read by nobody)
     if constexpr (MODE != kPair) {
       const float none[4] = {0.f, 0.f, 0.f, 0.f};
       for (int i = threadIdx.x; i < rows * (kF8TileN / 4); i += kF8Threads) {
         const int n = n0 + i % (kF8TileN / 4) * 4;
-        if (n < N) store4(a.y, (int64_t)(row0 + i / (kF8TileN / 4)) * N + n, N - n, a.dt, none);
+        if (n < N) store4(y, (int64_t)(row0 + i / (kF8TileN / 4)) * N + n, N - n, a.dt, none);
       }
     }
     return;
@@ -126,7 +128,7 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, F8Gri
   const int64_t matrix = (int64_t)mat * N * K;
   i32x4_t wr{};
   if constexpr (MODE != kColsOfWeights) {
-    const int which = MODE == kPair ? wave >> 2 : 0;  // waves 4 to 7 copy the up rows
+    const int which = MODE == kPair ? wave >> 2 : product;  // waves 4 to 7 copy the up rows
     wr = uniform(words_of(a.m[which].w + matrix + (int64_t)n0 * K, at_most_4g((int64_t)(N - n0) * K)));
   }
   // where the scales of the wave's half of the weight rows are (past the last block its own again, of rows that are never stored)
@@ -135,7 +137,7 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, F8Gri
     const int second = wave & 1, block = MODE == kPair ? nt : n0 / kF8Run + second < n_blocks ? n0 / kF8Run + second : n_blocks - 1;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      w_scale[i] = MODE == kPair ? a.m[second].s + ((int64_t)mat * n_blocks + block) * runs : MODE == kRowsOfWeights ? a.m[0].s + ((int64_t)mat * n_blocks + block) * runs
+      w_scale[i] = MODE == kPair ? a.m[second].s + ((int64_t)mat * n_blocks + block) * runs : MODE == kRowsOfWeights ? a.m[product].s + ((int64_t)mat * n_blocks + block) * runs
                                                                                                                      : a.m[i].s + (int64_t)mat * runs * n_blocks + block;
   }
   // Token rows and all scales, XC + 2 copies.  (Every wave copies scales, several the same: with a branch around them the compiler puts the sums' arithmetic off past it.)
@@ -434,7 +436,7 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, F8Gri
         const u32x4_f8 v = *reinterpret_cast<const u32x4_f8 *>(own + r * 128 + lane % 8 * 16);
         const int row = (r0 / 32 * 2 + wm) * 32 + r % 32;
         if (row < rows && n < N) {
-          unsigned char *const to = static_cast<unsigned char *>(a.y) + ((int64_t)(row0 + row) * N + n) * SIZE;
+          unsigned char *const to = static_cast<unsigned char *>(y) + ((int64_t)(row0 + row) * N + n) * SIZE;
           if (n + EACH <= N) {
             __builtin_memcpy(to, &v, 16);
           } else {
@@ -497,7 +499,7 @@ static hipError_t launch_tiles(const F8Product &p, hipStream_t st) {
   }
   if (each > (int64_t)1 << 19) return hipErrorInvalidValue;  // (a launch has less than 2^32 threads)
   const unsigned used = (unsigned)((steps + g.part_steps - 1) / g.part_steps);
-  f8_tiles_kernel<TM, MODE, F32><<<dim3((unsigned)(each * 8), used), kF8Threads, lds, st>>>(p, g);
+  f8_tiles_kernel<TM, MODE, F32><<<dim3((unsigned)(each * 8), used, p.y1 ? 2 : 1), kF8Threads, lds, st>>>(p, g);
   if (used > 1) f8_parts_kernel<<<dim3((unsigned)((p.N + 1023) / 1024), (unsigned)p.rows), 256, 0, st>>>(p.parts, (int)used, p.rows, p.N, p.bias, p.dt, p.y);
   return hipGetLastError();
 }
@@ -513,14 +515,6 @@ hipError_t launch_f8_tiles(const F8Product &p, hipStream_t st) {
   if (p.rows == 0) return hipSuccess;
   if (p.h) return launch_mode<kPair>(p, st);
   if (!p.transpose) return launch_mode<kColsOfWeights>(p, st);
-  if (p.y1) {  // two products: one after the other
-    F8Product q = p;
-    q.y1 = nullptr;
-    if (hipError_t e = launch_mode<kRowsOfWeights>(q, st); e != hipSuccess) return e;
-    q.m[0] = p.m[1];
-    q.y = p.y1;
-    return launch_mode<kRowsOfWeights>(q, st);
-  }
   return launch_mode<kRowsOfWeights>(p, st);
 }
 

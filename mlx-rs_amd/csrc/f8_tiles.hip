@@ -398,7 +398,7 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, F8Gri
           const int r = (2 * t + wm) * 32 + ln, exponent = (int)(__float_as_uint(most) >> 23);
           const int by = exponent < 27 ? -114 : exponent - 141;  // (the least values a little less exactly)
           down[t] = __uint_as_float((uint32_t)(127 - by) << 23);
-          if (half == 0 && r < rows && column * 64 < N) a.y_scales[(int64_t)column * a.rows + row0 + r] = __uint_as_float((uint32_t)(127 + by) << 23);
+          if (half == 0 && r < rows && column * 64 < N) a.y_scales[(int64_t)(row0 + r) * ((N + 63) / 64) + column] = __uint_as_float((uint32_t)(127 + by) << 23);
         }
       }
     }

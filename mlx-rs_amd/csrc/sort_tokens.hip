@@ -161,7 +161,7 @@ __device__ __forceinline__ void load_octets(Octet<DT> (&v)[N], const void *rows,
 
 // A thread eight columns of a token; its slots' rows eight at a time, all their loads in flight together.  Blocks of 256 threads: of 64, the launch of blocks is what it waits
 // for (8192 tokens of 2048 bf16 and eight slots: 80 us).
-// IN, DT: types of the rows and of the result.  SCALED: the rows' values are times scales[column / 64][row].
+// IN, DT: types of the rows and of the result.  SCALED: the rows' values are times scales[row][column / 64].
 template <int IN, int DT, bool SCALED>
 __global__ __launch_bounds__(kSortThreads) void unsort_kernel(const void *__restrict__ rows, const float *__restrict__ scales, const void *__restrict__ weights, int w_dtype, const int32_t *__restrict__ inverse,
                                                               int64_t T, int k, int H, int lanes_log2, void *__restrict__ out) {
@@ -184,7 +184,7 @@ __global__ __launch_bounds__(kSortThreads) void unsort_kernel(const void *__rest
     load_octets(v, rows, row, H, h, n);
     if constexpr (SCALED)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] *= scales[h / 64 * (T * k) + (row[j] < 0 ? 0 : row[j])];
+      for (int j = 0; j < 8; ++j) w[j] *= scales[(row[j] < 0 ? 0 : row[j]) * ((H + 63) / 64) + h / 64];
 #pragma unroll
     for (int j = 0; j < 8; ++j)
 #pragma unroll

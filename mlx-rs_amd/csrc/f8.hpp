@@ -36,6 +36,7 @@ struct F8Product {
   int raw_dt;
   const uint32_t *order;    // sorted row r reads x row order[r] / k_div; nullptr: r
   int k_div;
+  const uint32_t *ids;      // instead of order and list, for a few rows: row r is of x row r / k_div and matrix ids[r] (none, if there is no such one), a piece of its own
   const uint4 *list;        // the pieces of at most f8_tile_rows rows that the matrices' rows are cut into, and rows of no matrix, which are zeros of y (f8_list).  nullptr: one
   int n_mats;               // matrix, all rows
   int64_t rows;             // of y
@@ -128,7 +129,13 @@ constexpr int64_t kSortSmall = 2048;  // pairs up to which one launch sorts, and
 // lists (up to kSortSmall pairs): made beside it
 hipError_t launch_sort_tokens(const SortTokens &a, const void *x, int dt, int H, void *rows, void *scratch, hipStream_t st, const F8Lists &lists = F8Lists());
 // weights nullptr: sums without weights (the sorting's gradient).  out of type dt; rows of type dt, or scaled float16 (y_scales), or float32 for fewer bits of dt
-hipError_t launch_unsort_made(const void *rows, const float *y_scales, const void *weights, int w_dtype, const int32_t *inverse, int64_t T, int k, int H, int dt, void *out,
+// Places: a slot's row is inverse[slot], or, inverse nullptr, the slot's own if ids names one of E experts there.
+struct Places {
+  const int32_t *inverse;
+  const uint32_t *ids = nullptr;
+  int E = 0;
+};
+hipError_t launch_unsort_made(const void *rows, const float *y_scales, const void *weights, int w_dtype, const Places &places, int64_t T, int k, int H, int dt, void *out,
                               hipStream_t st);
 hipError_t launch_unsort_tokens(const void *rows, const void *weights, int w_dtype, const int32_t *inverse, int64_t T, int k, int H, int dt, void *out,
                                 hipStream_t st);
@@ -190,6 +197,10 @@ struct F8Piece {
   uint32_t row, rows;
 };
 __device__ __forceinline__ F8Piece f8_piece(const F8Product &p, uint32_t tile, uint32_t m) {
+  if (p.ids) {
+    const uint32_t e = p.ids[m];
+    return {__builtin_amdgcn_readfirstlane((int)(e < (uint32_t)p.n_mats ? e : (uint32_t)p.n_mats)), m, 1u};
+  }
   if (!p.list) {
     const uint32_t row = m * tile, total = (uint32_t)p.rows;
     return {0, row, row >= total ? 0u : total - row < tile ? total - row : tile};

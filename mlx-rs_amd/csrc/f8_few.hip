@@ -37,7 +37,7 @@ __global__ __launch_bounds__(kFewWaves *kWave) void f8_few_kernel(F8Product a) {
   const uint8_t *const w = m.w + (int64_t)piece.mat * a.N * a.K + (int64_t)(n0 + ln < a.N ? n0 + ln : a.N - 1) * a.K;
   const float *const ws = m.s + ((int64_t)piece.mat * f8_runs(a.N) + n0 / kF8Run) * runs;
   auto source = [&](uint32_t r) __attribute__((always_inline)) {
-    const int64_t at = a.order ? a.order[r] / (uint32_t)a.k_div : r;
+    const int64_t at = a.order ? a.order[r] / (uint32_t)a.k_div : a.ids ? r / (uint32_t)a.k_div : r;
     return at < a.x.rows ? at : 0;  // (never followed out of the rows)
   };
   u32x4_f8 wv[AHEAD][2];
@@ -155,9 +155,9 @@ __global__ __launch_bounds__(kFewWaves *kWave) void f8_few_kernel(F8Product a) {
 }
 
 int f8_tile_rows(const F8Product &p) {
-  const int64_t mats = p.list ? p.n_mats : 1, avg = p.rows / mats;
+  const int64_t mats = p.list || p.ids ? p.n_mats : 1, avg = p.rows / mats;
   // One matrix: 4096 x 4096, 16 / 32 / 48 / 64 rows in pieces of 32 take 10 / 12 / 16 / 17 us.
-  if (p.transpose && !p.h && !p.pair_sum && p.rows <= (p.list ? 16 * mats : 48)) return avg > 4 ? 32 : 16;
+  if (p.transpose && !p.h && !p.pair_sum && p.rows <= (p.list || p.ids ? 16 * mats : 48)) return avg > 4 ? 32 : 16;
   // Tiles of 64 / 128 rows to float32, us: 16 matrices of 1792 x 2048 at 56, 72, 100, 160 rows each 29 / 31, 31 / 37, 45 / 39, 51 / 42; 128 of 768 x 2048 72 / 77, 94 / 87, 127 / 99,
   // 171 / 142.  To bfloat16, of 64 / 128 / 256 rows: the 128 at 40, 72, 100, 128, 200 rows 50 / 51 / 53, 81 / 63 / 67, 105 / 73 / 79, 117 / 96 / 90, 168 / 133 / 107; the 16, which have
   // fewer tiles than there are CUs, at 56, 100, 200, 260 rows 24 / 24 / 26, 41 / 26 / 29, 48 / 32 / 41, 54 / 50 / 43.
@@ -170,7 +170,7 @@ hipError_t launch_f8_few(const F8Product &p, hipStream_t st) {
   if (p.rows == 0) return hipSuccess;
   const unsigned tiles = (unsigned)((p.N + 15) / 16) * (p.y1 ? 2 : 1);
   const int tile = f8_tile_rows(p);
-  const int64_t pieces = p.list ? f8_most_pieces(p.rows, p.n_mats, tile) : (p.rows + tile - 1) / tile;
+  const int64_t pieces = p.ids ? p.rows : p.list ? f8_most_pieces(p.rows, p.n_mats, tile) : (p.rows + tile - 1) / tile;
   const size_t own = p.raw ? f8_own_bytes(p) : 0;
   auto launch = [&](auto *kernel) {
     kernel<<<dim3(tiles, (unsigned)pieces), kFewWaves * kWave, own, st>>>(p);

@@ -302,13 +302,11 @@ int mi_moe_switch_glu_f8(const void *x, const uint32_t *topk_idx, const void *to
   list_for(d, lists, 1, ws.list[1]);
   // A token or a few: the lists come beside the sorting, rows are rounded where they are multiplied.  One token's slots as a rule name an expert each: they are not sorted (4 us of 24;
   // named more than once, an expert's weights are read as often).
-  const bool in_blocks = P <= kSortSmall && f8_in_blocks(p, T) && f8_in_blocks(d, T), as_they_are = in_blocks && T == 1 && top_k <= n_experts;
-  Places places{ws.inverse};
+  const bool in_blocks = P <= kSortSmall && f8_in_blocks(p, T) && f8_in_blocks(d, T), as_they_are = in_blocks && T == 1 && top_k <= n_experts && f8_token_bytes(d) <= 32 * 1024;
   if (as_they_are) {
     p.ids = d.ids = topk_idx;
     p.order = nullptr;
     p.list = d.list = nullptr;
-    places = {nullptr, topk_idx, n_experts};
   } else MI_HIP(launch_sort_tokens({topk_idx, T, top_k, n_experts, ws.order, ws.inverse, ws.offsets}, nullptr, dtype, hidden, nullptr, ws.sort, st, in_blocks ? lists : F8Lists()));
   if (in_blocks) {
     p.raw = x;
@@ -319,9 +317,13 @@ int mi_moe_switch_glu_f8(const void *x, const uint32_t *topk_idx, const void *to
     MI_HIP(launch_quantize_f8_rows(x, dtype, T, hidden, ws.x.out(T, hidden), st, lists));
   }
   MI_HIP(launch_f8_product(p, st));
+  if (as_they_are) {
+    MI_HIP(launch_f8_token(d, topk_w, w_dtype, out, dtype, st));
+    return 0;
+  }
   if (few && !in_blocks) MI_HIP(launch_swiglu_f8(ws.g, ws.u, P, intermediate, ws.h.out(P, intermediate), st));
   MI_HIP(launch_f8_product(d, st));
-  MI_HIP(launch_unsort_made(ws.y, d.y_scales, topk_w, w_dtype, places, T, top_k, hidden, dtype, out, st));
+  MI_HIP(launch_unsort_made(ws.y, d.y_scales, topk_w, w_dtype, ws.inverse, T, top_k, hidden, dtype, out, st));
   return 0;
 } MI_CATCH("switch_glu_f8")
 
@@ -385,7 +387,7 @@ int mi_moe_switch_glu_f8_grad(const void *dout, const void *x, const uint32_t *t
   MI_HIP(launch_f8_product(b, st));
   MI_HIP(launch_swiglu_f8_grad({ws.g, ws.u, ws.dh, topk_w, w_dtype, ws.order, ws.offsets, n_experts, P, intermediate, ws.h.codes, ws.h.scales, dweights}, st));
   MI_HIP(launch_f8_product(d, st));
-  MI_HIP(launch_unsort_made(ws.y, ws.y_scales, nullptr, 0, {ws.inverse}, T, top_k, hidden, dtype, dx, st));
+  MI_HIP(launch_unsort_made(ws.y, ws.y_scales, nullptr, 0, ws.inverse, T, top_k, hidden, dtype, dx, st));
   return 0;
 } MI_CATCH("switch_glu_f8_grad")
 

@@ -83,6 +83,9 @@ struct F8Lists {
 };
 hipError_t launch_f8_few(const F8Product &p, hipStream_t st);    // a few rows a matrix (f8_few.hip); transposed only
 hipError_t launch_f8_tiles(const F8Product &p, hipStream_t st);  // tiles (f8_tiles.hip)
+// One token's rows (ids): down's product on raw and raw_up, and the sum over the slots, into out [N] of type dt.
+size_t f8_token_bytes(const F8Product &p);
+hipError_t launch_f8_token(const F8Product &p, const void *weights, int w_dtype, void *out, int dt, hipStream_t st);
 inline hipError_t launch_f8_product(const F8Product &p, hipStream_t st) { return f8_few_rows(p) ? launch_f8_few(p, st) : launch_f8_tiles(p, st); }
 
 // f8_rows.hip.  Codes go to `codes` + row * code_stride, the scale of a row's run j to scales[row * row_stride + j * run_stride].
@@ -129,13 +132,7 @@ constexpr int64_t kSortSmall = 2048;  // pairs up to which one launch sorts, and
 // lists (up to kSortSmall pairs): made beside it
 hipError_t launch_sort_tokens(const SortTokens &a, const void *x, int dt, int H, void *rows, void *scratch, hipStream_t st, const F8Lists &lists = F8Lists());
 // weights nullptr: sums without weights (the sorting's gradient).  out of type dt; rows of type dt, or scaled float16 (y_scales), or float32 for fewer bits of dt
-// Places: a slot's row is inverse[slot], or, inverse nullptr, the slot's own if ids names one of E experts there.
-struct Places {
-  const int32_t *inverse;
-  const uint32_t *ids = nullptr;
-  int E = 0;
-};
-hipError_t launch_unsort_made(const void *rows, const float *y_scales, const void *weights, int w_dtype, const Places &places, int64_t T, int k, int H, int dt, void *out,
+hipError_t launch_unsort_made(const void *rows, const float *y_scales, const void *weights, int w_dtype, const int32_t *inverse, int64_t T, int k, int H, int dt, void *out,
                               hipStream_t st);
 hipError_t launch_unsort_tokens(const void *rows, const void *weights, int w_dtype, const int32_t *inverse, int64_t T, int k, int H, int dt, void *out,
                                 hipStream_t st);

@@ -163,7 +163,7 @@ __device__ __forceinline__ void load_octets(Octet<DT> (&v)[N], const void *rows,
 // for (8192 tokens of 2048 bf16 and eight slots: 80 us).
 // IN, DT: types of the rows and of the result.  SCALED: the rows' values are times scales[row][column / 64].
 template <int IN, int DT, bool SCALED>
-__global__ __launch_bounds__(kSortThreads) void unsort_kernel(const void *__restrict__ rows, const float *__restrict__ scales, const void *__restrict__ weights, int w_dtype, Places places,
+__global__ __launch_bounds__(kSortThreads) void unsort_kernel(const void *__restrict__ rows, const float *__restrict__ scales, const void *__restrict__ weights, int w_dtype, const int32_t *__restrict__ inverse,
                                                               int64_t T, int k, int H, int lanes_log2, void *__restrict__ out) {
   const int lanes = 1 << lanes_log2;
   const int64_t t = (int64_t)blockIdx.x * (kSortThreads >> lanes_log2) + (threadIdx.x >> lanes_log2);
@@ -177,7 +177,7 @@ __global__ __launch_bounds__(kSortThreads) void unsort_kernel(const void *__rest
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int64_t s = t * k + (s0 + j < k ? s0 + j : k - 1);
-      const int64_t at = places.inverse ? places.inverse[s] : places.ids[s] < (uint32_t)places.E ? s : -1;
+      const int32_t at = inverse[s];
       row[j] = s0 + j < k && at >= 0 && at < T * k ? at : -1;
       w[j] = weights ? value_of(weights, s, w_dtype) : 1.f;
     }
@@ -197,21 +197,21 @@ __global__ __launch_bounds__(kSortThreads) void unsort_kernel(const void *__rest
 }
 
 template <int IN, int DT, bool SCALED = false>
-static hipError_t launch_unsort(const void *rows, const float *scales, const void *weights, int w_dtype, const Places &places, int64_t T, int k, int H, void *out, hipStream_t st) {
+static hipError_t launch_unsort(const void *rows, const float *scales, const void *weights, int w_dtype, const int32_t *inverse, int64_t T, int k, int H, void *out, hipStream_t st) {
   if (T == 0) return hipSuccess;
   const TokenGrid g(H, kSortThreads);
-  unsort_kernel<IN, DT, SCALED><<<dim3((unsigned)((T + g.tokens - 1) / g.tokens), (unsigned)g.columns), kSortThreads, 0, st>>>(rows, scales, weights, w_dtype, places, T, k, H,
+  unsort_kernel<IN, DT, SCALED><<<dim3((unsigned)((T + g.tokens - 1) / g.tokens), (unsigned)g.columns), kSortThreads, 0, st>>>(rows, scales, weights, w_dtype, inverse, T, k, H,
                                                                                                                               __builtin_ctz((unsigned)g.lanes), out);
   return hipGetLastError();
 }
 hipError_t launch_unsort_tokens(const void *rows, const void *weights, int w_dtype, const int32_t *inverse, int64_t T, int k, int H, int dt, void *out, hipStream_t st) {
   auto *const launch = dt == 0 ? &launch_unsort<0, 0> : dt == 1 ? &launch_unsort<1, 1> : &launch_unsort<2, 2>;
-  return launch(rows, nullptr, weights, w_dtype, {inverse}, T, k, H, out, st);
+  return launch(rows, nullptr, weights, w_dtype, inverse, T, k, H, out, st);
 }
-hipError_t launch_unsort_made(const void *rows, const float *y_scales, const void *weights, int w_dtype, const Places &places, int64_t T, int k, int H, int dt, void *out,
+hipError_t launch_unsort_made(const void *rows, const float *y_scales, const void *weights, int w_dtype, const int32_t *inverse, int64_t T, int k, int H, int dt, void *out,
                               hipStream_t st) {
   auto *const launch = y_scales ? (dt == 0 ? &launch_unsort<1, 0, true> : &launch_unsort<1, 1, true>) : dt == 0 ? &launch_unsort<2, 0> : &launch_unsort<2, 1>;
-  return launch(rows, y_scales, weights, w_dtype, places, T, k, H, out, st);
+  return launch(rows, y_scales, weights, w_dtype, inverse, T, k, H, out, st);
 }
 
 __device__ __forceinline__ float wave_sum_f32(float v) {  // in a fixed order

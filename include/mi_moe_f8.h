@@ -56,8 +56,8 @@ int mi_moe_linear_f8(const void *x, const void *w, const float *scales, const vo
                      int32_t N, int32_t K, int32_t transpose, int32_t dtype, void *y, void *workspace,
                      size_t workspace_bytes, void *stream);
 /* The same for rows sorted by expert (mi_moe_sort_tokens): matrix e of w [n_experts, N, K] (or [n_experts, K, N]) for the rows from offsets[e] to offsets[e + 1]; rows of y
- * behind the last are zeros.  offsets ascend from 0 to at most `rows`: others reach no memory but the operands', and leave rows of y that are not in any expert's range as they
- * were.  n_experts 1..512. */
+ * behind the last are zeros.  offsets ascend from 0 to at most `rows`: others reach no memory but the operands', and what rows of y hold that are in no expert's range is not
+ * said.  n_experts 1..512. */
 int mi_moe_grouped_linear_f8(const void *x, const void *w, const float *scales, const uint32_t *offsets,
                              int64_t rows, int32_t n_experts, int32_t N, int32_t K, int32_t transpose,
                              int32_t dtype, void *y, void *workspace, size_t workspace_bytes, void *stream);

@@ -87,7 +87,7 @@ int linear(const char *who, const void *x, const void *w, const float *scales, c
   lists.n_mats = E;
   lists.rows = M;
   if (offsets) list_for(p, lists, 0, list);
-  else p.parts = reinterpret_cast<float *>(c.take<char>(f8_parts_bytes(M, N)));
+  p.parts = reinterpret_cast<float *>(c.take<char>(f8_parts_bytes(M, N)));
   if (!offsets && f8_in_blocks(p, M)) {
     p.raw = x;
     p.raw_dt = dtype;
@@ -110,6 +110,7 @@ struct ExpertsWs {
   RowsIn h;         // rows of pairs: h, or dg and du side by side
   void *y;          // of pairs, for the sum over slots: float32, or scaled float16
   float *y_scales;
+  float *parts;     // gradients: of a few rows an expert
   size_t bytes;
   ExpertsWs(void *at, int64_t T, int H, int I, int E, int k, bool grad) : ExpertsWs(Carver(at), T, T * k, H, I, E, k, grad) {}
 
@@ -118,7 +119,8 @@ struct ExpertsWs {
       : order(c.take<uint32_t>((size_t)P)), offsets(c.take<uint32_t>((size_t)E + 1)), inverse(c.take<int32_t>((size_t)P)),
         list{c.take<uint4>((size_t)f8_list_places(P, E)), c.take<uint4>((size_t)f8_list_places(P, E)), c.take<uint4>((size_t)f8_list_places(P, E))}, sort(c.take<char>(sort_tokens_bytes(T, k, E))),
         x(c, T, H), dout(c, grad ? T : 0, H), g(c.take<float>(float_rows(P, E, grad) * I)), u(c.take<float>(float_rows(P, E, grad) * I)), dh(c.take<float>(grad ? (size_t)P * I : 0)),
-        h(c, P, I, grad ? 2 : 1), y(c.take<char>(y_bytes(P, H, E))), y_scales(c.take<float>((size_t)P * ((H + 63) / 64))), bytes(c.off + 256) {}
+        h(c, P, I, grad ? 2 : 1), y(c.take<char>(y_bytes(P, H, E))), y_scales(c.take<float>((size_t)P * ((H + 63) / 64))),
+        parts(reinterpret_cast<float *>(c.take<char>(grad ? f8_parts_bytes(P < (int64_t)16 * E ? P : (int64_t)16 * E, H > I ? H : I) : 0))), bytes(c.off + 256) {}
   static size_t y_bytes(int64_t P, int H, int E) {
     const size_t halves = (size_t)P * H * 2, floats = (size_t)(P < (int64_t)16 * E ? P : (int64_t)16 * E) * H * 4;  // (few rows an expert: floats)
     return halves > floats ? halves : floats;
@@ -373,6 +375,16 @@ int mi_moe_switch_glu_f8_grad(const void *dout, const void *x, const uint32_t *t
   d.y = ws.y;
   d.y_scales = ws.y_scales;
   d.dt = dtype;
+  if (P <= (int64_t)16 * n_experts) {  // (room for float32 rows, and for parts)
+    b.parts = d.parts = ws.parts;
+    d.list = ws.list[1];
+    if (f8_plan(d).parts > 1) {
+      d.dt = MI_MOE_DTYPE_F32;
+      d.y_scales = nullptr;
+    } else {
+      d.parts = nullptr;
+    }
+  }
   // three lists, the forward products' beside the rounding of x, the others' beside that of dout
   F8Lists lists, back;
   lists.offsets = back.offsets = ws.offsets;
@@ -387,7 +399,7 @@ int mi_moe_switch_glu_f8_grad(const void *dout, const void *x, const uint32_t *t
   MI_HIP(launch_f8_product(b, st));
   MI_HIP(launch_swiglu_f8_grad({ws.g, ws.u, ws.dh, topk_w, w_dtype, ws.order, ws.offsets, n_experts, P, intermediate, ws.h.codes, ws.h.scales, dweights}, st));
   MI_HIP(launch_f8_product(d, st));
-  MI_HIP(launch_unsort_made(ws.y, ws.y_scales, nullptr, 0, ws.inverse, T, top_k, hidden, dtype, dx, st));
+  MI_HIP(launch_unsort_made(ws.y, d.y_scales, nullptr, 0, ws.inverse, T, top_k, hidden, dtype, dx, st));
   return 0;
 } MI_CATCH("switch_glu_f8_grad")
 

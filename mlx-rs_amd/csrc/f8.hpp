@@ -50,16 +50,21 @@ struct F8Product {
   float *y_scales;  // tiles: y is float16 whatever dt, a row's values of 64 columns times a power of two of their own, [rows][columns / 64] (the other way round
                     // the sum over the slots of 4096 tokens read a line for every scale and took 40 us, not 37).  Rows that are summed over
                     // slots afterwards: rounded to bfloat16 here and once more behind the sum, the experts' results were 1.5 times as far off as with one rounding.
-  float *parts;  // one matrix: room for the sums of blocks that share a tile's summed axis (f8_parts_bytes), or nullptr
+  float *parts;  // room for the sums of blocks that share a tile's summed axis (f8_parts_bytes), or nullptr: none do
   uint8_t *h;  // gate/up pairs: silu(gate) * up in e4m3, as F8Rows
   float *hs;
 };
 // Parts are made where tiles of 64 x 256 and more are fewer than the chip's CUs: kF8MostParts of a product at most, 256 tiles of all of them.
 constexpr int kF8MostParts = 16;
+constexpr int64_t kF8PartsMost = (int64_t)256 * 256 * 256;  // values
 inline size_t f8_parts_bytes(int64_t M, int N) {
-  const size_t all = (size_t)M * N * 4 * kF8MostParts, most = (size_t)256 * 256 * 256 * 4;
-  return all < most ? all : most;
+  const int64_t all = M * N * kF8MostParts;
+  return (size_t)(all < kF8PartsMost ? all : kF8PartsMost) * 4;
 }
+struct F8Plan {
+  int tile, parts;
+};
+F8Plan f8_plan(const F8Product &p);  // (f8_tiles.hip)
 // Rows of a piece: what the product's kernel takes at once (16 or 32: the one for a few rows).
 int f8_tile_rows(const F8Product &p);
 inline bool f8_few_rows(const F8Product &p) { return f8_tile_rows(p) < 64; }

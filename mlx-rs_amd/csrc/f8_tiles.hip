@@ -12,7 +12,7 @@
 namespace mi_moe {
 
 enum F8Mode { kRowsOfWeights, kPair, kColsOfWeights };  // matrices [N][K]; two such, into h; matrices [K][N]
-constexpr int kF8TileN = 256, kF8Threads = 512;
+constexpr int kF8TileN = 256, kF8Threads = 512, kF8FewPieces = 32;
 constexpr uint32_t kF8Outside = 0xfffffff0u;  // an offset past every descriptor's end: zeros
 
 // 4 bytes a lane into LDS, at `to` + 4 lane
@@ -84,6 +84,9 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, F8Gri
   if (!a.list) {
     mt = (xcd % (uint32_t)g.xcds_m) * (uint32_t)g.m_each + q % (uint32_t)g.m_each;
     nt = (xcd / (uint32_t)g.xcds_m) * (uint32_t)g.n_each + q / (uint32_t)g.m_each;
+  } else if (g.m_tiles < kF8FewPieces) {  // (too few pieces to give each XCD as many: 26 rows at one matrix of 2128 x 1792 took 23 us, all on one, not 16)
+    mt = blockIdx.x % (uint32_t)g.m_tiles;
+    nt = blockIdx.x / (uint32_t)g.m_tiles;
   } else {
     mt = q / (uint32_t)g.n_tiles * 8 + xcd;
     nt = q % (uint32_t)g.n_tiles;
@@ -101,9 +104,11 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, F8Gri
   if (mat == a.n_mats) {  // rows of no matrix (scaled ones are read by nobody)
     if constexpr (MODE != kPair) {
       const float none[4] = {0.f, 0.f, 0.f, 0.f};
+      const bool part = g.part_steps < steps;
+      void *const to = part ? a.parts + (int64_t)blockIdx.y * a.rows * N : y;
       for (int i = threadIdx.x; i < rows * (kF8TileN / 4); i += kF8Threads) {
         const int n = n0 + i % (kF8TileN / 4) * 4;
-        if (n < N) store4(y, (int64_t)(row0 + i / (kF8TileN / 4)) * N + n, N - n, a.dt, none);
+        if (n < N) store4(to, (int64_t)(row0 + i / (kF8TileN / 4)) * N + n, N - n, part ? 2 : a.dt, none);
       }
     }
     return;
@@ -450,25 +455,28 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, F8Gri
   }
 }
 
-// One matrix: the tile, and how many blocks share a tile's summed axis where the tiles alone leave CUs idle, by the time they take.  Us, measured: a launch 6; a stage 0.65 with a few
+// How many blocks share a tile's summed axis where the tiles alone leave CUs idle, and for one matrix the tile, by the time they take.  Us, measured: a launch 6; a stage 0.65 with a few
 // blocks and 1.1 with one on every CU (64 token rows), 1.0 and 1.45 (128), 1.7 and 2.2 (256); a join of parts 3, their bytes out and back 2.5 MB each.
-struct F8Plan {
-  int tile, parts;
-};
-static F8Plan f8_dense_plan(const F8Product &p) {
+static F8Plan plan_of(const F8Product &p, int tile, int64_t tiles, F8Plan best, double &least) {
+  const int steps = f8_runs(p.K) * (p.pair_sum ? 2 : 1);
+  for (int parts = 1; parts <= (p.parts ? kF8MostParts : 1); parts *= 2) {
+    if (parts > 1 && (steps < 2 * parts || tiles * parts > 256 || (int64_t)parts * p.rows * p.N > kF8PartsMost)) break;
+    const double full = (double)(tiles * parts < 256 ? tiles * parts : 256) / 256, few = tile == 64 ? 0.65 : tile == 128 ? 1.0 : 1.7;
+    const double t = (double)((tiles * parts + 255) / 256) * ((steps + parts - 1) / parts) * (few + 0.45 * full) + (parts > 1 ? 3.0 + (double)parts * p.rows * p.N * 8 / 2.5e6 : 0.0);
+    if (t < least) least = t, best = {tile, parts};
+  }
+  return best;
+}
+F8Plan f8_plan(const F8Product &p) {
   F8Plan best{64, 1};
   double least = 1e30;
-  const int steps = f8_runs(p.K);
-  for (int tile : {64, 128, 256}) {
-    if (tile == 256 && p.dt == 2) continue;
-    const int64_t tiles = ((p.rows + tile - 1) / tile) * ((p.N + kF8TileN - 1) / kF8TileN);
-    for (int parts = 1; parts <= (p.parts ? kF8MostParts : 1); parts *= 2) {
-      if (parts > 1 && (steps < 2 * parts || tiles * parts > 256)) break;
-      const double full = (double)(tiles * parts < 256 ? tiles * parts : 256) / 256, few = tile == 64 ? 0.65 : tile == 128 ? 1.0 : 1.7;
-      const double t = (double)((tiles * parts + 255) / 256) * ((steps + parts - 1) / parts) * (few + 0.45 * full) + (parts > 1 ? 3.0 + (double)parts * p.rows * p.N * 8 / 2.5e6 : 0.0);
-      if (t < least) least = t, best = {tile, parts};
-    }
+  const int64_t columns = (p.N + kF8TileN - 1) / kF8TileN;
+  if (p.list) {  // (as many pieces as there are matrices with rows, if each has a few)
+    best.tile = f8_tile_rows(p);
+    return p.parts ? plan_of(p, best.tile, (p.rows / best.tile + (p.n_mats < p.rows ? p.n_mats : p.rows)) * columns, best, least) : best;
   }
+  for (int tile : {64, 128, 256})
+    if (tile != 256 || p.dt != 2) best = plan_of(p, tile, (p.rows + tile - 1) / tile * columns, best, least);
   return best;
 }
 
@@ -484,11 +492,11 @@ static hipError_t launch_tiles(const F8Product &p, hipStream_t st) {
     if (dev >= 0 && dev < kMaxDevices) raised[dev].store(true, std::memory_order_release);
   }
   const int64_t n_tiles = (p.N + (MODE == kPair ? 127 : kF8TileN - 1)) / (MODE == kPair ? 128 : kF8TileN), m_tiles = p.list ? f8_most_pieces(p.rows, p.n_mats, TM) : (p.rows + TM - 1) / TM;
-  const int steps = f8_runs(p.K) * (p.pair_sum ? 2 : 1), parts = p.list ? 1 : f8_dense_plan(p).parts;
+  const int steps = f8_runs(p.K) * (p.pair_sum ? 2 : 1), parts = f8_plan(p).parts;
   F8Grid g{(int)m_tiles, (int)n_tiles, 1, (int)m_tiles, (int)((n_tiles + 7) / 8), (steps + parts - 1) / parts};
   int64_t each;  // blocks of an XCD
   if (p.list) {
-    each = (m_tiles + 7) / 8 * n_tiles;
+    each = m_tiles < kF8FewPieces ? (m_tiles * n_tiles + 7) / 8 : (m_tiles + 7) / 8 * n_tiles;
   } else {
     for (int xm = 2; xm <= 8; xm *= 2) {
       const int m_each = (int)((m_tiles + xm - 1) / xm), n_each = (int)((n_tiles + 8 / xm - 1) / (8 / xm));
@@ -506,7 +514,7 @@ static hipError_t launch_tiles(const F8Product &p, hipStream_t st) {
 
 template <F8Mode MODE>
 static hipError_t launch_mode(const F8Product &p, hipStream_t st) {
-  const int tile = p.list ? f8_tile_rows(p) : f8_dense_plan(p).tile;
+  const int tile = f8_plan(p).tile;
   if (p.dt == 2) return tile == 128 ? launch_tiles<128, MODE, true>(p, st) : launch_tiles<64, MODE, true>(p, st);
   return tile == 256 ? launch_tiles<256, MODE, false>(p, st) : tile == 128 ? launch_tiles<128, MODE, false>(p, st) : launch_tiles<64, MODE, false>(p, st);
 }

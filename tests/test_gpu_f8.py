@@ -160,6 +160,25 @@ def test_grouped(counts, behind, transpose, dtype):
         o.within(y, want, off, f"grouped {counts} {behind} {transpose} {dtype}")
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("counts", ["few", "ragged"])
+def test_grouped_along_a_long_axis(counts, dtype):
+    """Few tiles of many stages: blocks that share a tile's summed axis, rows of no expert among theirs."""
+    from mlx_rs_amd import ops
+    counts = COUNTS[counts]
+    N, K = 2576, 144
+    gen = gen_of(sum(counts))
+    w, s = o.bank(gen, N, K, len(counts))
+    ends = [0]
+    for c in counts:
+        ends.append(ends[-1] + c)
+    x = rows_of(gen, ends[-1] + 7, N, dtype)
+    y = ops.grouped_linear_f8(x, w, s, torch.tensor(ends, device="cuda", dtype=torch.int32), False)
+    want, off = grouped_oracle(x, w, s, ends, False, dtype)
+    assert not y[ends[-1]:].any()
+    o.within(y, want, off, f"along {counts} {dtype}")
+
+
 def test_many_experts():
     from mlx_rs_amd import ops
     gen = gen_of(1)
@@ -252,7 +271,7 @@ def experts_oracle(x, inds, weights, gate, up, down, dout=None):
     return (out, off) if dout is None else (out, off, dw, dw_off)
 
 
-EXPERTS = [(1, 1, 1, 16, 16), (1, 8, 128, 256, 192), (5, 2, 4, 144, 272), (40, 2, 4, 256, 128), (300, 2, 4, 272, 400), (700, 1, 2, 128, 256), (130, 4, 64, 128, 112)]
+EXPERTS = [(1, 1, 1, 16, 16), (1, 8, 128, 256, 192), (5, 2, 4, 144, 272), (40, 2, 4, 256, 128), (300, 2, 4, 272, 400), (700, 1, 2, 128, 256), (130, 4, 64, 128, 112), (3, 2, 8, 256, 2064), (20, 2, 3, 1296, 1040)]
 
 
 @pytest.mark.parametrize("padded", [False, True])

@@ -272,16 +272,6 @@ int mi_moe_switch_glu_f8(const void *x, const uint32_t *topk_idx, const void *to
   p.N = intermediate;
   p.K = hidden;
   p.dt = MI_MOE_DTYPE_F32;
-  const bool few = f8_few_rows(p);
-  if (few) {
-    p.y = ws.g;
-    p.y1 = ws.u;
-  } else {
-    // (results of float16 would show what the f8 instructions lose of gate and up, in the codes that it changes)
-    p.dt = dtype == MI_MOE_DTYPE_F16 ? MI_MOE_DTYPE_F32 : dtype;
-    p.h = ws.h.codes;
-    p.hs = ws.h.scales;
-  }
   F8Product d{};
   d.x = ws.h.as(P);
   d.k_div = 1;
@@ -294,6 +284,20 @@ int mi_moe_switch_glu_f8(const void *x, const uint32_t *topk_idx, const void *to
   d.y = ws.y;
   d.list = ws.list[1];
   d.dt = dtype;
+  // A token or a few: the lists come beside the sorting, rows are rounded where they are multiplied.  More of them go to the tiles, where silu(gate) * up is made in a block's registers,
+  // from two rows an expert on (32 / 64 / 256 tokens, 8 of 128 experts of 2048 x 768: 113 / 150 / 232 us on the kernels for a few rows, 99 / 126 / 148 on tiles).
+  const bool in_blocks = P <= kSortSmall && f8_in_blocks(p, T) && f8_in_blocks(d, T);
+  if (!in_blocks) p.few = d.few = 1;
+  const bool few = f8_few_rows(p);
+  if (few) {
+    p.y = ws.g;
+    p.y1 = ws.u;
+  } else {
+    // (results of float16 would show what the f8 instructions lose of gate and up, in the codes that it changes)
+    p.dt = dtype == MI_MOE_DTYPE_F16 ? MI_MOE_DTYPE_F32 : dtype;
+    p.h = ws.h.codes;
+    p.hs = ws.h.scales;
+  }
   if (f8_few_rows(d)) d.dt = MI_MOE_DTYPE_F32;
   else d.y_scales = ws.y_scales;
   F8Lists lists;
@@ -302,9 +306,8 @@ int mi_moe_switch_glu_f8(const void *x, const uint32_t *topk_idx, const void *to
   lists.rows = P;
   list_for(p, lists, 0, ws.list[0]);
   list_for(d, lists, 1, ws.list[1]);
-  // A token or a few: the lists come beside the sorting, rows are rounded where they are multiplied.  One token's slots as a rule name an expert each: they are not sorted (4 us of 24;
-  // named more than once, an expert's weights are read as often).
-  const bool in_blocks = P <= kSortSmall && f8_in_blocks(p, T) && f8_in_blocks(d, T), as_they_are = in_blocks && T == 1 && top_k <= n_experts && f8_token_bytes(d) <= 32 * 1024;
+  // One token's slots as a rule name an expert each: they are not sorted (4 us of 24; named more than once, an expert's weights are read as often).
+  const bool as_they_are = in_blocks && T == 1 && top_k <= n_experts && f8_token_bytes(d) <= 32 * 1024;
   if (as_they_are) {
     p.ids = d.ids = topk_idx;
     p.order = nullptr;

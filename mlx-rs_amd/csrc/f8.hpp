@@ -39,6 +39,7 @@ struct F8Product {
   const uint32_t *ids;      // instead of order and list, for a few rows: row r is of x row r / k_div and matrix ids[r] (none, if there is no such one), a piece of its own
   const uint4 *list;        // the pieces of at most f8_tile_rows rows that the matrices' rows are cut into, and rows of no matrix, which are zeros of y (f8_list).  nullptr: one
   int n_mats;               // matrix, all rows
+  int few;                  // with a list, how many rows a matrix on average the kernel for a few rows takes; 0: what is best for this product alone (f8_tile_rows)
   int64_t rows;             // of y
   F8Mat m[2];               // the second one: of a gate/up pair (y1 or h), or of a second half of the summed axis (pair_sum)
   bool transpose;           // matrices [N][K], else [K][N]

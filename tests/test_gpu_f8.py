@@ -271,7 +271,7 @@ def experts_oracle(x, inds, weights, gate, up, down, dout=None):
     return (out, off) if dout is None else (out, off, dw, dw_off)
 
 
-EXPERTS = [(1, 1, 1, 16, 16), (1, 8, 128, 256, 192), (5, 2, 4, 144, 272), (40, 2, 4, 256, 128), (300, 2, 4, 272, 400), (700, 1, 2, 128, 256), (130, 4, 64, 128, 112), (3, 2, 8, 256, 2064), (20, 2, 3, 1296, 1040)]
+EXPERTS = [(1, 1, 1, 16, 16), (1, 8, 128, 256, 192), (5, 2, 4, 144, 272), (40, 2, 4, 256, 128), (300, 2, 4, 272, 400), (700, 1, 2, 128, 256), (130, 4, 64, 128, 112), (3, 2, 8, 256, 2064), (20, 2, 3, 1296, 1040), (40, 1, 64, 256, 144)]
 
 
 @pytest.mark.parametrize("padded", [False, True])

@@ -274,7 +274,7 @@ int mi_moe_switch_glu_f8(const void *x, const uint32_t *topk_idx, const void *to
   p.dt = MI_MOE_DTYPE_F32;
   F8Product d{};
   d.x = ws.h.as(P);
-  d.k_div = 1;
+  d.k_div = top_k;
   d.n_mats = n_experts;
   d.rows = P;
   d.m[0] = d.m[1] = mat(experts->down, experts->down_scales);
@@ -284,9 +284,12 @@ int mi_moe_switch_glu_f8(const void *x, const uint32_t *topk_idx, const void *to
   d.y = ws.y;
   d.list = ws.list[1];
   d.dt = dtype;
-  // A token or a few: the lists come beside the sorting, rows are rounded where they are multiplied.  More of them go to the tiles, where silu(gate) * up is made in a block's registers,
+  // A few tokens: the lists come beside the sorting, rows are rounded where they are multiplied.  More of them go to the tiles, where silu(gate) * up is made in a block's registers,
   // from two rows an expert on (32 / 64 / 256 tokens, 8 of 128 experts of 2048 x 768: 113 / 150 / 232 us on the kernels for a few rows, 99 / 126 / 148 on tiles).
-  const bool in_blocks = P <= kSortSmall && f8_in_blocks(p, T) && f8_in_blocks(d, T);
+  // Slots of one or two tokens, and of four among many experts, as a rule name an expert each: they are not sorted, each has a piece and the sum over them comes with down (1, 2, 4 tokens as
+  // above: 24, 34, 46 us sorted, 19, 22, 37 so; 4 tokens, 2 of 16 experts of 4096 x 1536: 45, 49.  An expert that is named twice is read as often).
+  const bool unsorted = T <= 4 && (T <= 2 ? P : 4 * P) <= n_experts && f8_few_rows(p) && f8_few_rows(d) && f8_runs(hidden) <= 64 && f8_token_bytes(d) <= 32 * 1024;
+  const bool in_blocks = unsorted || (P <= kSortSmall && f8_in_blocks(p, T) && f8_in_blocks(d, T));
   if (!in_blocks) p.few = d.few = 1;
   const bool few = f8_few_rows(p);
   if (few) {
@@ -306,9 +309,7 @@ int mi_moe_switch_glu_f8(const void *x, const uint32_t *topk_idx, const void *to
   lists.rows = P;
   list_for(p, lists, 0, ws.list[0]);
   list_for(d, lists, 1, ws.list[1]);
-  // One token's slots as a rule name an expert each: they are not sorted (4 us of 24; named more than once, an expert's weights are read as often).
-  const bool as_they_are = in_blocks && T == 1 && top_k <= n_experts && f8_token_bytes(d) <= 32 * 1024;
-  if (as_they_are) {
+  if (unsorted) {
     p.ids = d.ids = topk_idx;
     p.order = nullptr;
     p.list = d.list = nullptr;
@@ -322,7 +323,7 @@ int mi_moe_switch_glu_f8(const void *x, const uint32_t *topk_idx, const void *to
     MI_HIP(launch_quantize_f8_rows(x, dtype, T, hidden, ws.x.out(T, hidden), st, lists));
   }
   MI_HIP(launch_f8_product(p, st));
-  if (as_they_are) {
+  if (unsorted) {
     MI_HIP(launch_f8_token(d, topk_w, w_dtype, out, dtype, st));
     return 0;
   }

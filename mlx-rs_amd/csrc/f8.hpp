@@ -72,7 +72,7 @@ inline bool f8_few_rows(const F8Product &p) { return f8_tile_rows(p) < 64; }
 // Whether the blocks of a product for a few rows round them by themselves, where a matrix has `most` rows as a rule.  (A piece may hold as many as its kernel takes, of tokens that
 // name an expert more than once: there is room for them.)
 inline size_t f8_own_bytes(const F8Product &p) {
-  const int tile = f8_tile_rows(p);
+  const int tile = p.ids ? 1 : f8_tile_rows(p);
   return (size_t)(p.rows < tile ? p.rows : tile) * (size_t)(f8_row_bytes(p.K) + 16 + 4 * f8_runs(p.K));
 }
 inline bool f8_in_blocks(const F8Product &p, int64_t most) { return f8_few_rows(p) && most * f8_runs(p.K) <= 64 && f8_own_bytes(p) <= 48 * 1024; }
@@ -89,7 +89,7 @@ struct F8Lists {
 };
 hipError_t launch_f8_few(const F8Product &p, hipStream_t st);    // a few rows a matrix (f8_few.hip); transposed only
 hipError_t launch_f8_tiles(const F8Product &p, hipStream_t st);  // tiles (f8_tiles.hip)
-// One token's rows (ids): down's product on raw and raw_up, and the sum over the slots, into out [N] of type dt.
+// Rows of a token or two (ids; k_div of each): down's product on raw and raw_up, and the sum over the slots, into out [tokens][N] of type dt.
 size_t f8_token_bytes(const F8Product &p);
 hipError_t launch_f8_token(const F8Product &p, const void *weights, int w_dtype, void *out, int dt, hipStream_t st);
 inline hipError_t launch_f8_product(const F8Product &p, hipStream_t st) { return f8_few_rows(p) ? launch_f8_few(p, st) : launch_f8_tiles(p, st); }

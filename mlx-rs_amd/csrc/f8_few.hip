@@ -168,17 +168,19 @@ __global__ __launch_bounds__(kFewWaves *kWave) void f8_few_kernel(F8Product a) {
   }
 }
 
-// One token: down, and the sum over its slots.  A block has 16 columns of the result, its sixteen waves share the slots and, of a slot's summed axis, every `each`th run; rows are
+// A token or two: down, and the sum over a token's k_div slots.  A block has 16 columns of a token's result, its sixteen waves share the slots and, of a slot's summed axis, every `each`th run; rows are
 // rounded as above.  The slots' rows are summed over the waves, then weighted and summed in the slots' order, all in float32.  A launch less than with rows in memory.
 constexpr int kTokenWaves = 16, kTokenSlots = 32;
 __global__ __launch_bounds__(kTokenWaves *kWave) void f8_token_kernel(F8Product a, const void *__restrict__ weights, int w_dtype, void *__restrict__ out, int out_dt) {
   constexpr int AHEAD = 4;
+  const uint32_t first = blockIdx.y * (uint32_t)a.k_div;  // the token's first pair
+  const uint32_t *const ids = a.ids + first;
   extern __shared__ __align__(16) uint8_t own_rows[];  // [slots][whole runs + 16], then scales [slots][runs]
   __shared__ float sums[kTokenSlots][16];  // [slot][wave of the slot's]: no more than sixteen of both, or one wave a slot
   __shared__ float slot_weight[kTokenSlots];
   __shared__ bool slot_named[kTokenSlots];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ln = lane & 15, part = lane >> 4, n0 = (int)blockIdx.x * 16;
-  const int slots = (int)a.rows, runs = f8_runs(a.K), wide = runs * kF8Run;
+  const int slots = a.k_div, runs = f8_runs(a.K), wide = runs * kF8Run;
   const int at_once = slots < kTokenWaves ? slots : kTokenWaves, each = kTokenWaves / at_once;  // slots at once, waves of a slot
   const int mine = wave % each, turns = (runs + each - 1) / each, all = wave / each < at_once ? (slots - wave / each + at_once - 1) / at_once * turns : 0;
   float *const own_scales = reinterpret_cast<float *>(own_rows + slots * (wide + 16));
@@ -196,7 +198,7 @@ __global__ __launch_bounds__(kTokenWaves *kWave) void f8_token_kernel(F8Product 
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
       const Item it = item(i0 + i);
-      const uint32_t e = a.ids[it.slot];
+      const uint32_t e = ids[it.slot];
       const bool named = it.there && e < (uint32_t)a.n_mats;
       const int64_t mat = named ? e : 0;
       const uint8_t *const w = a.m[0].w + (mat * a.N + (n0 + ln < a.N ? n0 + ln : a.N - 1)) * a.K;
@@ -211,12 +213,12 @@ __global__ __launch_bounds__(kTokenWaves *kWave) void f8_token_kernel(F8Product 
   };
   fetch(0);
   if ((int)threadIdx.x < slots) {  // (loaded where they are used, one after the other, they took 0.7 us)
-    slot_named[threadIdx.x] = a.ids[threadIdx.x] < (uint32_t)a.n_mats;
-    slot_weight[threadIdx.x] = value_of(weights, threadIdx.x, w_dtype);
+    slot_named[threadIdx.x] = ids[threadIdx.x] < (uint32_t)a.n_mats;
+    slot_weight[threadIdx.x] = value_of(weights, first + threadIdx.x, w_dtype);
   }
   for (int at = threadIdx.x / 16; at < slots * runs; at += kTokenWaves * kWave / 16) {
     const int r = at / runs, run = at - r * runs;
-    round_run<kGateUp>(a, r, run, own_rows + r * (wide + 16), own_scales + r * runs);
+    round_run<kGateUp>(a, first + r, run, own_rows + r * (wide + 16), own_scales + r * runs);
   }
   __syncthreads();
   f32x4_t acc = {};
@@ -248,11 +250,11 @@ __global__ __launch_bounds__(kTokenWaves *kWave) void f8_token_kernel(F8Product 
     for (int w = 0; w < each; ++w) row += sums[slot * each + w][threadIdx.x];
     y = __builtin_fmaf(slot_weight[slot], row, y);
   }
-  put_value(out, n, out_dt, y);
+  put_value(out, (int64_t)blockIdx.y * a.N + n, out_dt, y);
 }
-size_t f8_token_bytes(const F8Product &p) { return (size_t)p.rows * (size_t)(f8_row_bytes(p.K) + 16 + 4 * f8_runs(p.K)); }
+size_t f8_token_bytes(const F8Product &p) { return (size_t)p.k_div * (size_t)(f8_row_bytes(p.K) + 16 + 4 * f8_runs(p.K)); }
 hipError_t launch_f8_token(const F8Product &p, const void *weights, int w_dtype, void *out, int dt, hipStream_t st) {
-  f8_token_kernel<<<(unsigned)((p.N + 15) / 16), kTokenWaves * kWave, f8_token_bytes(p), st>>>(p, weights, w_dtype, out, dt);
+  f8_token_kernel<<<dim3((unsigned)((p.N + 15) / 16), (unsigned)(p.rows / p.k_div)), kTokenWaves * kWave, f8_token_bytes(p), st>>>(p, weights, w_dtype, out, dt);
   return hipGetLastError();
 }
 

@@ -317,7 +317,7 @@ def test_the_same_expert_twice_and_nobody_at_all():
     assert ops.switch_glu_f8(x[:0], twice[:0], w[:0], gate, up, down).shape == (0, 128)
 
 
-@pytest.mark.parametrize("T,k,H", [(1, 4, 1024), (1, 8, 256), (1, 16, 2048), (2, 32, 2048), (4, 8, 1024), (7, 3, 1040), (16, 16, 128), (40, 8, 256)])
+@pytest.mark.parametrize("T,k,H", [(1, 4, 1024), (1, 8, 256), (2, 4, 4096), (4, 2, 1040), (3, 2, 144), (1, 16, 2048), (2, 32, 2048), (4, 8, 1024), (7, 3, 1040), (16, 16, 128), (40, 8, 256)])
 def test_few_tokens_all_at_one_expert(T, k, H):
     """A matrix with more rows than tokens: pieces as long as the kernels for a few rows take."""
     from mlx_rs_amd import ops

@@ -159,10 +159,11 @@ __device__ __forceinline__ void load_octets(Octet<DT> (&v)[N], const void *rows,
   }
 }
 
-// A thread eight columns of a token; its slots' rows eight at a time, all their loads in flight together.  Blocks of 256 threads: of 64, the launch of blocks is what it waits
+// A thread eight columns of a token; its slots' rows N at a time, all their loads in flight together.  Blocks of 256 threads: of 64, the launch of blocks is what it waits
 // for (8192 tokens of 2048 bf16 and eight slots: 80 us).
+// N: eight, or of fewer slots two or four, where the loads for slots past the last one took as long as those for the slots (4096 tokens of 2048 bf16, one and four slots: 20 and 22 us, 10 and 15 so).
 // IN, DT: types of the rows and of the result.  SCALED: the rows' values are times scales[row][column / 64].
-template <int IN, int DT, bool SCALED>
+template <int IN, int DT, bool SCALED, int N>
 __global__ __launch_bounds__(kSortThreads) void unsort_kernel(const void *__restrict__ rows, const float *__restrict__ scales, const void *__restrict__ weights, int w_dtype, const int32_t *__restrict__ inverse,
                                                               int64_t T, int k, int H, int lanes_log2, void *__restrict__ out) {
   const int lanes = 1 << lanes_log2;
@@ -170,12 +171,12 @@ __global__ __launch_bounds__(kSortThreads) void unsort_kernel(const void *__rest
   const int h = (int)(blockIdx.y * lanes + (threadIdx.x & (lanes - 1))) * 8, n = H - h;
   if (n <= 0 || t >= T) return;
   float acc[8] = {};
-  for (int s0 = 0; s0 < k; s0 += 8) {
-    Octet<IN> v[8];
-    float w[8];
-    int64_t row[8];
+  for (int s0 = 0; s0 < k; s0 += N) {
+    Octet<IN> v[N];
+    float w[N];
+    int64_t row[N];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < N; ++j) {
       const int64_t s = t * k + (s0 + j < k ? s0 + j : k - 1);
       const int32_t at = inverse[s];
       row[j] = s0 + j < k && at >= 0 && at < T * k ? at : -1;
@@ -184,9 +185,9 @@ __global__ __launch_bounds__(kSortThreads) void unsort_kernel(const void *__rest
     load_octets(v, rows, row, H, h, n);
     if constexpr (SCALED)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] *= scales[(row[j] < 0 ? 0 : row[j]) * ((H + 63) / 64) + h / 64];
+      for (int j = 0; j < N; ++j) w[j] *= scales[(row[j] < 0 ? 0 : row[j]) * ((H + 63) / 64) + h / 64];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
+    for (int j = 0; j < N; ++j)
 #pragma unroll
       for (int i = 0; i < 8; ++i) acc[i] = row[j] >= 0 ? __builtin_fmaf(w[j], v[j].at(i), acc[i]) : acc[i];  // (not multiplied by zero: row or weight may be infinite)
   }
@@ -200,8 +201,9 @@ template <int IN, int DT, bool SCALED = false>
 static hipError_t launch_unsort(const void *rows, const float *scales, const void *weights, int w_dtype, const int32_t *inverse, int64_t T, int k, int H, void *out, hipStream_t st) {
   if (T == 0) return hipSuccess;
   const TokenGrid g(H, kSortThreads);
-  unsort_kernel<IN, DT, SCALED><<<dim3((unsigned)((T + g.tokens - 1) / g.tokens), (unsigned)g.columns), kSortThreads, 0, st>>>(rows, scales, weights, w_dtype, inverse, T, k, H,
-                                                                                                                              __builtin_ctz((unsigned)g.lanes), out);
+  auto *const kernel = k > 4 ? &unsort_kernel<IN, DT, SCALED, 8> : k > 2 ? &unsort_kernel<IN, DT, SCALED, 4> : &unsort_kernel<IN, DT, SCALED, 2>;
+  kernel<<<dim3((unsigned)((T + g.tokens - 1) / g.tokens), (unsigned)g.columns), kSortThreads, 0, st>>>(rows, scales, weights, w_dtype, inverse, T, k, H,
+                                                                                                         __builtin_ctz((unsigned)g.lanes), out);
   return hipGetLastError();
 }
 hipError_t launch_unsort_tokens(const void *rows, const void *weights, int w_dtype, const int32_t *inverse, int64_t T, int k, int H, int dt, void *out, hipStream_t st) {

@@ -226,8 +226,8 @@ __device__ __forceinline__ float wave_sum_f32(float v) {  // in a fixed order
   return (lane(0) + lane(16)) + (lane(32) + lane(48));
 }
 
-// A block a token; four slots' rows in flight at once.  A wave's share of a slot's dot product is kept in LDS from one pass over the columns to the next.
-template <int DT>
+// A block a token; N slots' rows in flight at once: four, or two or three where that leaves out none (4096 tokens of 2048 bf16, one slot: 16 us, 13 so; 1000 of 2045 f16, six: 16.5, 15.5).  A wave's share of a slot's dot product is kept in LDS from one pass over the columns to the next.
+template <int DT, int N>
 __global__ __launch_bounds__(kSortThreads) void unsort_grad_kernel(const void *__restrict__ dout, const void *__restrict__ rows, const void *__restrict__ weights, int w_dtype,
                                                                    const int32_t *__restrict__ inverse, int64_t T, int k, int H, void *__restrict__ drows,
                                                                    void *__restrict__ dweights) {
@@ -237,12 +237,12 @@ __global__ __launch_bounds__(kSortThreads) void unsort_grad_kernel(const void *_
   for (int h0 = 0; h0 < H; h0 += kSortThreads * 8) {
     const int h = h0 + (int)threadIdx.x * 8, n = H - h;
     const Octet<DT> g = load_octet<DT>(dout, t * H + (n > 0 ? h : 0), n > 0 ? n : 0);
-    for (int s0 = 0; s0 < k; s0 += 4) {
-      Octet<DT> v[4];
-      int64_t row[4], read[4];
-      float w[4];
+    for (int s0 = 0; s0 < k; s0 += N) {
+      Octet<DT> v[N];
+      int64_t row[N], read[N];
+      float w[N];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < N; ++j) {
         const int s = s0 + j < k ? s0 + j : k - 1;
         const int32_t at = inverse[t * k + s];
         row[j] = at >= 0 ? at : ~at;
@@ -252,7 +252,7 @@ __global__ __launch_bounds__(kSortThreads) void unsort_grad_kernel(const void *_
       }
       load_octets(v, rows, read, H, h, n);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < N; ++j) {
         Octet<DT> o{};
         float dot = 0.f;
         if (read[j] >= 0) {
@@ -277,7 +277,11 @@ __global__ __launch_bounds__(kSortThreads) void unsort_grad_kernel(const void *_
 hipError_t launch_unsort_tokens_grad(const void *dout, const void *rows, const void *weights, int w_dtype, const int32_t *inverse, int64_t T, int k, int H, int dt,
                                      void *drows, void *dweights, hipStream_t st) {
   if (T == 0) return hipSuccess;
-  auto *const kernel = dt == 0 ? &unsort_grad_kernel<0> : dt == 1 ? &unsort_grad_kernel<1> : &unsort_grad_kernel<2>;
+  auto of = [&](auto dt_of) {
+    constexpr int DT = decltype(dt_of)::value;
+    return k <= 2 ? &unsort_grad_kernel<DT, 2> : k % 3 == 0 && k < 12 ? &unsort_grad_kernel<DT, 3> : &unsort_grad_kernel<DT, 4>;
+  };
+  auto *const kernel = dt == 0 ? of(std::integral_constant<int, 0>()) : dt == 1 ? of(std::integral_constant<int, 1>()) : of(std::integral_constant<int, 2>());
   kernel<<<(unsigned)T, kSortThreads, 0, st>>>(dout, rows, weights, w_dtype, inverse, T, k, H, drows, dweights);
   return hipGetLastError();
 }

@@ -211,8 +211,10 @@ class SwitchGluF8:
 
     def __init__(self, gate_proj, up_proj, down_proj):
         self.gate_proj, self.up_proj, self.down_proj = gate_proj, up_proj, down_proj
-        self._banks = tuple((p.weight, p.scales) for p in (gate_proj, up_proj, down_proj))
         self.training = False
+
+    def _banks(self):
+        return tuple((p.weight, p.scales) for p in (self.gate_proj, self.up_proj, self.down_proj))
 
     def training_mode(self, mode):
         """The experts compute the same in training (module.rs:44-50)."""
@@ -220,10 +222,10 @@ class SwitchGluF8:
 
     def forward(self, x, inds, weights):
         """x: bfloat16 or float16 [..., H]; inds int32 and weights [..., top_k] (``ops.select_experts``, ``ops.route``) -> [..., H]."""
-        return ops.switch_glu_f8(x, inds, weights, *self._banks)
+        return ops.switch_glu_f8(x, inds, weights, *self._banks())
 
     __call__ = forward
 
     def gradient(self, dout, x, inds, weights):
         """(dx, dweights) for the gradient dout that arrives at forward's result."""
-        return ops.switch_glu_f8_grad(dout, x, inds, weights, *self._banks)
+        return ops.switch_glu_f8_grad(dout, x, inds, weights, *self._banks())

@@ -250,9 +250,6 @@ typedef uint32_t u32x4_f8 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ f32x16_t mfma_f8_32(i32x8_t a, i32x8_t b, f32x16_t c) {
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
 }
-__device__ __forceinline__ f32x4_t mfma_f8_16(i32x8_t a, i32x8_t b, f32x4_t c) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
-}
 // eight codes as bf16 (exact)
 __device__ __forceinline__ bf16x8_t codes_to_bf16(uint32_t lo, uint32_t hi) {
   typedef __bf16 pair_t __attribute__((ext_vector_type(2)));

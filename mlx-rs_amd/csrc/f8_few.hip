@@ -1,10 +1,11 @@
 // Product of a few rows a matrix with e4m3 weights: one token's or a decode batch's linear layers and experts.  Memory bound: a matrix's codes are read once for up to
 // 16 TG rows.
 //
-// A block of four waves computes 16 weight rows (the rows of a 16x16x128 matrix instruction) for up to 16 TG token rows (its columns).  The waves share the summed
+// A block of four waves computes 16 weight rows (the rows of 16x16x32 matrix instructions) for up to 16 TG token rows (their columns).  The waves share the summed
 // axis, every fourth run of 128 values each; a lane's 32 bytes of a run are two pieces of 16, at 16 (l / 16) and 64 bytes on, for codes and rows alike (which values a lane
-// multiplies is free as long as both sides agree), so that one load takes 64 consecutive bytes of a weight row.  Codes go from memory into the instruction's
-// registers, nothing is unpacked; token rows come the same way out of L2.  A run's sums are scaled in float32; the waves' sums meet in LDS in a fixed order.
+// multiplies is free as long as both sides agree), so that one load takes 64 consecutive bytes of a weight row.  Codes go from memory into registers and there to bf16, where their
+// products are exact and sums float32 (f8.hpp; on the f8 instructions, which take the codes as they are, a launch waits for the same bytes: 300 rows at 128 matrices of 768 x 2048
+// 37 us either way, one row of 4096 x 4096 6.8); token rows come the same way out of L2.  A run's sums are scaled in float32; the waves' sums meet in LDS in a fixed order.
 #include "f8.hpp"
 #include "octets.hpp"
 
@@ -50,21 +51,16 @@ __device__ __forceinline__ void round_run(const F8Product &a, int64_t from_row, 
 struct FewRow {
   u32x4_f8 v[2];
 };
-template <bool F32>
 __device__ __forceinline__ f32x4_t few_run(const u32x4_f8 (&w)[2], const FewRow &x) {
   f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
-  if constexpr (F32) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+  for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int p = 0; p < 2; ++p)
-        sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes_to_bf16(w[h][2 * p], w[h][2 * p + 1]), codes_to_bf16(x.v[h][2 * p], x.v[h][2 * p + 1]), sum, 0, 0, 0);
-  } else {
-    sum = mfma_f8_16(__builtin_bit_cast(i32x8_t, w), __builtin_bit_cast(i32x8_t, x), sum);
-  }
+    for (int p = 0; p < 2; ++p)
+      sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes_to_bf16(w[h][2 * p], w[h][2 * p + 1]), codes_to_bf16(x.v[h][2 * p], x.v[h][2 * p + 1]), sum, 0, 0, 0);
   return sum;
 }
-template <int TG, bool F32, F8In IN>  // F32: on the bf16 instructions
+template <int TG, F8In IN>
 __global__ __launch_bounds__(kFewWaves *kWave) void f8_few_kernel(F8Product a) {
   constexpr int AHEAD = TG == 1 ? 4 : 2;  // runs whose loads are in flight at once
   extern __shared__ __align__(16) uint8_t own_rows[];  // [rows][whole runs + 16], then scales [rows][runs]
@@ -147,7 +143,7 @@ __global__ __launch_bounds__(kFewWaves *kWave) void f8_few_kernel(F8Product a) {
     for (int i = 0; i < AHEAD; ++i)
 #pragma unroll
       for (int t = 0; t < TG; ++t) {
-        const f32x4_t sum = few_run<F32>(wv[i], xv[i][t]);
+        const f32x4_t sum = few_run(wv[i], xv[i][t]);
         const float f = s[i] * sx[i][t];
 #pragma unroll
         for (int v = 0; v < 4; ++v) acc[t][v] = __builtin_fmaf(sum[v], f, acc[t][v]);
@@ -228,7 +224,7 @@ __global__ __launch_bounds__(kTokenWaves *kWave) void f8_token_kernel(F8Product 
     for (int i = 0; i < AHEAD; ++i) {
       const Item it = item(i0 + i);
       const uint8_t *const x = own_rows + it.slot * (wide + 16) + it.run * kF8Run + part * 16;
-      const f32x4_t sum = few_run<true>(wv[i], {*reinterpret_cast<const u32x4_f8 *>(x), *reinterpret_cast<const u32x4_f8 *>(x + 64)});
+      const f32x4_t sum = few_run(wv[i], {*reinterpret_cast<const u32x4_f8 *>(x), *reinterpret_cast<const u32x4_f8 *>(x + 64)});
       const float f = it.there ? s[i] * own_scales[it.slot * runs + it.run] : 0.f;
 #pragma unroll
       for (int v = 0; v < 4; ++v) acc[v] = __builtin_fmaf(sum[v], f, acc[v]);
@@ -284,8 +280,7 @@ hipError_t launch_f8_few(const F8Product &p, hipStream_t st) {
   };
   auto kind = [&](auto in_of) {
     constexpr F8In IN = decltype(in_of)::value;
-    if (p.dt == 2) return tile == 32 ? launch(&f8_few_kernel<2, true, IN>) : launch(&f8_few_kernel<1, true, IN>);
-    return tile == 32 ? launch(&f8_few_kernel<2, false, IN>) : launch(&f8_few_kernel<1, false, IN>);
+    return tile == 32 ? launch(&f8_few_kernel<2, IN>) : launch(&f8_few_kernel<1, IN>);
   };
   return !p.raw ? kind(std::integral_constant<F8In, kCodes>()) : !p.raw_up ? kind(std::integral_constant<F8In, kRaw>()) : kind(std::integral_constant<F8In, kGateUp>());
 }

@@ -48,8 +48,8 @@ int mi_moe_dequantize_f8(const void *codes, const float *scales, int64_t rows, i
 /* ---- The linear layer on such weights: y = q(x) . W^T + linear_bias (transpose), or y = q(x) . W, which is its gradient with respect to its input.
  * q: rows to e4m3 with a scale for each run of 128 values, as mi_moe_quantize_f8 makes them.  x [M, K], y [M, N] and linear_bias [N] (transpose only; or NULL) of element
  * type dtype, sums in float32, each result rounded once.  W [N, K] (transpose; K a multiple of 16) or [K, N] (N a multiple of 16), 16-byte aligned; scales of its blocks.
- * M N and M K up to 2^35, N and K up to 2^22.  16-bit results are summed on the f8 matrix instructions, whose sums over a run are off by up to 2^-11 of its largest
- * product; float32 results are not.  A row's scale times a block's is made in float32 and has to lie in its range.
+ * M N and M K up to 2^35, N and K up to 2^22.  bfloat16 results may be summed on the f8 matrix instructions, whose sums over a run are off by up to 2^-11 of its largest
+ * product; float16 and float32 results are not.  A row's scale times a block's is made in float32 and has to lie in its range.
  * workspace >= mi_moe_linear_f8_workspace_size, 16-byte aligned. ---- */
 int mi_moe_linear_f8_workspace_size(int64_t M, int32_t N, int32_t K, size_t *bytes);
 int mi_moe_linear_f8(const void *x, const void *w, const float *scales, const void *linear_bias, int64_t M,

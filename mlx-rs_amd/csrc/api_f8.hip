@@ -296,8 +296,7 @@ int mi_moe_switch_glu_f8(const void *x, const uint32_t *topk_idx, const void *to
     p.y = ws.g;
     p.y1 = ws.u;
   } else {
-    // (results of float16 would show what the f8 instructions lose of gate and up, in the codes that it changes)
-    p.dt = dtype == MI_MOE_DTYPE_F16 ? MI_MOE_DTYPE_F32 : dtype;
+    p.dt = dtype;  // (which instructions)
     p.h = ws.h.codes;
     p.hs = ws.h.scales;
   }

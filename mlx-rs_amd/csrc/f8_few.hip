@@ -264,7 +264,7 @@ int f8_tile_rows(const F8Product &p) {
   // Tiles of 64 / 128 rows to float32, us: 16 matrices of 1792 x 2048 at 56, 72, 100, 160 rows each 29 / 31, 31 / 37, 45 / 39, 51 / 42; 128 of 768 x 2048 72 / 77, 94 / 87, 127 / 99,
   // 171 / 142.  To bfloat16, of 64 / 128 / 256 rows: the 128 at 40, 72, 100, 128, 200 rows 50 / 51 / 53, 81 / 63 / 67, 105 / 73 / 79, 117 / 96 / 90, 168 / 133 / 107; the 16, which have
   // fewer tiles than there are CUs, at 56, 100, 200, 260 rows 24 / 24 / 26, 41 / 26 / 29, 48 / 32 / 41, 54 / 50 / 43.
-  if (p.dt == 2) return avg > 64 ? 128 : 64;
+  if (f8_exact(p)) return avg > 64 ? 128 : 64;
   return avg > (tiles >= 256 ? 112 : 208) ? 256 : avg > 48 ? 128 : 64;
 }
 

@@ -69,7 +69,8 @@ __global__ __launch_bounds__(256) void f8_parts_kernel(const float *__restrict__
   store4(y, row * N + n, N - n, dt, sum);
 }
 
-template <int TM, F8Mode MODE, bool F32>
+// EXACT: on the bf16 instructions (f8_exact).  WIDE: results are float32.
+template <int TM, F8Mode MODE, bool EXACT, bool WIDE>
 __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, F8Grid g) {
   typedef F8Stage<TM> L;
   constexpr int XC = TM / 64, MT = TM / 64;  // copies of token rows a wave; sub-tiles of 32 token rows a wave
@@ -223,7 +224,7 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, F8Gri
     return v;
   };
   auto multiply = [&](const i32x8_t &w, const i32x8_t &x, f32x16_t sum) __attribute__((always_inline)) {
-    if constexpr (F32) {
+    if constexpr (EXACT) {
 #pragma unroll
       for (int p = 0; p < 4; ++p)
         sum = __builtin_amdgcn_mfma_f32_32x32x16_bf16(codes_to_bf16((uint32_t)w[2 * p], (uint32_t)w[2 * p + 1]), codes_to_bf16((uint32_t)x[2 * p], (uint32_t)x[2 * p + 1]), sum, 0, 0, 0);
@@ -373,12 +374,12 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, F8Gri
         }
     }
   } else {
-    constexpr int SIZE = F32 ? 4 : 2, EACH = 16 / SIZE, PASSES = F32 ? 2 : 1;  // bytes of a value, values of a piece; 64 weight rows at once, or 32
+    constexpr int SIZE = WIDE ? 4 : 2, EACH = 16 / SIZE, PASSES = WIDE ? 2 : 1;  // bytes of a value, values of a piece; 64 weight rows at once, or 32
     unsigned char *const own = lds + wave * (32 * MT * 128);
     float down[MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t) down[t] = 1.f;
-    if constexpr (!F32) {
+    if constexpr (!WIDE) {
       if (a.y_scales) {
         // to within 2^15, by the exponent of the largest of a row's 64 values
         const int column = n0 / 64 + wn;
@@ -410,7 +411,7 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, F8Gri
 #pragma unroll
     for (int pass = 0; pass < PASSES; ++pass) {
 #pragma unroll
-      for (int i = pass; i < (F32 ? pass + 1 : 2); ++i)
+      for (int i = pass; i < (WIDE ? pass + 1 : 2); ++i)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           float bias[4] = {0.f, 0.f, 0.f, 0.f};
@@ -427,9 +428,9 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, F8Gri
             float o[4];
 #pragma unroll
             for (int v = 0; v < 4; ++v) o[v] = __builtin_fmaf(acc[t][i][4 * g + v], down[t], bias[v]);
-            const int piece = F32 ? 2 * g + half : i * 4 + g;
-            unsigned char *const to = own + r * 128 + (piece ^ f8_turn(r)) * 16 + (F32 ? 0 : half * 8);
-            if constexpr (F32) *reinterpret_cast<f32x4_t *>(to) = f32x4_t{o[0], o[1], o[2], o[3]};
+            const int piece = WIDE ? 2 * g + half : i * 4 + g;
+            unsigned char *const to = own + r * 128 + (piece ^ f8_turn(r)) * 16 + (WIDE ? 0 : half * 8);
+            if constexpr (WIDE) *reinterpret_cast<f32x4_t *>(to) = f32x4_t{o[0], o[1], o[2], o[3]};
             else if (a.dt == 0 && !a.y_scales) *reinterpret_cast<uint2 *>(to) = make_uint2(cvt_pk_bf16(o[0], o[1]), cvt_pk_bf16(o[2], o[3]));
             else *reinterpret_cast<uint2 *>(to) = make_uint2(pack_f16(o[0], o[1]), pack_f16(o[2], o[3]));
           }
@@ -477,11 +478,11 @@ F8Plan f8_plan(const F8Product &p) {
     return p.parts ? plan_of(p, best.tile, (p.rows / best.tile + (p.n_mats < p.rows ? p.n_mats : p.rows)) * columns, best, least) : best;
   }
   for (int tile : {64, 128, 256})
-    if (tile != 256 || p.dt != 2) best = plan_of(p, tile, (p.rows + tile - 1) / tile * columns, best, least);
+    if (tile != 256 || !f8_exact(p)) best = plan_of(p, tile, (p.rows + tile - 1) / tile * columns, best, least);
   return best;
 }
 
-template <int TM, F8Mode MODE, bool F32>
+template <int TM, F8Mode MODE, bool EXACT, bool WIDE>
 static hipError_t launch_tiles(const F8Product &p, hipStream_t st) {
   constexpr size_t lds = f8_tiles_lds(TM);
   constexpr int kMaxDevices = 64;
@@ -489,7 +490,7 @@ static hipError_t launch_tiles(const F8Product &p, hipStream_t st) {
   int dev = 0;
   if (hipError_t e = hipGetDevice(&dev); e != hipSuccess) return e;
   if (dev < 0 || dev >= kMaxDevices || !raised[dev].load(std::memory_order_acquire)) {
-    if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&f8_tiles_kernel<TM, MODE, F32>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds); e != hipSuccess) return e;
+    if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&f8_tiles_kernel<TM, MODE, EXACT, WIDE>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds); e != hipSuccess) return e;
     if (dev >= 0 && dev < kMaxDevices) raised[dev].store(true, std::memory_order_release);
   }
   const int64_t n_tiles = (p.N + (MODE == kPair ? 127 : kF8TileN - 1)) / (MODE == kPair ? 128 : kF8TileN), m_tiles = p.list ? f8_most_pieces(p.rows, p.n_mats, TM) : (p.rows + TM - 1) / TM;
@@ -508,7 +509,7 @@ static hipError_t launch_tiles(const F8Product &p, hipStream_t st) {
   }
   if (each > (int64_t)1 << 19) return hipErrorInvalidValue;  // (a launch has less than 2^32 threads)
   const unsigned used = (unsigned)((steps + g.part_steps - 1) / g.part_steps);
-  f8_tiles_kernel<TM, MODE, F32><<<dim3((unsigned)(each * 8), used, p.y1 ? 2 : 1), kF8Threads, lds, st>>>(p, g);
+  f8_tiles_kernel<TM, MODE, EXACT, WIDE><<<dim3((unsigned)(each * 8), used, p.y1 ? 2 : 1), kF8Threads, lds, st>>>(p, g);
   if (used > 1) f8_parts_kernel<<<dim3((unsigned)((p.N + 1023) / 1024), (unsigned)p.rows), 256, 0, st>>>(p.parts, (int)used, p.rows, p.N, p.bias, p.dt, p.y);
   return hipGetLastError();
 }
@@ -516,8 +517,11 @@ static hipError_t launch_tiles(const F8Product &p, hipStream_t st) {
 template <F8Mode MODE>
 static hipError_t launch_mode(const F8Product &p, hipStream_t st) {
   const int tile = f8_plan(p).tile;
-  if (p.dt == 2) return tile == 128 ? launch_tiles<128, MODE, true>(p, st) : launch_tiles<64, MODE, true>(p, st);
-  return tile == 256 ? launch_tiles<256, MODE, false>(p, st) : tile == 128 ? launch_tiles<128, MODE, false>(p, st) : launch_tiles<64, MODE, false>(p, st);
+  if (!f8_exact(p))
+    return tile == 256 ? launch_tiles<256, MODE, false, false>(p, st) : tile == 128 ? launch_tiles<128, MODE, false, false>(p, st) : launch_tiles<64, MODE, false, false>(p, st);
+  if constexpr (MODE != kPair)
+    if (p.dt == 2) return tile == 128 ? launch_tiles<128, MODE, true, true>(p, st) : launch_tiles<64, MODE, true, true>(p, st);
+  return tile == 128 ? launch_tiles<128, MODE, true, false>(p, st) : launch_tiles<64, MODE, true, false>(p, st);
 }
 
 hipError_t launch_f8_tiles(const F8Product &p, hipStream_t st) {

@@ -52,3 +52,37 @@ def test_a_few_rows(M, dtype, kind):
     o.within(linear(), want, off, f"linear {M} {dtype} {kind}")
     if M <= 4:
         o.within(grouped(), want, off, f"grouped {M} {dtype} {kind}")
+
+
+@pytest.mark.parametrize("kind", ["pairs", "eights"])
+@pytest.mark.parametrize("transpose", [True, False])
+@pytest.mark.parametrize("dtype", DTYPES[1:])
+@pytest.mark.parametrize("M", [1, 40, 100, 300])
+def test_float16_and_float32_in_tiles(M, dtype, transpose, kind):
+    linear, grouped, want, off = calls(M, dtype, transpose, kind)
+    o.within(linear(), want, off, f"linear {M} {dtype} {transpose} {kind}")
+    o.within(grouped(), want, off, f"grouped {M} {dtype} {transpose} {kind}")
+
+
+def down_of_large_products(T, dtype):
+    """gate = up = 1 makes every value of h silu(4) * 4, of which all codes are 448; down's products are 448 * 448 and -448 * 448 in every eight, and small ones of one sign.
+    What the experts give, what they should, and by what that may be off but for down's sums: the roundings of silu and of h's scale (2^-20 for all of them), float32's of the sum."""
+    from mlx_rs_amd import ops
+    K = 256
+    ones = torch.ones((2, K, 128), device="cuda").to(o.F8), torch.full((2, 2, 1), 4.0 / 128, device="cuda")
+    w = torch.full((128, K), 0.0625, device="cuda", dtype=torch.float64)
+    w[:, 1::8], w[:, 6::8] = 448.0, -448.0
+    w[::2] = w[::2] * torch.where(w[::2].abs() < 1, 7.0, 1.0)
+    down = w.float().to(o.F8).expand(2, 128, K).contiguous(), torch.full((2, 1, 2), 2.0 ** -9, device="cuda")
+    x = torch.ones((T, 128), device="cuda", dtype=dtype)
+    inds = torch.tensor([0, 1], device="cuda", dtype=torch.int32).expand(T, 2).contiguous()
+    y = ops.switch_glu_f8(x, inds, torch.full((T, 2), 0.5, device="cuda"), ones, ones, down)
+    h = 16.0 / (1.0 + torch.exp(torch.tensor(-4.0, dtype=torch.float64))).item() * 2.0 ** -9
+    want = (w.sum(1) * h).expand(T, 128)
+    return y, want, want.abs() * 2.0 ** -20 + (w.abs().sum(1) * h * (K + 2) * 2.0 ** -24).expand(T, 128)
+
+
+@pytest.mark.parametrize("T,dtype", [(1, torch.bfloat16), (1, torch.float16), (3, torch.bfloat16), (3, torch.float16), (40, torch.float16), (300, torch.float16)])
+def test_experts_whose_down_has_large_products(T, dtype):
+    y, want, off = down_of_large_products(T, dtype)
+    o.within(y, want, off + off.new_tensor(2.0 ** -11) * want.abs(), f"experts {T} {dtype}")  # (the rows on their way to the sum over slots have 11 bits)

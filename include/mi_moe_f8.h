@@ -67,8 +67,9 @@ int mi_moe_grouped_linear_f8(const void *x, const void *w, const float *scales, 
  *   out[t] = sum over s of topk_w[t][s] * q(silu(q(x[t]) . gate_e^T) * (q(x[t]) . up_e^T)) . down_e^T,   e = topk_idx[t][s]
  * gate, up [n_experts, intermediate, hidden], down [n_experts, hidden, intermediate], scales of their blocks (f32 [n_experts, ceil(rows / 128), ceil(cols / 128)]); 16-byte
  * aligned; hidden and intermediate multiples of 16, up to 2^22; x and out [T, hidden] bfloat16 or float16; topk_w of element type w_dtype.  Products are summed as mi_moe_linear_f8's of
- * x's type (with bfloat16, a code of the rounded silu(gate) * up that lies at a border may so be its neighbour).  Experts' results are summed over the slots in float32, from 11 significant bits of each or more (of those below 2^-28 of the largest of 64 beside each other, fewer).  Slots that name no expert have no part in
- * it.  T * hidden, each rounded up to whole runs of 128, below 2^32; T * top_k up to 2^24 - 1, and times hidden or intermediate up to 2^35.
+ * x's type (with bfloat16, a code of the rounded silu(gate) * up that lies at a border may so be its neighbour).  Experts' results are summed over the slots in float32, those of
+ * bfloat16 tokens from 11 significant bits of each or more (of those below 2^-28 of the largest of 64 beside each other, fewer).  Slots that name no expert have no part in it.
+ * T * hidden, each rounded up to whole runs of 128, below 2^32; T * top_k up to 2^24 - 1, and times hidden or intermediate up to 2^35.
  * workspace >= mi_moe_switch_glu_f8_workspace_size (grad: of the gradient), 16-byte aligned. ---- */
 typedef struct {
   const void *gate;

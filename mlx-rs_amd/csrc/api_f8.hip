@@ -1,6 +1,8 @@
 // C ABI of the experts and linear layers on e4m3 weights (include/mi_moe_f8.h): validation, workspaces and the launch sequences.
 #include "../../include/mi_moe_f8.h"
 
+#include <algorithm>
+
 #include "entries.hpp"
 #include "f8.hpp"
 
@@ -121,10 +123,15 @@ struct ExpertsWs {
         x(c, T, H), dout(c, grad ? T : 0, H), g(c.take<float>(float_rows(P, E, grad) * I)), u(c.take<float>(float_rows(P, E, grad) * I)), dh(c.take<float>(grad ? (size_t)P * I : 0)),
         h(c, P, I, grad ? 2 : 1), y(c.take<char>(y_bytes(P, H, E))), y_scales(c.take<float>((size_t)P * ((H + 63) / 64))),
         parts(reinterpret_cast<float *>(c.take<char>(grad ? f8_parts_bytes(P < (int64_t)16 * E ? P : (int64_t)16 * E, H > I ? H : I) : 0))), bytes(c.off + 256) {}
-  static size_t y_bytes(int64_t P, int H, int E) {
-    const size_t halves = (size_t)P * H * 2, floats = (size_t)(P < (int64_t)16 * E ? P : (int64_t)16 * E) * H * 4;  // (few rows an expert: floats)
-    return halves > floats ? halves : floats;
+  static size_t y_bytes(int64_t P, int H, int E) {  // halves, or floats: of few rows an expert (all columns), or of some columns at a time
+    return std::max({(size_t)P * H * 2, (size_t)std::min(P, (int64_t)16 * E) * H * 4, (size_t)P * half_columns(H) * 4});
   }
+  static int half_columns(int H) { return std::min(H, ((H + kF8TileN - 1) / kF8TileN + 1) / 2 * kF8TileN); }  // whole tiles
+
+ public:
+  static int float_columns(int64_t P, int H, int E) { return P <= (int64_t)16 * E ? H : half_columns(H); }  // columns of float32 rows that y holds
+
+ private:
   static size_t float_rows(int64_t P, int E, bool grad) { return (size_t)(grad || P <= (int64_t)16 * E ? P : (int64_t)16 * E); }  // (never less for more tokens)
 };
 
@@ -141,6 +148,18 @@ int check_switch(const char *who, const mi_moe_f8_experts *e, const void *x, con
   if (!aligned16(e->gate) || !aligned16(e->up) || !aligned16(e->down)) return fail("%s: weights must be 16-byte aligned", who);
   if (!x || !idx || !w) return fail("%s: x, topk_idx and topk_w must be non-NULL", who);
   return 0;
+}
+
+// A product of sorted rows, and the sums of tokens' rows over the slots, `columns` at a time.
+hipError_t product_to_tokens(F8Product p, int columns, const void *weights, int w_dtype, const int32_t *inverse, int64_t T, int k, int dt, void *out, hipStream_t st) {
+  const int H = p.N;
+  for (int n = 0; n < H; n += columns) {
+    const int count = std::min(columns, H - n);
+    if (count < H) p.n_first = n, p.n_count = count;
+    if (hipError_t e = launch_f8_product(p, st); e != hipSuccess) return e;
+    if (hipError_t e = launch_unsort_made(p.y, p.y_scales, weights, w_dtype, inverse, T, k, count, dt, static_cast<uint16_t *>(out) + n, H, st); e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 F8Mat mat(const void *w, const float *s) { return {static_cast<const uint8_t *>(w), s}; }
@@ -300,7 +319,7 @@ int mi_moe_switch_glu_f8(const void *x, const uint32_t *topk_idx, const void *to
     p.h = ws.h.codes;
     p.hs = ws.h.scales;
   }
-  if (f8_few_rows(d)) d.dt = MI_MOE_DTYPE_F32;
+  if (f8_few_rows(d) || dtype == MI_MOE_DTYPE_F16) d.dt = MI_MOE_DTYPE_F32;
   else d.y_scales = ws.y_scales;
   F8Lists lists;
   lists.offsets = ws.offsets;
@@ -327,8 +346,7 @@ int mi_moe_switch_glu_f8(const void *x, const uint32_t *topk_idx, const void *to
     return 0;
   }
   if (few && !in_blocks) MI_HIP(launch_swiglu_f8(ws.g, ws.u, P, intermediate, ws.h.out(P, intermediate), st));
-  MI_HIP(launch_f8_product(d, st));
-  MI_HIP(launch_unsort_made(ws.y, d.y_scales, topk_w, w_dtype, ws.inverse, T, top_k, hidden, dtype, out, st));
+  MI_HIP(product_to_tokens(d, d.y_scales ? hidden : ExpertsWs::float_columns(P, hidden, n_experts), topk_w, w_dtype, ws.inverse, T, top_k, dtype, out, st));
   return 0;
 } MI_CATCH("switch_glu_f8")
 
@@ -376,8 +394,15 @@ int mi_moe_switch_glu_f8_grad(const void *dout, const void *x, const uint32_t *t
   d.N = hidden;
   d.K = intermediate;
   d.y = ws.y;
-  d.y_scales = ws.y_scales;
-  d.dt = dtype;
+  int columns = hidden;
+  if (dtype == MI_MOE_DTYPE_F16) {
+    d.dt = MI_MOE_DTYPE_F32;
+    if (hidden <= 3 * (int64_t)intermediate) d.y = ws.g;  // (to dh: read by then.  1000 tokens through 2 of 16 experts of 2048 x 1792: 183 us, with half of the columns at a time 231)
+    else columns = ExpertsWs::float_columns(P, hidden, n_experts);
+  } else {
+    d.dt = dtype;
+    d.y_scales = ws.y_scales;
+  }
   if (P <= (int64_t)16 * n_experts) {  // (room for float32 rows, and for parts)
     b.parts = d.parts = ws.parts;
     d.list = ws.list[1];
@@ -401,8 +426,7 @@ int mi_moe_switch_glu_f8_grad(const void *dout, const void *x, const uint32_t *t
   MI_HIP(launch_f8_product(p, st));
   MI_HIP(launch_f8_product(b, st));
   MI_HIP(launch_swiglu_f8_grad({ws.g, ws.u, ws.dh, topk_w, w_dtype, ws.order, ws.offsets, n_experts, P, intermediate, ws.h.codes, ws.h.scales, dweights}, st));
-  MI_HIP(launch_f8_product(d, st));
-  MI_HIP(launch_unsort_made(ws.y, d.y_scales, nullptr, 0, ws.inverse, T, top_k, hidden, dtype, dx, st));
+  MI_HIP(product_to_tokens(d, columns, nullptr, 0, ws.inverse, T, top_k, dtype, dx, st));
   return 0;
 } MI_CATCH("switch_glu_f8_grad")
 

@@ -47,20 +47,23 @@ struct F8Product {
   bool transpose;           // matrices [N][K], else [K][N]
   bool pair_sum;
   int N, K;
+  int n_first, n_count;     // tiles: the columns of y that are computed, from a multiple of kF8TileN on, and as many values a row of y has; n_count 0: all N
   const void *bias;
   void *y, *y1;
   int dt;
-  float *y_scales;  // tiles: y is float16 whatever dt, a row's values of 64 columns times a power of two of their own, [rows][columns / 64] (the other way round
+  float *y_scales;  // tiles, bfloat16: y is float16, a row's values of 64 columns times a power of two of their own, [rows][columns / 64] (the other way round
                     // the sum over the slots of 4096 tokens read a line for every scale and took 40 us, not 37).  Rows that are summed over
-                    // slots afterwards: rounded to bfloat16 here and once more behind the sum, the experts' results were 1.5 times as far off as with one rounding.
+                    // slots afterwards: rounded to bfloat16 here and once more behind the sum, the experts' results were 1.5 times as far off as with one rounding.  (Those to be summed to float16
+                    // would be 1.4 times as far off with these: they are float32, some columns at a time.)
   float *parts;  // room for the sums of blocks that share a tile's summed axis (f8_parts_bytes), or nullptr: none do
   uint8_t *h;  // gate/up pairs: silu(gate) * up in e4m3, as F8Rows
   float *hs;
 };
 // Whether tiles sum on the bf16 instructions: for results (or, of gate/up pairs, tokens) of float16 and float32.  Us, to float16, so and on the f8 instructions, rounding of the rows and all:
-// 4096^3 157 and 87, 1000 x 4096 x 4096 49 and 39, its gradient 56 and 46; 4096 tokens through 8 of 128 experts of 2048 x 768 527 and 478.
+// 4096^3 157 and 87, 1000 x 4096 x 4096 49 and 39, its gradient 56 and 46; 4096 tokens through 8 of 128 experts of 2048 x 768 570 and 478.
 inline bool f8_exact(const F8Product &p) { return p.dt != 0; }
 // Parts are made where tiles of 64 x 256 and more are fewer than the chip's CUs: kF8MostParts of a product at most, 256 tiles of all of them.
+constexpr int kF8TileN = 256;  // columns of a tile
 constexpr int kF8MostParts = 16;
 constexpr int64_t kF8PartsMost = (int64_t)256 * 256 * 256;  // values
 inline size_t f8_parts_bytes(int64_t M, int N) {
@@ -142,9 +145,9 @@ constexpr int64_t kSortSmall = 2048;  // pairs up to which one launch sorts, and
 // rows != nullptr: the sorted rows of x, those that no slot names zeros
 // lists (up to kSortSmall pairs): made beside it
 hipError_t launch_sort_tokens(const SortTokens &a, const void *x, int dt, int H, void *rows, void *scratch, hipStream_t st, const F8Lists &lists = F8Lists());
-// weights nullptr: sums without weights (the sorting's gradient).  out of type dt; rows of type dt, or scaled float16 (y_scales), or float32 for fewer bits of dt
+// weights nullptr: sums without weights (the sorting's gradient).  out of type dt, its rows out_stride values from each other; rows of type dt, or scaled float16 (y_scales), or float32 for fewer bits of dt
 hipError_t launch_unsort_made(const void *rows, const float *y_scales, const void *weights, int w_dtype, const int32_t *inverse, int64_t T, int k, int H, int dt, void *out,
-                              hipStream_t st);
+                              int out_stride, hipStream_t st);
 hipError_t launch_unsort_tokens(const void *rows, const void *weights, int w_dtype, const int32_t *inverse, int64_t T, int k, int H, int dt, void *out,
                                 hipStream_t st);
 hipError_t launch_unsort_tokens_grad(const void *dout, const void *rows, const void *weights, int w_dtype, const int32_t *inverse, int64_t T, int k, int H, int dt,

@@ -12,7 +12,7 @@
 namespace mi_moe {
 
 enum F8Mode { kRowsOfWeights, kPair, kColsOfWeights };  // matrices [N][K]; two such, into h; matrices [K][N]
-constexpr int kF8TileN = 256, kF8Threads = 512, kF8FewPieces = 32;
+constexpr int kF8Threads = 512, kF8FewPieces = 32;
 constexpr uint32_t kF8Outside = 0xfffffff0u;  // an offset past every descriptor's end: zeros
 
 // 4 bytes a lane into LDS, at `to` + 4 lane
@@ -45,6 +45,7 @@ constexpr size_t f8_tiles_lds(int tm) {  // two stages, and what a thread copies
 struct F8Grid {
   int m_tiles, n_tiles, xcds_m, m_each, n_each;  // one matrix: xcds_m XCDs along the token rows, rectangles of m_each x n_each tiles
   int part_steps;                                // stages of a block: fewer than all where blocks share a tile, whose sums then go to a.parts
+  int n_first, n_end;                            // columns of y (F8Product)
 };
 
 // Sums of parts, in their order, a bias added, rounded.
@@ -99,17 +100,18 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, F8Gri
   if (rows == 0) return;
   const int lane = threadIdx.x & 63, ln = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 2, wn = wave & 3;
-  const int n0 = nt * (MODE == kPair ? 128 : kF8TileN);
+  const int n0 = MODE == kPair ? nt * 128 : g.n_first + nt * kF8TileN, n_end = g.n_end;
+  const int64_t y_stride = n_end - g.n_first;  // (column n of y's row r: r y_stride + n - n_first)
   const int product = MODE == kRowsOfWeights ? (int)blockIdx.z : 0;  // (two at most, of the same rows)
   void *const y = product ? a.y1 : a.y;
   if (mat == a.n_mats) {  // rows of no matrix (scaled ones are read by nobody)
     if constexpr (MODE != kPair) {
       const float none[4] = {0.f, 0.f, 0.f, 0.f};
       const bool part = g.part_steps < steps;
-      void *const to = part ? a.parts + (int64_t)blockIdx.y * a.rows * N : y;
+      void *const to = part ? a.parts + (int64_t)blockIdx.y * a.rows * N : y;  // (parts: of all columns)
       for (int i = threadIdx.x; i < rows * (kF8TileN / 4); i += kF8Threads) {
         const int n = n0 + i % (kF8TileN / 4) * 4;
-        if (n < N) store4(to, (int64_t)(row0 + i / (kF8TileN / 4)) * N + n, N - n, part ? 2 : a.dt, none);
+        if (n < n_end) store4(to, (row0 + i / (kF8TileN / 4)) * y_stride + n - g.n_first, n_end - n, part ? 2 : a.dt, none);
       }
     }
     return;
@@ -441,14 +443,14 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, F8Gri
         const int r = r0 + lane / 8, n = n0 + wn * 64 + pass * 32 + ((lane % 8) ^ f8_turn(r)) * EACH;
         const u32x4_f8 v = *reinterpret_cast<const u32x4_f8 *>(own + r * 128 + lane % 8 * 16);
         const int row = (r0 / 32 * 2 + wm) * 32 + r % 32;
-        if (row < rows && n < N) {
-          unsigned char *const to = static_cast<unsigned char *>(y) + ((int64_t)(row0 + row) * N + n) * SIZE;
-          if (n + EACH <= N) {
+        if (row < rows && n < n_end) {
+          unsigned char *const to = static_cast<unsigned char *>(y) + ((row0 + row) * y_stride + n - g.n_first) * SIZE;
+          if (n + EACH <= n_end) {
             __builtin_memcpy(to, &v, 16);
           } else {
 #pragma unroll
             for (int e = 0; e < EACH; ++e)
-              if (n + e < N) __builtin_memcpy(to + e * SIZE, reinterpret_cast<const unsigned char *>(&v) + e * SIZE, SIZE);
+              if (n + e < n_end) __builtin_memcpy(to + e * SIZE, reinterpret_cast<const unsigned char *>(&v) + e * SIZE, SIZE);
           }
         }
       }
@@ -493,9 +495,10 @@ static hipError_t launch_tiles(const F8Product &p, hipStream_t st) {
     if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&f8_tiles_kernel<TM, MODE, EXACT, WIDE>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds); e != hipSuccess) return e;
     if (dev >= 0 && dev < kMaxDevices) raised[dev].store(true, std::memory_order_release);
   }
-  const int64_t n_tiles = (p.N + (MODE == kPair ? 127 : kF8TileN - 1)) / (MODE == kPair ? 128 : kF8TileN), m_tiles = p.list ? f8_most_pieces(p.rows, p.n_mats, TM) : (p.rows + TM - 1) / TM;
+  const int n_end = p.n_count ? p.n_first + p.n_count : p.N;
+  const int64_t n_tiles = (n_end - p.n_first + (MODE == kPair ? 127 : kF8TileN - 1)) / (MODE == kPair ? 128 : kF8TileN), m_tiles = p.list ? f8_most_pieces(p.rows, p.n_mats, TM) : (p.rows + TM - 1) / TM;
   const int steps = f8_runs(p.K) * (p.pair_sum ? 2 : 1), parts = f8_plan(p).parts;
-  F8Grid g{(int)m_tiles, (int)n_tiles, 1, (int)m_tiles, (int)((n_tiles + 7) / 8), (steps + parts - 1) / parts};
+  F8Grid g{(int)m_tiles, (int)n_tiles, 1, (int)m_tiles, (int)((n_tiles + 7) / 8), (steps + parts - 1) / parts, p.n_first, n_end};
   int64_t each;  // blocks of an XCD
   if (p.list) {
     each = m_tiles < kF8FewPieces ? (m_tiles * n_tiles + 7) / 8 : (m_tiles + 7) / 8 * n_tiles;

@@ -165,7 +165,7 @@ __device__ __forceinline__ void load_octets(Octet<DT> (&v)[N], const void *rows,
 // IN, DT: types of the rows and of the result.  SCALED: the rows' values are times scales[row][column / 64].
 template <int IN, int DT, bool SCALED, int N>
 __global__ __launch_bounds__(kSortThreads) void unsort_kernel(const void *__restrict__ rows, const float *__restrict__ scales, const void *__restrict__ weights, int w_dtype, const int32_t *__restrict__ inverse,
-                                                              int64_t T, int k, int H, int lanes_log2, void *__restrict__ out) {
+                                                              int64_t T, int k, int H, int lanes_log2, void *__restrict__ out, int out_stride) {
   const int lanes = 1 << lanes_log2;
   const int64_t t = (int64_t)blockIdx.x * (kSortThreads >> lanes_log2) + (threadIdx.x >> lanes_log2);
   const int h = (int)(blockIdx.y * lanes + (threadIdx.x & (lanes - 1))) * 8, n = H - h;
@@ -194,26 +194,27 @@ __global__ __launch_bounds__(kSortThreads) void unsort_kernel(const void *__rest
   Octet<DT> o;
 #pragma unroll
   for (int i = 0; i < 8; i += 2) o.put2(i, acc[i], acc[i + 1]);
-  store_octet<DT>(out, t * H + h, n, o);
+  store_octet<DT>(out, t * out_stride + h, n, o);
 }
 
 template <int IN, int DT, bool SCALED = false>
-static hipError_t launch_unsort(const void *rows, const float *scales, const void *weights, int w_dtype, const int32_t *inverse, int64_t T, int k, int H, void *out, hipStream_t st) {
+static hipError_t launch_unsort(const void *rows, const float *scales, const void *weights, int w_dtype, const int32_t *inverse, int64_t T, int k, int H, void *out, int out_stride,
+                                hipStream_t st) {
   if (T == 0) return hipSuccess;
   const TokenGrid g(H, kSortThreads);
   auto *const kernel = k > 4 ? &unsort_kernel<IN, DT, SCALED, 8> : k > 2 ? &unsort_kernel<IN, DT, SCALED, 4> : &unsort_kernel<IN, DT, SCALED, 2>;
   kernel<<<dim3((unsigned)((T + g.tokens - 1) / g.tokens), (unsigned)g.columns), kSortThreads, 0, st>>>(rows, scales, weights, w_dtype, inverse, T, k, H,
-                                                                                                         __builtin_ctz((unsigned)g.lanes), out);
+                                                                                                         __builtin_ctz((unsigned)g.lanes), out, out_stride);
   return hipGetLastError();
 }
 hipError_t launch_unsort_tokens(const void *rows, const void *weights, int w_dtype, const int32_t *inverse, int64_t T, int k, int H, int dt, void *out, hipStream_t st) {
   auto *const launch = dt == 0 ? &launch_unsort<0, 0> : dt == 1 ? &launch_unsort<1, 1> : &launch_unsort<2, 2>;
-  return launch(rows, nullptr, weights, w_dtype, inverse, T, k, H, out, st);
+  return launch(rows, nullptr, weights, w_dtype, inverse, T, k, H, out, H, st);
 }
 hipError_t launch_unsort_made(const void *rows, const float *y_scales, const void *weights, int w_dtype, const int32_t *inverse, int64_t T, int k, int H, int dt, void *out,
-                              hipStream_t st) {
+                              int out_stride, hipStream_t st) {
   auto *const launch = y_scales ? (dt == 0 ? &launch_unsort<1, 0, true> : &launch_unsort<1, 1, true>) : dt == 0 ? &launch_unsort<2, 0> : &launch_unsort<2, 1>;
-  return launch(rows, y_scales, weights, w_dtype, inverse, T, k, H, out, st);
+  return launch(rows, y_scales, weights, w_dtype, inverse, T, k, H, out, out_stride, st);
 }
 
 __device__ __forceinline__ float wave_sum_f32(float v) {  // in a fixed order

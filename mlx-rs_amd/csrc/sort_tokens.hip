@@ -183,13 +183,15 @@ __global__ __launch_bounds__(kSortThreads) void unsort_kernel(const void *__rest
       w[j] = weights ? value_of(weights, s, w_dtype) : 1.f;
     }
     load_octets(v, rows, row, H, h, n);
+    float scale[N];  // (of the values, which are what they were with it; with the weight it may leave float32's range where their products do not)
     if constexpr (SCALED)
 #pragma unroll
-      for (int j = 0; j < N; ++j) w[j] *= scales[(row[j] < 0 ? 0 : row[j]) * ((H + 63) / 64) + h / 64];
+      for (int j = 0; j < N; ++j) scale[j] = scales[(row[j] < 0 ? 0 : row[j]) * ((H + 63) / 64) + h / 64];
 #pragma unroll
     for (int j = 0; j < N; ++j)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) acc[i] = row[j] >= 0 ? __builtin_fmaf(w[j], v[j].at(i), acc[i]) : acc[i];  // (not multiplied by zero: row or weight may be infinite)
+      for (int i = 0; i < 8; ++i)
+        acc[i] = row[j] >= 0 ? __builtin_fmaf(w[j], SCALED ? v[j].at(i) * scale[j] : v[j].at(i), acc[i]) : acc[i];  // (not multiplied by zero: row or weight may be infinite)
   }
   Octet<DT> o;
 #pragma unroll

@@ -46,6 +46,7 @@ struct F8Grid {
   int m_tiles, n_tiles, xcds_m, m_each, n_each;  // one matrix: xcds_m XCDs along the token rows, rectangles of m_each x n_each tiles
   int part_steps;                                // stages of a block: fewer than all where blocks share a tile, whose sums then go to a.parts
   int n_first, n_end;                            // columns of y (F8Product)
+  uint32_t first;                                // block, where a product takes more than one launch
 };
 
 // Sums of parts, in their order, a bias added, rounded.
@@ -81,14 +82,14 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, F8Gri
   const int begin = (int)blockIdx.y * g.part_steps, end = begin + g.part_steps < steps ? begin + g.part_steps : steps;
   // Blocks go round the eight XCDs, each of which has an L2 of its own.  One matrix: an XCD takes a rectangle of tiles.  Several: all tiles of a piece go to one XCD.  (A matrix's
   // pieces beside each other on one XCD, and blocks that take tile after tile, were tried: fewer misses of L2, and no faster, or slower by what the shares differ in time.)
-  const uint32_t xcd = blockIdx.x & 7, q = blockIdx.x >> 3;
+  const uint32_t block = g.first + blockIdx.x, xcd = block & 7, q = block >> 3;
   uint32_t mt, nt;
   if (!a.list) {
     mt = (xcd % (uint32_t)g.xcds_m) * (uint32_t)g.m_each + q % (uint32_t)g.m_each;
     nt = (xcd / (uint32_t)g.xcds_m) * (uint32_t)g.n_each + q / (uint32_t)g.m_each;
   } else if (g.m_tiles < kF8FewPieces) {  // (too few pieces to give each XCD as many: 26 rows at one matrix of 2128 x 1792 took 23 us, all on one, not 16)
-    mt = blockIdx.x % (uint32_t)g.m_tiles;
-    nt = blockIdx.x / (uint32_t)g.m_tiles;
+    mt = block % (uint32_t)g.m_tiles;
+    nt = block / (uint32_t)g.m_tiles;
   } else {
     mt = q / (uint32_t)g.n_tiles * 8 + xcd;
     nt = q % (uint32_t)g.n_tiles;
@@ -498,7 +499,7 @@ static hipError_t launch_tiles(const F8Product &p, hipStream_t st) {
   const int n_end = p.n_count ? p.n_first + p.n_count : p.N;
   const int64_t n_tiles = (n_end - p.n_first + (MODE == kPair ? 127 : kF8TileN - 1)) / (MODE == kPair ? 128 : kF8TileN), m_tiles = p.list ? f8_most_pieces(p.rows, p.n_mats, TM) : (p.rows + TM - 1) / TM;
   const int steps = f8_runs(p.K) * (p.pair_sum ? 2 : 1), parts = f8_plan(p).parts;
-  F8Grid g{(int)m_tiles, (int)n_tiles, 1, (int)m_tiles, (int)((n_tiles + 7) / 8), (steps + parts - 1) / parts, p.n_first, n_end};
+  F8Grid g{(int)m_tiles, (int)n_tiles, 1, (int)m_tiles, (int)((n_tiles + 7) / 8), (steps + parts - 1) / parts, p.n_first, n_end, 0};
   int64_t each;  // blocks of an XCD
   if (p.list) {
     each = m_tiles < kF8FewPieces ? (m_tiles * n_tiles + 7) / 8 : (m_tiles + 7) / 8 * n_tiles;
@@ -510,9 +511,12 @@ static hipError_t launch_tiles(const F8Product &p, hipStream_t st) {
     }
     each = (int64_t)g.m_each * g.n_each;
   }
-  if (each > (int64_t)1 << 19) return hipErrorInvalidValue;  // (a launch has less than 2^32 threads)
   const unsigned used = (unsigned)((steps + g.part_steps - 1) / g.part_steps);
-  f8_tiles_kernel<TM, MODE, EXACT, WIDE><<<dim3((unsigned)(each * 8), used, p.y1 ? 2 : 1), kF8Threads, lds, st>>>(p, g);
+  constexpr int64_t most = (int64_t)1 << 22;  // blocks of a launch, which has less than 2^32 threads
+  for (int64_t first = 0; first < each * 8; first += most) {
+    g.first = (uint32_t)first;
+    f8_tiles_kernel<TM, MODE, EXACT, WIDE><<<dim3((unsigned)(each * 8 - first < most ? each * 8 - first : most), used, p.y1 ? 2 : 1), kF8Threads, lds, st>>>(p, g);
+  }
   if (used > 1) f8_parts_kernel<<<dim3((unsigned)((p.N + 1023) / 1024), (unsigned)p.rows), 256, 0, st>>>(p.parts, (int)used, p.rows, p.N, p.bias, p.dt, p.y);
   return hipGetLastError();
 }

@@ -86,7 +86,9 @@ int mi_moe_switch_glu_f8(const void *x, const uint32_t *topk_idx, const void *to
                          int32_t n_experts, int32_t top_k, int32_t dtype, void *out, void *workspace,
                          size_t workspace_bytes, void *stream);
 /* Its gradients with respect to x and topk_w, from dout, the gradient at out; nothing of the forward call is needed (gate and up are computed again).  Roundings to e4m3
- * pass a gradient on as it is; dout and the gradients at gate and up are themselves rounded to e4m3 by runs of 128 ahead of their products with the weights.
+ * pass a gradient on as it is: what is differentiated is the call above without the rounding of h = silu(gate) * up, on rounded x.  So dweights[t][s] is the product of h as float32
+ * with the gradient at it, not of the codes that the forward call makes of h (a few percent of its length).  dout and the gradients at gate and up are themselves rounded to e4m3 by
+ * runs of 128 ahead of their products with the weights.
  * dx [T, hidden] of element type dtype, dweights [T, top_k] of element type w_dtype (zeros in slots that name no expert). */
 int mi_moe_switch_glu_f8_grad(const void *dout, const void *x, const uint32_t *topk_idx, const void *topk_w,
                               int32_t w_dtype, const mi_moe_f8_experts *experts, int64_t T, int32_t hidden,

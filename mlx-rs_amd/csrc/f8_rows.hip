@@ -185,6 +185,7 @@ hipError_t launch_swiglu_f8(const float *g, const float *u, int64_t rows, int co
 }
 
 // With s = sigmoid(g) and the slot's weight w:  dg = w dh u s (1 + g (1 - s)),  du = w dh g s,  dw = sum over the row of dh (g s u).
+// (dw of g s u itself, not of the codes that the forward call makes of it: the rounding is passed through as in dg and du.)
 // A block a row, its threads over the runs of both gradients; the weight's sum in float32, a thread's values in order, then the threads' in a fixed tree.
 __global__ __launch_bounds__(kRowThreads) void swiglu_f8_grad_kernel(F8SwigluGrad a) {
   __shared__ float sums[kRowThreads / kWave];

@@ -856,7 +856,7 @@ def switch_glu_f8(x, inds, weights, gate, up, down):
 
 def switch_glu_f8_grad(dout, x, inds, weights, gate, up, down):
     """The gradients of switch_glu_f8 with respect to x and the routing weights: (dx, dweights), of x's and weights' shapes and types.  Roundings to e4m3 pass a gradient on as
-    it is; nothing of the forward call is needed."""
+    it is: dweights is made of silu(gate) * up ahead of its rounding.  Nothing of the forward call is needed."""
     out = _native("switch_glu_f8_grad", dout, x, inds, weights, *gate, *up, *down)
     if out is not None:
         return out

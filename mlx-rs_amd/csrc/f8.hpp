@@ -14,12 +14,9 @@
 // tiles fast (4096 x 4096 x 4096 89 us, 157 on the bf16 ones; 4096 tokens through 8 of 128 experts of 2048 x 768 377 and 519).
 #pragma once
 #include "common.hpp"
+#include "f8_rule.hpp"
 
 namespace mi_moe {
-
-constexpr int kF8Run = 128;
-__host__ __device__ constexpr int f8_runs(int n) { return (n + kF8Run - 1) / kF8Run; }
-__host__ __device__ inline int64_t f8_row_bytes(int k) { return (int64_t)f8_runs(k) * kF8Run; }  // of a row of codes in a workspace: whole runs, zeros behind the last value
 
 // rows in e4m3 as the products read them: codes [rows][whole runs], scales [runs][rows]
 struct F8Rows {
@@ -62,20 +59,12 @@ struct F8Product {
 // Whether tiles sum on the bf16 instructions: for results (or, of gate/up pairs, tokens) of float16 and float32.  Us, to float16, so and on the f8 instructions, rounding of the rows and all:
 // 4096^3 157 and 87, 1000 x 4096 x 4096 49 and 39, its gradient 56 and 46; 4096 tokens through 8 of 128 experts of 2048 x 768 570 and 478.
 inline bool f8_exact(const F8Product &p) { return p.dt != 0; }
-// Parts are made where tiles of 64 x 256 and more are fewer than the chip's CUs: kF8MostParts of a product at most, 256 tiles of all of them.
-constexpr int kF8TileN = 256;  // columns of a tile
-constexpr int kF8MostParts = 16;
-constexpr int64_t kF8PartsMost = (int64_t)256 * 256 * 256;  // values
-inline size_t f8_parts_bytes(int64_t M, int N) {
-  const int64_t all = M * N * kF8MostParts;
-  return (size_t)(all < kF8PartsMost ? all : kF8PartsMost) * 4;
+inline F8Sizes f8_sizes(const F8Product &p) {
+  const bool by_matrix = p.list || p.ids;
+  return {p.rows, p.N, p.K, by_matrix ? p.n_mats : 1, by_matrix, p.list != nullptr, p.transpose, p.h != nullptr, p.pair_sum, f8_exact(p), p.parts != nullptr, p.few};
 }
-struct F8Plan {
-  int tile, parts;
-};
-F8Plan f8_plan(const F8Product &p);  // (f8_tiles.hip)
-// Rows of a piece: what the product's kernel takes at once (16 or 32: the one for a few rows).
-int f8_tile_rows(const F8Product &p);
+inline int f8_tile_rows(const F8Product &p) { return f8_tile_rows(f8_sizes(p)); }
+inline F8Plan f8_plan(const F8Product &p) { return f8_plan(f8_sizes(p)); }
 inline bool f8_few_rows(const F8Product &p) { return f8_tile_rows(p) < 64; }
 // Whether the blocks of a product for a few rows round them by themselves, where a matrix has `most` rows as a rule.  (A piece may hold as many as its kernel takes, of tokens that
 // name an expert more than once: there is room for them.)

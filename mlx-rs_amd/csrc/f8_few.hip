@@ -254,20 +254,6 @@ hipError_t launch_f8_token(const F8Product &p, const void *weights, int w_dtype,
   return hipGetLastError();
 }
 
-int f8_tile_rows(const F8Product &p) {
-  const int64_t mats = p.list || p.ids ? p.n_mats : 1, avg = p.rows / mats;
-  // One matrix: 4096 x 4096, 16 / 32 / 48 / 64 rows in pieces of 32 take 10 / 12 / 16 / 17 us.  By expert, this kernel / tiles, us: 128 matrices of 768 x 2048 at 2, 4, 6, 16 rows each
-  // 34 / 40, 39 / 41, 49 / 41, 62 / 43; 16 of 1792 x 2048, whose tiles are half as many as the CUs, at 4, 8, 12, 16 rows 18 / 20, 21 / 21, 22 / 22, 24 / 22.
-  const int64_t tiles = (p.N + (p.h ? 127 : 255)) / (p.h ? 128 : 256) * mats;
-  const int64_t few = !(p.list || p.ids) ? 48 : p.few ? p.few : tiles >= 256 ? 4 : 12;
-  if (p.transpose && !p.h && !p.pair_sum && p.rows <= few * mats) return avg > 4 ? 32 : 16;
-  // Tiles of 64 / 128 rows to float32, us: 16 matrices of 1792 x 2048 at 56, 72, 100, 160 rows each 29 / 31, 31 / 37, 45 / 39, 51 / 42; 128 of 768 x 2048 72 / 77, 94 / 87, 127 / 99,
-  // 171 / 142.  To bfloat16, of 64 / 128 / 256 rows: the 128 at 40, 72, 100, 128, 200 rows 50 / 51 / 53, 81 / 63 / 67, 105 / 73 / 79, 117 / 96 / 90, 168 / 133 / 107; the 16, which have
-  // fewer tiles than there are CUs, at 56, 100, 200, 260 rows 24 / 24 / 26, 41 / 26 / 29, 48 / 32 / 41, 54 / 50 / 43.
-  if (f8_exact(p)) return avg > 64 ? 128 : 64;
-  return avg > (tiles >= 256 ? 112 : 208) ? 256 : avg > 48 ? 128 : 64;
-}
-
 hipError_t launch_f8_few(const F8Product &p, hipStream_t st) {
   if (p.rows == 0) return hipSuccess;
   const unsigned tiles = (unsigned)((p.N + 15) / 16) * (p.y1 ? 2 : 1);

@@ -459,32 +459,6 @@ __global__ __launch_bounds__(kF8Threads) void f8_tiles_kernel(F8Product a, F8Gri
   }
 }
 
-// How many blocks share a tile's summed axis where the tiles alone leave CUs idle, and for one matrix the tile, by the time they take.  Us, measured: a launch 6; a stage 0.65 with a few
-// blocks and 1.1 with one on every CU (64 token rows), 1.0 and 1.45 (128), 1.7 and 2.2 (256); a join of parts 3, their bytes out and back 2.5 MB each.
-// By expert weights come from memory and not out of L2: a stage with a block on every CU 1.6 (64 token rows), a join 5.
-static F8Plan plan_of(const F8Product &p, int tile, int64_t tiles, F8Plan best, double &least) {
-  const int steps = f8_runs(p.K) * (p.pair_sum ? 2 : 1);
-  for (int parts = 1; parts <= (p.parts ? kF8MostParts : 1); parts *= 2) {
-    if (parts > 1 && (steps < 2 * parts || tiles * parts > 256 || (int64_t)parts * p.rows * p.N > kF8PartsMost)) break;
-    const double full = (double)(tiles * parts < 256 ? tiles * parts : 256) / 256, few = tile == 64 ? 0.65 : tile == 128 ? 1.0 : 1.7;
-    const double t = (double)((tiles * parts + 255) / 256) * ((steps + parts - 1) / parts) * (few + (p.list ? 0.95 : 0.45) * full) + (parts > 1 ? (p.list ? 5.0 : 3.0) + (double)parts * p.rows * p.N * 8 / 2.5e6 : 0.0);
-    if (t < least) least = t, best = {tile, parts};
-  }
-  return best;
-}
-F8Plan f8_plan(const F8Product &p) {
-  F8Plan best{64, 1};
-  double least = 1e30;
-  const int64_t columns = (p.N + kF8TileN - 1) / kF8TileN;
-  if (p.list) {  // (as many pieces as there are matrices with rows, if each has a few)
-    best.tile = f8_tile_rows(p);
-    return p.parts ? plan_of(p, best.tile, (p.rows / best.tile + (p.n_mats < p.rows ? p.n_mats : p.rows)) * columns, best, least) : best;
-  }
-  for (int tile : {64, 128, 256})
-    if (tile != 256 || !f8_exact(p)) best = plan_of(p, tile, (p.rows + tile - 1) / tile * columns, best, least);
-  return best;
-}
-
 template <int TM, F8Mode MODE, bool EXACT, bool WIDE>
 static hipError_t launch_tiles(const F8Product &p, hipStream_t st) {
   constexpr size_t lds = f8_tiles_lds(TM);

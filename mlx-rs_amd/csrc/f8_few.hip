@@ -5,7 +5,7 @@
 // axis, every fourth run of 128 values each; a lane's 32 bytes of a run are two pieces of 16, at 16 (l / 16) and 64 bytes on, for codes and rows alike (which values a lane
 // multiplies is free as long as both sides agree), so that one load takes 64 consecutive bytes of a weight row.  Codes go from memory into registers and there to bf16, where their
 // products are exact and sums float32 (f8.hpp; on the f8 instructions, which take the codes as they are, a launch waits for the same bytes: 300 rows at 128 matrices of 768 x 2048
-// 37 us either way, one row of 4096 x 4096 6.8); token rows come the same way out of L2.  A run's sums are scaled in float32; the waves' sums meet in LDS in a fixed order.
+// 37.4 us, 38.4 so; 16 rows of 4096 x 4096 11.7, 11.6; one 6.9, 7.3); token rows come the same way out of L2.  A run's sums are scaled in float32; the waves' sums meet in LDS in a fixed order.
 #include "f8.hpp"
 #include "octets.hpp"
 
@@ -61,7 +61,7 @@ __device__ __forceinline__ f32x4_t few_run(const u32x4_f8 (&w)[2], const FewRow 
   return sum;
 }
 template <int TG, F8In IN>
-__global__ __launch_bounds__(kFewWaves *kWave) void f8_few_kernel(F8Product a) {
+__global__ __launch_bounds__(kFewWaves *kWave, 5) void f8_few_kernel(F8Product a) {
   constexpr int AHEAD = TG == 1 ? 4 : 2;  // runs whose loads are in flight at once
   extern __shared__ __align__(16) uint8_t own_rows[];  // [rows][whole runs + 16], then scales [rows][runs]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ln = lane & 15, part = lane >> 4;
@@ -139,6 +139,7 @@ __global__ __launch_bounds__(kFewWaves *kWave) void f8_few_kernel(F8Product a) {
         sx[i][t] = IN == kCodes ? xs[t][(int64_t)j * a.x.rows] : xs[t][j];
       }
     }
+    __builtin_amdgcn_sched_barrier(0);  // (all loads ahead of the products: in between, and with one wave a SIMD less, 16 rows of 4096 x 4096 took 12.4 us, not 11.6)
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i)
 #pragma unroll

@@ -52,12 +52,21 @@ int check_linear(const char *who, const void *x, const void *w, const float *sca
   if (!aligned16(w)) return fail("%s: w must be 16-byte aligned", who);
   return 0;
 }
-size_t linear_bytes(int64_t M, int N, int K) {
-  Carver c(nullptr);
-  RowsIn(c, M, K);
-  c.take<uint4>((size_t)f8_list_places(M, kMostExperts));
-  c.take<char>(f8_parts_bytes(M, N));
-  return c.off + 256;
+// What linear() keeps in its workspace; parts only where the rows are few enough for them.
+struct LinearWs {
+  RowsIn x;
+  uint4 *list;
+  float *parts;
+  size_t bytes;
+  LinearWs(void *at, int64_t M, int N, int K) : LinearWs(Carver(at), M, N, K) {}
+
+ private:
+  LinearWs(Carver c, int64_t M, int N, int K)
+      : x(c, M, K), list(c.take<uint4>((size_t)f8_list_places(M, kMostExperts))),
+        parts(M <= f8_parts_rows(N, f8_runs(K)) ? reinterpret_cast<float *>(c.take<char>(f8_parts_bytes(M, N, f8_runs(K)))) : nullptr), bytes(c.off + 256) {}
+};
+size_t linear_bytes(int64_t M, int N, int K) {  // (never less for more rows: parts may be room that a larger product's rows take)
+  return std::max(LinearWs(nullptr, M, N, K).bytes, LinearWs(nullptr, std::min(M, f8_parts_rows(N, f8_runs(K))), N, K).bytes);
 }
 // A list for a product, or none for one matrix.
 void list_for(F8Product &p, F8Lists &lists, int i, uint4 *at) {
@@ -70,11 +79,9 @@ void list_for(F8Product &p, F8Lists &lists, int i, uint4 *at) {
 int linear(const char *who, const void *x, const void *w, const float *scales, const void *bias, const uint32_t *offsets, int64_t M, int E, int32_t N, int32_t K, int32_t transpose,
            int32_t dtype, void *y, void *workspace, size_t workspace_bytes, hipStream_t st) {
   if (check_workspace(who, workspace, workspace_bytes, linear_bytes(M, N, K))) return 1;
-  Carver c(workspace);
-  const RowsIn q(c, M, K);
-  uint4 *const list = c.take<uint4>((size_t)f8_list_places(M, kMostExperts));
+  const LinearWs ws(workspace, M, N, K);
   F8Product p{};
-  p.x = q.as(M);
+  p.x = ws.x.as(M);
   p.n_mats = E;
   p.rows = M;
   p.m[0] = p.m[1] = {static_cast<const uint8_t *>(w), scales};
@@ -88,15 +95,15 @@ int linear(const char *who, const void *x, const void *w, const float *scales, c
   lists.offsets = offsets;
   lists.n_mats = E;
   lists.rows = M;
-  if (offsets) list_for(p, lists, 0, list);
-  p.parts = reinterpret_cast<float *>(c.take<char>(f8_parts_bytes(M, N)));
+  if (offsets) list_for(p, lists, 0, ws.list);
+  p.parts = ws.parts;
   if (!offsets && f8_in_blocks(p, M)) {
     p.raw = x;
     p.raw_dt = dtype;
     MI_HIP(launch_f8_product(p, st));
     return 0;
   }
-  MI_HIP(launch_quantize_f8_rows(x, dtype, M, K, q.out(M, K), st, lists));
+  MI_HIP(launch_quantize_f8_rows(x, dtype, M, K, ws.x.out(M, K), st, lists));
   MI_HIP(launch_f8_product(p, st));
   return 0;
 }
@@ -122,7 +129,10 @@ struct ExpertsWs {
         list{c.take<uint4>((size_t)f8_list_places(P, E)), c.take<uint4>((size_t)f8_list_places(P, E)), c.take<uint4>((size_t)f8_list_places(P, E))}, sort(c.take<char>(sort_tokens_bytes(T, k, E))),
         x(c, T, H), dout(c, grad ? T : 0, H), g(c.take<float>(float_rows(P, E, grad) * I)), u(c.take<float>(float_rows(P, E, grad) * I)), dh(c.take<float>(grad ? (size_t)P * I : 0)),
         h(c, P, I, grad ? 2 : 1), y(c.take<char>(y_bytes(P, H, E))), y_scales(c.take<float>((size_t)P * ((H + 63) / 64))),
-        parts(reinterpret_cast<float *>(c.take<char>(grad ? f8_parts_bytes(P < (int64_t)16 * E ? P : (int64_t)16 * E, H > I ? H : I) : 0))), bytes(c.off + 256) {}
+        parts(reinterpret_cast<float *>(c.take<char>(grad ? parts_bytes(std::min(P, (int64_t)16 * E), H, I) : 0))), bytes(c.off + 256) {}
+  static size_t parts_bytes(int64_t rows, int H, int I) {  // the gradient at h, of H stages' values by I columns, and that at x
+    return std::max(f8_parts_bytes(rows, I, f8_stages(H, false)), f8_parts_bytes(rows, H, f8_stages(I, true)));
+  }
   static size_t y_bytes(int64_t P, int H, int E) {  // halves, or floats: of few rows an expert (all columns), or of some columns at a time
     return std::max({(size_t)P * H * 2, (size_t)std::min(P, (int64_t)16 * E) * H * 4, (size_t)P * half_columns(H) * 4});
   }

@@ -40,12 +40,19 @@ inline int f8_tile_rows(const F8Sizes &p) {
   return avg > (tiles >= 256 ? 112 : 208) ? 256 : avg > 48 ? 128 : 64;
 }
 
-// Parts are made where tiles of 64 x 256 and more are fewer than the chip's CUs: kF8MostParts of a product at most, 256 tiles of all of them.
+// Parts are made where tiles of 64 x 256 and more are fewer than the chip's CUs: kF8MostParts of a product at most, 256 tiles of all of them, two stages or more each.  A join costs by the parts' values
+// and saves by the stages: beyond 2^11 values for each value of the summed axis it does not pay.
 constexpr int kF8MostParts = 16;
-constexpr int64_t kF8PartsMost = (int64_t)256 * 256 * 256;  // values
-inline size_t f8_parts_bytes(int64_t M, int N) {
-  const int64_t all = M * N * kF8MostParts;
-  return (size_t)(all < kF8PartsMost ? all : kF8PartsMost) * 4;
+constexpr int f8_stages(int K, bool pair_sum) { return f8_runs(K) * (pair_sum ? 2 : 1); }
+constexpr int64_t f8_most_parts_values(int stages) {
+  const int64_t most = (int64_t)stages * kF8Run << 11, tiles = (int64_t)256 * 256 * 256;
+  return stages < 4 ? 0 : most < tiles ? most : tiles;
+}
+// the most rows of which parts are made, and room for them; with more rows never less
+constexpr int64_t f8_parts_rows(int N, int stages) { return f8_most_parts_values(stages) / (2 * (int64_t)N); }
+inline size_t f8_parts_bytes(int64_t M, int N, int stages) {
+  const int64_t all = M * N * kF8MostParts, most = f8_most_parts_values(stages);
+  return (size_t)(all < most ? all : most) * 4;
 }
 struct F8Plan {
   int tile, parts;
@@ -54,9 +61,9 @@ struct F8Plan {
 // blocks and 1.1 with one on every CU (64 token rows), 1.0 and 1.45 (128), 1.7 and 2.2 (256); a join of parts 3, their bytes out and back 2.5 MB each.
 // By expert weights come from memory and not out of L2: a stage with a block on every CU 1.6 (64 token rows), a join 5.
 inline F8Plan f8_plan_of(const F8Sizes &p, int tile, int64_t tiles, F8Plan best, double &least) {
-  const int steps = f8_runs(p.K) * (p.pair_sum ? 2 : 1);
+  const int steps = f8_stages(p.K, p.pair_sum);
   for (int parts = 1; parts <= (p.parts ? kF8MostParts : 1); parts *= 2) {
-    if (parts > 1 && (steps < 2 * parts || tiles * parts > 256 || (int64_t)parts * p.rows * p.N > kF8PartsMost)) break;
+    if (parts > 1 && (steps < 2 * parts || tiles * parts > 256 || (int64_t)parts * p.rows * p.N > f8_most_parts_values(steps))) break;
     const double full = (double)(tiles * parts < 256 ? tiles * parts : 256) / 256, few = tile == 64 ? 0.65 : tile == 128 ? 1.0 : 1.7;
     const double t = (double)((tiles * parts + 255) / 256) * ((steps + parts - 1) / parts) * (few + (p.pieces ? 0.95 : 0.45) * full) + (parts > 1 ? (p.pieces ? 5.0 : 3.0) + (double)parts * p.rows * p.N * 8 / 2.5e6 : 0.0);
     if (t < least) least = t, best = {tile, parts};

@@ -16,7 +16,7 @@ extern "C" int plan(long rows, int N, int K, int mats, int transpose, int exact,
   const F8Plan p = f8_plan(sizes(rows, N, K, mats, transpose, exact, pair_sum));
   return p.tile * 100 + p.parts;
 }
-extern "C" long parts_bytes(long M, int N) { return (long)f8_parts_bytes(M, N); }
+extern "C" long parts_bytes(long M, int N, int K, int pair_sum) { return M <= f8_parts_rows(N, f8_stages(K, pair_sum != 0)) ? (long)f8_parts_bytes(M, N, f8_stages(K, pair_sum != 0)) : 0; }
 """
 
 
@@ -32,7 +32,7 @@ def load(d):
     lib.parts_bytes.restype = C.c_long
     for fn in (lib.tile_rows, lib.plan):
         fn.argtypes = [C.c_long] + [C.c_int] * 6
-    lib.parts_bytes.argtypes = [C.c_long, C.c_int]
+    lib.parts_bytes.argtypes = [C.c_long] + [C.c_int] * 3
     return lib
 
 
@@ -62,5 +62,24 @@ def test_parts_have_room(rule):
                     for transpose, exact in ((True, False), (True, True), (False, False), (False, True)):
                         tile, parts = kernel(rule, rows, N, K, mats, transpose, exact)
                         assert tile in ((16, 32, 64, 128) if exact else (16, 32, 64, 128, 256)) and (tile >= 64 or transpose)
-                        assert parts == 1 or parts * rows * N * 4 <= rule.parts_bytes(rows, N)
+                        assert parts == 1 or parts * rows * N * 4 <= rule.parts_bytes(rows, N, K, False)
                         assert parts == 1 or 2 * parts <= (K + 127) // 128
+
+
+def test_workspaces_hold_no_parts_where_there_are_none():
+    from mlx_rs_amd import load_library
+    lib = load_library()
+
+    def linear(M, N, K):
+        n = C.c_size_t()
+        assert lib.mi_moe_linear_f8_workspace_size(M, N, K, C.byref(n)) == 0
+        return n.value
+
+    def rows(M, K):  # codes and scales, and the list of 512 matrices' pieces
+        return M * -(-K // 128) * 132 + 16 * (M // 16 + min(M, 513)) + 2048
+
+    assert linear(4096, 4096, 4096) <= rows(1024, 4096) + (33 << 20)  # (as much as for 1024 rows, which may come in parts)
+    assert linear(32768, 4096, 4096) <= rows(32768, 4096) and linear(4096, 4096, 256) <= rows(4096, 256)
+    for N, K in ((4096, 4096), (1, 16), (16384, 512), (256, 65536), (1000, 1040)):
+        sizes = [linear(M, N, K) for M in list(range(0, 5000, 7)) + [10000, 100000, 300000]]
+        assert sizes == sorted(sizes)

@@ -54,6 +54,15 @@ def test_kernels_by_size(rule, shape, want, exact):
     assert kernel(rule, **shape, exact=True) == exact
 
 
+def test_the_gpu_tests_reach_every_tile(rule):
+    torch = pytest.importorskip("torch")  # noqa: F841
+    import test_gpu_f8_large as t
+    for transpose in (True, False):
+        assert [kernel(rule, *shape, transpose=transpose) for shape in t.DENSE] == [(256, 1), (128, 1), (256, 1), (256, 1), (128, 2), (256, 8), (64, 4)]
+        assert [kernel(rule, *shape, transpose=transpose, exact=True) for shape in t.DENSE] == [(128, 1), (128, 1), (128, 1), (128, 1), (128, 2), (128, 4), (64, 4)]
+    assert kernel(rule, *t.SHARED, mats=1) == (256, 4) and kernel(rule, *t.SHARED, mats=1, exact=True) == (128, 4)
+
+
 def test_parts_have_room(rule):
     for rows in (1, 16, 49, 64, 100, 256, 300, 1000, 2048, 4096, 10000, 32768, 1 << 20):
         for N in (1, 16, 256, 1000, 4096, 16384, 1 << 20):

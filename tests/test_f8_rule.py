@@ -60,7 +60,7 @@ def test_the_gpu_tests_reach_every_tile(rule):
     for transpose in (True, False):
         assert [kernel(rule, *shape, transpose=transpose) for shape in t.DENSE] == [(256, 1), (128, 1), (256, 1), (256, 1), (128, 2), (256, 8), (64, 4)]
         assert [kernel(rule, *shape, transpose=transpose, exact=True) for shape in t.DENSE] == [(128, 1), (128, 1), (128, 1), (128, 1), (128, 2), (128, 4), (64, 4)]
-    assert kernel(rule, *t.SHARED, mats=1) == (256, 4) and kernel(rule, *t.SHARED, mats=1, exact=True) == (128, 4)
+    assert kernel(rule, *t.SHARED, mats=1) == (256, 4) and kernel(rule, *t.SHARED, mats=1, exact=True) == (128, 1)
 
 
 def test_parts_have_room(rule):

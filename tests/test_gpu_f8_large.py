@@ -61,7 +61,7 @@ def test_grouped_by_many_pieces_and_columns(transpose, dtype):
             o.within(y[at], want, off, f"grouped {e} {transpose} {dtype}")
 
 
-SHARED = (507, 250, 1040)  # rows by one matrix: listed pieces of 256 rows (128 in float16 and float32), of which four blocks share a tile
+SHARED = (507, 250, 1040)  # rows by one matrix: listed pieces of 256 rows, a tile of which four blocks share (of 128 rows and one block in float16 and float32)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

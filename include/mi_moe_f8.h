@@ -2,7 +2,8 @@
  * mi_moe_f8.h -- experts and linear layers whose weights are 8-bit floating point (e4m3: sign, four bits of exponent, three of mantissa, largest value 448, no
  * infinity), with a float32 scale for each block of 128 x 128, as checkpoints in that form hold them; tokens sorted by expert and back; and the gradients of all of
  * these for fine-tuning on frozen weights.  Same library, same conventions as mi_moe.h: int status and mi_moe_last_error, device pointers, work enqueued on `stream`,
- * nothing allocated and nothing kept by a call; arrays are row-major and contiguous, and need no more alignment than their elements' unless a comment says so.
+ * nothing allocated and nothing kept by a call; arrays are row-major and contiguous, and need no more alignment than their elements' unless a comment says so.  What a call writes
+ * overlaps none of its operands.
  */
 #ifndef MI_MOE_F8_H
 #define MI_MOE_F8_H
@@ -32,7 +33,7 @@ int mi_moe_sort_tokens_grad(const void *drows, const int32_t *inverse, int64_t T
  * w_dtype.  What rows hold where no slot names them has no part in it, whatever it is.  A place in `inverse` outside the T * top_k rows counts as no expert. */
 int mi_moe_unsort_tokens(const void *rows, const void *topk_w, int32_t w_dtype, const int32_t *inverse,
                          int64_t T, int32_t top_k, int32_t hidden, int32_t dtype, void *out, void *stream);
-/* Its gradients: drows (zeros in the rows of slots that name no expert) and dweights [T, top_k] of element type w_dtype (zeros in such slots).  drows must not be rows. */
+/* Its gradients: drows (zeros in the rows of slots that name no expert) and dweights [T, top_k] of element type w_dtype (zeros in such slots). */
 int mi_moe_unsort_tokens_grad(const void *dout, const void *rows, const void *topk_w, int32_t w_dtype,
                               const int32_t *inverse, int64_t T, int32_t top_k, int32_t hidden, int32_t dtype,
                               void *drows, void *dweights, void *stream);
@@ -69,7 +70,7 @@ int mi_moe_grouped_linear_f8(const void *x, const void *w, const float *scales, 
  * aligned; hidden and intermediate multiples of 16, up to 2^22; x and out [T, hidden] bfloat16 or float16; topk_w of element type w_dtype.  Products are summed as mi_moe_linear_f8's of
  * x's type (with bfloat16, a code of the rounded silu(gate) * up that lies at a border may so be its neighbour).  Experts' results are summed over the slots in float32, those of
  * bfloat16 tokens from 11 significant bits of each or more (of those below 2^-28 of the largest of 64 beside each other, fewer).  Slots that name no expert have no part in it.
- * T * hidden, each rounded up to whole runs of 128, below 2^32; T * top_k up to 2^24 - 1, and times hidden or intermediate up to 2^35.
+ * T times hidden, this rounded up to whole runs of 128, below 2^32 - 256; T * top_k up to 2^24 - 1, and times hidden or intermediate up to 2^35.
  * workspace >= mi_moe_switch_glu_f8_workspace_size (grad: of the gradient), 16-byte aligned. ---- */
 typedef struct {
   const void *gate;

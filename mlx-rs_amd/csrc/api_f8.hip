@@ -79,6 +79,7 @@ void list_for(F8Product &p, F8Lists &lists, int i, uint4 *at) {
 int linear(const char *who, const void *x, const void *w, const float *scales, const void *bias, const uint32_t *offsets, int64_t M, int E, int32_t N, int32_t K, int32_t transpose,
            int32_t dtype, void *y, void *workspace, size_t workspace_bytes, hipStream_t st) {
   if (check_workspace(who, workspace, workspace_bytes, linear_bytes(M, N, K))) return 1;
+  if (y == x) return fail("%s: y must not be x", who);
   const LinearWs ws(workspace, M, N, K);
   F8Product p{};
   p.x = ws.x.as(M);
@@ -190,6 +191,7 @@ int mi_moe_sort_tokens(const void *x, const uint32_t *topk_idx, int64_t T, int32
   if (check_types("sort_tokens", dtype) || check_slots("sort_tokens", T, top_k, hidden) || check_experts("sort_tokens", n_experts)) return 1;
   if (!offsets || (T > 0 && (!topk_idx || !order || !inverse || (rows && !x)))) return fail("sort_tokens: topk_idx, order, inverse, offsets, and x with rows, must be non-NULL");
   if (check_workspace("sort_tokens", workspace, workspace_bytes, sort_tokens_bytes(T, top_k, n_experts))) return 1;
+  if (rows && rows == x && T > 0) return fail("sort_tokens: rows must not be x");
   MI_HIP(launch_sort_tokens({topk_idx, T, top_k, n_experts, order, inverse, offsets}, x, dtype, hidden, rows, workspace, static_cast<hipStream_t>(stream)));
   return 0;
 } MI_CATCH("sort_tokens")
@@ -198,6 +200,7 @@ int mi_moe_sort_tokens_grad(const void *drows, const int32_t *inverse, int64_t T
   if (check_types("sort_tokens_grad", dtype) || check_slots("sort_tokens_grad", T, top_k, hidden)) return 1;
   if (T == 0) return 0;
   if (!drows || !inverse || !dx) return fail("sort_tokens_grad: drows, inverse and dx must be non-NULL");
+  if (dx == drows) return fail("sort_tokens_grad: dx must not be drows");
   MI_HIP(launch_unsort_tokens(drows, nullptr, 0, inverse, T, top_k, hidden, dtype, dx, static_cast<hipStream_t>(stream)));
   return 0;
 } MI_CATCH("sort_tokens_grad")
@@ -207,6 +210,7 @@ int mi_moe_unsort_tokens(const void *rows, const void *topk_w, int32_t w_dtype, 
   if (check_types("unsort_tokens", dtype, w_dtype) || check_slots("unsort_tokens", T, top_k, hidden)) return 1;
   if (T == 0) return 0;
   if (!rows || !topk_w || !inverse || !out) return fail("unsort_tokens: rows, topk_w, inverse and out must be non-NULL");
+  if (out == rows) return fail("unsort_tokens: out must not be rows");
   MI_HIP(launch_unsort_tokens(rows, topk_w, w_dtype, inverse, T, top_k, hidden, dtype, out, static_cast<hipStream_t>(stream)));
   return 0;
 } MI_CATCH("unsort_tokens")
@@ -216,7 +220,7 @@ int mi_moe_unsort_tokens_grad(const void *dout, const void *rows, const void *to
   if (check_types("unsort_tokens_grad", dtype, w_dtype) || check_slots("unsort_tokens_grad", T, top_k, hidden)) return 1;
   if (T == 0) return 0;
   if (!dout || !rows || !topk_w || !inverse || !drows || !dweights) return fail("unsort_tokens_grad: dout, rows, topk_w, inverse, drows and dweights must be non-NULL");
-  if (rows == drows) return fail("unsort_tokens_grad: drows must not be rows");
+  if (drows == rows || drows == dout) return fail("unsort_tokens_grad: drows must not be %s", drows == rows ? "rows" : "dout");
   MI_HIP(launch_unsort_tokens_grad(dout, rows, topk_w, w_dtype, inverse, T, top_k, hidden, dtype, drows, dweights, static_cast<hipStream_t>(stream)));
   return 0;
 } MI_CATCH("unsort_tokens_grad")

@@ -57,7 +57,7 @@ struct F8Product {
   float *hs;
 };
 // Whether tiles sum on the bf16 instructions: for results (or, of gate/up pairs, tokens) of float16 and float32.  Us, to float16, so and on the f8 instructions, rounding of the rows and all:
-// 4096^3 157 and 87, 1000 x 4096 x 4096 49 and 39, its gradient 56 and 46; 4096 tokens through 8 of 128 experts of 2048 x 768 570 and 478.
+// 4096^3 143 and 87, 1000 x 4096 x 4096 47 and 39, its gradient 53 and 46; 4096 tokens through 8 of 128 experts of 2048 x 768 540 and 478.
 inline bool f8_exact(const F8Product &p) { return p.dt != 0; }
 inline F8Sizes f8_sizes(const F8Product &p) {
   const bool by_matrix = p.list || p.ids;

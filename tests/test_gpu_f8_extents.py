@@ -7,7 +7,14 @@ import f8_cases as o  # noqa: E402
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(autouse=True)
+def give_back():
+    yield
+    torch.cuda.empty_cache()
+
+
 def needs(gigabytes):
+    torch.cuda.empty_cache()
     if torch.cuda.mem_get_info()[0] < gigabytes * 1e9:
         pytest.skip(f"needs {gigabytes} GB of memory")
 
